@@ -485,6 +485,56 @@ int mva_paged_mixed_run(const void* q, int64_t q_token_stride, int64_t q_head_st
                         int num_kv_heads, int head_dim, int page_size, float softmax_scale, int dtype,
                         void* stream);
 
+/*
+ * ---- MXFP4 cache ----
+ * A K or V cache in 4 bits: [num_pages][num_kv_heads] blocks of 1088 bytes, a
+ * block per page of 16 tokens and KV head: token t's 128 e2m1 codes at byte
+ * 64*t (element 2i in the low four bits of byte i), then its four E8M0 scales
+ * (2^(byte - 127), 255: NaN), one for 32 elements, at byte 1024 + 4*t.  Blocks
+ * lie page_stride_bytes / head_stride_bytes apart (multiples of 16, K and V
+ * alike).  Reduced-precision caches have no counterpart in the reference.
+ */
+
+/*
+ * Quantises row t of key and value (num_kv_heads rows of 128 elements, unit
+ * inner stride, 16-byte aligned) into slot slot_mapping[t] (page * 16 + token;
+ * slots < 0 or past the cache are skipped; the others must be distinct).
+ * Groups of 32 take the smallest scale 2^e with max|x| <= 7 * 2^e, e <= 125
+ * (bf16) or 13 (fp16); codes are x / 2^e to nearest even.  A group with an
+ * infinity or a NaN gets scale byte 255 and codes 0.
+ */
+int mva_kv_store_mxfp4(const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                       int64_t value_token_stride, int64_t value_head_stride, void* k_cache, void* v_cache,
+                       int64_t num_pages, int64_t page_stride_bytes, int64_t head_stride_bytes,
+                       const void* slot_mapping, int slot_is_int64, int64_t num_tokens, int num_kv_heads,
+                       int head_dim, int dtype, void* stream);
+
+/*
+ * The rows that the caches hold at slot_mapping, into key and value
+ * (arguments as mva_kv_store_mxfp4).  Slots < 0 or past the cache give zeros.
+ */
+int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stride, void* value,
+                      int64_t value_token_stride, int64_t value_head_stride, const void* k_cache,
+                      const void* v_cache, int64_t num_pages, int64_t page_stride_bytes, int64_t head_stride_bytes,
+                      const void* slot_mapping, int slot_is_int64, int64_t num_tokens, int num_kv_heads,
+                      int head_dim, int dtype, void* stream);
+
+/*
+ * mva_paged_decode over MXFP4 caches, with piece lists (wave_extra; no
+ * claims).  With counts ([3] int32 on the device) it is the fixed-shape launch
+ * of mva_paged_decode_graph: num_items, num_waves and num_merges are then
+ * capacities.  The workspace is mva_paged_decode's.
+ */
+int mva_paged_decode_mxfp4(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                           const void* v_cache, int64_t num_pages, int64_t page_stride_bytes,
+                           int64_t head_stride_bytes, const int32_t* block_tables, int64_t block_table_stride,
+                           const int32_t* seq_lens, const int32_t* counts, const int32_t* items, int64_t num_items,
+                           int64_t num_waves, const int32_t* wave_extra, int waves_per_group, const int32_t* merges,
+                           int64_t num_merges, int64_t num_part_slots, void* out, int64_t out_token_stride,
+                           int64_t out_head_stride, void* workspace, int64_t workspace_bytes, int num_q_heads,
+                           int num_kv_heads, int head_dim, int page_size, float softmax_scale, int dtype,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,36 @@ _SIGNATURES = {
             _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p,  # heads, head_dim, page, scale, dtype, stream
         ],
     ),
+    "mva_kv_store_mxfp4": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # key, value and their token and head strides
+            _c_void_p, _c_void_p, _i64, _i64, _i64,  # k_cache, v_cache, num_pages, page and head strides (bytes)
+            _c_void_p, _i32, _i64, _i32, _i32, _i32, _c_void_p,  # slots, int64 slots, tokens, heads, dim, dtype, stream
+        ],
+    ),
+    "mva_kv_load_mxfp4": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
+            _c_void_p, _c_void_p, _i64, _i64, _i64,
+            _c_void_p, _i32, _i64, _i32, _i32, _i32, _c_void_p,
+        ],
+    ),
+    "mva_paged_decode_mxfp4": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64,  # q, q_token_stride, q_head_stride
+            _c_void_p, _c_void_p, _i64, _i64, _i64,  # k_cache, v_cache, num_pages, page and head strides (bytes)
+            _c_void_p, _i64, _c_void_p,  # block_tables, block_table_stride, seq_lens
+            _c_void_p, _c_void_p, _i64, _i64,  # counts, items, num_items, num_waves
+            _c_void_p, _i32,  # wave_extra, waves_per_group
+            _c_void_p, _i64, _i64,  # merges, num_merges, num_part_slots
+            _c_void_p, _i64, _i64,  # out, out_token_stride, out_head_stride
+            _c_void_p, _i64,  # workspace, workspace_bytes
+            _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p,  # heads, head_dim, page, scale, dtype, stream
+        ],
+    ),
     "mva_decode_plan_listed_rows": (_i64, [_i64, _i64, _i32, _i32, _i32]),
     "mva_decode_plan_listed": (
         _i32,
@@ -204,7 +234,7 @@ _SIGNATURES = {
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 # The C ABI revision these signatures describe (mva_abi_version()).
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

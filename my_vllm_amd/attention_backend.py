@@ -631,6 +631,13 @@ class MI355XAttentionBackendMixin:
                       f"the batch has {common.num_prefill_seqs}")
         return reason
 
+    def _decode_schedule(self, total_pages: int) -> str:
+        return decode_schedule(total_pages, self.num_kv_heads, forced=self.decode_schedule_override)
+
+    def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
+        """(page ranges, wavefronts per workgroup) of a decode launch with piece lists."""
+        return decode_ranges(int(decode_counts.sum()), len(decode_counts), self.num_kv_heads, device)
+
     # ---- per-step metadata and plan ------------------------------------------
     def build_metadata(self, common) -> MI355XAttentionMetadata:
         check_common_metadata(common, require_cuda=self.require_device_metadata, common_type=self.common_type)
@@ -726,15 +733,13 @@ class MI355XAttentionBackendMixin:
                                     f"(partial slot, KV head) pairs, the decode plan has "
                                     f"{num_part_slots * self.num_kv_heads}")
             if not one_launch:
-                schedule = decode_schedule(int(decode_counts.sum()), self.num_kv_heads,
-                                           forced=self.decode_schedule_override)
+                schedule = self._decode_schedule(int(decode_counts.sum()))
                 if schedule == "listed":
                     if self.decode_waves_override:
                         groups, waves_per_group = listed_decode_groups(self.num_kv_heads, block_tables.device,
                                                                        override=self.decode_waves_override)
                     else:
-                        groups, waves_per_group = decode_ranges(int(decode_counts.sum()), len(decode_counts),
-                                                                self.num_kv_heads, block_tables.device)
+                        groups, waves_per_group = self._decode_ranges(decode_counts, block_tables.device)
                     items, wave_extra, num_decode_waves, num_part_slots, merges = plan_decode_listed(
                         decode_counts, common.num_prefill_seqs, common.num_prefill_tokens, self.num_kv_heads, groups
                     )
@@ -954,8 +959,11 @@ class MI355XAttentionBackendMixin:
                 raise RuntimeError("fused KV store: a new row's slot is not its sequence's last position; "
                                    "the cache holds the row, but this step's attention did not see it there")
             return out
-        (store if store is not None else ops.store_kvcache)(k, v, k_cache, v_cache, slot_mapping)
+        (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
         return self.forward(q, k, v, k_cache, v_cache, plan)
+
+    def _store_rows(self, k, v, k_cache, v_cache, slot_mapping) -> None:
+        ops.store_kvcache(k, v, k_cache, v_cache, slot_mapping)
 
     def forward(self, q, k, v, k_cache, v_cache, plan) -> torch.Tensor:
         metadata = plan_metadata(plan, MI355XAttentionMetadata, self.backend_name, self.plan_type)
@@ -1312,6 +1320,87 @@ class MI355XSplitAttentionBackend(MI355XAttentionBackend):
     default_attention_mode = "split"
 
 
+class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
+    """The backend over an MXFP4 cache: K and V in 4 bits, ``uint8`` caches of
+    ``ops.mxfp4_cache_shape`` (136 bytes a token and KV head instead of 512).
+
+    ``dtype`` is that of queries and outputs.  Rows go in through
+    ``ops.store_kvcache_mxfp4`` (``layers.MXFP4KVCacheStore``), which
+    :meth:`forward_with_kv_store` calls.  DECODE and its graphs, PREFILL and
+    WARMUP run as on the base; a MIXED batch runs as prefill + decode launches
+    (route MIXED_SPLIT) in both attention modes."""
+
+    backend_name = "mi355x_mxfp4"
+
+    def _store_rows(self, k, v, k_cache, v_cache, slot_mapping) -> None:
+        ops.store_kvcache_mxfp4(k, v, k_cache, v_cache, slot_mapping)
+
+    def _backend_mixed_reason(self) -> str | None:
+        return "MIXED batches over an MXFP4 cache run as prefill + decode launches"
+
+    def _decode_schedule(self, total_pages: int) -> str:
+        if self.decode_schedule_override not in (None, "listed"):
+            raise ValueError("decode over an MXFP4 cache runs piece lists only")
+        return "listed"
+
+    def _validate_inputs(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+        if q.device.type != "cuda" or q.dtype != self.dtype:
+            raise ValueError("query must be a CUDA tensor with the backend dtype")
+        if q.ndim != 3 or q.shape[1:] != (self.num_q_heads, self.head_dim):
+            raise ValueError("query must have shape [tokens, num_q_heads, head_dim]")
+        if q.stride(2) != 1:
+            raise ValueError("query must have unit stride in head_dim")
+        expected_tail = (self.num_kv_heads, ops.MXFP4_PAGE_BYTES)
+        for name, cache in (("key", k_cache), ("value", v_cache)):
+            if cache.device != q.device or cache.dtype != torch.uint8:
+                raise ValueError(f"{name} cache must be uint8 on the query device")
+            if cache.ndim != 3 or cache.shape[1:] != expected_tail:
+                raise ValueError(f"{name} cache must have shape [pages, num_kv_heads, {ops.MXFP4_PAGE_BYTES}]")
+            if cache.stride(2) != 1 or cache.stride(1) != ops.MXFP4_PAGE_BYTES:
+                raise ValueError(f"{name} cache pages must be contiguous")
+        if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+            raise ValueError("key and value caches must share shape and layout")
+
+    def forward_with_kv_store(self, q, k, v, k_cache, v_cache, slot_mapping, plan, store=None) -> torch.Tensor:
+        """The step's K/V rows quantised into the cache (``store``, or
+        ``ops.store_kvcache_mxfp4``), then :meth:`forward`."""
+        (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
+        return self.forward(q, k, v, k_cache, v_cache, plan)
+
+    def _run_decode(self, q, k_cache, v_cache, common, metadata: MI355XAttentionMetadata, output) -> None:
+        group = self.num_q_heads // self.num_kv_heads
+        ws_bytes = ops.decode_workspace_bytes(metadata.num_decode_part_slots, self.num_kv_heads, group)
+        ops.paged_decode_mxfp4(
+            q, k_cache, v_cache, metadata.block_tables, metadata.seq_lens,
+            metadata.decode_items, metadata.num_decode_items, metadata.num_decode_waves,
+            metadata.decode_merges, metadata.num_decode_merges, metadata.num_decode_part_slots,
+            output, self._get_workspace(ws_bytes, q.device), self.softmax_scale,
+            metadata.decode_wave_extra, metadata.decode_waves_per_group, validate=False,
+        )
+
+    def _run_decode_graph(self, q, k_cache, v_cache, state: MI355XFullDecodeGraphState) -> None:
+        counts, items, wave_extra, merges = state.views()
+        ops.paged_decode_mxfp4(
+            q, k_cache, v_cache, state.block_tables_buffer, state.seq_lens_buffer,
+            items, items.shape[0], wave_extra.numel() - 1, merges, merges.shape[0], state.part_slot_capacity,
+            state.output, state.workspace, self.softmax_scale, wave_extra, state.waves_per_group, counts=counts,
+            validate=False,
+        )
+
+    def _run_prefill(self, q, k_cache, v_cache, common, metadata: MI355XAttentionMetadata, output) -> None:
+        workspace, planned, key = self._take_prefill_plan(metadata, q.device)
+        ops.paged_prefill_mxfp4(
+            q, k_cache, v_cache, metadata.block_tables, metadata.seq_lens, metadata.query_start_loc,
+            common.num_prefill_seqs, metadata.prefill_max_tiles, workspace, output, self.softmax_scale,
+            planned=planned,
+        )
+        self._keep_prefill_plan(metadata, workspace, key)
+
+
+class MI355XMXFP4AttentionBackend(MI355XMXFP4AttentionBackendMixin, AttentionBackend):
+    """gfx950 backend over an MXFP4 cache ("mi355x_mxfp4")."""
+
+
 def integrate(registry: Any, base: type, plan_type: type, route_type: type, batch_type_enum: type,
               common_type: type, names: tuple[str, str] = ("mi355x", "mi355x_split")) -> tuple[type, type]:
     """Build the backend on another contract's classes and register it.
@@ -1339,6 +1428,8 @@ __all__ = [
     "MI355XAttentionBackend",
     "MI355XAttentionBackendMixin",
     "MI355XAttentionMetadata",
+    "MI355XMXFP4AttentionBackend",
+    "MI355XMXFP4AttentionBackendMixin",
     "MI355XSplitAttentionBackend",
     "integrate",
     "make_decode_plan",

@@ -1,0 +1,183 @@
+// The MXFP4 KV cache's writer and reader (format: mxfp4.h).
+//
+// Store: every group of 32 elements x of a K or V row becomes codes
+// rne(x / 2^e) and the byte e + 127, where 2^e is the smallest power of two
+// with max|x| <= 7 * 2^e: the largest element is then off by at most one unit
+// 2^e (half its step), where the smallest 2^e with max|x| < 8 * 2^e would cut
+// values up to 7.99 down to 6.  Division by a power of two is exact, so a code
+// depends on one rounding only.  e stops at 125 (bf16) or 13 (fp16), which
+// keeps every value read back finite in the row's type.  A group that holds an
+// infinity or a NaN becomes byte 255 (NaN) with codes 0.
+//
+// Both are bound by memory (324 bytes a row of one KV head): 16 lanes take a
+// row, 16 bytes of bf16/fp16 and 4 bytes of codes a lane; a group's maximum is
+// two lane exchanges away.  A workgroup takes 16 tokens of one head, so the
+// codes of consecutive tokens leave as whole lines.
+#include "mva_capi.h"
+#include "mxfp4.h"
+
+namespace mva {
+namespace {
+
+constexpr int kRowLanes = 16;
+constexpr int kRowsPerBlock = 16;
+
+// Maximum of both 16-bit halves over the four lanes of a group.
+__device__ inline uint32_t group_max(uint32_t m) {
+  m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+  return max(m, (uint32_t)__shfl_xor((int)m, 2));
+}
+
+// Where a slot's row of one head lies, or false: a negative slot or one past the cache.
+template <typename SlotT>
+__device__ inline bool slot_block(SlotT slot, int64_t num_pages, int64_t page_stride, int64_t head_stride, int head,
+                                  int64_t& block, int& token) {
+  const int64_t page = (int64_t)slot >> 4;
+  token = (int)slot & (kFp4PageTokens - 1);
+  block = page * page_stride + head * head_stride;
+  return (int64_t)slot >= 0 && page < num_pages;
+}
+
+// blockIdx.y: K heads, then V heads.
+template <typename T, typename SlotT>
+__global__ __launch_bounds__(kRowLanes* kRowsPerBlock) void kv_store_mxfp4_kernel(
+    const T* __restrict__ key, int64_t key_stride, int64_t key_head_stride, const T* __restrict__ value,
+    int64_t value_stride, int64_t value_head_stride, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
+    int64_t num_pages, int64_t page_stride, int64_t head_stride, const SlotT* __restrict__ slots, int64_t num_tokens,
+    int num_heads) {
+  typedef Fp4<T> F;
+  const int sub = threadIdx.x & (kRowLanes - 1);
+  const int64_t t = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x / kRowLanes);
+  if (t >= num_tokens) return;  // the 16 lanes of a row leave together
+  const bool is_v = (int)blockIdx.y >= num_heads;
+  const int h = (int)blockIdx.y - (is_v ? num_heads : 0);
+  int64_t block;
+  int token;
+  if (!slot_block(slots[t], num_pages, page_stride, head_stride, h, block, token)) return;
+  const T* row = is_v ? value + t * value_stride + h * value_head_stride : key + t * key_stride + h * key_head_stride;
+  const u32x4 x = ld16<u32x4>(row + 8 * sub);
+  // Magnitudes order as their bits do, in both halves of a word.
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max((x[i] >> 16) & 0x7fffu, x[i] & 0x7fffu));
+  m = group_max(m);
+  const bool finite = m < F::kInfBits;
+  // The exponent of the maximum, one more where its mantissa is above 1.75;
+  // 4 and 7 lie two binades above 1.
+  const int e = (int)((F::f32_bits(m) + 0x1fffffu) >> 23) - 2;
+  const uint32_t byte = finite ? (uint32_t)min(max(e, 0), F::kMaxScale) : 255u;
+  const float scale = byte == 0 ? 0x1p-127f : fp4_scale(byte);
+  uint32_t codes = 0;
+  if (finite) {
+    codes = F::template pack<0>(codes, x[0], scale);
+    codes = F::template pack<1>(codes, x[1], scale);
+    codes = F::template pack<2>(codes, x[2], scale);
+    codes = F::template pack<3>(codes, x[3], scale);
+  }
+  uint8_t* dst = (is_v ? v_cache : k_cache) + block;
+  *(uint32_t*)(dst + token * kFp4RowBytes + 4 * sub) = codes;
+  if ((sub & 3) == 0) dst[kFp4ScaleOffset + token * kFp4RowScales + (sub >> 2)] = (uint8_t)byte;
+}
+
+template <typename T, typename SlotT>
+__global__ __launch_bounds__(kRowLanes* kRowsPerBlock) void kv_load_mxfp4_kernel(
+    T* __restrict__ key, int64_t key_stride, int64_t key_head_stride, T* __restrict__ value, int64_t value_stride,
+    int64_t value_head_stride, const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
+    int64_t num_pages, int64_t page_stride, int64_t head_stride, const SlotT* __restrict__ slots, int64_t num_tokens,
+    int num_heads) {
+  const int sub = threadIdx.x & (kRowLanes - 1);
+  const int64_t t = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x / kRowLanes);
+  if (t >= num_tokens) return;
+  const bool is_v = (int)blockIdx.y >= num_heads;
+  const int h = (int)blockIdx.y - (is_v ? num_heads : 0);
+  T* row = is_v ? value + t * value_stride + h * value_head_stride : key + t * key_stride + h * key_head_stride;
+  typename Elem<T>::v8 y = {};
+  int64_t block;
+  int token;
+  if (slot_block(slots[t], num_pages, page_stride, head_stride, h, block, token)) {
+    const uint8_t* src = (is_v ? v_cache : k_cache) + block;
+    const uint32_t codes = *(const uint32_t*)(src + token * kFp4RowBytes + 4 * sub);
+    y = fp4_unpack8<T>(codes, fp4_scale(src[kFp4ScaleOffset + token * kFp4RowScales + (sub >> 2)]));
+  }
+  st16(row + 8 * sub, y);
+}
+
+// The checks that both directions share; *rc is set when the call ends here.
+bool rows_ready(const void* key, int64_t ks, int64_t khs, const void* value, int64_t vs, int64_t vhs,
+                const void* k_cache, const void* v_cache, int64_t num_pages, int64_t page_stride, int64_t head_stride,
+                const void* slots, int64_t num_tokens, int num_kv_heads, int head_dim, int dtype, int* rc) {
+  *rc = 0;
+  auto fail = [&](const char* what) {
+    *rc = set_error(what);
+    return false;
+  };
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_pages < 0) return fail("kv cache mxfp4: invalid sizes");
+  if (head_dim != 4 * kFp4Group) return fail("kv cache mxfp4: head_dim must be 128");
+  if (dtype != kBF16 && dtype != kF16) return fail("kv cache mxfp4: dtype must be bf16 or fp16");
+  if (num_tokens == 0) return false;
+  if (num_kv_heads > 32767) return fail("kv cache mxfp4: too many KV heads for one launch");
+  if ((num_tokens + kRowsPerBlock - 1) / kRowsPerBlock > 0xffffff)  // 2^32 threads a grid dimension
+    return fail("kv cache mxfp4: too many tokens for one launch");
+  if (!key || !value || !slots || (num_pages > 0 && (!k_cache || !v_cache)))
+    return fail("kv cache mxfp4: null buffer");
+  if (((uint64_t)(uintptr_t)key | (uint64_t)(uintptr_t)value | (uint64_t)(ks * 2) | (uint64_t)(khs * 2) |
+       (uint64_t)(vs * 2) | (uint64_t)(vhs * 2)) % 16)
+    return fail("kv cache mxfp4: key / value rows must be 16-byte aligned");
+  if (((uint64_t)(uintptr_t)k_cache | (uint64_t)(uintptr_t)v_cache | (uint64_t)page_stride | (uint64_t)head_stride) % 16)
+    return fail("kv cache mxfp4: cache buffers and strides must be 16-byte aligned");
+  return true;
+}
+
+}  // namespace
+}  // namespace mva
+
+extern "C" int mva_kv_store_mxfp4(const void* key, int64_t key_token_stride, int64_t key_head_stride,
+                                  const void* value, int64_t value_token_stride, int64_t value_head_stride,
+                                  void* k_cache, void* v_cache, int64_t num_pages, int64_t page_stride_bytes,
+                                  int64_t head_stride_bytes, const void* slot_mapping, int slot_is_int64,
+                                  int64_t num_tokens, int num_kv_heads, int head_dim, int dtype, void* stream) {
+  using namespace mva;
+  int rc;
+  if (!rows_ready(key, key_token_stride, key_head_stride, value, value_token_stride, value_head_stride, k_cache,
+                  v_cache, num_pages, page_stride_bytes, head_stride_bytes, slot_mapping, num_tokens, num_kv_heads,
+                  head_dim, dtype, &rc))
+    return rc;
+  if (num_pages == 0) return 0;
+  const dim3 grid((uint32_t)((num_tokens + kRowsPerBlock - 1) / kRowsPerBlock), (uint32_t)(2 * num_kv_heads));
+  auto go = [&](auto type, auto slot) {
+    typedef decltype(type) T;
+    typedef decltype(slot) S;
+    hipLaunchKernelGGL((kv_store_mxfp4_kernel<T, S>), grid, dim3(kRowLanes * kRowsPerBlock), 0, (hipStream_t)stream,
+                       (const T*)key, key_token_stride, key_head_stride, (const T*)value, value_token_stride,
+                       value_head_stride, (uint8_t*)k_cache, (uint8_t*)v_cache, num_pages, page_stride_bytes,
+                       head_stride_bytes, (const S*)slot_mapping, num_tokens, num_kv_heads);
+  };
+  if (dtype == kBF16) slot_is_int64 ? go(__bf16{}, int64_t{}) : go(__bf16{}, int32_t{});
+  else slot_is_int64 ? go(_Float16{}, int64_t{}) : go(_Float16{}, int32_t{});
+  return check_launch("kv_store_mxfp4");
+}
+
+extern "C" int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stride, void* value,
+                                 int64_t value_token_stride, int64_t value_head_stride, const void* k_cache,
+                                 const void* v_cache, int64_t num_pages, int64_t page_stride_bytes,
+                                 int64_t head_stride_bytes, const void* slot_mapping, int slot_is_int64,
+                                 int64_t num_tokens, int num_kv_heads, int head_dim, int dtype, void* stream) {
+  using namespace mva;
+  int rc;
+  if (!rows_ready(key, key_token_stride, key_head_stride, value, value_token_stride, value_head_stride, k_cache,
+                  v_cache, num_pages, page_stride_bytes, head_stride_bytes, slot_mapping, num_tokens, num_kv_heads,
+                  head_dim, dtype, &rc))
+    return rc;
+  const dim3 grid((uint32_t)((num_tokens + kRowsPerBlock - 1) / kRowsPerBlock), (uint32_t)(2 * num_kv_heads));
+  auto go = [&](auto type, auto slot) {
+    typedef decltype(type) T;
+    typedef decltype(slot) S;
+    hipLaunchKernelGGL((kv_load_mxfp4_kernel<T, S>), grid, dim3(kRowLanes * kRowsPerBlock), 0, (hipStream_t)stream,
+                       (T*)key, key_token_stride, key_head_stride, (T*)value, value_token_stride, value_head_stride,
+                       (const uint8_t*)k_cache, (const uint8_t*)v_cache, num_pages, page_stride_bytes,
+                       head_stride_bytes, (const S*)slot_mapping, num_tokens, num_kv_heads);
+  };
+  if (dtype == kBF16) slot_is_int64 ? go(__bf16{}, int64_t{}) : go(__bf16{}, int32_t{});
+  else slot_is_int64 ? go(_Float16{}, int64_t{}) : go(_Float16{}, int32_t{});
+  return check_launch("kv_load_mxfp4");
+}

@@ -5,6 +5,8 @@ bound to this package's gfx950 kernels through ``providers.resolve``.
   times ``x[..., I:]``; attribute ``provider_name``.
 * ``KVCacheStore`` (nanovllm/layers/attention.py:44-101): slot_mapping scatter
   of K/V rows into the paged cache; attribute ``kv_store_provider_name``.
+* ``MXFP4KVCacheStore``: the same over a cache held in 4 bits (no counterpart
+  in the reference).
 * ``RMSNorm`` (nanovllm/layers/layernorm.py:7-154): ``forward(x)``,
   ``forward(x, residual)`` and ``forward_inplace(x, residual)``; attributes
   ``rms_provider_name`` and ``add_rms_provider_name``.
@@ -50,6 +52,20 @@ class KVCacheStore(CustomOp):
 
     def forward_cuda(self, key, value, k_cache, v_cache, slot_mapping) -> None:
         ops.store_kvcache(key, value, k_cache, v_cache, slot_mapping)
+
+
+class MXFP4KVCacheStore(CustomOp):
+    """Quantise K/V tensors into a paged MXFP4 cache (``ops.mxfp4_cache_shape``);
+    its provider is that of ``kv_cache_store``."""
+
+    op_name = "kv_cache_store"
+
+    def __init__(self, custom_op_config: CustomOpConfig | None = None) -> None:
+        super().__init__(custom_op_config)
+        self.kv_store_provider_name = providers.resolve(self)
+
+    def forward_cuda(self, key, value, k_cache, v_cache, slot_mapping) -> None:
+        ops.store_kvcache_mxfp4(key, value, k_cache, v_cache, slot_mapping)
 
 
 class RMSNorm(CustomOp):
@@ -120,4 +136,4 @@ class RotaryEmbedding(CustomOp):
         )
 
 
-__all__ = ["KVCacheStore", "RMSNorm", "RotaryEmbedding", "SiluAndMul", "rope_table"]
+__all__ = ["KVCacheStore", "MXFP4KVCacheStore", "RMSNorm", "RotaryEmbedding", "SiluAndMul", "rope_table"]

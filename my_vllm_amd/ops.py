@@ -879,3 +879,245 @@ def paged_mixed_run(
         workspace.data_ptr(), workspace.numel() * workspace.element_size(),
         *_tail_args(q, k_cache, softmax_scale),
     )
+
+
+# ---- MXFP4 cache --------------------------------------------------------------
+
+# Bytes of one page of one KV head in an MXFP4 cache (kFp4BlockBytes): 16 tokens
+# of 64 bytes of codes, then their 4 scale bytes each.
+MXFP4_PAGE_BYTES = 1088
+
+
+def mxfp4_cache_shape(num_pages: int, num_kv_heads: int) -> tuple[int, int, int]:
+    """Shape of one ``uint8`` MXFP4 cache (K or V) of ``num_pages`` pages of 16
+    tokens: 136 bytes a token and KV head for K and V, where bf16 takes 512.
+
+    A block ``cache[page, head]`` holds the page's 16 rows of 128 elements as
+    e2m1 codes (element ``2i`` in the low four bits of byte ``i``), 64 bytes a
+    row, then four E8M0 scale bytes a row, one for 32 elements.  A zeroed cache
+    holds zeros."""
+    return int(num_pages), int(num_kv_heads), MXFP4_PAGE_BYTES
+
+
+def _check_mxfp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, device: torch.device) -> None:
+    """What the kernels rely on: device memory in blocks of 1088 bytes, K and V
+    of one layout (only K's strides cross the ABI), no two blocks overlapping."""
+    for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.size(2) != MXFP4_PAGE_BYTES:
+            raise TypeError(f"{name} must be a uint8 [pages, num_kv_heads, {MXFP4_PAGE_BYTES}] MXFP4 cache")
+        if cache.device != device:
+            raise RuntimeError(f"{name} must be on the device of the other tensors")
+        if cache.stride(2) != 1 or any(cache.size(d) > 1 and cache.stride(d) < MXFP4_PAGE_BYTES for d in (0, 1)):
+            raise ValueError(f"{name} blocks must be contiguous and apart")
+    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+        raise ValueError("k_cache and v_cache must share shape and layout")
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """``_native.call`` with ``device`` current: a stream handle alone does not
+    name the device of its default stream."""
+    if device.index == torch.cuda.current_device():
+        _native.call(name, *args)
+        return
+    with torch.cuda.device(device):
+        _native.call(name, *args)
+
+
+def _dense_slots(slot_mapping: torch.Tensor, num_tokens: int, device: torch.device) -> torch.Tensor:
+    if slot_mapping.numel() != num_tokens:
+        raise ValueError("slot_mapping must contain one slot per token")
+    if slot_mapping.dtype not in (torch.int32, torch.int64):
+        raise TypeError("slot_mapping must be int32 or int64")
+    if slot_mapping.device != device:
+        raise RuntimeError("slot_mapping must be on the device of the other tensors")
+    return slot_mapping.reshape(-1).contiguous()  # the kernels index it densely
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` if its rows start at multiples of 16 bytes, else a copy."""
+    bits = x.data_ptr() | x.stride(0) * 2 | x.stride(1) * 2
+    return x if bits % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
+def store_kvcache_mxfp4(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+) -> None:
+    """Quantise K/V rows into an MXFP4 cache by ``slot_mapping`` (``page * 16 +
+    offset``; a slot that is negative or past the cache is skipped).
+
+    ``key``/``value`` are bf16/fp16 ``[N, Hkv, 128]`` with unit inner stride
+    (views of a packed projection work); the caches ``uint8`` of
+    :func:`mxfp4_cache_shape`, K and V of one layout.  Each 32 elements share the
+    smallest power-of-two scale under which the largest of them is at most 7
+    (it is then stored as 4 or 6, off by at most 1) and are rounded to the
+    nearest code, ties to even.  Scales stop at 2^125 (bf16) or 2^13 (fp16), so
+    that every value read back is finite; a group that holds an infinity or a
+    NaN reads back as NaN.  The slots >= 0 of one call must be distinct."""
+    if key.dim() != 3 or value.shape != key.shape or key.size(2) != HEAD_DIM:
+        raise ValueError(f"key and value must both have shape [tokens, num_kv_heads, {HEAD_DIM}]")
+    num_tokens, num_heads, _ = key.shape
+    if not key.is_cuda or value.device != key.device:
+        raise RuntimeError("store_kvcache_mxfp4 expects CUDA tensors on one device")
+    if key.dtype not in _native.DTYPE_CODES or value.dtype != key.dtype:
+        raise TypeError("key and value must both be bfloat16 or float16")
+    if key.stride(-1) != 1 or value.stride(-1) != 1:
+        raise ValueError("key/value must have unit stride in the head dimension")
+    _check_mxfp4_caches(k_cache, v_cache, key.device)
+    if k_cache.size(1) != num_heads:
+        raise ValueError("the cache must have the key's number of KV heads")
+    slots = _dense_slots(slot_mapping, num_tokens, key.device)
+    if num_tokens == 0 or num_heads == 0:
+        return
+    key, value = _aligned_rows(key), _aligned_rows(value)
+    _call_on(
+        key.device, "mva_kv_store_mxfp4",
+        key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.size(0), k_cache.stride(0), k_cache.stride(1),
+        slots.data_ptr(), int(slots.dtype == torch.int64), num_tokens, num_heads, HEAD_DIM,
+        _native.dtype_code(key.dtype), _native.stream_handle(key.device),
+    )
+
+
+def load_kvcache_mxfp4(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    dtype: torch.dtype = torch.bfloat16,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The K and V rows that an MXFP4 cache holds at ``slot_mapping``, as new
+    ``[N, Hkv, 128]`` tensors of ``dtype`` (bf16 or fp16): exactly the values
+    that the attention reads.  A slot that is negative or past the cache gives
+    zeros.  (Values that a bf16 row put beyond fp16's range round to it as
+    usual.)"""
+    if not k_cache.is_cuda:
+        raise RuntimeError("load_kvcache_mxfp4 expects CUDA tensors")
+    _check_mxfp4_caches(k_cache, v_cache, k_cache.device)
+    if dtype not in _native.DTYPE_CODES:
+        raise TypeError("load_kvcache_mxfp4 reads rows as bfloat16 or float16")
+    num_tokens, num_heads = slot_mapping.numel(), k_cache.size(1)
+    slots = _dense_slots(slot_mapping, num_tokens, k_cache.device)
+    key = torch.empty((num_tokens, num_heads, HEAD_DIM), dtype=dtype, device=k_cache.device)
+    value = torch.empty_like(key)
+    if key.numel() == 0:
+        return key, value
+    _call_on(
+        key.device, "mva_kv_load_mxfp4",
+        key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.size(0), k_cache.stride(0), k_cache.stride(1),
+        slots.data_ptr(), int(slots.dtype == torch.int64), num_tokens, num_heads, HEAD_DIM,
+        _native.dtype_code(dtype), _native.stream_handle(key.device),
+    )
+    return key, value
+
+
+def _check_paged_mxfp4(q, out, k_cache, v_cache, int32_arrays=(), buffers=()) -> None:
+    """:func:`_check_paged` over MXFP4 caches."""
+    device = q.device
+    if not q.is_cuda:
+        raise RuntimeError("paged attention expects CUDA tensors")
+    if out.device != device:
+        raise RuntimeError("paged attention: out must be on the query's device")
+    if q.dtype not in _native.DTYPE_CODES or out.dtype != q.dtype:
+        raise TypeError("paged attention: query and out must share bfloat16 or float16")
+    for name, t in (("query", q), ("out", out)):
+        if t.dim() != 3 or t.size(2) != HEAD_DIM or t.stride(2) != 1:
+            raise ValueError(f"paged attention: {name} must be [tokens, heads, {HEAD_DIM}] with unit inner stride")
+    if out.shape[1] != q.shape[1] or out.shape[0] < q.shape[0]:
+        raise ValueError("paged attention: out must hold the query's rows")
+    _check_mxfp4_caches(k_cache, v_cache, device)
+    for name, t in int32_arrays:
+        if t is None:
+            continue
+        dense = t.stride(-1) == 1 if name == "block_tables" else t.is_contiguous()
+        if t.device != device or t.dtype != torch.int32 or not dense:
+            raise ValueError(f"paged attention: {name} must be a dense int32 CUDA tensor on the query's device")
+    for name, t in buffers:
+        if t is not None and (t.device != device or not t.is_contiguous()):
+            raise ValueError(f"paged attention: {name} must be a contiguous CUDA tensor on the query's device")
+
+
+def paged_decode_mxfp4(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    items: torch.Tensor,
+    num_items: int,
+    num_waves: int,
+    merges: torch.Tensor | None,
+    num_merges: int,
+    num_part_slots: int,
+    out: torch.Tensor,
+    workspace: torch.Tensor | None,
+    softmax_scale: float,
+    wave_extra: torch.Tensor,
+    waves_per_group: int = 1,
+    *,
+    counts: torch.Tensor | None = None,
+    validate: bool = True,
+) -> None:
+    """:func:`paged_decode` over MXFP4 caches, with piece lists (``wave_extra``).
+
+    With ``counts`` (int32 ``[3]`` on the device) it is the fixed-shape launch
+    of :func:`paged_decode_graph`: ``counts`` holds this step's ``{num_items,
+    num_waves, num_merges}`` and the scalar arguments are capacities."""
+    if validate:
+        _check_paged_mxfp4(q, out, k_cache, v_cache,
+                           (("block_tables", block_tables), ("seq_lens", seq_lens), ("items", items),
+                            ("merges", merges), ("wave_extra", wave_extra), ("counts", counts)),
+                           (("workspace", workspace),))
+        if counts is not None and counts.numel() < 3:
+            raise ValueError("graph decode needs 3 counts")
+    _call_on(
+        q.device, "mva_paged_decode_mxfp4",
+        q.data_ptr(), q.stride(0), q.stride(1),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], k_cache.stride(0), k_cache.stride(1),
+        block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(),
+        counts.data_ptr() if counts is not None else 0, items.data_ptr(), int(num_items), int(num_waves),
+        wave_extra.data_ptr() if wave_extra is not None else 0, int(waves_per_group),
+        merges.data_ptr() if merges is not None else 0, int(num_merges), int(num_part_slots),
+        out.data_ptr(), out.stride(0), out.stride(1),
+        workspace.data_ptr() if workspace is not None else 0,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0,
+        q.shape[1], k_cache.shape[1], q.shape[2], PAGE_SIZE, float(softmax_scale),
+        _native.dtype_code(q.dtype), _native.stream_handle(q.device),
+    )
+
+
+def paged_prefill_mxfp4(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    num_seqs: int,
+    max_tiles: int,
+    workspace: torch.Tensor,
+    out: torch.Tensor,
+    softmax_scale: float,
+    *,
+    validate: bool = True,
+    planned: bool = False,
+) -> None:
+    """:func:`paged_prefill` over MXFP4 caches: the pages of the batch are read
+    back into rows of the query's type, which the prefill kernel then takes."""
+    if validate:
+        _check_paged_mxfp4(q, out, k_cache, v_cache,
+                           (("block_tables", block_tables), ("seq_lens", seq_lens),
+                            ("query_start_loc", query_start_loc)), (("workspace", workspace),))
+    tables = block_tables[:num_seqs]
+    if tables.numel() == 0:
+        return
+    offsets = torch.arange(PAGE_SIZE, device=q.device)
+    slots = torch.where(tables[..., None] >= 0, tables.long()[..., None] * PAGE_SIZE + offsets, -1)
+    key, value = load_kvcache_mxfp4(k_cache, v_cache, slots, q.dtype)
+    shape = (tables.numel(), PAGE_SIZE, k_cache.shape[1], HEAD_DIM)
+    pages = torch.arange(tables.numel(), dtype=torch.int32, device=q.device).view(tables.shape)
+    paged_prefill(q, key.view(shape), value.view(shape), pages, seq_lens, query_start_loc, num_seqs, max_tiles,
+                  workspace, out, softmax_scale, planned=planned)

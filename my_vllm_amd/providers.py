@@ -50,7 +50,7 @@ _TABLE = {
     for spec in (
         KernelProvider("silu_and_mul", ("mva_silu_and_mul",),
                        frozenset({"custom_cuda", "adaptive_cuda", "flashinfer"})),
-        KernelProvider("kv_cache_store", ("mva_kv_store",), frozenset({"native_triton"})),
+        KernelProvider("kv_cache_store", ("mva_kv_store", "mva_kv_store_mxfp4"), frozenset({"native_triton"})),
         KernelProvider("rms_norm", ("mva_rms_norm",), frozenset({"flashinfer"})),
         KernelProvider("fused_add_rms_norm", ("mva_fused_add_rms_norm",), frozenset({"flashinfer"})),
         KernelProvider("rotary_embedding", ("mva_qk_norm_rope_store",), frozenset({"flashinfer"})),
