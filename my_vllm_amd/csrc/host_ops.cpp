@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/my_vllm_amd.h"
@@ -415,6 +416,128 @@ PyObject* forward_inputs_ok(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- MXFP4 caches ----
+
+constexpr int64_t kFp4Block = 1088;
+
+// Whether both are MXFP4 caches of one layout on `device`, which is current
+// (another device takes the general path, which makes it current).
+bool fp4_caches(const Tensor* kc, const Tensor* vc, c10::Device device) {
+  if (!kc || !vc || kc->dim() != 3 || kc->sizes() != vc->sizes() || kc->strides() != vc->strides() ||
+      kc->size(2) != kFp4Block || kc->stride(2) != 1)
+    return false;
+  for (const Tensor* c : {kc, vc})
+    if (c->scalar_type() != at::kByte || c->device() != device) return false;
+  for (int d : {0, 1})
+    if (kc->size(d) > 1 && kc->stride(d) < kFp4Block) return false;
+  return device.index() == c10::hip::current_device();
+}
+
+// Rows that start at multiples of 16 bytes.
+bool aligned_rows(const Tensor& t) {
+  return (((uint64_t)(uintptr_t)ptr(t)) | (uint64_t)(t.stride(0) * 2) | (uint64_t)(t.stride(1) * 2)) % 16 == 0;
+}
+
+// (key, value, k_cache, v_cache, slot_mapping): True when launched.
+PyObject* store_kvcache_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 5) return none();
+    const Tensor *k = plain(a[0]), *v = plain(a[1]), *kc = plain(a[2]), *vc = plain(a[3]), *slots = plain(a[4]);
+    if (!k || !v || !slots || !head_rows(*k, *k) || !head_rows(*v, *k) || k->sizes() != v->sizes() ||
+        k->numel() == 0 || !fp4_caches(kc, vc, k->device()) || kc->size(1) != k->size(1) ||
+        !slot_list(*slots, *k, k->size(0)) || !aligned_rows(*k) || !aligned_rows(*v))
+      return none();
+    const int code = dtype_code(*k);
+    if (code < 0) return none();
+    void* const stream = stream_of(*k);
+    const int status = unlocked(
+        mva_kv_store_mxfp4, ptr(*k), k->stride(0), k->stride(1), ptr(*v), v->stride(0), v->stride(1), ptr(*kc),
+        ptr(*vc), kc->size(0), kc->stride(0), kc->stride(1), ptr(*slots), slots->scalar_type() == at::kLong,
+        k->size(0), (int)k->size(1), kHeadDim, code, stream);
+    return launched("mva_kv_store_mxfp4", status);
+  });
+}
+
+// (k_cache, v_cache, slot_mapping, MVA_DTYPE_* of the rows): (key, value).
+PyObject* load_kvcache_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int64_t code;
+    if (n != 4 || !as_int(a[3], &code) || (code != MVA_DTYPE_BF16 && code != MVA_DTYPE_F16)) return none();
+    const Tensor *kc = plain(a[0]), *vc = plain(a[1]), *slots = plain(a[2]);
+    if (!kc || !slots || !fp4_caches(kc, vc, kc->device()) || !slot_list(*slots, *kc, slots->numel()) ||
+        slots->numel() == 0 || kc->size(1) == 0)
+      return none();
+    const int64_t tokens = slots->numel(), heads = kc->size(1);
+    const auto options =
+        kc->options().dtype(code == MVA_DTYPE_BF16 ? at::kBFloat16 : at::kHalf).requires_grad(false);
+    const Tensor key = at::empty({tokens, heads, kHeadDim}, options), value = at::empty({tokens, heads, kHeadDim}, options);
+    void* const stream = stream_of(*kc);
+    const int status = unlocked(
+        mva_kv_load_mxfp4, ptr(key), key.stride(0), key.stride(1), ptr(value), value.stride(0), value.stride(1),
+        ptr(*kc), ptr(*vc), kc->size(0), kc->stride(0), kc->stride(1), ptr(*slots),
+        slots->scalar_type() == at::kLong, tokens, (int)heads, kHeadDim, (int)code, stream);
+    if (status != 0) return launched("mva_kv_load_mxfp4", status, nullptr);
+    PyObject* pair = PyTuple_New(2);
+    if (pair == nullptr) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(key));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(value));
+    return pair;
+  });
+}
+
+// The paged operators' shared tensors, checked as ops._check_paged_mxfp4 does.
+struct PagedFp4 : Paged {
+  bool read(PyObject* q_, PyObject* kc_, PyObject* vc_, PyObject* bt_, PyObject* sl_, PyObject* out_) {
+    q = plain(q_), kc = plain(kc_), vc = plain(vc_), bt = plain(bt_), sl = plain(sl_), out = plain(out_);
+    if (!q || !bt || !sl || !out || !head_rows(*q, *q) || !head_rows(*out, *q) || out->size(1) != q->size(1) ||
+        out->size(0) < q->size(0))
+      return false;
+    code = dtype_code(*q);
+    return code >= 0 && fp4_caches(kc, vc, q->device()) && bt->dim() == 2 && bt->stride(1) == 1 &&
+           bt->scalar_type() == at::kInt && bt->device() == q->device() && ints(sl);
+  }
+};
+
+// (q, k_cache, v_cache, block_tables, seq_lens, counts | None, items,
+//  num_items, num_waves, merges | None, num_merges, num_part_slots, out,
+//  workspace, scale, wave_extra, waves_per_group): True when launched.
+PyObject* paged_decode_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    PagedFp4 p;
+    int64_t items_n, waves, merges_n, slots_n, per_group;
+    double scale;
+    if (n != 17 || !p.read(a[0], a[1], a[2], a[3], a[4], a[12])) return none();
+    const Tensor *counts = a[5] == Py_None ? nullptr : plain(a[5]), *items = plain(a[6]);
+    const Tensor *merges = a[9] == Py_None ? nullptr : plain(a[9]), *ws = plain(a[13]), *extra = plain(a[15]);
+    if ((a[5] != Py_None && (!p.ints(counts) || counts->numel() < 3)) || !p.ints(items) ||
+        (a[9] != Py_None && !p.ints(merges)) || !p.ints(extra) || !p.bytes(ws) || !as_int(a[7], &items_n) ||
+        !as_int(a[8], &waves) || !as_int(a[10], &merges_n) || !as_int(a[11], &slots_n) || !as_float(a[14], &scale) ||
+        !as_int(a[16], &per_group))
+      return none();
+    const Tensor &q = *p.q, &kc = *p.kc, &out = *p.out;
+    void* const stream = stream_of(q);
+    const int status = unlocked(
+        mva_paged_decode_mxfp4, ptr(q), q.stride(0), q.stride(1), ptr(kc), ptr(*p.vc), kc.size(0), kc.stride(0),
+        kc.stride(1), words(p.bt), p.bt->stride(0), words(p.sl), words(counts), words(items), items_n, waves,
+        words(extra), (int)per_group, words(merges), merges_n, slots_n, ptr(out), out.stride(0), out.stride(1),
+        ptr(*ws), nbytes(ws), (int)q.size(1), (int)kc.size(1), kHeadDim, 16, (float)scale, p.code, stream);
+    return launched("mva_paged_decode_mxfp4", status);
+  });
+}
+
+// (q, k_cache, v_cache, MVA_DTYPE_* of the backend, num_q_heads, num_kv_heads): forward_inputs_ok over MXFP4 caches.
+PyObject* forward_inputs_ok_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int64_t code, hq, hkv;
+    if (n != 6 || !as_int(a[3], &code) || !as_int(a[4], &hq) || !as_int(a[5], &hkv)) return none();
+    const Tensor *q = plain(a[0]), *kc = plain(a[1]), *vc = plain(a[2]);
+    if (!q || dtype_code(*q) != code || !head_rows(*q, *q) || q->size(1) != hq || !fp4_caches(kc, vc, q->device()) ||
+        kc->size(1) != hkv || kc->stride(1) != kFp4Block)
+      return none();
+    Py_RETURN_TRUE;
+  });
+}
+
 // (device index): number of the graph capture that torch's current stream of
 // the device is in, or 0.
 PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -435,6 +558,8 @@ PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef kMethods[] = {MVA_METHOD(silu_and_mul),       MVA_METHOD(rms_norm),      MVA_METHOD(fused_add_rms_norm),
                           MVA_METHOD(qk_norm_rope_store), MVA_METHOD(paged_decode),  MVA_METHOD(paged_prefill),
                           MVA_METHOD(paged_mixed),        MVA_METHOD(forward_inputs_ok), MVA_METHOD(capture_id),
+                          MVA_METHOD(store_kvcache_mxfp4), MVA_METHOD(load_kvcache_mxfp4),
+                          MVA_METHOD(paged_decode_mxfp4), MVA_METHOD(forward_inputs_ok_mxfp4),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "mva_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -957,6 +957,8 @@ def store_kvcache_mxfp4(
     nearest code, ties to even.  Scales stop at 2^125 (bf16) or 2^13 (fp16), so
     that every value read back is finite; a group that holds an infinity or a
     NaN reads back as NaN.  The slots >= 0 of one call must be distinct."""
+    if _native.host_ops().store_kvcache_mxfp4(key, value, k_cache, v_cache, slot_mapping):
+        return
     if key.dim() != 3 or value.shape != key.shape or key.size(2) != HEAD_DIM:
         raise ValueError(f"key and value must both have shape [tokens, num_kv_heads, {HEAD_DIM}]")
     num_tokens, num_heads, _ = key.shape
@@ -993,6 +995,9 @@ def load_kvcache_mxfp4(
     that the attention reads.  A slot that is negative or past the cache gives
     zeros.  (Values that a bf16 row put beyond fp16's range round to it as
     usual.)"""
+    fast = _native.host_ops().load_kvcache_mxfp4(k_cache, v_cache, slot_mapping, _native.DTYPE_CODES.get(dtype))
+    if fast is not None:
+        return fast
     if not k_cache.is_cuda:
         raise RuntimeError("load_kvcache_mxfp4 expects CUDA tensors")
     _check_mxfp4_caches(k_cache, v_cache, k_cache.device)
@@ -1066,6 +1071,10 @@ def paged_decode_mxfp4(
     With ``counts`` (int32 ``[3]`` on the device) it is the fixed-shape launch
     of :func:`paged_decode_graph`: ``counts`` holds this step's ``{num_items,
     num_waves, num_merges}`` and the scalar arguments are capacities."""
+    if _native.host_ops().paged_decode_mxfp4(q, k_cache, v_cache, block_tables, seq_lens, counts, items, num_items,
+                                             num_waves, merges, num_merges, num_part_slots, out, workspace,
+                                             softmax_scale, wave_extra, waves_per_group):
+        return
     if validate:
         _check_paged_mxfp4(q, out, k_cache, v_cache,
                            (("block_tables", block_tables), ("seq_lens", seq_lens), ("items", items),
