@@ -13,20 +13,16 @@
 //    that scale in one instruction a pair, exactly.  The contraction may take
 //    the 128 dimensions in any order, so lane group j holds dimensions 32j..
 //    and Q is loaded to match: S^T = K Q^T by 16x16x32 MFMAs, fp32.
-//  * V: ds_read_b64_tr_b4 turns 16 tokens x 16 dimensions of codes, so that a
-//    lane holds one dimension of 16 tokens, the A operand of O^T += V^T P^T.
-//    Its scales run along tokens there, so the codes convert with scale 1 and
-//    P takes the scales: P_g[t] = P[t] * 2^(b[t][g] - 127) for the four groups
-//    g of dimensions.
-//  * The tokens of the S^T tiles are dealt so that lane group j gets the 16
-//    tokens of page j of the tile, in order: tile i of four takes rows 4i..4i+3
-//    of each page.  P then lies as the PV MFMA wants it, without a shuffle.
-//  * P is rounded to bf16 for the product, whatever the query's type: its
-//    products with the scales need bf16's exponents, and 2^-9 relative is far
-//    below the cache's own rounding (up to 2^-3).  Row sums stay in fp32.
-//
-// Tokens past a sequence's end or its piece get S = -inf and P_g = 0; codes are
-// always finite, so nothing else of a stale row can reach the result.
+//  * V: O^T += V^T P^T wants a lane to hold one dimension of eight tokens, and a
+//    token's scales run along its dimensions.  So a lane takes one group of one
+//    token from LDS, converts it with its scale, exactly, and writes the rows
+//    back to LDS (over the codes, which every lane has read by then), from where
+//    ds_read_b64_tr_b16 transposes them.  Transposing the codes instead
+//    (ds_read_b64_tr_b4) leaves the scales to P, four scaled copies of it: 32
+//    more conversions and 128 more multiplies and byte extracts a tile, and P
+//    times a scale leaves fp16's range.
+// Tokens past a sequence's end or its piece get S = -inf and V = 0: nothing of a
+// stale row, whose scales may be NaN, can reach the result.
 #pragma once
 
 #include "mxfp4.h"
@@ -49,81 +45,102 @@ constexpr int kFp4TileBytes = kFp4TileVScales + kFp4TileTokens * kFp4RowScales; 
 constexpr int kFp4WaveLdsBytes = 2 * kFp4TileBytes;
 
 // One tile's copies into LDS at byte address `lds`, ten loads, then a wait for
-// everything before them: page j's codes of K and V from kb[j] / vb[j] (uniform)
-// + the lane's offset koff[j] / voff, and both tiles' scales, 4 bytes a lane,
-// from ks / vs.  With kQ the query fragments at `q` (4 x 16 bytes) are requested
-// first, so the wait covers them too.  One asm statement: see paged_decode.h.
+// everything before them: page j's codes of K and V, 16 bytes a lane, from k[j]
+// and v[j], and both scale blocks, 4 bytes a lane, from ks and vs.
 struct Fp4Copy {
-  const uint8_t* kb[kFp4TilePages];
-  const uint8_t* vb[kFp4TilePages];
+  const uint8_t* k[kFp4TilePages];
+  const uint8_t* v[kFp4TilePages];
   const uint8_t* ks;
   const uint8_t* vs;
 };
 
-#define MVA_FP4_TILE_DMA                          \
-  "s_mov_b32 %[m0s], m0\n\t"                      \
-  "s_mov_b32 m0, %[l]\n\t"                        \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[ko0], %[k0]\n\t"     \
-  "s_add_u32 m0, %[l], 0x400\n\t"                 \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[ko1], %[k1]\n\t"     \
-  "s_add_u32 m0, %[l], 0x800\n\t"                 \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[ko2], %[k2]\n\t"     \
-  "s_add_u32 m0, %[l], 0xc00\n\t"                 \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[ko3], %[k3]\n\t"     \
-  "s_add_u32 m0, %[l], 0x1000\n\t"                \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[vo], %[v0]\n\t"      \
-  "s_add_u32 m0, %[l], 0x1400\n\t"                \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[vo], %[v1]\n\t"      \
-  "s_add_u32 m0, %[l], 0x1800\n\t"                \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[vo], %[v2]\n\t"      \
-  "s_add_u32 m0, %[l], 0x1c00\n\t"                \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dwordx4 %[vo], %[v3]\n\t"      \
-  "s_add_u32 m0, %[l], 0x2000\n\t"                \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dword %[ks], off\n\t"          \
-  "s_add_u32 m0, %[l], 0x2100\n\t"                \
-  "s_nop 0\n\t"                                   \
-  "global_load_lds_dword %[vs], off\n\t"          \
-  "s_mov_b32 m0, %[m0s]\n\t"                      \
+#define MVA_FP4_TILE_DMA                   \
+  "s_mov_b32 %[m0s], m0\n\t"               \
+  "s_mov_b32 m0, %[l]\n\t"                 \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[k0], off\n\t" \
+  "s_add_u32 m0, %[l], 0x400\n\t"          \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[k1], off\n\t" \
+  "s_add_u32 m0, %[l], 0x800\n\t"          \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[k2], off\n\t" \
+  "s_add_u32 m0, %[l], 0xc00\n\t"          \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[k3], off\n\t" \
+  "s_add_u32 m0, %[l], 0x1000\n\t"         \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[v0], off\n\t" \
+  "s_add_u32 m0, %[l], 0x1400\n\t"         \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[v1], off\n\t" \
+  "s_add_u32 m0, %[l], 0x1800\n\t"         \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[v2], off\n\t" \
+  "s_add_u32 m0, %[l], 0x1c00\n\t"         \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dwordx4 %[v3], off\n\t" \
+  "s_add_u32 m0, %[l], 0x2000\n\t"         \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dword %[ks], off\n\t"   \
+  "s_add_u32 m0, %[l], 0x2100\n\t"         \
+  "s_nop 0\n\t"                            \
+  "global_load_lds_dword %[vs], off\n\t"   \
+  "s_mov_b32 m0, %[m0s]\n\t"               \
   "s_waitcnt vmcnt(10)"
 
 static_assert(kFp4TileV == 0x1000 && kFp4TileKScales == 0x2000 && kFp4TileVScales == 0x2100, "the copies' LDS layout");
 
-#define MVA_FP4_TILE_IN                                                                                         \
-  [l] "s"(lds), [ko0] "v"(koff[0]), [ko1] "v"(koff[1]), [ko2] "v"(koff[2]), [ko3] "v"(koff[3]), [vo] "v"(voff), \
-      [k0] "s"(c.kb[0]), [k1] "s"(c.kb[1]), [k2] "s"(c.kb[2]), [k3] "s"(c.kb[3]), [v0] "s"(c.vb[0]),            \
-      [v1] "s"(c.vb[1]), [v2] "s"(c.vb[2]), [v3] "s"(c.vb[3]), [ks] "v"(c.ks), [vs] "v"(c.vs)
+#define MVA_FP4_TILE_IN                                                                                          \
+  [l] "s"(lds), [k0] "v"(c.k[0]), [k1] "v"(c.k[1]), [k2] "v"(c.k[2]), [k3] "v"(c.k[3]), [v0] "v"(c.v[0]),        \
+      [v1] "v"(c.v[1]), [v2] "v"(c.v[2]), [v3] "v"(c.v[3]), [ks] "v"(c.ks), [vs] "v"(c.vs)
 
-__device__ inline void fp4_tile_copy(const Fp4Copy& c, const uint32_t (&koff)[4], uint32_t voff, uint32_t lds) {
+__device__ inline void fp4_tile_copy(const Fp4Copy& c, uint32_t lds) {
   uint32_t m0_saved;
   lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile(MVA_FP4_TILE_DMA : [m0s] "=&s"(m0_saved) : MVA_FP4_TILE_IN : "memory", "scc");
 }
 
-__device__ inline void fp4_tile_copy_q(const Fp4Copy& c, const uint32_t (&koff)[4], uint32_t voff, uint32_t lds,
-                                       const void* q, u32x4 (&qv)[4]) {
+// The first tile of a piece: also requests, ahead of the tile, so that the wait
+// covers them, the query fragments at `q` (4 x 16 bytes) and the piece's page
+// table words at t0 and t1.
+struct Fp4Piece {
+  u32x4 q[4];
+  int lo, hi;
+};
+__device__ inline void fp4_tile_copy_first(const Fp4Copy& c, uint32_t lds, const void* q, const int32_t* t0,
+                                           const int32_t* t1, Fp4Piece& out) {
   uint32_t m0_saved;
   lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile(
+      "global_load_dword %[lo], %[t0], off\n\t"
+      "global_load_dword %[hi], %[t1], off\n\t"
       "global_load_dwordx4 %[q0], %[qp], off\n\t"
       "global_load_dwordx4 %[q1], %[qp], off offset:16\n\t"
       "global_load_dwordx4 %[q2], %[qp], off offset:32\n\t"
       "global_load_dwordx4 %[q3], %[qp], off offset:48\n\t" MVA_FP4_TILE_DMA
-      : [m0s] "=&s"(m0_saved), [q0] "=&v"(qv[0]), [q1] "=&v"(qv[1]), [q2] "=&v"(qv[2]), [q3] "=&v"(qv[3])
-      : MVA_FP4_TILE_IN, [qp] "v"(q)
+      : [m0s] "=&s"(m0_saved), [lo] "=&v"(out.lo), [hi] "=&v"(out.hi), [q0] "=&v"(out.q[0]), [q1] "=&v"(out.q[1]),
+        [q2] "=&v"(out.q[2]), [q3] "=&v"(out.q[3])
+      : MVA_FP4_TILE_IN, [qp] "v"(q), [t0] "v"(t0), [t1] "v"(t1)
       : "memory", "scc");
 }
 
 #undef MVA_FP4_TILE_DMA
 #undef MVA_FP4_TILE_IN
+
+// Maximum and sum over the four lane groups of a wavefront, without LDS.
+__device__ inline float groups_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float groups_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
 
 // One wavefront of a decode launch over piece lists (see decode_wave); `lds` is
 // its kFp4WaveLdsBytes of LDS.
@@ -155,66 +172,94 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
   int nx = max(sload(p.wave_extra, wave), 0);
   const int nx_end = min(sload(p.wave_extra, wave + 1), N);
 
-  // Per-lane offsets.  A page's codes lie in LDS token by token, 64 bytes each,
-  // with 16-byte chunk ch of a token at slot ch ^ j (K, page j of the tile) or
-  // ch ^ (token / 4) (V): then the 16 tokens that a K read takes (four of each
-  // page) and the 16 of a V read fall on different banks.
-  uint32_t koff[4];
+  // Per-lane offsets.  K codes lie in LDS token by token, 64 bytes each, with
+  // 16-byte chunk ch of token t at slot ch ^ (t / 4): the 16 tokens that a read
+  // takes at one chunk then fall on different banks.  V codes lie in lane order.
+  const uint32_t koff = (uint32_t)((lane >> 2) * kFp4RowBytes + (((lane & 3) ^ (lane >> 4)) << 4));
+  const uint32_t voff = (uint32_t)(lane << 4);
+  const int kread = c * kFp4RowBytes + ((q4 ^ (c >> 2)) << 4);
+  const int ksread = kFp4TileKScales + c * kFp4RowScales + q4;
+  // Converted V rows of two pages, 256 bytes a token, 16-byte chunk ch of token t
+  // at slot ch ^ vswz(t).  This lane writes chunks 4 (lane % 4) + u of token
+  // lane / 4, and supplies token 4 q4 + c / 4, dimensions 16 mt + 4 (c % 4) .. + 3
+  // to a transposed read, which gives it dimension 16 mt + c of tokens 4 q4 .. + 3.
+  auto vswz = [](int t) { return 2 * (t & 3) | ((t >> 2) & 1) << 3; };
+  const int vtok = lane >> 2;
+  int vwrite[4], vread[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) koff[j] = (uint32_t)((lane >> 2) * kFp4RowBytes + (((lane & 3) ^ j) << 4));
-  const uint32_t voff = (uint32_t)((lane >> 2) * kFp4RowBytes + (((lane & 3) ^ (lane >> 4)) << 4));
-  const int kread = (c >> 2) * kFp4ScaleOffset + (c & 3) * kFp4RowBytes + ((q4 ^ (c >> 2)) << 4);
-  const int ksread = kFp4TileKScales + (c >> 2) * 64 + (c & 3) * 4 + q4;
-  int vread[4];
+  for (int u = 0; u < 4; ++u) vwrite[u] = vtok * 256 + ((4 * (lane & 3) + u) ^ vswz(vtok)) * 16;
+  const int rtok = 4 * q4 + (c >> 2);
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
-    vread[g] = kFp4TileV + q4 * kFp4ScaleOffset + c * kFp4RowBytes + ((g ^ (c >> 2)) << 4);
-  const int vsread = kFp4TileVScales + q4 * 64;
+  for (int u = 0; u < 4; ++u) vread[u] = rtok * 256 + ((2 * u + ((c >> 1) & 1)) ^ vswz(rtok)) * 16 + (c & 1) * 8;
 
   // The tile to copy next: tile ft of piece F, its page ids, and whether it
-  // opens a piece.
+  // opens a piece.  A piece's first page ids come by scalar loads, one piece
+  // ahead; the others from its table words, lane L of lo / hi holding page L and
+  // 64 + L, which arrive with its first tile.
   i32x8 F = desc_at(wave);
   int ft = 0;
   bool fvalid = true, fnew = true;
-  int ids[kFp4TilePages];
-  auto load_ids = [&]() {
-    const int32_t* row = p.block_tables + (int64_t)F[0] * p.bt_stride + F[1];
+  int id0, id1, id2, id3;
+  Fp4Piece piece;
+  auto good_id = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pages ? id : 0; };
+  auto bt_row = [&]() { return p.block_tables + (int64_t)F[0] * p.bt_stride + F[1]; };
+  auto open_ids = [&]() {
     const int last = max(F[2] - F[1] - 1, 0);
-#pragma unroll
-    for (int j = 0; j < kFp4TilePages; ++j) ids[j] = sload(row, min(kFp4TilePages * ft + j, last));
+    id0 = good_id(sload(bt_row(), 0));
+    id1 = good_id(sload(bt_row(), min(1, last)));
+    id2 = good_id(sload(bt_row(), min(2, last)));
+    id3 = good_id(sload(bt_row(), min(3, last)));
   };
-  load_ids();
+  open_ids();
   auto advance = [&]() {
     ++ft;
-    fnew = false;
-    if (kFp4TilePages * ft >= F[2] - F[1]) {
-      fvalid = nx < nx_end;
-      if (!fvalid) return;
-      F = desc_at(nx);
-      ++nx;
-      ft = 0;
-      fnew = true;
+    fnew = kFp4TilePages * ft >= F[2] - F[1];
+    if (!fnew) {
+      const int words = kFp4TilePages * ft < 64 ? piece.lo : piece.hi;
+      const int at = (kFp4TilePages * ft) & 63;
+      id0 = __builtin_amdgcn_readlane(words, at);
+      id1 = __builtin_amdgcn_readlane(words, at + 1);
+      id2 = __builtin_amdgcn_readlane(words, at + 2);
+      id3 = __builtin_amdgcn_readlane(words, at + 3);
+      return;
     }
-    load_ids();
+    fvalid = nx < nx_end;
+    if (!fvalid) return;
+    F = desc_at(nx);
+    ++nx;
+    ft = 0;
+    open_ids();
   };
-  u32x4 qn[4];
-  const int scale_off = kFp4ScaleOffset + c * kFp4RowScales;
+  // This lane's addresses in page 0 of head F[7]; a page id adds page_stride,
+  // below 2^32 bytes.
+  const uint8_t *k_lane, *v_lane, *ks_lane, *vs_lane;
   auto copy_tile = [&](lds_u8* buf) {
-    Fp4Copy cp;
-    int64_t scale_page = 0;
-#pragma unroll
-    for (int j = 0; j < kFp4TilePages; ++j) {
-      const int id = (ids[j] >= 0 && ids[j] < p.num_pages) ? ids[j] : 0;
-      const int64_t off = (int64_t)id * p.page_stride + (int64_t)F[7] * p.head_stride;
-      cp.kb[j] = (const uint8_t*)p.k_cache + off;
-      cp.vb[j] = (const uint8_t*)p.v_cache + off;
-      if (q4 == j) scale_page = off;
+    if (fnew) {
+      const int64_t head = (int64_t)F[7] * p.head_stride;
+      k_lane = (const uint8_t*)p.k_cache + head + koff;
+      v_lane = (const uint8_t*)p.v_cache + head + voff;
+      ks_lane = (const uint8_t*)p.k_cache + head + kFp4ScaleOffset + c * kFp4RowScales;
+      vs_lane = (const uint8_t*)p.v_cache + head + kFp4ScaleOffset + c * kFp4RowScales;
     }
-    cp.ks = (const uint8_t*)p.k_cache + scale_page + scale_off;
-    cp.vs = (const uint8_t*)p.v_cache + scale_page + scale_off;
+    Fp4Copy cp;
+    const uint32_t stride = (uint32_t)p.page_stride;
+    auto page = [&](const uint8_t* lane_base, int id) { return lane_base + (uint64_t)(uint32_t)id * stride; };
+    cp.k[0] = page(k_lane, id0), cp.k[1] = page(k_lane, id1), cp.k[2] = page(k_lane, id2), cp.k[3] = page(k_lane, id3);
+    cp.v[0] = page(v_lane, id0), cp.v[1] = page(v_lane, id1), cp.v[2] = page(v_lane, id2), cp.v[3] = page(v_lane, id3);
+    int mine = id0;  // the page whose scales this lane copies
+    mine = q4 == 1 ? id1 : mine;
+    mine = q4 == 2 ? id2 : mine;
+    mine = q4 == 3 ? id3 : mine;
+    cp.ks = page(ks_lane, mine), cp.vs = page(vs_lane, mine);
     const uint32_t at = (uint32_t)(uintptr_t)buf;
-    if (fnew) fp4_tile_copy_q(cp, koff, voff, at, q_addr(F), qn);
-    else fp4_tile_copy(cp, koff, voff, at);
+    if (fnew) {
+      const int last = max(F[2] - F[1] - 1, 0);
+      fp4_tile_copy_first(cp, at, q_addr(F), bt_row() + min(lane, last), bt_row() + min(64 + lane, last), piece);
+      piece.lo = good_id(piece.lo);
+      piece.hi = good_id(piece.hi);
+    } else {
+      fp4_tile_copy(cp, at);
+    }
   };
 
   i32x8 X = F;  // the piece being computed
@@ -225,7 +270,7 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
   float m, l;  // reference max (log2 domain) of g = c; this lane's share of the denominator
   auto open_piece = [&]() {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) qf[j] = q_lane ? __builtin_bit_cast(V8, qn[j]) : V8{};
+    for (int j = 0; j < 4; ++j) qf[j] = q_lane ? __builtin_bit_cast(V8, piece.q[j]) : V8{};
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
@@ -233,79 +278,129 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
   };
 
   // `valid`: tokens of the tile that count; below 64 on an edge tile.
-  auto compute = [&](const lds_u8* buf, int valid, auto edge_tag) __attribute__((always_inline)) {
-    constexpr bool edge = decltype(edge_tag)::value;
-    f32x4 sc[4];  // sc[i][r] = S[token 4 i + r of page q4][g = c]
+  auto compute = [&](lds_u8* buf, int valid) __attribute__((always_inline)) {
+    const bool edge = valid < kFp4TileTokens;  // wave-uniform
+    u32x4 vw[4];  // page i's codes of token lane / 4, group lane % 4
+    uint32_t vs[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const u32x4 w = lds_ld16<u32x4>(buf + kread + i * 4 * kFp4RowBytes);
-      const float ks = fp4_scale((uint32_t)buf[ksread + 16 * i]);
-      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc = Elem<T>::mfma16(fp4_unpack8<T>(w[j], ks), qf[j], acc);
-      sc[i] = acc;
+      vw[i] = lds_ld16<u32x4>(buf + kFp4TileV + i * kFp4ScaleOffset + voff);
+      vs[i] = buf[kFp4TileVScales + 64 * i + lane];
     }
-    const int mine = valid - kPageSize * q4;  // valid tokens of this lane's page
-    float tmax = -INFINITY;
+    u32x4 kw[4];
+    float ks[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      kw[i] = lds_ld16<u32x4>(buf + kread + i * kFp4ScaleOffset);
+      ks[i] = fp4_scale((uint32_t)buf[ksread + 64 * i]);
+    }
+    f32x4 sc[4];  // sc[i][r] = S[token 4 q4 + r of page i][g = c]
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (edge) {
-          if (4 * i + r >= mine) sc[i][r] = -INFINITY;
+    for (int i = 0; i < 4; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // The four pages' sums in turn: one alone is a chain of dependent MFMAs.
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[i] = Elem<T>::mfma16(fp4_unpack8<T>(kw[i][j], ks[i]), qf[j], sc[i]);
+      __builtin_amdgcn_sched_barrier(0);  // not all conversions at once: registers
+    }
+    // Rows of pages 2 half and 2 half + 1 over the tile's codes.  LDS works in
+    // order for a wavefront: reads before these writes see the codes, and the
+    // second half's writes come after the first half's reads.
+    auto write_v = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = 2 * half + k;
+        u32x4 w = vw[i];
+        uint32_t byte = vs[i];
+        if (edge) {
+          const bool live = kPageSize * i + vtok < valid;
+          byte = live ? byte : 127u;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[u] = live ? w[u] : 0u;
         }
-        tmax = fmaxf(tmax, sc[i][r]);
+        const float scale = fp4_scale(byte);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          lds_st16(buf + k * kDecodePageBytes + vwrite[u], fp4_unpack8<T>(w[u], scale));
+        __builtin_amdgcn_sched_barrier(0);
       }
-    tmax = wave_max16(tmax) * p.scale_log2;  // scale > 0 commutes with max
-    // Move the reference max only when it grows by > 8 (p stays <= 2^8).
-    const bool grow = tmax > m + 8.0f;
-    if (__any(grow)) {
+    };
+    wave_lds_fence();
+    write_v(0);
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (kPageSize * i + 4 * q4 + r >= valid) sc[i][r] = -INFINITY;
+    }
+    // P = 2^(S * scale - m), packed, and this lane's sum of it.
+    V8 pf[2];
+    auto exponentials = [&](float m_use) __attribute__((always_inline)) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float pr = fast_exp2(sc[i][r] * p.scale_log2 - m_use);
+          sum[r] += pr;
+          pf[i >> 1][4 * (i & 1) + r] = (T)pr;
+        }
+      return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    // The reference maximum moves only when a score exceeds it by more than 8
+    // (P stays <= 2^8).  A sum below 128 shows that none does, as every P is
+    // below 128 then (2^7.01 covers the rounding of S * scale and m + 8 while
+    // |m| < 2^20), so most tiles take no maximum.
+    float sum = exponentials(m);
+    if (__any(!(sum < 128.f && __builtin_fabsf(m) < 0x1p20f))) {
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sc[i][r]);
+      tmax = groups_max(tmax) * p.scale_log2;  // scale > 0 commutes with max
+      const bool grow = tmax > m + 8.0f;
       const float m_new = grow ? tmax : m;
       const float alpha = grow ? fast_exp2(m - m_new) : 1.0f;  // m = -inf -> 0
       m = m_new;
       l *= alpha;
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) o[mt] *= alpha;
+      sum = exponentials(m == -INFINITY ? 0.f : m);
     }
-    const float m_use = (m == -INFINITY) ? 0.f : m;
+    l += sum;
+    // d-tile mt: tokens 4 q4 .. + 3 of the half's two pages.
+    auto read_v = [&](V8 (&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sc[i][r] = fast_exp2(sc[i][r] * p.scale_log2 - m_use);
-        l += sc[i][r];
+      for (int mt = 0; mt < 8; ++mt) {
+        // Chunks of d-tile mt lie 8 chunks, one bit of the slot, from those of mt - 4.
+        const lds_u8* a = buf + (mt < 4 ? vread[mt] : vread[mt - 4] ^ 128);
+        v[mt] = __builtin_bit_cast(
+            V8, __builtin_shufflevector(lds_ld_tr16(a), lds_ld_tr16(a + kDecodePageBytes), 0, 1, 2, 3, 4, 5, 6, 7));
       }
-    u32x4 vs[4];  // vs[i][r]: the four scale bytes of token 4 i + r
+    };
+    V8 v[8];
+    __builtin_amdgcn_sched_barrier(0);
+    wave_lds_fence();
+    read_v(v);
+    wave_lds_fence();
+    __builtin_amdgcn_sched_barrier(0);
+    write_v(1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vs[i] = lds_ld16<u32x4>(buf + vsread + 16 * i);
+    for (int mt = 0; mt < 8; ++mt) o[mt] = Elem<T>::mfma16(v[mt], pf[0], o[mt]);
+    __builtin_amdgcn_sched_barrier(0);
+    wave_lds_fence();
+    read_v(v);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      bf16x8 pg[2];  // tokens 0-7 and 8-15
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = sc[i][r] * fp4_scale((vs[i][r] >> (8 * g)) & 0xffu);
-          if constexpr (edge) {
-            if (4 * i + r >= mine) x = 0.f;  // a stale scale may be NaN
-          }
-          pg[i >> 1][4 * (i & 1) + r] = (__bf16)x;
-        }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            (__attribute__((address_space(3))) i32x2*)(buf + vread[g] + 8 * half));
-        f32x4& acc = o[2 * g + half];
-        acc = Elem<__bf16>::mfma16(fp4_unpack8<__bf16>((uint32_t)v[0], 1.f), pg[0], acc);
-        acc = Elem<__bf16>::mfma16(fp4_unpack8<__bf16>((uint32_t)v[1], 1.f), pg[1], acc);
-      }
-    }
+    for (int mt = 0; mt < 8; ++mt) o[mt] = Elem<T>::mfma16(v[mt], pf[1], o[mt]);
   };
 
   // End of piece X: the final output, or its split-K partial (normalised o and
   // log2-sum-exp) for the merge kernel.
   auto finish_piece = [&]() __attribute__((always_inline)) {
-    const float l_tot = wave_sum16(l);
+    const float l_tot = groups_sum(l);
     const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
     const int h = X[7];
     if (!q_lane) return;
@@ -347,8 +442,7 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
     wave_lds_fence();
     const int begin = X[1] + kFp4TilePages * xt;
     const int valid = min(seq_len, X[2] * kPageSize) - begin * kPageSize;
-    if (valid < kFp4TileTokens) compute(cur, valid, std::true_type{});
-    else compute(cur, valid, std::false_type{});
+    compute(cur, valid);
     wave_lds_fence();
     buf ^= 1;
     ++xt;

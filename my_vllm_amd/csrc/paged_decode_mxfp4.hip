@@ -59,6 +59,8 @@ extern "C" int mva_paged_decode_mxfp4(const void* q, int64_t q_token_stride, int
   if (wave_extra == nullptr && num_items > 0) return set_error("paged attention mxfp4: piece lists (wave_extra) needed");
   if (((uint64_t)page_stride_bytes | (uint64_t)head_stride_bytes) % 16)
     return set_error("paged attention mxfp4: cache strides must be 16-byte aligned");
+  if (page_stride_bytes < 0 || page_stride_bytes > 0xffffffffLL)
+    return set_error("paged attention mxfp4: pages must lie less than 4 GiB apart");
   if (dtype != kBF16 && dtype != kF16) return set_error("paged attention: dtype must be bf16 or fp16");
   Fp4DecodeParams p;
   const int rc = fill_decode_params(p, q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, 0, 0,
