@@ -286,8 +286,8 @@ def plan_decode_listed(
     :func:`ops.decode_merge_list` would give it), from the library's native
     planner ``mva_decode_plan_listed``."""
     counts = _plan_counts(block_counts)
-    if not 1 <= max_piece_pages <= ops.MAX_CHUNK_PAGES:
-        raise ValueError("piece length must be in [1, 128] pages")
+    if max_piece_pages != ops.ANY_PIECE_PAGES and not 1 <= max_piece_pages <= ops.MAX_CHUNK_PAGES:
+        raise ValueError("piece length must be in [1, 128] pages, or ANY_PIECE_PAGES")
     n = counts.size
     if n == 0:
         empty = np.zeros((0, ops.DECODE_ITEM_INTS), np.int32)
@@ -500,6 +500,8 @@ class MI355XAttentionBackendMixin:
     # after each fused launch (a device read) and raise if a row's slot was
     # not its sequence's last position.
     check_fused_store: bool = False
+    # Longest piece of a decode plan with piece lists.
+    _max_piece_pages = ops.MAX_CHUNK_PAGES
 
     def __init__(
         self,
@@ -636,7 +638,13 @@ class MI355XAttentionBackendMixin:
 
     def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
         """(page ranges, wavefronts per workgroup) of a decode launch with piece lists."""
+        if self.decode_waves_override:
+            return self._most_decode_ranges(device)
         return decode_ranges(int(decode_counts.sum()), len(decode_counts), self.num_kv_heads, device)
+
+    def _most_decode_ranges(self, device: torch.device) -> tuple[int, int]:
+        """The same for the largest batch: what a captured launch is sized for."""
+        return listed_decode_groups(self.num_kv_heads, device, override=self.decode_waves_override)
 
     # ---- per-step metadata and plan ------------------------------------------
     def build_metadata(self, common) -> MI355XAttentionMetadata:
@@ -735,13 +743,10 @@ class MI355XAttentionBackendMixin:
             if not one_launch:
                 schedule = self._decode_schedule(int(decode_counts.sum()))
                 if schedule == "listed":
-                    if self.decode_waves_override:
-                        groups, waves_per_group = listed_decode_groups(self.num_kv_heads, block_tables.device,
-                                                                       override=self.decode_waves_override)
-                    else:
-                        groups, waves_per_group = self._decode_ranges(decode_counts, block_tables.device)
+                    groups, waves_per_group = self._decode_ranges(decode_counts, block_tables.device)
                     items, wave_extra, num_decode_waves, num_part_slots, merges = plan_decode_listed(
-                        decode_counts, common.num_prefill_seqs, common.num_prefill_tokens, self.num_kv_heads, groups
+                        decode_counts, common.num_prefill_seqs, common.num_prefill_tokens, self.num_kv_heads, groups,
+                        self._max_piece_pages
                     )
                 else:
                     items, num_decode_waves, num_part_slots, merges = plan_decode_claims(
@@ -1094,8 +1099,7 @@ class MI355XAttentionBackendMixin:
         graph_device = torch.device(device)
         if graph_device.type != "cuda":
             raise ValueError("full decode graph state must be on CUDA")
-        groups, waves_per_group = listed_decode_groups(self.num_kv_heads, graph_device,
-                                                       override=self.decode_waves_override)
+        groups, waves_per_group = self._most_decode_ranges(graph_device)
         caps = graph_decode_capacities(batch_size, page_indices_capacity, self.num_kv_heads, groups)
         group = self.num_q_heads // self.num_kv_heads
         plan_ints = graph_plan_buffer_ints(caps["item_capacity"], caps["wave_capacity"], caps["merge_capacity"])
@@ -1162,7 +1166,8 @@ class MI355XAttentionBackendMixin:
         # KV heads): replays run what an eager launch runs.
         if host is None or host[3] > state.groups:
             counts = np.diff(np.asarray(metadata.kv_indptr, dtype=np.int64))
-            items, wave_extra, _, _, merges = plan_decode_listed(counts, 0, 0, self.num_kv_heads, state.groups)
+            items, wave_extra, _, _, merges = plan_decode_listed(counts, 0, 0, self.num_kv_heads, state.groups,
+                                                                 self._max_piece_pages)
         else:
             items, wave_extra, merges, _ = host
         # Staging buffers alternate: the one refilled now was last copied two
@@ -1320,6 +1325,18 @@ class MI355XSplitAttentionBackend(MI355XAttentionBackend):
     default_attention_mode = "split"
 
 
+# Wavefronts per CU of a decode launch over an MXFP4 cache (kFp4WaveLdsBytes of
+# LDS each).
+_MXFP4_WAVES_PER_CU = 12
+
+
+def mxfp4_decode_ranges(num_kv_heads: int, device: torch.device | None = None,
+                        override: int | None = None) -> tuple[int, int]:
+    """(page ranges, wavefronts per workgroup) of a decode launch over an MXFP4 cache."""
+    waves = max(1, int(override)) if override else _num_cus(device) * _MXFP4_WAVES_PER_CU
+    return max(1, waves // num_kv_heads), _MXFP4_WAVES_PER_CU
+
+
 class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
     """The backend over an MXFP4 cache: K and V in 4 bits, ``uint8`` caches of
     ``ops.mxfp4_cache_shape`` (136 bytes a token and KV head instead of 512).
@@ -1331,6 +1348,7 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
     (route MIXED_SPLIT) in both attention modes."""
 
     backend_name = "mi355x_mxfp4"
+    _max_piece_pages = ops.ANY_PIECE_PAGES
 
     def _store_rows(self, k, v, k_cache, v_cache, slot_mapping) -> None:
         ops.store_kvcache_mxfp4(k, v, k_cache, v_cache, slot_mapping)
@@ -1342,6 +1360,12 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
         if self.decode_schedule_override not in (None, "listed"):
             raise ValueError("decode over an MXFP4 cache runs piece lists only")
         return "listed"
+
+    def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
+        return self._most_decode_ranges(device)
+
+    def _most_decode_ranges(self, device: torch.device) -> tuple[int, int]:
+        return mxfp4_decode_ranges(self.num_kv_heads, device, self.decode_waves_override)
 
     def _validate_inputs(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
         if _native.host_ops().forward_inputs_ok_mxfp4(q, k_cache, v_cache, _native.DTYPE_CODES[self.dtype],

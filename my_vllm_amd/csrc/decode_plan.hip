@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kItemInts = 8;
 constexpr int kMaxPiecePages = 128;  // the decode kernel's longest piece
+constexpr int kAnyPiecePages = 0x7fffffff;  // piece lists not cut further: the MXFP4 decode kernel takes any length
 
 struct Piece {
   int64_t begin, end;  // absolute page offsets in the batch
@@ -79,7 +80,7 @@ int64_t collect_merges(const int32_t* items, int64_t num_items, int32_t* merges,
 extern "C" int64_t mva_decode_plan_listed_rows(int64_t num_seqs, int64_t total_pages, int num_kv_heads,
                                                int num_groups, int max_piece_pages) {
   if (num_seqs < 0 || total_pages < 0 || num_kv_heads <= 0 || num_groups <= 0 || max_piece_pages < 1 ||
-      max_piece_pages > mva::kMaxPiecePages)
+      (max_piece_pages > mva::kMaxPiecePages && max_piece_pages != mva::kAnyPiecePages))
     return -1;
   if (num_seqs == 0) return 0;
   const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(num_groups, total_pages));
@@ -98,8 +99,8 @@ extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_s
   if (num_seqs < 0 || num_kv_heads <= 0 || num_groups <= 0 || out_counts == nullptr || wave_extra == nullptr ||
       wave_extra_len < 1)
     return set_error("decode plan: invalid arguments");
-  if (max_piece_pages < 1 || max_piece_pages > kMaxPiecePages)
-    return set_error("decode plan: piece length must be in [1, 128] pages");
+  if (max_piece_pages < 1 || (max_piece_pages > kMaxPiecePages && max_piece_pages != kAnyPiecePages))
+    return set_error("decode plan: piece length must be in [1, 128] pages, or unlimited (INT_MAX)");
   for (int i = 0; i < 4; ++i) out_counts[i] = 0;
   if (num_seqs == 0) {
     wave_extra[0] = 0;

@@ -3,10 +3,10 @@
 //
 //   o = sum_j softmax_j(scale * q . K[j]) V[j],  K, V = code * 2^(byte - 127)
 //
-// A wavefront streams its pieces (sequence, KV head, page range) in tiles of
-// four pages, 64 tokens: 4 KB of codes and 256 bytes of scales of K, as much of
-// V.  Both go from memory into LDS by global_load_lds, double-buffered, the
-// next tile in flight while this one is computed.
+// A wavefront streams its pieces (sequence, KV head, page range) in tiles of two
+// pages, 32 tokens: 2 KB of codes and 128 bytes of scales of K, as much of V.
+// Both go from memory into LDS by global_load_lds, in three buffers: two tiles in
+// flight while one is computed, twelve wavefronts per CU.
 //
 //  * K: a lane reads the 16 bytes of one token's 32-element group, which is
 //    also what one scale covers, and converts them to the query's type with
@@ -35,98 +35,56 @@ struct Fp4DecodeParams : DecodeParams {
   int64_t head_stride;  // bytes between the blocks of a page's KV heads
 };
 
-constexpr int kFp4TilePages = 4;
+constexpr int kFp4TilePages = 2;
 constexpr int kFp4TileTokens = kFp4TilePages * kPageSize;
-// A tile in LDS: K codes, V codes, K scales, V scales.
+// A tile in LDS: K codes, V codes, then the scales of both pages of K and of V.
 constexpr int kFp4TileV = kFp4TilePages * kFp4ScaleOffset;
 constexpr int kFp4TileKScales = 2 * kFp4TileV;
 constexpr int kFp4TileVScales = kFp4TileKScales + kFp4TileTokens * kFp4RowScales;
-constexpr int kFp4TileBytes = kFp4TileVScales + kFp4TileTokens * kFp4RowScales;  // 8704
-constexpr int kFp4WaveLdsBytes = 2 * kFp4TileBytes;
+constexpr int kFp4TileBytes = kFp4TileVScales + kFp4TileTokens * kFp4RowScales;  // 4352
+constexpr int kFp4TileBufs = 3;
+constexpr int kFp4WaveLdsBytes = kFp4TileBufs * kFp4TileBytes;  // 13056: twelve wavefronts in 160 KB
+constexpr int kFp4TileLoads = 2 * kFp4TilePages + 1;
+// Pages whose ids a wavefront holds at a time, four table words a lane.
+constexpr int kFp4RunPages = 256;
 
-// One tile's copies into LDS at byte address `lds`, ten loads, then a wait for
-// everything before them: page j's codes of K and V, 16 bytes a lane, from k[j]
-// and v[j], and both scale blocks, 4 bytes a lane, from ks and vs.
+// A tile's copies into LDS at byte address `lds`: the codes of its pages of K and
+// of V, 16 bytes a lane, 1 KB each, from a[0] .. a[3], and its scales, 4 bytes a
+// lane, from w (lane group j: K pages 0 and 1, V pages 0 and 1).  One asm
+// statement (see paged_decode.h), which first waits for this wavefront's LDS
+// reads of the buffer.
 struct Fp4Copy {
-  const uint8_t* k[kFp4TilePages];
-  const uint8_t* v[kFp4TilePages];
-  const uint8_t* ks;
-  const uint8_t* vs;
+  const uint8_t* a[4];
+  const uint8_t* w;
 };
 
-#define MVA_FP4_TILE_DMA                   \
-  "s_mov_b32 %[m0s], m0\n\t"               \
-  "s_mov_b32 m0, %[l]\n\t"                 \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[k0], off\n\t" \
-  "s_add_u32 m0, %[l], 0x400\n\t"          \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[k1], off\n\t" \
-  "s_add_u32 m0, %[l], 0x800\n\t"          \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[k2], off\n\t" \
-  "s_add_u32 m0, %[l], 0xc00\n\t"          \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[k3], off\n\t" \
-  "s_add_u32 m0, %[l], 0x1000\n\t"         \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[v0], off\n\t" \
-  "s_add_u32 m0, %[l], 0x1400\n\t"         \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[v1], off\n\t" \
-  "s_add_u32 m0, %[l], 0x1800\n\t"         \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[v2], off\n\t" \
-  "s_add_u32 m0, %[l], 0x1c00\n\t"         \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dwordx4 %[v3], off\n\t" \
-  "s_add_u32 m0, %[l], 0x2000\n\t"         \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dword %[ks], off\n\t"   \
-  "s_add_u32 m0, %[l], 0x2100\n\t"         \
-  "s_nop 0\n\t"                            \
-  "global_load_lds_dword %[vs], off\n\t"   \
-  "s_mov_b32 m0, %[m0s]\n\t"               \
-  "s_waitcnt vmcnt(10)"
+static_assert(kFp4TileV == 0x800 && kFp4TileKScales == 0x1000 && kFp4TileVScales == 0x1080, "the copies' LDS layout");
 
-static_assert(kFp4TileV == 0x1000 && kFp4TileKScales == 0x2000 && kFp4TileVScales == 0x2100, "the copies' LDS layout");
-
-#define MVA_FP4_TILE_IN                                                                                          \
-  [l] "s"(lds), [k0] "v"(c.k[0]), [k1] "v"(c.k[1]), [k2] "v"(c.k[2]), [k3] "v"(c.k[3]), [v0] "v"(c.v[0]),        \
-      [v1] "v"(c.v[1]), [v2] "v"(c.v[2]), [v3] "v"(c.v[3]), [ks] "v"(c.ks), [vs] "v"(c.vs)
-
-__device__ inline void fp4_tile_copy(const Fp4Copy& c, uint32_t lds) {
-  uint32_t m0_saved;
-  lds = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile(MVA_FP4_TILE_DMA : [m0s] "=&s"(m0_saved) : MVA_FP4_TILE_IN : "memory", "scc");
-}
-
-// The first tile of a piece: also requests, ahead of the tile, so that the wait
-// covers them, the query fragments at `q` (4 x 16 bytes) and the piece's page
-// table words at t0 and t1.
-struct Fp4Piece {
-  u32x4 q[4];
-  int lo, hi;
-};
-__device__ inline void fp4_tile_copy_first(const Fp4Copy& c, uint32_t lds, const void* q, const int32_t* t0,
-                                           const int32_t* t1, Fp4Piece& out) {
+__device__ inline void fp4_copy_tile(const Fp4Copy& c, uint32_t lds) {
   uint32_t m0_saved;
   lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile(
-      "global_load_dword %[lo], %[t0], off\n\t"
-      "global_load_dword %[hi], %[t1], off\n\t"
-      "global_load_dwordx4 %[q0], %[qp], off\n\t"
-      "global_load_dwordx4 %[q1], %[qp], off offset:16\n\t"
-      "global_load_dwordx4 %[q2], %[qp], off offset:32\n\t"
-      "global_load_dwordx4 %[q3], %[qp], off offset:48\n\t" MVA_FP4_TILE_DMA
-      : [m0s] "=&s"(m0_saved), [lo] "=&v"(out.lo), [hi] "=&v"(out.hi), [q0] "=&v"(out.q[0]), [q1] "=&v"(out.q[1]),
-        [q2] "=&v"(out.q[2]), [q3] "=&v"(out.q[3])
-      : MVA_FP4_TILE_IN, [qp] "v"(q), [t0] "v"(t0), [t1] "v"(t1)
+      "s_mov_b32 %[m0s], m0\n\t"
+      "s_mov_b32 m0, %[l]\n\t"
+      "s_waitcnt lgkmcnt(0)\n\t"
+      "global_load_lds_dwordx4 %[a0], off\n\t"
+      "s_add_u32 m0, %[l], 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %[a1], off\n\t"
+      "s_add_u32 m0, %[l], 0x800\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %[a2], off\n\t"
+      "s_add_u32 m0, %[l], 0xc00\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %[a3], off\n\t"
+      "s_add_u32 m0, %[l], 0x1000\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %[w], off\n\t"
+      "s_mov_b32 m0, %[m0s]"
+      : [m0s] "=&s"(m0_saved)
+      : [l] "s"(lds), [a0] "v"(c.a[0]), [a1] "v"(c.a[1]), [a2] "v"(c.a[2]), [a3] "v"(c.a[3]), [w] "v"(c.w)
       : "memory", "scc");
 }
-
-#undef MVA_FP4_TILE_DMA
-#undef MVA_FP4_TILE_IN
 
 // Maximum and sum over the four lane groups of a wavefront, without LDS.
 __device__ inline float groups_max(float v) {
@@ -144,8 +102,22 @@ __device__ inline float groups_sum(float v) {
 
 // One wavefront of a decode launch over piece lists (see decode_wave); `lds` is
 // its kFp4WaveLdsBytes of LDS.
+//
+// A piece goes in runs of up to 256 pages.  A run loads its queries and page table
+// words, copies its first three tiles, and then computes tile after tile, copying
+// into each buffer the tile three further on.  Nothing of the next run is
+// requested before the run has ended: its wavefront waits for that, the others of
+// the CU do not, and the loop stays short (at the start of a launch fetching its
+// code counts: a form with the next piece's first tiles in flight was twice the
+// code and 1-2 us slower on small batches, level on large ones).
+//
+// `progress` (LDS, one int per wavefront of the workgroup, or nullptr): the
+// wavefronts `slot` % 4 share a SIMD, whose issue favours the oldest.  Each
+// publishes the tiles it has done and runs at the higher priority the fewer of
+// its two partners are behind it, so the three stay level.
 template <typename T>
-__device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* lds) {
+__device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* lds, int* progress = nullptr,
+                                  int slot = 0) {
   typedef typename Elem<T>::v8 V8;
   typedef typename Elem<T>::v4 V4;
   const int lane = threadIdx.x & 63;
@@ -164,8 +136,9 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
   // Lane (q4, c) of the B operand holds Q[g = c][32 q4 + 8 j .. +8]; lanes
   // c >= G read head 0 of the group (in bounds) and are zeroed.
   auto q_addr = [&](const i32x8& d) -> const T* {
-    const int g = q_lane ? c : 0;
-    return (const T*)p.q + (int64_t)d[6] * p.q_tok_stride + (int64_t)(d[7] * G + g) * p.q_head_stride + 32 * q4;
+    int g = d[7] * G + (q_lane ? c : 0);
+    asm volatile("" : "+v"(g));  // made for each piece, not held in registers
+    return (const T*)p.q + (int64_t)d[6] * p.q_tok_stride + (int64_t)g * p.q_head_stride + 32 * q4;
   };
   // This wavefront's list: piece `wave`, then entries [nx, nx_end), clamped to
   // the item array.
@@ -179,175 +152,111 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
   const uint32_t voff = (uint32_t)(lane << 4);
   const int kread = c * kFp4RowBytes + ((q4 ^ (c >> 2)) << 4);
   const int ksread = kFp4TileKScales + c * kFp4RowScales + q4;
-  // Converted V rows of two pages, 256 bytes a token, 16-byte chunk ch of token t
-  // at slot ch ^ vswz(t).  This lane writes chunks 4 (lane % 4) + u of token
+  // Converted V rows of one page, 256 bytes a token, 16-byte chunk ch of token t
+  // at slot ch ^ vswz(t): 16 lanes of a write take 16 slots, 32 lanes of a
+  // transposed read take all 256 bytes of banks.  This lane writes chunks 4 (lane % 4) + u of token
   // lane / 4, and supplies token 4 q4 + c / 4, dimensions 16 mt + 4 (c % 4) .. + 3
   // to a transposed read, which gives it dimension 16 mt + c of tokens 4 q4 .. + 3.
-  auto vswz = [](int t) { return 2 * (t & 3) | ((t >> 2) & 1) << 3; };
+  auto vswz = [](int t) { return (t & 3) | (t & 1) << 2 | (t & 4) << 1; };
   const int vtok = lane >> 2;
-  int vwrite[4], vread[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) vwrite[u] = vtok * 256 + ((4 * (lane & 3) + u) ^ vswz(vtok)) * 16;
   const int rtok = 4 * q4 + (c >> 2);
-#pragma unroll
-  for (int u = 0; u < 4; ++u) vread[u] = rtok * 256 + ((2 * u + ((c >> 1) & 1)) ^ vswz(rtok)) * 16 + (c & 1) * 8;
+  const int vwrite = vtok * 256 + ((4 * (lane & 3)) ^ vswz(vtok)) * 16;            // chunk u: ^ 16 u
+  const int vread = rtok * 256 + (((c >> 1) & 1) ^ vswz(rtok)) * 16 + (c & 1) * 8;  // d-tile mt: ^ 32 mt
 
-  // The tile to copy next: tile ft of piece F, its page ids, and whether it
-  // opens a piece.  A piece's first page ids come by scalar loads, one piece
-  // ahead; the others from its table words, lane L of lo / hi holding page L and
-  // 64 + L, which arrive with its first tile.
-  i32x8 F = desc_at(wave);
-  int ft = 0;
-  bool fvalid = true, fnew = true;
-  int id0, id1, id2, id3;
-  Fp4Piece piece;
-  auto good_id = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pages ? id : 0; };
-  auto bt_row = [&]() { return p.block_tables + (int64_t)F[0] * p.bt_stride + F[1]; };
-  auto open_ids = [&]() {
-    const int last = max(F[2] - F[1] - 1, 0);
-    id0 = good_id(sload(bt_row(), 0));
-    id1 = good_id(sload(bt_row(), min(1, last)));
-    id2 = good_id(sload(bt_row(), min(2, last)));
-    id3 = good_id(sload(bt_row(), min(3, last)));
-  };
-  open_ids();
-  auto advance = [&]() {
-    ++ft;
-    fnew = kFp4TilePages * ft >= F[2] - F[1];
-    if (!fnew) {
-      const int words = kFp4TilePages * ft < 64 ? piece.lo : piece.hi;
-      const int at = (kFp4TilePages * ft) & 63;
-      id0 = __builtin_amdgcn_readlane(words, at);
-      id1 = __builtin_amdgcn_readlane(words, at + 1);
-      id2 = __builtin_amdgcn_readlane(words, at + 2);
-      id3 = __builtin_amdgcn_readlane(words, at + 3);
-      return;
-    }
-    fvalid = nx < nx_end;
-    if (!fvalid) return;
-    F = desc_at(nx);
-    ++nx;
-    ft = 0;
-    open_ids();
-  };
-  // This lane's addresses in page 0 of head F[7]; a page id adds page_stride,
-  // below 2^32 bytes.
-  const uint8_t *k_lane, *v_lane, *ks_lane, *vs_lane;
-  auto copy_tile = [&](lds_u8* buf) {
-    if (fnew) {
-      const int64_t head = (int64_t)F[7] * p.head_stride;
-      k_lane = (const uint8_t*)p.k_cache + head + koff;
-      v_lane = (const uint8_t*)p.v_cache + head + voff;
-      ks_lane = (const uint8_t*)p.k_cache + head + kFp4ScaleOffset + c * kFp4RowScales;
-      vs_lane = (const uint8_t*)p.v_cache + head + kFp4ScaleOffset + c * kFp4RowScales;
-    }
-    Fp4Copy cp;
-    const uint32_t stride = (uint32_t)p.page_stride;
-    auto page = [&](const uint8_t* lane_base, int id) { return lane_base + (uint64_t)(uint32_t)id * stride; };
-    cp.k[0] = page(k_lane, id0), cp.k[1] = page(k_lane, id1), cp.k[2] = page(k_lane, id2), cp.k[3] = page(k_lane, id3);
-    cp.v[0] = page(v_lane, id0), cp.v[1] = page(v_lane, id1), cp.v[2] = page(v_lane, id2), cp.v[3] = page(v_lane, id3);
-    int mine = id0;  // the page whose scales this lane copies
-    mine = q4 == 1 ? id1 : mine;
-    mine = q4 == 2 ? id2 : mine;
-    mine = q4 == 3 ? id3 : mine;
-    cp.ks = page(ks_lane, mine), cp.vs = page(vs_lane, mine);
-    const uint32_t at = (uint32_t)(uintptr_t)buf;
-    if (fnew) {
-      const int last = max(F[2] - F[1] - 1, 0);
-      fp4_tile_copy_first(cp, at, q_addr(F), bt_row() + min(lane, last), bt_row() + min(64 + lane, last), piece);
-      piece.lo = good_id(piece.lo);
-      piece.hi = good_id(piece.hi);
-    } else {
-      fp4_tile_copy(cp, at);
-    }
-  };
-
-  i32x8 X = F;  // the piece being computed
+  i32x8 X = desc_at(wave);  // the piece being computed
+  i32x8 N_ = X;             // the one after it
   int seq_len = sload(p.seq_lens, X[0]);
-  int xt = 0;
+  auto good_id = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pages ? id : 0; };
+  // This lane's addresses in page 0 of head X[7]; a page id adds page_stride,
+  // below 2^32 bytes.
+  const uint8_t *k_lane, *v_lane, *sc_lane;
+  auto tile_at = [&](int id0, int id1) {
+    auto page = [&](const uint8_t* lane_base, int id) {
+      return lane_base + (uint64_t)(uint32_t)id * (uint32_t)p.page_stride;
+    };
+    return Fp4Copy{{page(k_lane, id0), page(k_lane, id1), page(v_lane, id0), page(v_lane, id1)},
+                   page(sc_lane, (q4 & 1) ? id1 : id0)};
+  };
   V8 qf[4];
   f32x4 o[8];  // o[mt][r] = O^T[d = 16 mt + 4 q4 + r][g = c]
   float m, l;  // reference max (log2 domain) of g = c; this lane's share of the denominator
-  auto open_piece = [&]() {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) qf[j] = q_lane ? __builtin_bit_cast(V8, piece.q[j]) : V8{};
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m = -INFINITY;
-    l = 0.f;
-  };
-
   // `valid`: tokens of the tile that count; below 64 on an edge tile.
   auto compute = [&](lds_u8* buf, int valid) __attribute__((always_inline)) {
     const bool edge = valid < kFp4TileTokens;  // wave-uniform
-    u32x4 vw[4];  // page i's codes of token lane / 4, group lane % 4
-    uint32_t vs[4];
+    u32x4 vw[2];  // page i's codes of token lane / 4, group lane % 4
+    uint32_t vs[2];
+    u32x4 kw[2];
+    float ks[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vw[i] = lds_ld16<u32x4>(buf + kFp4TileV + i * kFp4ScaleOffset + voff);
-      vs[i] = buf[kFp4TileVScales + 64 * i + lane];
-    }
-    u32x4 kw[4];
-    float ks[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       kw[i] = lds_ld16<u32x4>(buf + kread + i * kFp4ScaleOffset);
       ks[i] = fp4_scale((uint32_t)buf[ksread + 64 * i]);
     }
-    f32x4 sc[4];  // sc[i][r] = S[token 4 q4 + r of page i][g = c]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // The four pages' sums in turn: one alone is a chain of dependent MFMAs.
+    for (int i = 0; i < 2; ++i) {
+      vw[i] = lds_ld16<u32x4>(buf + kFp4TileV + i * kFp4ScaleOffset + voff);
+      vs[i] = buf[kFp4TileVScales + 64 * i + lane];
+    }
+    f32x4 sc[2];  // sc[i][r] = S[token 4 q4 + r of page i][g = c]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // The two pages' sums in turn: one alone is a chain of dependent MFMAs.
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[i] = Elem<T>::mfma16(fp4_unpack8<T>(kw[i][j], ks[i]), qf[j], sc[i]);
-      __builtin_amdgcn_sched_barrier(0);  // not all conversions at once: registers
+      for (int i = 0; i < 2; ++i) sc[i] = Elem<T>::mfma16(fp4_unpack8<T>(kw[i][j], ks[i]), qf[j], sc[i]);
+      if (j & 1) __builtin_amdgcn_sched_barrier(0);  // not all conversions at once: registers
     }
-    // Rows of pages 2 half and 2 half + 1 over the tile's codes.  LDS works in
-    // order for a wavefront: reads before these writes see the codes, and the
-    // second half's writes come after the first half's reads.
-    auto write_v = [&](int half) __attribute__((always_inline)) {
+    // Rows of page i over the tile's codes, and their transposed reads.  LDS works
+    // in order for a wavefront: the reads of codes above come before the first
+    // page's writes, its transposed reads before the second page's writes.
+    auto write_v = [&](int i) __attribute__((always_inline)) {
+      u32x4 w = vw[i];
+      uint32_t byte = vs[i];
+      if (edge) {
+        const bool live = kPageSize * i + vtok < valid;
+        byte = live ? byte : 127u;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int i = 2 * half + k;
-        u32x4 w = vw[i];
-        uint32_t byte = vs[i];
-        if (edge) {
-          const bool live = kPageSize * i + vtok < valid;
-          byte = live ? byte : 127u;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) w[u] = live ? w[u] : 0u;
-        }
-        const float scale = fp4_scale(byte);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          lds_st16(buf + k * kDecodePageBytes + vwrite[u], fp4_unpack8<T>(w[u], scale));
-        __builtin_amdgcn_sched_barrier(0);
+        for (int u = 0; u < 4; ++u) w[u] = live ? w[u] : 0u;
       }
+      const float scale = fp4_scale(byte);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) lds_st16(buf + (vwrite ^ (16 * u)), fp4_unpack8<T>(w[u], scale));
     };
+    // v[mt]: dimension 16 mt + c of tokens 4 q4 .. + 3 of the page.
+    auto read_v = [&](s16x4 (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) v[mt] = lds_ld_tr16(buf + (vread ^ (32 * mt)));
+    };
+    s16x4 v0[8], v1[8];
     wave_lds_fence();
     write_v(0);
+    wave_lds_fence();
+    read_v(v0);
+    wave_lds_fence();
+    write_v(1);
+    wave_lds_fence();
+    read_v(v1);
     if (edge) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (kPageSize * i + 4 * q4 + r >= valid) sc[i][r] = -INFINITY;
     }
     // P = 2^(S * scale - m), packed, and this lane's sum of it.
-    V8 pf[2];
+    V8 pf;
     auto exponentials = [&](float m_use) __attribute__((always_inline)) {
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float pr = fast_exp2(sc[i][r] * p.scale_log2 - m_use);
-          sum[r] += pr;
-          pf[i >> 1][4 * (i & 1) + r] = (T)pr;
+          sum[r & 1] += pr;
+          pf[4 * i + r] = (T)pr;
         }
-      return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      return sum[0] + sum[1];
     };
     // The reference maximum moves only when a score exceeds it by more than 8
     // (P stays <= 2^8).  A sum below 128 shows that none does, as every P is
@@ -357,7 +266,7 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
     if (__any(!(sum < 128.f && __builtin_fabsf(m) < 0x1p20f))) {
       float tmax = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, sc[i][r]);
       tmax = groups_max(tmax) * p.scale_log2;  // scale > 0 commutes with max
@@ -371,30 +280,10 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
       sum = exponentials(m == -INFINITY ? 0.f : m);
     }
     l += sum;
-    // d-tile mt: tokens 4 q4 .. + 3 of the half's two pages.
-    auto read_v = [&](V8 (&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        // Chunks of d-tile mt lie 8 chunks, one bit of the slot, from those of mt - 4.
-        const lds_u8* a = buf + (mt < 4 ? vread[mt] : vread[mt - 4] ^ 128);
-        v[mt] = __builtin_bit_cast(
-            V8, __builtin_shufflevector(lds_ld_tr16(a), lds_ld_tr16(a + kDecodePageBytes), 0, 1, 2, 3, 4, 5, 6, 7));
-      }
-    };
-    V8 v[8];
-    __builtin_amdgcn_sched_barrier(0);
-    wave_lds_fence();
-    read_v(v);
-    wave_lds_fence();
-    __builtin_amdgcn_sched_barrier(0);
-    write_v(1);
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) o[mt] = Elem<T>::mfma16(v[mt], pf[0], o[mt]);
-    __builtin_amdgcn_sched_barrier(0);
-    wave_lds_fence();
-    read_v(v);
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) o[mt] = Elem<T>::mfma16(v[mt], pf[1], o[mt]);
+    for (int mt = 0; mt < 8; ++mt)
+      o[mt] = Elem<T>::mfma16(
+          __builtin_bit_cast(V8, __builtin_shufflevector(v0[mt], v1[mt], 0, 1, 2, 3, 4, 5, 6, 7)), pf, o[mt]);
   };
 
   // End of piece X: the final output, or its split-K partial (normalised o and
@@ -404,8 +293,10 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
     const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
     const int h = X[7];
     if (!q_lane) return;
+    int hc = h * G + c;
+    asm volatile("" : "+v"(hc));  // its address is made here, not held in registers through the stream
     if (X[4] == 1) {
-      T* op = (T*)p.out + (int64_t)X[6] * p.out_tok_stride + (int64_t)(h * G + c) * p.out_head_stride + 4 * q4;
+      T* op = (T*)p.out + (int64_t)X[6] * p.out_tok_stride + (int64_t)hc * p.out_head_stride + 4 * q4;
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) {
         V4 w;
@@ -415,45 +306,83 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
       }
       return;
     }
-    const int64_t slot = (int64_t)(X[5] + X[3]) * Hkv + h;
-    float* po = p.part_o + (slot * G + c) * kHeadDim + 4 * q4;
+    const int64_t row = (int64_t)(X[5] + X[3]) * Hkv * G + hc;
+    float* po = p.part_o + row * kHeadDim + 4 * q4;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) store16_device_untracked(po + 16 * mt, __builtin_bit_cast(u32x4, o[mt] * inv));
-    if (q4 == 0) store4_device_untracked(&p.part_lse[slot * G + c], l_tot > 0.f ? m + fast_log2(l_tot) : -INFINITY);
+    if (q4 == 0) store4_device_untracked(&p.part_lse[row], l_tot > 0.f ? m + fast_log2(l_tot) : -INFINITY);
   };
 
-  // ---- tile stream: tile k + 1 is copied while tile k is computed -----------
-  copy_tile(lds);
-  advance();
-  open_piece();
-  int buf = 0;
+  int done = 0;
+  const int mate1 = slot < 8 ? slot + 4 : slot - 8, mate2 = slot < 4 ? slot + 8 : slot - 4;
+  auto keep_level = [&]() {
+    if (!progress) return;
+    if (lane == 0) progress[slot] = done;
+    const int a = __builtin_amdgcn_readfirstlane(*(volatile int*)&progress[mate1]);
+    const int b = __builtin_amdgcn_readfirstlane(*(volatile int*)&progress[mate2]);
+    const int behind = (a < done ? 1 : 0) + (b < done ? 1 : 0);
+    if (behind == 0) __builtin_amdgcn_s_setprio(2);
+    else if (behind == 1) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+    ++done;
+  };
+
+  // ---- piece by piece, run by run -------------------------------------------
+  static_assert(kFp4TileBufs == 3 && kFp4TilePages == 2, "the run's copies and waits");
   for (;;) {
-    lds_u8* const cur = lds + buf * kFp4TileBytes;
-    lds_u8* const nxt = lds + (buf ^ 1) * kFp4TileBytes;
-    const bool more = fvalid, piece_ends = fnew || !fvalid;
-    const i32x8 Y = F;
-    const int y_len = sload(p.seq_lens, Y[0]);
-    if (more) {
-      copy_tile(nxt);
-      advance();
-    } else {
-      __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    const bool more = nx < nx_end;
+    if (more) N_ = desc_at(nx);
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+    const int64_t head = (int64_t)X[7] * p.head_stride;
+    k_lane = (const uint8_t*)p.k_cache + head + koff;
+    v_lane = (const uint8_t*)p.v_cache + head + voff;
+    sc_lane = (const uint8_t*)(q4 < 2 ? p.k_cache : p.v_cache) + head + kFp4ScaleOffset + c * kFp4RowScales;
+    for (int first = X[1]; first < X[2]; first += kFp4RunPages) {
+      const int pages = min(X[2] - first, kFp4RunPages);
+      const int tiles = (pages + 1) >> 1;
+      const int32_t* const row = p.block_tables + (int64_t)X[0] * p.bt_stride + first;
+      int words[kFp4RunPages / 64];  // lane L of words[k]: page 64 k + L of the run
+#pragma unroll
+      for (int k = 0; k < kFp4RunPages / 64; ++k) words[k] = row[min(64 * k + lane, pages - 1)];
+      const T* const q = q_addr(X);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[j] = ld16<V8>(q + 8 * j);
+#pragma unroll
+      for (int k = 0; k < kFp4RunPages / 64; ++k) words[k] = good_id(words[k]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[j] = q_lane ? qf[j] : V8{};
+      const int tokens = min(seq_len, X[2] * kPageSize) - first * kPageSize;  // of the run on
+      lds_u8* buf = lds;
+      for (int t = -kFp4TileBufs; t < tiles; ++t) {
+        if (t >= 0) {
+          if (t + 2 < tiles) __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * kFp4TileLoads));
+          else if (t + 1 < tiles) __builtin_amdgcn_s_waitcnt(waitcnt_vm(kFp4TileLoads));
+          else __builtin_amdgcn_s_waitcnt(kVmcnt0);
+          wave_lds_fence();
+          compute(buf, tokens - t * kFp4TileTokens);
+          wave_lds_fence();
+        }
+        const int page = kFp4TilePages * (t + kFp4TileBufs);
+        if (page < pages) {
+          const int word = page < 128 ? (page < 64 ? words[0] : words[1]) : (page < 192 ? words[2] : words[3]);
+          fp4_copy_tile(
+              tile_at(__builtin_amdgcn_readlane(word, page & 63), __builtin_amdgcn_readlane(word, (page & 63) + 1)),
+              (uint32_t)(uintptr_t)buf);
+        }
+        buf = buf == lds + (kFp4TileBufs - 1) * kFp4TileBytes ? lds : buf + kFp4TileBytes;
+        keep_level();
+      }
     }
-    wave_lds_fence();
-    const int begin = X[1] + kFp4TilePages * xt;
-    const int valid = min(seq_len, X[2] * kPageSize) - begin * kPageSize;
-    compute(cur, valid);
-    wave_lds_fence();
-    buf ^= 1;
-    ++xt;
-    if (!piece_ends) continue;
     finish_piece();
     if (!more) break;
-    X = Y;
-    xt = 0;
-    seq_len = y_len;
-    open_piece();
+    X = N_;
+    ++nx;
+    seq_len = sload(p.seq_lens, X[0]);
   }
+  if (progress && lane == 0) progress[slot] = 0x3fffffff;  // no longer in the way
   __builtin_amdgcn_s_waitcnt(kVmcnt0);
 }
 

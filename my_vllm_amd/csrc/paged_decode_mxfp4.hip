@@ -18,14 +18,19 @@ int launch_decode_merge(const DecodeParams& p, const int32_t* merges, int64_t nu
 
 namespace {
 
+// kWaves wavefronts per workgroup, each with private LDS buffers; wavefront w of
+// workgroup b is decode wavefront b * kWaves + w.
 template <typename T, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void paged_decode_mxfp4_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))) void paged_decode_mxfp4_kernel(
     Fp4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * kFp4WaveLdsBytes];
+  // Tiles done by the wavefronts; one without work reads as far ahead.
+  __shared__ int progress[kWaves];
   const int w = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wave = (int)blockIdx.x * kWaves + w;
+  if (kWaves == 12 && (threadIdx.x & 63) == 0) progress[w] = 0x3fffffff;
   if (wave >= p.num_waves) return;
-  decode_wave_mxfp4<T>(p, wave, (lds_u8*)lds + w * kFp4WaveLdsBytes);
+  decode_wave_mxfp4<T>(p, wave, (lds_u8*)lds + w * kFp4WaveLdsBytes, kWaves == 12 ? progress : nullptr, w);
 }
 
 template <typename T>
@@ -35,8 +40,8 @@ int launch(const Fp4DecodeParams& p, int waves_per_group, hipStream_t s) {
     case 1: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 1>), dim3(blocks), dim3(64), 0, s, p); break;
     case 2: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 2>), dim3(blocks), dim3(128), 0, s, p); break;
     case 4: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 4>), dim3(blocks), dim3(256), 0, s, p); break;
-    case 8: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 8>), dim3(blocks), dim3(512), 0, s, p); break;
-    default: return set_error("paged attention: waves_per_group must be 1, 2, 4 or 8");
+    case 12: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 12>), dim3(blocks), dim3(768), 0, s, p); break;
+    default: return set_error("paged attention mxfp4: waves_per_group must be 1, 2, 4 or 12");
   }
   return check_launch("paged_decode_mxfp4");
 }

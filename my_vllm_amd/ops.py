@@ -25,6 +25,9 @@ PAGE_SIZE = 16
 DECODE_ITEM_INTS = 8
 # Longest piece one decode work item may cover (kMaxChunkPages).
 MAX_CHUNK_PAGES = 128
+# Piece length of a plan whose pieces are not cut any further (kAnyPiecePages):
+# paged_decode_mxfp4 takes pieces of any length, paged_decode of MAX_CHUNK_PAGES.
+ANY_PIECE_PAGES = 0x7fffffff
 # Query rows per prefill workgroup (kPrefillRows): G heads x 128 // G tokens.
 PREFILL_ROWS = 128
 # Query rows per tile of the planned prefill (mva_paged_prefill,
