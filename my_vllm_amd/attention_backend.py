@@ -639,11 +639,11 @@ class MI355XAttentionBackendMixin:
     def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
         """(page ranges, wavefronts per workgroup) of a decode launch with piece lists."""
         if self.decode_waves_override:
-            return self._most_decode_ranges(device)
+            return self._most_decode_ranges(int(decode_counts.sum()), device)
         return decode_ranges(int(decode_counts.sum()), len(decode_counts), self.num_kv_heads, device)
 
-    def _most_decode_ranges(self, device: torch.device) -> tuple[int, int]:
-        """The same for the largest batch: what a captured launch is sized for."""
+    def _most_decode_ranges(self, total_pages: int, device: torch.device) -> tuple[int, int]:
+        """The same for a batch of at most ``total_pages``: what a captured launch is sized for."""
         return listed_decode_groups(self.num_kv_heads, device, override=self.decode_waves_override)
 
     # ---- per-step metadata and plan ------------------------------------------
@@ -1099,7 +1099,7 @@ class MI355XAttentionBackendMixin:
         graph_device = torch.device(device)
         if graph_device.type != "cuda":
             raise ValueError("full decode graph state must be on CUDA")
-        groups, waves_per_group = self._most_decode_ranges(graph_device)
+        groups, waves_per_group = self._most_decode_ranges(page_indices_capacity, graph_device)
         caps = graph_decode_capacities(batch_size, page_indices_capacity, self.num_kv_heads, groups)
         group = self.num_q_heads // self.num_kv_heads
         plan_ints = graph_plan_buffer_ints(caps["item_capacity"], caps["wave_capacity"], caps["merge_capacity"])
@@ -1325,16 +1325,32 @@ class MI355XSplitAttentionBackend(MI355XAttentionBackend):
     default_attention_mode = "split"
 
 
-# Wavefronts per CU of a decode launch over an MXFP4 cache (kFp4WaveLdsBytes of
-# LDS each).
-_MXFP4_WAVES_PER_CU = 12
+# A decode launch over an MXFP4 cache: (wavefronts per CU, wavefronts per
+# workgroup) of batches below and from _MXFP4_LARGE_BYTES of K and V.  Twelve
+# wavefronts, whose priorities keep the three of a SIMD level, fill a CU's LDS;
+# eight leave fewer split-K chunks and start sooner.  Call, microseconds, 12 / 8:
+# 56 sequences of 8192-32768 tokens at 64 / 8 heads (1.4 GB) 251 / 264, 28
+# (0.7 GB) 117 / 122, 14 (0.4 GB) 70.0 / 65.6; 64 of 128-2048 at 16 / 8 26.4 /
+# 23.6; one of 30001 at 32 / 8 20.0 / 17.1.
+_MXFP4_LARGE_BYTES = 512 << 20
+_MXFP4_WAVES = ((8, 4), (12, 12))
+# Pages a range has at least, two tiles.  Ranges of one / four / sixteen pages:
+# one sequence of 30000 tokens at 8 / 1 heads 24.6 / 13.6 / 15.5, eight of
+# 256-1024 at 16 / 8 12.9 / 12.6 / 16.3.
+_MXFP4_RANGE_PAGES = 4
 
 
-def mxfp4_decode_ranges(num_kv_heads: int, device: torch.device | None = None,
+def mxfp4_decode_ranges(total_pages: int, num_kv_heads: int, device: torch.device | None = None,
                         override: int | None = None) -> tuple[int, int]:
-    """(page ranges, wavefronts per workgroup) of a decode launch over an MXFP4 cache."""
-    waves = max(1, int(override)) if override else _num_cus(device) * _MXFP4_WAVES_PER_CU
-    return max(1, waves // num_kv_heads), _MXFP4_WAVES_PER_CU
+    """(page ranges, wavefronts per workgroup) of a decode launch over an MXFP4
+    cache; ``override`` (a backend's ``decode_waves_override``) sets the
+    wavefront count the ranges share."""
+    large = total_pages * num_kv_heads * 2 * ops.MXFP4_PAGE_BYTES >= _MXFP4_LARGE_BYTES
+    waves_per_cu, per_group = _MXFP4_WAVES[large]
+    if override:
+        return max(1, int(override) // num_kv_heads), per_group
+    ranges = _num_cus(device) * waves_per_cu // num_kv_heads
+    return max(1, min(ranges, total_pages // _MXFP4_RANGE_PAGES)), per_group
 
 
 class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
@@ -1362,10 +1378,10 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
         return "listed"
 
     def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
-        return self._most_decode_ranges(device)
+        return mxfp4_decode_ranges(int(decode_counts.sum()), self.num_kv_heads, device, self.decode_waves_override)
 
-    def _most_decode_ranges(self, device: torch.device) -> tuple[int, int]:
-        return mxfp4_decode_ranges(self.num_kv_heads, device, self.decode_waves_override)
+    def _most_decode_ranges(self, total_pages: int, device: torch.device) -> tuple[int, int]:
+        return mxfp4_decode_ranges(total_pages, self.num_kv_heads, device, self.decode_waves_override)
 
     def _validate_inputs(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
         if _native.host_ops().forward_inputs_ok_mxfp4(q, k_cache, v_cache, _native.DTYPE_CODES[self.dtype],

@@ -356,7 +356,10 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
       for (int j = 0; j < 4; ++j) qf[j] = q_lane ? qf[j] : V8{};
       const int tokens = min(seq_len, X[2] * kPageSize) - first * kPageSize;  // of the run on
       lds_u8* buf = lds;
-      for (int t = -kFp4TileBufs; t < tiles; ++t) {
+      int t = -kFp4TileBufs;
+      asm volatile("" : "+s"(t));  // one copy of the loop's code: no peeled first turns
+#pragma unroll 1
+      for (; t < tiles; ++t) {
         if (t >= 0) {
           if (t + 2 < tiles) __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * kFp4TileLoads));
           else if (t + 1 < tiles) __builtin_amdgcn_s_waitcnt(waitcnt_vm(kFp4TileLoads));
