@@ -535,6 +535,18 @@ int mva_paged_decode_mxfp4(const void* q, int64_t q_token_stride, int64_t q_head
                            int num_kv_heads, int head_dim, int page_size, float softmax_scale, int dtype,
                            void* stream);
 
+/*
+ * mva_paged_prefill (planned == 0) or mva_paged_prefill_run (planned != 0: the
+ * workspace holds the batch's plan, from either kind of cache) over MXFP4 caches.
+ */
+int mva_paged_prefill_mxfp4(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                            const void* v_cache, int64_t num_pages, int64_t page_stride_bytes,
+                            int64_t head_stride_bytes, const int32_t* block_tables, int64_t block_table_stride,
+                            const int32_t* seq_lens, const int32_t* query_start_loc, int64_t num_seqs,
+                            int64_t max_tiles, void* workspace, int64_t workspace_bytes, int planned, void* out,
+                            int64_t out_token_stride, int64_t out_head_stride, int num_q_heads, int num_kv_heads,
+                            int head_dim, int page_size, float softmax_scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

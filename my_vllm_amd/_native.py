@@ -149,6 +149,17 @@ _SIGNATURES = {
             _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p,  # heads, head_dim, page, scale, dtype, stream
         ],
     ),
+    "mva_paged_prefill_mxfp4": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64,  # q, q_token_stride, q_head_stride
+            _c_void_p, _c_void_p, _i64, _i64, _i64,  # k_cache, v_cache, num_pages, page and head strides (bytes)
+            _c_void_p, _i64, _c_void_p, _c_void_p,  # block_tables, stride, seq_lens, query_start_loc
+            _i64, _i64, _c_void_p, _i64, _i32,  # num_seqs, max_tiles, workspace, workspace_bytes, planned
+            _c_void_p, _i64, _i64,  # out, out_token_stride, out_head_stride
+            _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p,
+        ],
+    ),
     "mva_decode_plan_listed_rows": (_i64, [_i64, _i64, _i32, _i32, _i32]),
     "mva_decode_plan_listed": (
         _i32,

@@ -525,6 +525,29 @@ PyObject* paged_decode_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// (q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, num_seqs,
+//  max_tiles, workspace, out, scale, planned): True when launched.
+PyObject* paged_prefill_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    PagedFp4 p;
+    int64_t seqs, tiles;
+    double scale;
+    if (n != 12 || !p.read(a[0], a[1], a[2], a[3], a[4], a[9])) return none();
+    const Tensor *qsl = plain(a[5]), *ws = plain(a[8]);
+    if (!p.ints(qsl) || !p.bytes(ws) || !as_int(a[6], &seqs) || !as_int(a[7], &tiles) || !as_float(a[10], &scale) ||
+        !PyBool_Check(a[11]))
+      return none();
+    const Tensor &q = *p.q, &kc = *p.kc, &out = *p.out;
+    void* const stream = stream_of(q);
+    const int status = unlocked(
+        mva_paged_prefill_mxfp4, ptr(q), q.stride(0), q.stride(1), ptr(kc), ptr(*p.vc), kc.size(0), kc.stride(0),
+        kc.stride(1), words(p.bt), p.bt->stride(0), words(p.sl), words(qsl), seqs, tiles, ptr(*ws), nbytes(ws),
+        (int)(a[11] == Py_True), ptr(out), out.stride(0), out.stride(1), (int)q.size(1), (int)kc.size(1), kHeadDim, 16,
+        (float)scale, p.code, stream);
+    return launched("mva_paged_prefill_mxfp4", status);
+  });
+}
+
 // (q, k_cache, v_cache, MVA_DTYPE_* of the backend, num_q_heads, num_kv_heads): forward_inputs_ok over MXFP4 caches.
 PyObject* forward_inputs_ok_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -559,7 +582,8 @@ PyMethodDef kMethods[] = {MVA_METHOD(silu_and_mul),       MVA_METHOD(rms_norm), 
                           MVA_METHOD(qk_norm_rope_store), MVA_METHOD(paged_decode),  MVA_METHOD(paged_prefill),
                           MVA_METHOD(paged_mixed),        MVA_METHOD(forward_inputs_ok), MVA_METHOD(capture_id),
                           MVA_METHOD(store_kvcache_mxfp4), MVA_METHOD(load_kvcache_mxfp4),
-                          MVA_METHOD(paged_decode_mxfp4), MVA_METHOD(forward_inputs_ok_mxfp4),
+                          MVA_METHOD(paged_decode_mxfp4), MVA_METHOD(paged_prefill_mxfp4),
+                          MVA_METHOD(forward_inputs_ok_mxfp4),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "mva_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

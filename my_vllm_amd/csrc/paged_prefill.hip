@@ -416,9 +416,8 @@ __device__ __attribute__((always_inline)) inline void leave_prefill_plan(int32_t
 // ahead (prefill_items_pingpong), so the grid never waits on dispatch and
 // faster CUs simply run more tiles; once their head's queue is exhausted
 // they take the remaining tiles of the other heads.
-template <typename T, bool kPieces>
-__global__ __launch_bounds__(kPrefillPPThreads) void paged_prefill_stream_kernel(PrefillParams p,
-                                                                                 int32_t* __restrict__ plan) {
+template <typename T, bool kPieces, typename P>
+__global__ __launch_bounds__(kPrefillPPThreads) void paged_prefill_stream_kernel(P p, int32_t* __restrict__ plan) {
   __shared__ __attribute__((aligned(16))) uint8_t tiles[kPrefillPPLdsBytes];
   __shared__ int nextq[8];
   const int h = (int)(blockIdx.x % (uint32_t)p.num_kv_heads);
@@ -432,9 +431,8 @@ __global__ __launch_bounds__(kPrefillPPThreads) void paged_prefill_stream_kernel
 
 // The fixed form, for a batch of at most one tile per workgroup of a head: no
 // claims, and tiles may be cut into split-K pieces (plan_pieces).
-template <typename T>
-__global__ __launch_bounds__(kPrefillPPThreads) void paged_prefill_fixed_kernel(PrefillParams p,
-                                                                                int32_t* __restrict__ plan) {
+template <typename T, typename P>
+__global__ __launch_bounds__(kPrefillPPThreads) void paged_prefill_fixed_kernel(P p, int32_t* __restrict__ plan) {
   __shared__ __attribute__((aligned(16))) uint8_t tiles[kPrefillPPLdsBytes];
   __shared__ int nextq[8];
   const int h = (int)(blockIdx.x % (uint32_t)p.num_kv_heads);
@@ -777,8 +775,48 @@ int check_prefill_plan(int64_t max_tiles, const void* workspace, int64_t workspa
   return 0;
 }
 
-// Plans (plan_it) and/or streams (run_it) a prefill batch: the shared body
-// of mva_paged_prefill, mva_paged_prefill_plan and mva_paged_prefill_run.
+// Plans (plan_it) and/or streams (run_it) the prefill batch of `p`: the shared
+// body of the prefill entry points, over either kind of cache (P).
+template <typename P>
+int stream_prefill(P& p, int64_t num_seqs, int64_t max_tiles, void* workspace, int64_t workspace_bytes, int dtype,
+                   void* stream, bool plan_it, bool run_it) {
+  if (dtype != kBF16 && dtype != kF16) return set_error("paged attention: dtype must be bf16 or fp16");
+  if (mva_prefill_workspace_bytes(max_tiles) < 0) return set_error(kBadTileCapacity);
+  if (num_seqs == 0 || max_tiles == 0) return 0;
+  int rc = check_prefill_plan(max_tiles, workspace, workspace_bytes, p.num_kv_heads);
+  if (rc) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  int32_t* plan = (int32_t*)workspace;
+  p.tile_tokens = kPrefillPPRows / p.group;
+  // Persistent grid: one workgroup per CU (96 KB of LDS and two waves per
+  // SIMD each), a whole number per KV head, also where the tiles are fewer:
+  // they may be planned as pieces.
+  int64_t per_head = (int64_t)device_cu_count() / p.num_kv_heads;
+  per_head = per_head < 1 ? 1 : per_head;
+  const PlanForm form = plan_form(max_tiles, per_head);
+  if (plan_it) {
+    rc = launch_prefill_plan(p, num_seqs, max_tiles, plan, workspace_bytes, per_head, per_head * p.num_kv_heads, s);
+    if (rc) return rc;
+  }
+  if (!run_it) return 0;
+  const dim3 grid((uint32_t)(per_head * p.num_kv_heads));
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kPrefillPPThreads), 0, s, p, plan); };
+  if (form == PlanForm::kFixed) {
+    if (dtype == kBF16) launch(paged_prefill_fixed_kernel<__bf16, P>);
+    else launch(paged_prefill_fixed_kernel<_Float16, P>);
+    return check_launch("paged_prefill");
+  }
+  const bool pieces = form == PlanForm::kTurns;
+  if (dtype == kBF16) {
+    if (pieces) launch(paged_prefill_stream_kernel<__bf16, true, P>);
+    else launch(paged_prefill_stream_kernel<__bf16, false, P>);
+  } else {
+    if (pieces) launch(paged_prefill_stream_kernel<_Float16, true, P>);
+    else launch(paged_prefill_stream_kernel<_Float16, false, P>);
+  }
+  return check_launch("paged_prefill");
+}
+
 int prefill_launch(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                    const void* v_cache, int64_t num_pages, int64_t page_stride, int64_t token_stride,
                    const int32_t* block_tables, int64_t block_table_stride, const int32_t* seq_lens,
@@ -787,48 +825,12 @@ int prefill_launch(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                    int num_q_heads, int num_kv_heads, int head_dim, int page_size, float softmax_scale, int dtype,
                    void* stream, bool plan_it, bool run_it) {
   PrefillParams p;
-  int rc = fill_prefill_params(p, q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, page_stride,
-                               token_stride, block_tables, block_table_stride, seq_lens, query_start_loc,
-                               num_seqs, out, out_token_stride, out_head_stride, num_q_heads,
-                               num_kv_heads, head_dim, page_size, softmax_scale);
+  const int rc = fill_prefill_params(p, q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, page_stride,
+                                     token_stride, block_tables, block_table_stride, seq_lens, query_start_loc,
+                                     num_seqs, out, out_token_stride, out_head_stride, num_q_heads, num_kv_heads,
+                                     head_dim, page_size, softmax_scale);
   if (rc) return rc;
-  if (dtype != kBF16 && dtype != kF16) return set_error("paged attention: dtype must be bf16 or fp16");
-  if (mva_prefill_workspace_bytes(max_tiles) < 0) return set_error(kBadTileCapacity);
-  if (num_seqs == 0 || max_tiles == 0) return 0;
-  rc = check_prefill_plan(max_tiles, workspace, workspace_bytes, num_kv_heads);
-  if (rc) return rc;
-  hipStream_t s = (hipStream_t)stream;
-  int32_t* plan = (int32_t*)workspace;
-  p.tile_tokens = kPrefillPPRows / p.group;
-  // Persistent grid: one workgroup per CU (96 KB of LDS and two waves per
-  // SIMD each), a whole number per KV head, also where the tiles are fewer:
-  // they may be planned as pieces.
-  int64_t per_head = (int64_t)device_cu_count() / num_kv_heads;
-  per_head = per_head < 1 ? 1 : per_head;
-  const PlanForm form = plan_form(max_tiles, per_head);
-  if (plan_it) {
-    rc = launch_prefill_plan(p, num_seqs, max_tiles, plan, workspace_bytes, per_head, per_head * num_kv_heads, s);
-    if (rc) return rc;
-  }
-  if (!run_it) return 0;
-  const dim3 grid((uint32_t)(per_head * num_kv_heads));
-  if (form == PlanForm::kFixed) {
-    if (dtype == kBF16)
-      hipLaunchKernelGGL(paged_prefill_fixed_kernel<__bf16>, grid, dim3(kPrefillPPThreads), 0, s, p, plan);
-    else
-      hipLaunchKernelGGL(paged_prefill_fixed_kernel<_Float16>, grid, dim3(kPrefillPPThreads), 0, s, p, plan);
-    return check_launch("paged_prefill");
-  }
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kPrefillPPThreads), 0, s, p, plan); };
-  const bool pieces = form == PlanForm::kTurns;
-  if (dtype == kBF16) {
-    if (pieces) launch(paged_prefill_stream_kernel<__bf16, true>);
-    else launch(paged_prefill_stream_kernel<__bf16, false>);
-  } else {
-    if (pieces) launch(paged_prefill_stream_kernel<_Float16, true>);
-    else launch(paged_prefill_stream_kernel<_Float16, false>);
-  }
-  return check_launch("paged_prefill");
+  return stream_prefill(p, num_seqs, max_tiles, workspace, workspace_bytes, dtype, stream, plan_it, run_it);
 }
 
 // Stand-ins for the buffers a plan-only launch does not touch: they pass the
@@ -875,6 +877,28 @@ extern "C" int mva_paged_prefill_run(const void* q, int64_t q_token_stride, int6
                         block_tables, block_table_stride, seq_lens, query_start_loc, num_seqs, max_tiles, workspace,
                         workspace_bytes, out, out_token_stride, out_head_stride, num_q_heads, num_kv_heads, head_dim,
                         page_size, softmax_scale, dtype, stream, false, true);
+}
+
+extern "C" int mva_paged_prefill_mxfp4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                       const void* k_cache, const void* v_cache, int64_t num_pages,
+                                       int64_t page_stride_bytes, int64_t head_stride_bytes,
+                                       const int32_t* block_tables, int64_t block_table_stride,
+                                       const int32_t* seq_lens, const int32_t* query_start_loc, int64_t num_seqs,
+                                       int64_t max_tiles, void* workspace, int64_t workspace_bytes, int planned,
+                                       void* out, int64_t out_token_stride, int64_t out_head_stride, int num_q_heads,
+                                       int num_kv_heads, int head_dim, int page_size, float softmax_scale, int dtype,
+                                       void* stream) {
+  if (((uint64_t)page_stride_bytes | (uint64_t)head_stride_bytes) % 16)
+    return set_error("paged attention mxfp4: cache strides must be 16-byte aligned");
+  Fp4PrefillParams p;
+  const int rc = fill_prefill_params(p, q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, 0, 0,
+                                     block_tables, block_table_stride, seq_lens, query_start_loc, num_seqs, out,
+                                     out_token_stride, out_head_stride, num_q_heads, num_kv_heads, head_dim,
+                                     page_size, softmax_scale);
+  if (rc) return rc;
+  p.page_stride = page_stride_bytes;
+  p.head_stride = head_stride_bytes;
+  return stream_prefill(p, num_seqs, max_tiles, workspace, workspace_bytes, dtype, stream, planned == 0, true);
 }
 
 extern "C" int mva_paged_mixed(const void* q, int64_t q_token_stride, int64_t q_head_stride,

@@ -25,9 +25,17 @@
 // needs.
 #pragma once
 
+#include "mxfp4.h"
 #include "paged_prefill.h"
 
+#include <type_traits>
+
 namespace mva {
+
+// Prefill over an MXFP4 cache: page_stride counts bytes, tok_stride is unused.
+struct Fp4PrefillParams : PrefillParams {
+  int64_t head_stride;  // bytes between the blocks of a page's KV heads
+};
 
 constexpr int kPrefillPPRows = 256;     // query rows per workgroup
 constexpr int kPrefillPPThreads = 512;  // 8 wavefronts
@@ -205,10 +213,22 @@ __device__ __attribute__((always_inline)) inline bool settle_piece(int32_t* plan
 // known: no plan read, query load, copy wait or claim sits between items.
 // Only when A has a single tile does group 1 copy V(B, 0) at B's start
 // (it is first read at B's phase 2, after the wait that ends phase 1).
-template <typename T, int kGrp, bool kFixed, bool kPieces>
-__device__ __attribute__((always_inline)) inline void prefill_items_pingpong(const PrefillParams& p, int32_t* plan,
+//
+// Over an MXFP4 cache (P = Fp4PrefillParams) a page is copied in two steps: each
+// lane loads 16 bytes of codes and their scale into registers, and a later M
+// phase of the wave converts them (exactly) and writes the rows to the page's
+// place in LDS, four groups of four conversions and a 16-byte write between the
+// phase's MFMAs, whose issue slots the vector ALU does not need.  Loads go out
+// at the end of an M phase, so that they have two phases to arrive: group 0
+// loads K(t+2) after M(t) and writes it in M(t+1), phase 2t+2; group 1 loads
+// V(t+2) after M(t) and writes it in M(t+1), phase 2t+3.  Either is after the
+// last read of the buffer (phase 2t-1, 2t+1) and two phases before the first
+// (2t+4, 2t+6).
+template <typename T, int kGrp, bool kFixed, bool kPieces, typename P>
+__device__ __attribute__((always_inline)) inline void prefill_items_pingpong(const P& p, int32_t* plan,
                                                                              int h0, int rank, lds_u8* tiles, lds_i32* nextq) {
   typedef typename Elem<T>::v8 V8;
+  constexpr bool kFp4 = std::is_same<P, Fp4PrefillParams>::value;
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);  // 0..7
   const int slot = w & 3;  // page slot this wave copies
@@ -271,7 +291,58 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
   auto vbuf = [&](int x) { return tiles + (kPrefillPPBufs + x % kPrefillPPBufs) * kPrefillTileBytes; };
   // This wave's page of K (group 0) or V (group 1) of KV head `head`, global
   // tile x.
+  // MXFP4: the page in registers (its codes and scale byte, and the place of its
+  // rows).  K: this lane holds group lane / 16 of token lane %
+  // 16 and writes chunk u of four at 256 u, 16 lanes side by side.  V: group g =
+  // lane % 4 of token lane / 4; a row's chunks are neighbours there, so lanes of
+  // one token take them in different orders, u ^ g, to write to different banks.
+  u32x4 held_w = {};
+  uint32_t held_byte = 0;
+  lds_u8* held_at = nullptr;
+  bool held = false;
+  const int fp4_tok = kGrp == 0 ? lane & 15 : lane >> 2, fp4_grp = kGrp == 0 ? lane >> 4 : lane & 3;
+  const uint32_t fp4_codes = (uint32_t)(fp4_tok * kFp4RowBytes + fp4_grp * 16);
+  const uint32_t fp4_scales = (uint32_t)(kFp4ScaleOffset + fp4_tok * kFp4RowScales + fp4_grp);
+  const int fp4_rows = 1024 * fp4_grp + (kGrp == 0 ? 16 * fp4_tok : 64 * fp4_tok + 16 * fp4_grp);
+  auto write_chunk = [&](int u) __attribute__((always_inline)) {
+    if constexpr (kFp4) {
+      // Chunk u of K; of V chunk u ^ g, its codes already in word u.
+      const int off = kGrp == 0 ? fp4_rows + 256 * u : fp4_rows ^ (16 * u);
+      lds_st16(held_at + off, fp4_unpack8<T>(held_w[u], fp4_scale(held_byte)));
+    }
+  };
+  // Words in the order of their writes (V).
+  auto order_words = [&]() __attribute__((always_inline)) {
+    if constexpr (kFp4 && kGrp == 1) {
+      u32x4 x = held_w;
+      const bool b0 = lane & 1, b1 = lane & 2;
+      x = u32x4{b0 ? x[1] : x[0], b0 ? x[0] : x[1], b0 ? x[3] : x[2], b0 ? x[2] : x[3]};
+      held_w = u32x4{b1 ? x[2] : x[0], b1 ? x[3] : x[1], b1 ? x[0] : x[2], b1 ? x[1] : x[3]};
+    }
+  };
+  // The page held, at once.
+  auto write_held = [&]() __attribute__((always_inline)) {
+    if constexpr (kFp4) {
+      if (!held) return;
+      order_words();
+#pragma unroll
+      for (int u = 0; u < 4; ++u) write_chunk(u);
+      held = false;
+    }
+  };
   auto copy_page = [&](int x, int page, int head) __attribute__((always_inline)) {
+    if constexpr (kFp4) {
+      // A second page at one time (only items of one or two tiles ask for it)
+      // puts the first in its place: its buffer is free already.
+      write_held();
+      const uint8_t* src = (const uint8_t*)(kGrp == 0 ? p.k_cache : p.v_cache) +
+                           (int64_t)__builtin_amdgcn_readfirstlane(page) * p.page_stride + head * p.head_stride;
+      held_w = ld16<u32x4>(src + fp4_codes);
+      held_byte = src[fp4_scales];
+      held_at = (kGrp == 0 ? kbuf(x) : vbuf(x)) + 4096 * slot;
+      held = true;
+      return;
+    }
     const T* src = (const T*)(kGrp == 0 ? p.k_cache : p.v_cache) + head * kHeadDim;
     lds_u8* buf = kGrp == 0 ? kbuf(x) : vbuf(x);
     dma16_x4_saddr(src + (int64_t)__builtin_amdgcn_readfirstlane(page) * p.page_stride, kGrp == 0 ? koff : voff,
@@ -333,6 +404,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
   };
   // Waits until at most the last c page copies (4 loads each) are in flight.
   auto wait_copies = [&](int c) __attribute__((always_inline)) {
+    if constexpr (kFp4) return;  // its loads are waited for where they are used
     if (c >= 2) __builtin_amdgcn_s_waitcnt(waitcnt_vm(8));
     else if (c == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));
     else __builtin_amdgcn_s_waitcnt(kVmcnt0);
@@ -379,6 +451,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
   } else {
     copy_page(0, cur.pg0, cur_h);
   }
+  write_held();
   __builtin_amdgcn_s_waitcnt(kVmcnt0);
   if (!kFixed && turn == 0) {
     if (w == 0) {
@@ -431,8 +504,14 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
         st[1] = f32x16{};
       }
       if constexpr (with_pv) vf[0] = vread(vb, 0);
+      if constexpr (kFp4) {
+        if (held) order_words();
+      }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
+        if constexpr (kFp4) {
+          if (j % 4 == 2 && held) write_chunk(j / 4);
+        }
         if constexpr (with_qk) {
           if (j + 1 < 16) kf[(j + 1) & 1] = kread(kb, j + 1);
           st[j & 1] = Elem<T>::mfma32(kf[j & 1], qf[j >> 1], st[j & 1]);
@@ -445,6 +524,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
         // which would hold 48 fragments in registers at once.
         __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (kFp4) held = false;
       if constexpr (with_qk) pin_s();
       if constexpr (with_pv) pin_o();
     };
@@ -613,13 +693,15 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
     };
     // Phases 0 and 1.
     pg_next = kGrp == 0 ? pg2_next : __builtin_amdgcn_readfirstlane(cur.pg1);
-    int c = issue(0);
+    int c = 0;
+    if (!kFp4 || kGrp == 1) c = issue(0);
     // B's record (and group 0's tile-3 page) are loaded at the end of the
     // group's phase-0 / phase-1 M phase, where it waits for the other group
     // anyway (its LDS reads are done, so nothing waits behind the loads).
     if constexpr (kGrp == 0) {
       phase_m(0, yes, no);
       load_next();
+      if constexpr (kFp4) issue(0);
       pg_next = page_of(3);
       phase_barrier();
       phase_s(0);
@@ -628,13 +710,15 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
       phase_barrier();
       phase_m(0, yes, no);
       load_next();
+      if constexpr (kFp4) issue(1);
     }
     end_odd_phase(0, c);
     // Phases 2t and 2t+1, t = 1 .. n-1.
     for (int t = 1; t < n; ++t) {
-      c = issue(t);
+      if constexpr (!kFp4) c = issue(t);
       if constexpr (kGrp == 0) {
         phase_m(t, yes, yes);
+        if constexpr (kFp4) issue(t);
         phase_barrier();
         pg_next = page_of(t + 3);
         phase_s(t);
@@ -643,6 +727,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
         phase_s(t - 1);
         phase_barrier();
         phase_m(t, yes, yes);
+        if constexpr (kFp4) issue(t + 1);
       }
       end_odd_phase(t, c);
     }
@@ -653,11 +738,13 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
         load_q(nx, nh);
         if (tid == 0 && turn == 0) claim_ret = claim(claim_head);
       }
-      issue(n);
+      if constexpr (!kFp4) issue(n);
       phase_m(n, no, yes);
+      if constexpr (kFp4) issue(n);
       phase_barrier();
       // B's tile-2 page, loaded while this group waits for group 1's M(n).
       if (has_next) pg2_next = page_of_item(nx, 2);
+      write_held();
       __builtin_amdgcn_s_waitcnt(kVmcnt0);
       if (w == 0 && has_next && turn == 0) {
         const int r = claim_on(claim_ret, claim_head);
@@ -667,7 +754,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
         }
       }
     } else {
-      issue(n);
+      if constexpr (!kFp4) issue(n);
       if (has_next && n >= 2) load_q(nx, nh);
       // B's tile-2 page, in an S phase (no LDS read waits behind the load).
       if (has_next) pg2_next = page_of_item(nx, 2);
@@ -675,6 +762,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
       phase_barrier();
       if (has_next && n == 1) load_q(nx, nh);
       phase_m(n, no, yes);
+      write_held();
       __builtin_amdgcn_s_waitcnt(kVmcnt0);
     }
     phase_barrier();

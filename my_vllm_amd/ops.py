@@ -1117,19 +1117,22 @@ def paged_prefill_mxfp4(
     validate: bool = True,
     planned: bool = False,
 ) -> None:
-    """:func:`paged_prefill` over MXFP4 caches: the pages of the batch are read
-    back into rows of the query's type, which the prefill kernel then takes."""
+    """:func:`paged_prefill` over MXFP4 caches.  The tile plan is the same for
+    both kinds of cache."""
+    if _native.host_ops().paged_prefill_mxfp4(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, num_seqs,
+                                              max_tiles, workspace, out, softmax_scale, planned):
+        return
     if validate:
         _check_paged_mxfp4(q, out, k_cache, v_cache,
                            (("block_tables", block_tables), ("seq_lens", seq_lens),
                             ("query_start_loc", query_start_loc)), (("workspace", workspace),))
-    tables = block_tables[:num_seqs]
-    if tables.numel() == 0:
-        return
-    offsets = torch.arange(PAGE_SIZE, device=q.device)
-    slots = torch.where(tables[..., None] >= 0, tables.long()[..., None] * PAGE_SIZE + offsets, -1)
-    key, value = load_kvcache_mxfp4(k_cache, v_cache, slots, q.dtype)
-    shape = (tables.numel(), PAGE_SIZE, k_cache.shape[1], HEAD_DIM)
-    pages = torch.arange(tables.numel(), dtype=torch.int32, device=q.device).view(tables.shape)
-    paged_prefill(q, key.view(shape), value.view(shape), pages, seq_lens, query_start_loc, num_seqs, max_tiles,
-                  workspace, out, softmax_scale, planned=planned)
+    _call_on(
+        q.device, "mva_paged_prefill_mxfp4",
+        q.data_ptr(), q.stride(0), q.stride(1),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], k_cache.stride(0), k_cache.stride(1),
+        block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), query_start_loc.data_ptr(),
+        int(num_seqs), int(max_tiles), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        int(planned), out.data_ptr(), out.stride(0), out.stride(1),
+        q.shape[1], k_cache.shape[1], q.shape[2], PAGE_SIZE, float(softmax_scale),
+        _native.dtype_code(q.dtype), _native.stream_handle(q.device),
+    )
