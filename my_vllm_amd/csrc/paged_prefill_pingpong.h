@@ -218,7 +218,8 @@ __device__ __attribute__((always_inline)) inline bool settle_piece(int32_t* plan
 // lane loads 16 bytes of codes and their scale into registers, and a later M
 // phase of the wave converts them (exactly) and writes the rows to the page's
 // place in LDS, four groups of four conversions and a 16-byte write between the
-// phase's MFMAs, whose issue slots the vector ALU does not need.  Loads go out
+// phase's last MFMAs, whose issue slots the vector ALU does not need (at its first
+// ones: 1% slower).  Loads go out
 // at the end of an M phase, so that they have two phases to arrive: group 0
 // loads K(t+2) after M(t) and writes it in M(t+1), phase 2t+2; group 1 loads
 // V(t+2) after M(t) and writes it in M(t+1), phase 2t+3.  Either is after the
@@ -510,7 +511,7 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         if constexpr (kFp4) {
-          if (j % 4 == 2 && held) write_chunk(j / 4);
+          if (j >= 12 && held) write_chunk(j - 12);
         }
         if constexpr (with_qk) {
           if (j + 1 < 16) kf[(j + 1) & 1] = kread(kb, j + 1);

@@ -107,8 +107,8 @@ def _abi_store(**change):
     ({"dtype": 2}, "bf16 or fp16"),
     ({"tokens": -1}, "invalid sizes"),
     ({"heads": 0}, "invalid sizes"),
-    ({"heads": 40000}, "too many KV heads"),
-    ({"tokens": 1 << 40}, "too many tokens"),
+    ({"heads": 40000}, "at most 32767 KV heads"),
+    ({"tokens": (1 << 40) + 1}, "too many tokens"),
     ({"key": 0}, "null buffer"),
     ({"slots": 0}, "null buffer"),
     ({"kc": 0}, "null buffer"),
