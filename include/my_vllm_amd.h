@@ -501,7 +501,8 @@ int mva_paged_mixed_run(const void* q, int64_t q_token_stride, int64_t q_head_st
  * slots < 0 or past the cache are skipped; the others must be distinct).
  * Groups of 32 take the smallest scale 2^e with max|x| <= 7 * 2^e, e <= 125
  * (bf16) or 13 (fp16); codes are x / 2^e to nearest even.  A group with an
- * infinity or a NaN gets scale byte 255 and codes 0.
+ * infinity or a NaN gets scale byte 255 and codes 0.  At most 2^40 tokens and
+ * 32767 KV heads.
  */
 int mva_kv_store_mxfp4(const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
                        int64_t value_token_stride, int64_t value_head_stride, void* k_cache, void* v_cache,
@@ -521,7 +522,8 @@ int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stri
 
 /*
  * mva_paged_decode over MXFP4 caches, with piece lists (wave_extra; no
- * claims).  With counts ([3] int32 on the device) it is the fixed-shape launch
+ * claims), pieces of any length and waves_per_group 4 or 12.  Pages must lie
+ * less than 4 GiB apart.  With counts ([3] int32 on the device) it is the fixed-shape launch
  * of mva_paged_decode_graph: num_items, num_waves and num_merges are then
  * capacities.  The workspace is mva_paged_decode's.
  */

@@ -1467,6 +1467,17 @@ def integrate(registry: Any, base: type, plan_type: type, route_type: type, batc
     return unified, split
 
 
+def integrate_mxfp4(registry: Any, base: type, plan_type: type, route_type: type, batch_type_enum: type,
+                    common_type: type, name: str = "mi355x_mxfp4") -> type:
+    """:func:`integrate` for the backend over an MXFP4 cache: builds it on
+    another contract's classes, registers it under ``name`` and returns it."""
+    backend = type("MI355XMXFP4Backend", (MI355XMXFP4AttentionBackendMixin, base),
+                   {"__module__": __name__, "backend_name": name, "plan_type": plan_type, "route_type": route_type,
+                    "batch_type_enum": batch_type_enum, "common_type": common_type})
+    registry.register(name, backend)
+    return backend
+
+
 __all__ = [
     "MI355XAttentionBackend",
     "MI355XAttentionBackendMixin",
@@ -1475,6 +1486,7 @@ __all__ = [
     "MI355XMXFP4AttentionBackendMixin",
     "MI355XSplitAttentionBackend",
     "integrate",
+    "integrate_mxfp4",
     "make_decode_plan",
     "make_decode_plan_listed",
     "plan_decode_claims",

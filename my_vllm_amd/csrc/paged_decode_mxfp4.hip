@@ -26,7 +26,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))
   __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * kFp4WaveLdsBytes];
   // Tiles done by the wavefronts; one without work reads as far ahead.
   __shared__ int progress[kWaves];
-  const int w = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wave = (int)blockIdx.x * kWaves + w;
   if (kWaves == 12 && (threadIdx.x & 63) == 0) progress[w] = 0x3fffffff;
   if (wave >= p.num_waves) return;
@@ -37,11 +37,9 @@ template <typename T>
 int launch(const Fp4DecodeParams& p, int waves_per_group, hipStream_t s) {
   const uint32_t blocks = (uint32_t)((p.num_waves + waves_per_group - 1) / waves_per_group);
   switch (waves_per_group) {
-    case 1: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 1>), dim3(blocks), dim3(64), 0, s, p); break;
-    case 2: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 2>), dim3(blocks), dim3(128), 0, s, p); break;
     case 4: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 4>), dim3(blocks), dim3(256), 0, s, p); break;
     case 12: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 12>), dim3(blocks), dim3(768), 0, s, p); break;
-    default: return set_error("paged attention mxfp4: waves_per_group must be 1, 2, 4 or 12");
+    default: return set_error("paged attention mxfp4: waves_per_group must be 4 or 12");
   }
   return check_launch("paged_decode_mxfp4");
 }

@@ -1064,12 +1064,13 @@ def paged_decode_mxfp4(
     workspace: torch.Tensor | None,
     softmax_scale: float,
     wave_extra: torch.Tensor,
-    waves_per_group: int = 1,
+    waves_per_group: int = 4,
     *,
     counts: torch.Tensor | None = None,
     validate: bool = True,
 ) -> None:
-    """:func:`paged_decode` over MXFP4 caches, with piece lists (``wave_extra``).
+    """:func:`paged_decode` over MXFP4 caches, with piece lists (``wave_extra``),
+    pieces of any length and 4 or 12 wavefronts to a workgroup.
 
     With ``counts`` (int32 ``[3]`` on the device) it is the fixed-shape launch
     of :func:`paged_decode_graph`: ``counts`` holds this step's ``{num_items,

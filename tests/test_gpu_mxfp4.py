@@ -4,12 +4,13 @@ What the cache holds is compared exactly, bytes and values.  Attention is held
 to the bound that tests/_mxfp4.py derives from the roundings made.
 """
 
-import numpy as np
+import types
+
 import pytest
 import torch
 
-from my_vllm_amd import ops
-from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend
+from my_vllm_amd import _native, attention_backend, ops
+from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend, integrate_mxfp4
 from my_vllm_amd.contract import AttentionRoute, CommonAttentionMetadata
 from my_vllm_amd.custom_op import CustomOpConfig
 from my_vllm_amd.layers import MXFP4KVCacheStore
@@ -222,14 +223,21 @@ def test_decode(gpu, hq, hkv, dtype):
     _check(out, batch, k, v, dtype)
 
 
+@pytest.mark.parametrize("large", [False, True])
 @pytest.mark.parametrize("waves", [8, 24, 64, 512])
-def test_decode_with_long_piece_lists(gpu, monkeypatch, waves):
-    # Many pieces a wavefront, of every length modulo a tile, and pieces of more than 128 pages cut.
+def test_decode_with_long_piece_lists(gpu, monkeypatch, waves, large):
+    # Many pieces a wavefront, of every length modulo a tile, with one longer than a run of 256 pages; both
+    # workgroup sizes.
     set_decode_planning(monkeypatch, waves=waves)
-    ctx = [1, 16, 17, 33, 48, 64, 65, 100, 113, 128, 129, 200, 2500, 5, 31, 47]
+    if large:
+        monkeypatch.setattr(attention_backend, "_MXFP4_LARGE_BYTES", 0)
+    ctx = [1, 16, 17, 33, 48, 64, 65, 100, 113, 128, 129, 200, 8500, 5, 31, 47]
     batch = make_paged_batch(waves, [1] * len(ctx), ctx, 0, 16, 8)
     out, backend, plan, (_, _, k, v) = _forward(batch, gpu, BF16)
     assert plan.metadata.num_decode_waves <= max(waves, 8)
+    assert plan.metadata.decode_waves_per_group == (12 if large else 4)
+    if waves == 8:
+        assert (plan.metadata.decode_items[:, 2] - plan.metadata.decode_items[:, 1]).max() > 512
     _check(out, batch, k, v, BF16)
 
 
@@ -432,3 +440,129 @@ def test_two_backends_on_two_streams(gpu):
     torch.cuda.synchronize()
     assert all(torch.equal(o, outs[0]) for o in outs)
     _check(outs[0], batch, k, v, BF16)
+
+
+def test_caches_beyond_32_bit_offsets(gpu):
+    """K and V of more than 4 GiB each: rows stored, read back and attended to at their far end."""
+    hq, hkv, far = 16, 8, 4 << 30
+    pages = far // (hkv * 1088) + 40
+    ctx, q_lens = [500, 37], [1, 1]
+    batch = make_paged_batch(51, q_lens, ctx, 0, hq, hkv)
+    count = batch.k_cache.shape[0]
+    first = pages - count
+    caches = torch.empty(2, pages, hkv, 1088, dtype=torch.uint8, device=gpu)
+    assert first * hkv * 1088 > far - (1 << 20) and (pages - 1) * hkv * 1088 > far
+    k, v = mxfp4.cache_of(batch.k_cache), mxfp4.cache_of(batch.v_cache)
+    caches[0, first:], caches[1, first:] = k.to(gpu), v.to(gpu)
+    common = _on(batch.common, gpu)
+    tables = torch.where(common.block_tables >= 0, common.block_tables + first, -1)
+    common = type(common)(**{**common.__dict__, "block_tables": tables,
+                             "slot_mapping": common.slot_mapping + first * 16})
+    backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, BF16)
+    out = backend.forward_with_kv_store(batch.q.to(gpu), batch.k_new.to(gpu), batch.v_new.to(gpu), caches[0],
+                                        caches[1], common.slot_mapping, backend.build_plan(common))
+    slots = batch.common.slot_mapping.tolist()
+    mxfp4.store(batch.k_new, k, slots)
+    mxfp4.store(batch.v_new, v, slots)
+    _check(out, batch, k, v, BF16)
+    rows = ops.load_kvcache_mxfp4(caches[0], caches[1], common.slot_mapping)
+    for got, cache in zip(rows, (k, v)):
+        assert torch.equal(got.cpu().double(), mxfp4.values(cache).reshape(-1, hkv, 128)[slots])
+    # A prefill over the same pages.
+    chunk = make_paged_batch(51, [20, 37], ctx, 2, hq, hkv)
+    chunk_common = _on(chunk.common, gpu)
+    chunk_common = type(common)(**{**chunk_common.__dict__, "block_tables": tables})
+    out = backend.forward(chunk.q.to(gpu), None, None, caches[0], caches[1], backend.build_plan(chunk_common))
+    expected, spread, largest = mxfp4.attention(chunk.q, k, v, batch.common.block_tables, [20, 37], ctx)
+    assert_within(out, expected, attention_bound(expected, spread, largest, 500, BF16, BF16))
+
+
+def test_captured_steps_replay_beside_eager_ones(gpu):
+    """A prefill and a decode step captured as they are, replayed between eager steps of the same backend."""
+    hq, hkv = 32, 8
+    pre = make_paged_batch(61, [70, 200], [70 + 64, 200], 2, hq, hkv)
+    dec = make_paged_batch(62, [1] * 5, [300, 17, 90, 1000, 33], 0, hq, hkv)
+    backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, BF16)
+    steps = []
+    for batch in (pre, dec):
+        kd, vd, k, v = cache_pool(batch, gpu)
+        q = batch.q.to(gpu)
+        common = _on(batch.common, gpu)
+        plan = backend.build_plan(common)
+        eager = backend.forward(q, None, None, kd, vd, plan).clone()
+        _check(eager, batch, k, v, BF16)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = backend.forward(q, None, None, kd, vd, plan).clone()
+        steps.append((graph, out, eager, lambda q=q, kd=kd, vd=vd, c=common: backend.forward(
+            q, None, None, kd, vd, backend.build_plan(c))))
+    for _ in range(3):
+        for graph, out, eager, again in steps:
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+            (torch.randn(256, 256, device=gpu) @ torch.randn(256, 256, device=gpu)).sum().item()
+            assert torch.equal(again(), eager)
+
+
+def test_native_and_general_launches_agree(gpu, monkeypatch):
+    """Every operator through the native module and through ctypes: the same bits and the same errors."""
+    real = _native.host_ops()
+    names = [n for n in dir(real) if not n.startswith("_") and callable(getattr(real, n))]
+    batch = make_paged_batch(71, [1] * 3, [40, 300, 700], 0, 16, 8)
+    chunk = make_paged_batch(72, [30, 9], [100, 9], 2, 16, 8)
+    kd, vd, _, _ = cache_pool(batch, gpu)
+    kp, vp, _, _ = cache_pool(chunk, gpu)
+    rows = torch.randn(6, 8, 128, device=gpu).to(BF16)
+    slots = torch.tensor([3, 0, -1, 40, 41, 9], device=gpu)
+
+    def calls():
+        store = torch.zeros(2, 4, 8, 1088, dtype=torch.uint8, device=gpu)
+        ops.store_kvcache_mxfp4(rows, -rows, store[0], store[1], slots)
+        backend = MI355XMXFP4AttentionBackend(16, 8, 128, 16, BF16)
+        decode = backend.forward(batch.q.to(gpu), None, None, kd, vd, backend.build_plan(_on(batch.common, gpu)))
+        backend = MI355XMXFP4AttentionBackend(16, 8, 128, 16, BF16)
+        prefill = backend.forward(chunk.q.to(gpu), None, None, kp, vp, backend.build_plan(_on(chunk.common, gpu)))
+        return [store, decode, prefill, *ops.load_kvcache_mxfp4(store[0], store[1], slots, FP16)]
+
+    def errors():
+        found = []
+        backend = MI355XMXFP4AttentionBackend(16, 8, 128, 16, BF16)
+        plan = backend.build_plan(_on(batch.common, gpu))
+        q = batch.q.to(gpu)
+        odd = torch.empty(3 * 16 * 128 + 1, dtype=BF16, device=gpu)[1:].view(3, 16, 128)
+        for call in (lambda: backend.forward(odd, None, None, kd, vd, plan),
+                     lambda: backend.forward(q, None, None, kd, vd[:-1], plan),
+                     lambda: backend.forward(q.half(), None, None, kd, vd, plan),
+                     lambda: ops.store_kvcache_mxfp4(rows, rows[:, :4], kd, vd, slots),
+                     lambda: ops.load_kvcache_mxfp4(kd, vd.view(torch.int8), slots)):
+            with pytest.raises(Exception) as info:
+                call()
+            found.append((info.type, str(info.value)))
+        return found
+
+    fast, fast_errors = calls(), errors()
+    monkeypatch.setattr(_native, "_host", types.SimpleNamespace(
+        **{n: (real.capture_id if n == "capture_id" else lambda *a: None) for n in names}))
+    for a, b in zip(fast, calls()):
+        assert torch.equal(a, b)
+    assert errors() == fast_errors
+
+
+def test_foreign_contract_family(gpu):
+    from tests import _foreign_contract as foreign
+
+    registered = {}
+    registry = types.SimpleNamespace(register=lambda name, cls: registered.__setitem__(name, cls))
+    made = integrate_mxfp4(registry, foreign.ForeignBackendBase, foreign.ForeignPlan, foreign.ForeignRoute,
+                           foreign.ForeignBatchType, foreign.ForeignCommon)
+    assert registered == {"mi355x_mxfp4": made}
+    batch = make_paged_batch(81, [9, 1], [40, 77], 1, 16, 8)
+    kd, vd, k, v = cache_pool(batch, gpu)
+    common = foreign.ForeignCommon(**_on(batch.common, gpu).__dict__)
+    backend = made(16, 8, 128, 16, BF16)
+    plan = backend.build_plan(common)
+    assert type(plan) is foreign.ForeignPlan and plan.route is foreign.ForeignRoute.MIXED_SPLIT
+    _check(backend.forward(batch.q.to(gpu), None, None, kd, vd, plan), batch, k, v, BF16)

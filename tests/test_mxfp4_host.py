@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from my_vllm_amd import _native, ops
-from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend
+from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend, mxfp4_decode_ranges
 from my_vllm_amd.contract import AttentionRoute
 from my_vllm_amd.custom_op import CustomOpConfig
 from my_vllm_amd.layers import MXFP4KVCacheStore
@@ -131,7 +131,7 @@ def test_abi_takes_no_tokens():
 
 def _abi_decode(**change):
     args = dict(q=16, qts=2048, qhs=128, kc=16, vc=16, pages=4, ps=2176, hs=1088, bt=4, bts=4, sl=4, counts=0, items=32,
-                n=4, waves=4, extra=4, per=1, merges=0, nm=0, slots=0, out=16, ots=2048, ohs=128, ws=256,
+                n=4, waves=4, extra=4, per=4, merges=0, nm=0, slots=0, out=16, ots=2048, ohs=128, ws=256,
                 wsb=1 << 30, hq=16, hkv=2, dim=128, page=16, scale=0.1, dtype=0)
     args.update(change)
     return list(args.values()) + [0]
@@ -152,11 +152,54 @@ def _abi_decode(**change):
     ({"kc": 8}, "16-byte aligned"),
     ({"out": 4}, "8-byte aligned"),
     ({"wsb": 1024}, "workspace too small"),
-    ({"per": 3}, "waves_per_group"),
+    ({"per": 8}, "waves_per_group"),
+    ({"ps": 1 << 33}, "less than 4 GiB apart"),
 ])
 def test_abi_decode_refuses_before_any_launch(change, message):
     with pytest.raises(RuntimeError, match=message):
         _native.call("mva_paged_decode_mxfp4", *_abi_decode(**change))
+
+
+def _abi_prefill(**change):
+    args = dict(q=16, qts=2048, qhs=128, kc=16, vc=16, pages=4, ps=2176, hs=1088, bt=4, bts=4, sl=4, qsl=4, seqs=2,
+                tiles=3, ws=256, wsb=1 << 30, planned=0, out=16, ots=2048, ohs=128, hq=16, hkv=2, dim=128, page=16,
+                scale=0.1, dtype=0)
+    args.update(change)
+    return list(args.values()) + [0]
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"ps": 2184}, "16-byte aligned"),
+    ({"hs": 1090}, "16-byte aligned"),
+    ({"dtype": 2}, "bf16 or fp16"),
+    ({"dim": 64}, "head_dim must be 128"),
+    ({"page": 32}, "page_size must be 16"),
+    ({"hq": 15}, "multiple of num_kv_heads"),
+    ({"hq": 34}, "at most 16 query heads"),
+    ({"pages": 0}, "empty KV cache"),
+    ({"vc": 8}, "16-byte aligned"),
+    ({"out": 4}, "8-byte aligned"),
+    ({"wsb": 1024}, "workspace too small"),
+    ({"ws": 0}, "workspace too small"),
+    ({"ws": 8}, "16-byte aligned"),
+    ({"tiles": -1}, "invalid tile capacity"),
+    ({"seqs": -1}, "invalid sequence count"),
+    ({"hq": 256, "hkv": 128}, "at most 127 KV heads"),
+])
+def test_abi_prefill_refuses_before_any_launch(change, message):
+    with pytest.raises(RuntimeError, match=message):
+        _native.call("mva_paged_prefill_mxfp4", *_abi_prefill(**change))
+
+
+def test_decode_ranges():
+    # Ranges of four pages or more; twelve wavefronts a CU from half a gigabyte on.
+    assert mxfp4_decode_ranges(3, 8) == (1, 4)
+    assert mxfp4_decode_ranges(41, 8) == (10, 4)
+    assert mxfp4_decode_ranges(20000, 8) == (256, 4)
+    assert mxfp4_decode_ranges(40000, 8) == (384, 12)
+    assert mxfp4_decode_ranges(4000, 1) == (1000, 4)
+    assert mxfp4_decode_ranges(4000, 8, override=64) == (8, 4)
+    assert mxfp4_decode_ranges(4000, 300) == (10, 12)  # 2.6 GB
 
 
 class _HostBackend(MI355XMXFP4AttentionBackend):
