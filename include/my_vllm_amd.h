@@ -201,7 +201,8 @@ int mva_paged_decode(const void* q, int64_t q_token_stride, int64_t q_head_strid
  * G = min(num_groups, total pages) near-equal ranges (range g = pages
  * [g*T/G, (g+1)*T/G)); wavefront g*num_kv_heads + h streams KV head h of
  * range g, one piece per sequence the range touches, cut further to at most
- * max_piece_pages (1 .. 128).  wave_extra gets G*num_kv_heads + 1 entries
+ * max_piece_pages (1 .. 128, or INT_MAX for mva_paged_decode_mxfp4: no
+ * further cut).  wave_extra gets G*num_kv_heads + 1 entries
  * (the mva_paged_decode argument).  item_rows must be at least
  * mva_decode_plan_listed_rows(...), an upper bound on the rows written.
  */
@@ -521,11 +522,27 @@ int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stri
                       int head_dim, int dtype, void* stream);
 
 /*
+ * Host planner of mva_paged_decode_mxfp4 besides mva_decode_plan_listed: four
+ * wavefronts share every (sequence, KV head), in an order made for num_cus CUs.
+ * Unless always is nonzero it plans only where that is expected to be faster
+ * than page ranges; otherwise, and for no sequences, the counts are 0.  items holds
+ * num_seqs * num_kv_heads * 4 rows of 8 int32, wave_extra one entry more;
+ * out_counts = {items, wavefronts, 0 partial slots, 0 merges}.
+ */
+int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq, int64_t first_q_row,
+                           int num_kv_heads, int num_cus, int always, int32_t* items, int64_t item_rows,
+                           int32_t* wave_extra, int64_t wave_extra_len, int64_t* out_counts);
+
+/*
  * mva_paged_decode over MXFP4 caches, with piece lists (wave_extra; no
  * claims), pieces of any length and waves_per_group 4 or 12.  Pages must lie
- * less than 4 GiB apart.  With counts ([3] int32 on the device) it is the fixed-shape launch
- * of mva_paged_decode_graph: num_items, num_waves and num_merges are then
- * capacities.  The workspace is mva_paged_decode's.
+ * less than 4 GiB apart.  With counts ([3] int32 on the device) it is the
+ * fixed-shape launch of mva_paged_decode_graph: num_items, num_waves and
+ * num_merges are then capacities.  The workspace is mva_paged_decode's.
+ *
+ * The plan may be mva_decode_plan_shared's, whose pieces have part_base -1:
+ * wavefronts 4 i .. 4 i + 3 hold a quarter each of one segment and join in LDS
+ * (all pieces of a launch, one a wavefront, or none).
  */
 int mva_paged_decode_mxfp4(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                            const void* v_cache, int64_t num_pages, int64_t page_stride_bytes,

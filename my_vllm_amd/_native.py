@@ -161,6 +161,13 @@ _SIGNATURES = {
         ],
     ),
     "mva_decode_plan_listed_rows": (_i64, [_i64, _i64, _i32, _i32, _i32]),
+    "mva_decode_plan_shared": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32,  # block_counts, seqs, first_seq, first_q_row, heads, cus, always
+            _c_void_p, _i64, _c_void_p, _i64, _c_void_p,  # items, item_rows, wave_extra, its length, out_counts
+        ],
+    ),
     "mva_decode_plan_listed": (
         _i32,
         [

@@ -309,6 +309,23 @@ def plan_decode_listed(
     return items[:num_items], wave_extra, waves, slots, merges[:num_merges]
 
 
+def plan_decode_shared(block_counts: np.ndarray | tuple[int, ...], first_seq: int, first_q_row: int,
+                       num_kv_heads: int, num_cus: int, always: bool = False) -> tuple[np.ndarray, np.ndarray]:
+    """(items, wave_extra) of an MXFP4 decode launch in which four wavefronts share
+    each (sequence, KV head) and join in LDS, from the library's native planner
+    ``mva_decode_plan_shared``.  Unless ``always``, the plan is empty where page
+    ranges (:func:`plan_decode_listed`) are expected to be faster."""
+    counts = _plan_counts(block_counts)
+    rows = counts.size * int(num_kv_heads) * ops.MXFP4_SHARE_WAVES
+    items = np.empty((rows, ops.DECODE_ITEM_INTS), np.int32)
+    wave_extra = np.empty(rows + 1, np.int32)
+    out = np.zeros(4, np.int64)
+    _native.call("mva_decode_plan_shared", counts.ctypes.data, counts.size, int(first_seq), int(first_q_row),
+                 int(num_kv_heads), int(num_cus), int(always), items.ctypes.data, rows, wave_extra.ctypes.data, wave_extra.size,
+                 out.ctypes.data)
+    return items[:out[0]], wave_extra[:out[0] + 1]
+
+
 def make_decode_plan_listed(
     block_counts: np.ndarray | tuple[int, ...],
     first_seq: int,
@@ -639,12 +656,21 @@ class MI355XAttentionBackendMixin:
     def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
         """(page ranges, wavefronts per workgroup) of a decode launch with piece lists."""
         if self.decode_waves_override:
-            return self._most_decode_ranges(int(decode_counts.sum()), device)
+            return listed_decode_groups(self.num_kv_heads, device, override=self.decode_waves_override)
         return decode_ranges(int(decode_counts.sum()), len(decode_counts), self.num_kv_heads, device)
 
-    def _most_decode_ranges(self, total_pages: int, device: torch.device) -> tuple[int, int]:
-        """The same for a batch of at most ``total_pages``: what a captured launch is sized for."""
-        return listed_decode_groups(self.num_kv_heads, device, override=self.decode_waves_override)
+    def _plan_decode_lists(self, decode_counts: np.ndarray, first_seq: int, first_q_row: int, device: torch.device):
+        """(items, wave_extra, waves, partial slots, merges, page ranges, wavefronts
+        per workgroup) of a decode launch with piece lists."""
+        groups, waves_per_group = self._decode_ranges(decode_counts, device)
+        return (*plan_decode_listed(decode_counts, first_seq, first_q_row, self.num_kv_heads, groups,
+                                    self._max_piece_pages), groups, waves_per_group)
+
+    def _decode_graph_capacities(self, batch_size: int, total_pages: int, device: torch.device):
+        """(page ranges, wavefronts per workgroup, capacities) of a captured
+        launch for ``batch_size`` sequences of at most ``total_pages`` together."""
+        groups, waves_per_group = listed_decode_groups(self.num_kv_heads, device, override=self.decode_waves_override)
+        return groups, waves_per_group, graph_decode_capacities(batch_size, total_pages, self.num_kv_heads, groups)
 
     # ---- per-step metadata and plan ------------------------------------------
     def build_metadata(self, common) -> MI355XAttentionMetadata:
@@ -743,11 +769,9 @@ class MI355XAttentionBackendMixin:
             if not one_launch:
                 schedule = self._decode_schedule(int(decode_counts.sum()))
                 if schedule == "listed":
-                    groups, waves_per_group = self._decode_ranges(decode_counts, block_tables.device)
-                    items, wave_extra, num_decode_waves, num_part_slots, merges = plan_decode_listed(
-                        decode_counts, common.num_prefill_seqs, common.num_prefill_tokens, self.num_kv_heads, groups,
-                        self._max_piece_pages
-                    )
+                    (items, wave_extra, num_decode_waves, num_part_slots, merges, groups,
+                     waves_per_group) = self._plan_decode_lists(decode_counts, common.num_prefill_seqs,
+                                                                common.num_prefill_tokens, block_tables.device)
                 else:
                     items, num_decode_waves, num_part_slots, merges = plan_decode_claims(
                         decode_counts,
@@ -1099,8 +1123,7 @@ class MI355XAttentionBackendMixin:
         graph_device = torch.device(device)
         if graph_device.type != "cuda":
             raise ValueError("full decode graph state must be on CUDA")
-        groups, waves_per_group = self._most_decode_ranges(page_indices_capacity, graph_device)
-        caps = graph_decode_capacities(batch_size, page_indices_capacity, self.num_kv_heads, groups)
+        groups, waves_per_group, caps = self._decode_graph_capacities(batch_size, page_indices_capacity, graph_device)
         group = self.num_q_heads // self.num_kv_heads
         plan_ints = graph_plan_buffer_ints(caps["item_capacity"], caps["wave_capacity"], caps["merge_capacity"])
         ws_bytes = ops.decode_workspace_bytes(caps["part_slot_capacity"], self.num_kv_heads, group)
@@ -1373,15 +1396,35 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
         return "MIXED batches over an MXFP4 cache run as prefill + decode launches"
 
     def _decode_schedule(self, total_pages: int) -> str:
-        if self.decode_schedule_override not in (None, "listed"):
-            raise ValueError("decode over an MXFP4 cache runs piece lists only")
+        if self.decode_schedule_override not in (None, "listed", "shared"):
+            raise ValueError("decode over an MXFP4 cache runs piece lists or shared segments only")
         return "listed"
 
     def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
         return mxfp4_decode_ranges(int(decode_counts.sum()), self.num_kv_heads, device, self.decode_waves_override)
 
-    def _most_decode_ranges(self, total_pages: int, device: torch.device) -> tuple[int, int]:
-        return mxfp4_decode_ranges(total_pages, self.num_kv_heads, device, self.decode_waves_override)
+    def _plan_decode_lists(self, decode_counts: np.ndarray, first_seq: int, first_q_row: int, device: torch.device):
+        forced = self.decode_schedule_override
+        if forced == "shared" or (forced is None and self.decode_waves_override is None):
+            items, wave_extra = plan_decode_shared(decode_counts, first_seq, first_q_row, self.num_kv_heads,
+                                                   _num_cus(device), forced is not None)
+            if items.shape[0]:
+                no_merges = np.zeros((0, ops.DECODE_ITEM_INTS), np.int32)
+                return items, wave_extra, items.shape[0], 0, no_merges, 0, ops.MXFP4_SHARE_WAVES
+        return super()._plan_decode_lists(decode_counts, first_seq, first_q_row, device)
+
+    def _decode_graph_capacities(self, batch_size: int, total_pages: int, device: torch.device):
+        groups, waves_per_group = mxfp4_decode_ranges(total_pages, self.num_kv_heads, device,
+                                                      self.decode_waves_override)
+        caps = graph_decode_capacities(batch_size, total_pages, self.num_kv_heads, groups)
+        # A step may be a plan of shared segments.  Workgroups of twelve wavefronts
+        # only where one for each CU holds it: a CU takes no second one.
+        shared = batch_size * self.num_kv_heads * ops.MXFP4_SHARE_WAVES
+        if shared > 12 * _num_cus(device):
+            waves_per_group = 4
+        for name in ("item_capacity", "wave_capacity"):
+            caps[name] = max(caps[name], shared)
+        return groups, waves_per_group, caps
 
     def _validate_inputs(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
         if _native.host_ops().forward_inputs_ok_mxfp4(q, k_cache, v_cache, _native.DTYPE_CODES[self.dtype],
@@ -1490,6 +1533,7 @@ __all__ = [
     "make_decode_plan",
     "make_decode_plan_listed",
     "plan_decode_claims",
+    "plan_decode_shared",
     "plan_decode_listed",
     "resident_decode_waves",
 ]

@@ -14,7 +14,9 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <functional>
 #include <limits>
+#include <queue>
 #include <vector>
 
 namespace mva {
@@ -183,6 +185,93 @@ extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_s
   out_counts[1] = waves;
   out_counts[2] = slots;
   out_counts[3] = num_merges;
+  return 0;
+}
+
+// A segment (sequence, KV head) for every four wavefronts, which join in LDS: no
+// partials, no merges.  A wavefront takes a contiguous quarter of the segment's tiles
+// (two pages).
+//
+// Order: workgroups go to CUs in turn, and a CU holds three at a time.  Where all fit at
+// once, the longest num_cus segments come first, shortest of them first, then the
+// next num_cus longest first, and so on: every CU gets a long and a short one.  With
+// more, longest first, as the later ones go where there is room.  Longest first /
+// alternating, call in microseconds: 16 / 8 heads, 64 sequences of 128-2048 23.3 /
+// 20.6; 32 / 8, 64 of 100-6000 54.3 / 46.9, 80 of 1000-4000 52.6 / 50.2; 40 / 8, 200
+// of 128-4096 (1600 segments) 96.2 / 98.3.
+//
+// Unless `always`, only where that is faster than page ranges.  The unit is one tile of
+// each of the four wavefronts.  The longest queue of a CU, the segments handed out
+// longest first to the least loaded, takes M units of about 0.8 us after 5 us; ranges
+// take the mean A of a CU's units and 10 us, of which 4 are the merge kernel.  Measured
+// (call, microseconds, ranges / shared) on both sides of M <= 7 + A:
+//   32 / 8 heads, 8 sequences of 1000         M  8  A  2   12.3 / 10.9
+//   32 / 8, 32 of 1000                        M  8  A  8   16.6 / 12.3
+//   32 / 8, 200 of 100-200                    M  9  A  8   22.4 / 15.5
+//   16 / 8, 64 of 128-2048                    M 18  A 18   27.8 / 20.6
+//   32 / 8, 90 of 4000                        M 94  A 89   90.0 / 83.7
+//   32 / 8, one of 1200                       M 10  A  0    9.6 / 12.2
+//   32 / 8, 8 of 1800                         M 14  A  4   14.6 / 17.0
+//   16 / 4, 37 of 300-3000                    M 23  A  7   19.3 / 23.6
+//   32 / 8, 24 of 6000                        M 47  A 35   41.5 / 45.5
+//   16 / 4, 96 of 8000                        M 125 A 94   91.5 / 93.9
+extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
+                                      int64_t first_q_row, int num_kv_heads, int num_cus, int always, int32_t* items,
+                                      int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
+                                      int64_t* out_counts) {
+  using namespace mva;
+  constexpr int kShare = 4, kTilePages = 2, kPerCu = 3;
+  if (num_seqs < 0 || num_kv_heads <= 0 || num_cus <= 0 || out_counts == nullptr || wave_extra == nullptr ||
+      wave_extra_len < 1)
+    return set_error("decode plan: invalid arguments");
+  for (int i = 0; i < 4; ++i) out_counts[i] = 0;
+  wave_extra[0] = 0;
+  if (num_seqs == 0) return 0;
+  if (block_counts == nullptr || items == nullptr) return set_error("decode plan: invalid arguments");
+  if (!rows_fit_int32(first_seq, first_q_row, num_seqs))
+    return set_error("decode plan: sequence or query row index out of int32 range");
+  if (page_offsets(block_counts, num_seqs).empty()) return -1;
+  if (num_seqs > std::numeric_limits<int32_t>::max() / kShare / num_kv_heads)
+    return set_error("decode plan: more than 2^31-1 pieces");
+  const int64_t segments = num_seqs * num_kv_heads, waves = segments * kShare;
+  std::vector<int32_t> order((size_t)num_seqs);
+  for (int64_t s = 0; s < num_seqs; ++s) order[(size_t)s] = (int32_t)s;
+  std::stable_sort(order.begin(), order.end(),
+                   [&](int32_t a, int32_t b) { return block_counts[a] > block_counts[b]; });
+  if (!always) {
+    auto units = [&](int32_t s) { return (double)((block_counts[s] + kTilePages - 1) / kTilePages) / kShare; };
+    double mean = 0;
+    for (int32_t s : order) mean += units(s) * num_kv_heads / num_cus;
+    const double most = 7 + mean;
+    if (units(order[0]) > most) return 0;
+    std::priority_queue<double, std::vector<double>, std::greater<double>> load;
+    for (int i = 0; i < num_cus; ++i) load.push(0);
+    for (int32_t s : order)
+      for (int h = 0; h < num_kv_heads; ++h) {
+        const double after = load.top() + units(s);
+        if (after > most) return 0;
+        load.pop();
+        load.push(after);
+      }
+  }
+  if (waves > item_rows || wave_extra_len < waves + 1) return set_error("decode plan: item capacity too small");
+  // Place at = segment order[at / heads], head at % heads, sorted by length.
+  auto emit = [&](int64_t row, int64_t at) {
+    const int32_t s = order[(size_t)(at / num_kv_heads)];
+    const int64_t pages = block_counts[s], tiles = (pages + kTilePages - 1) / kTilePages;
+    for (int k = 0; k < kShare; ++k) {
+      const int64_t begin = tiles * k / kShare * kTilePages, end = tiles * (k + 1) / kShare * kTilePages;
+      write_piece(items + (row * kShare + k) * kItemInts, s, first_seq, first_q_row, begin, std::min(end, pages), k,
+                  kShare, -1, (int)(at % num_kv_heads));
+    }
+  };
+  const bool at_once = segments <= (int64_t)kPerCu * num_cus;
+  for (int64_t turn = 0, first = 0; first < segments; ++turn, first += num_cus) {
+    const int64_t end = std::min(segments, first + num_cus);
+    for (int64_t i = first; i < end; ++i) emit(i, at_once && turn % 2 == 0 ? end - 1 - (i - first) : i);
+  }
+  std::fill(wave_extra, wave_extra + waves + 1, (int32_t)waves);
+  out_counts[0] = out_counts[1] = waves;
   return 0;
 }
 

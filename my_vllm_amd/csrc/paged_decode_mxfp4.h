@@ -44,6 +44,13 @@ constexpr int kFp4TileVScales = kFp4TileKScales + kFp4TileTokens * kFp4RowScales
 constexpr int kFp4TileBytes = kFp4TileVScales + kFp4TileTokens * kFp4RowScales;  // 4352
 constexpr int kFp4TileBufs = 3;
 constexpr int kFp4WaveLdsBytes = kFp4TileBufs * kFp4TileBytes;  // 13056: twelve wavefronts in 160 KB
+// Wavefronts that share a segment, and where each leaves its m and l of 16 heads,
+// after its 16 rows of o.
+constexpr int kFp4ShareWaves = 4;
+constexpr int kFp4ShareMax = 16 * kHeadDim * 4;
+constexpr int kFp4ShareSum = kFp4ShareMax + 64;
+static_assert(kFp4ShareSum + 64 <= kFp4WaveLdsBytes, "a share fits its wavefront's LDS");
+typedef __attribute__((address_space(3))) float lds_f32;
 constexpr int kFp4TileLoads = 2 * kFp4TilePages + 1;
 // Pages whose ids a wavefront holds at a time, four table words a lane.
 constexpr int kFp4RunPages = 256;
@@ -100,8 +107,13 @@ __device__ inline float groups_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// One wavefront of a decode launch over piece lists (see decode_wave); `lds` is
-// its kFp4WaveLdsBytes of LDS.
+// One wavefront, number `slot` of its workgroup, of a decode launch over piece
+// lists (see decode_wave); `group_lds` is kFp4WaveLdsBytes for each wavefront of the workgroup.
+//
+// Wavefronts 4 i .. 4 i + 3 of a launch may instead share a segment (sequence, KV
+// head): each has one piece, a quarter of its pages and part_base -1, and the four
+// join in LDS, without partials in memory and the merge kernel after it.  Either all
+// pieces of a launch are shared or none.
 //
 // A piece goes in runs of up to 256 pages.  A run loads its queries and page table
 // words, copies its first three tiles, and then computes tile after tile, copying
@@ -112,12 +124,12 @@ __device__ inline float groups_sum(float v) {
 // code and 1-2 us slower on small batches, level on large ones).
 //
 // `progress` (LDS, one int per wavefront of the workgroup, or nullptr): the
-// wavefronts `slot` % 4 share a SIMD, whose issue favours the oldest.  Each
+// wavefronts of one `slot` % 4 share a SIMD, whose issue favours the oldest.  Each
 // publishes the tiles it has done and runs at the higher priority the fewer of
 // its two partners are behind it, so the three stay level.
 template <typename T>
-__device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* lds, int* progress = nullptr,
-                                  int slot = 0) {
+__device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* group_lds, int* progress, int slot) {
+  lds_u8* const lds = group_lds + slot * kFp4WaveLdsBytes;
   typedef typename Elem<T>::v8 V8;
   typedef typename Elem<T>::v4 V4;
   const int lane = threadIdx.x & 63;
@@ -286,10 +298,55 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* ld
           __builtin_bit_cast(V8, __builtin_shufflevector(v0[mt], v1[mt], 0, 1, 2, 3, 4, 5, 6, 7)), pf, o[mt]);
   };
 
-  // End of piece X: the final output, or its split-K partial (normalised o and
-  // log2-sum-exp) for the merge kernel.
+  // A piece of a shared segment (part_base -1): the four wavefronts of its share
+  // group leave their o, m and l in LDS, over their tiles, and join them together.
+  auto join_share = [&](float l_tot) __attribute__((always_inline)) {
+    // Row c of this wavefront, 16-byte chunk ch at slot ch ^ c: 16 lanes of a
+    // write take 16 slots.
+    if (q_lane) {
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) lds_st16(lds + c * 4 * kHeadDim + (((4 * mt + q4) ^ c) << 4), o[mt]);
+      if (q4 == 0) {
+        *(lds_f32*)(lds + kFp4ShareMax + 4 * c) = m;
+        *(lds_f32*)(lds + kFp4ShareSum + 4 * c) = l_tot;
+      }
+    }
+    __syncthreads();
+    lds_u8* const first = group_lds + (slot & ~(kFp4ShareWaves - 1)) * kFp4WaveLdsBytes;
+    for (int i = (slot & (kFp4ShareWaves - 1)) * 64 + lane; i < G * (kHeadDim / 4); i += 64 * kFp4ShareWaves) {
+      const int g = i >> 5, ch = i & 31;
+      float mw[kFp4ShareWaves], top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kFp4ShareWaves; ++w) {
+        mw[w] = *(lds_f32*)(first + w * kFp4WaveLdsBytes + kFp4ShareMax + 4 * g);
+        top = fmaxf(top, mw[w]);
+      }
+      const float m_use = top == -INFINITY ? 0.f : top;
+      f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFp4ShareWaves; ++w) {
+        const float a = fast_exp2(mw[w] - m_use);  // a wavefront without pages: m = -inf -> 0
+        den += a * *(lds_f32*)(first + w * kFp4WaveLdsBytes + kFp4ShareSum + 4 * g);
+        sum += a * lds_ld16<f32x4>(first + w * kFp4WaveLdsBytes + g * 4 * kHeadDim + ((ch ^ g) << 4));
+      }
+      const float inv = den > 0.f ? 1.0f / den : 0.f;
+      V4 y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = (T)(sum[r] * inv);
+      store8_untracked((T*)p.out + (int64_t)X[6] * p.out_tok_stride + (int64_t)(X[7] * G + g) * p.out_head_stride +
+                           4 * ch,
+                       __builtin_bit_cast(u32x2, y));
+    }
+  };
+  // End of piece X: the final output, its share of one, or its split-K partial
+  // (normalised o and log2-sum-exp) for the merge kernel.
   auto finish_piece = [&]() __attribute__((always_inline)) {
     const float l_tot = groups_sum(l);
+    if (X[5] < 0) {
+      join_share(l_tot);
+      return;
+    }
     const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
     const int h = X[7];
     if (!q_lane) return;

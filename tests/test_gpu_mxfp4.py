@@ -566,3 +566,71 @@ def test_foreign_contract_family(gpu):
     plan = backend.build_plan(common)
     assert type(plan) is foreign.ForeignPlan and plan.route is foreign.ForeignRoute.MIXED_SPLIT
     _check(backend.forward(batch.q.to(gpu), None, None, kd, vd, plan), batch, k, v, BF16)
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("hq,hkv,dtype", [(8, 8, BF16), (16, 8, FP16), (32, 2, BF16), (24, 8, FP16), (5, 1, BF16)])
+def test_shared_segments_of_every_length(gpu, monkeypatch, hq, hkv, dtype, large):
+    """Four wavefronts a segment: lengths that leave some of them without pages, and long ones."""
+    monkeypatch.setattr(MI355XMXFP4AttentionBackend, "decode_schedule_override", "shared")
+    ctx = [1, 15, 16, 17, 32, 33, 64, 65, 95, 96, 97, 128, 129, 300, 2047, 4500]
+    batch = make_paged_batch(hq, [1] * len(ctx), ctx, 0, hq, hkv, dtype=dtype)
+    k, v = mxfp4.cache_of(batch.k_cache), mxfp4.cache_of(batch.v_cache)
+    for cache, seed in ((k, 1), (v, 2)):
+        poison_stale(cache, batch.common.block_tables, ctx, seed)
+    backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, dtype)
+    plan = backend.build_plan(_on(batch.common, gpu))
+    metadata = plan.metadata
+    assert metadata.num_decode_waves == len(ctx) * hkv * 4 and metadata.num_decode_merges == 0
+    q, kd, vd = batch.q.to(gpu), k.to(gpu), v.to(gpu)
+    if not large:
+        _check(backend.forward(q, None, None, kd, vd, plan), batch, k, v, dtype)
+        return
+    # The same plan in workgroups of twelve.
+    out = torch.full_like(q, float("nan"))
+    ops.paged_decode_mxfp4(q, kd, vd, metadata.block_tables, metadata.seq_lens, metadata.decode_items,
+                           metadata.num_decode_items, metadata.num_decode_waves, None, 0, 0, out,
+                           torch.empty(ops.decode_workspace_bytes(0, hkv, hq // hkv), dtype=torch.uint8, device=gpu),
+                           backend.softmax_scale, metadata.decode_wave_extra, 12)
+    _check(out, batch, k, v, dtype)
+    assert torch.equal(out, backend.forward(q, None, None, kd, vd, plan))
+
+
+@pytest.mark.parametrize("large", [False, True])
+def test_one_graph_replays_shared_and_listed_steps(gpu, monkeypatch, large):
+    """Steps of one captured launch whose plans are of either kind, in workgroups of 4 and of 12."""
+    if large:
+        monkeypatch.setattr(attention_backend, "_MXFP4_LARGE_BYTES", 0)
+    hq, hkv, n, width = 16, 8, 6, 260
+    backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, BF16)
+    state = backend.create_full_decode_graph_state(n, n * width, gpu)
+    assert state.waves_per_group == (12 if large else 4)
+    caches = torch.zeros(2, *ops.mxfp4_cache_shape(n * width, hkv), dtype=torch.uint8, device=gpu)
+    q = torch.zeros(n, hq, 128, dtype=BF16, device=gpu)
+    graph, kinds = None, []
+    for seed, ctx in enumerate(([100, 7, 64, 300, 16, 1], [4100, 30, 17, 1000, 1, 900], [500] * 6, [4160] * 6)):
+        batch = make_paged_batch(seed, [1] * n, ctx, 0, hq, hkv)
+        k, v = mxfp4.cache_of(batch.k_cache), mxfp4.cache_of(batch.v_cache)
+        caches[0, :len(k)], caches[1, :len(v)] = k.to(gpu), v.to(gpu)
+        q.copy_(batch.q)
+        plan = backend.build_plan(_on(batch.common, gpu))
+        kinds.append(plan.metadata.num_decode_merges == 0)
+        eager = backend.forward(q, None, None, caches[0], caches[1], plan).clone()
+        _check(eager, batch, k, v, BF16)
+        assert backend.full_decode_graph_metadata_fits(state, plan)
+        backend.plan_full_decode_graph(state, plan)
+        backend.activate_full_decode_graph(state)
+        try:
+            if graph is None:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    backend.forward(q, None, None, caches[0], caches[1], plan)
+        finally:
+            backend.deactivate_full_decode_graph()
+        for _ in range(2):
+            state.output.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(state.output, eager)
+    assert kinds == [True, False, True, False]

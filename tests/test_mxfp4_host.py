@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from my_vllm_amd import _native, ops
-from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend, mxfp4_decode_ranges
+from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend, mxfp4_decode_ranges, plan_decode_shared
 from my_vllm_amd.contract import AttentionRoute
 from my_vllm_amd.custom_op import CustomOpConfig
 from my_vllm_amd.layers import MXFP4KVCacheStore
@@ -200,6 +200,71 @@ def test_decode_ranges():
     assert mxfp4_decode_ranges(4000, 1) == (1000, 4)
     assert mxfp4_decode_ranges(4000, 8, override=64) == (8, 4)
     assert mxfp4_decode_ranges(4000, 300) == (10, 12)  # 2.6 GB
+
+
+def test_shared_plan_covers_every_segment():
+    counts = np.array([5, 1, 40, 8, 1, 129], np.int64)
+    items, wave_extra = plan_decode_shared(counts, 3, 7, 5, 256, always=True)
+    assert items.shape == (6 * 5 * 4, 8) and (wave_extra == len(items)).all() and wave_extra.size == len(items) + 1
+    groups = items.reshape(-1, 4, 8)
+    assert (groups[:, :, [0, 6, 7]] == groups[:, :1, [0, 6, 7]]).all()  # four of one segment
+    assert (groups[:, :, 3] == np.arange(4)).all() and (items[:, 4] == 4).all() and (items[:, 5] == -1).all()
+    assert (items[:, 6] - items[:, 0] == 4).all()
+    assert len({(s, h) for s, h in groups[:, 0, [0, 7]].tolist()}) == 30
+    for group in groups:
+        pages = counts[group[0, 0] - 3]
+        assert group[0, 1] == 0 and group[3, 2] == pages
+        assert (group[1:, 1] == group[:-1, 2]).all() and (group[:, 2] >= group[:, 1]).all()
+        assert (group[:, 1] % 2 == 0).all() or pages < 8  # whole tiles
+        assert (group[:, 2] - group[:, 1]).max() <= 2 * -(-pages // 8)
+
+
+def test_shared_plan_order():
+    # All at once: every CU's workgroups (4 CUs, places i, i + 4, i + 8) sum to about the same.
+    counts = np.array([10, 3, 7, 1, 12, 5, 9, 2, 8, 4], np.int64)
+    pages = counts[plan_decode_shared(counts, 0, 0, 1, 4, always=True)[0][::4, 0]]
+    assert pages.tolist() == [8, 9, 10, 12, 7, 5, 4, 3, 1, 2]
+    # More than a CU holds: longest first.
+    pages = counts[plan_decode_shared(counts, 0, 0, 1, 3, always=True)[0][::4, 0]]
+    assert pages.tolist() == sorted(counts.tolist(), reverse=True)
+
+
+@pytest.mark.parametrize("counts,hkv,shared", [
+    ([1], 8, True),
+    ([33] * 8, 8, True),
+    ([63] * 32, 8, True),
+    ([13] * 200, 8, True),
+    ([2000], 8, False),
+    ([75], 8, False),
+    ([500] + [10] * 40, 8, False),
+    ([150] * 37, 4, False),
+    ([500] * 96, 4, False),  # 384 segments on 256 CUs: two on half of them
+])
+def test_shared_plans_where_they_are_expected_to_be_faster(counts, hkv, shared):
+    items, wave_extra = plan_decode_shared(counts, 0, 0, hkv, 256)
+    assert len(items) == (len(counts) * hkv * 4 if shared else 0) and wave_extra.size == len(items) + 1
+
+
+def test_shared_plan_refusals():
+    with pytest.raises(ValueError):
+        plan_decode_shared([3, 0], 0, 0, 8, 256)
+    with pytest.raises(RuntimeError, match="int32 range"):
+        plan_decode_shared([3, 3], 2 ** 31 - 1, 0, 8, 256)
+    counts, items = np.array([4], np.int64), np.zeros((8, 8), np.int32)
+    extra, out = np.zeros(9, np.int32), np.zeros(4, np.int64)
+
+    def call(hkv=1, cus=256, rows=8, words=9):
+        _native.call("mva_decode_plan_shared", counts.ctypes.data, 1, 0, 0, hkv, cus, 1, items.ctypes.data, rows,
+                     extra.ctypes.data, words, out.ctypes.data)
+
+    for change in ({"hkv": 0}, {"cus": 0}, {"words": 0}):
+        with pytest.raises(RuntimeError, match="invalid arguments"):
+            call(**change)
+    for change in ({"rows": 3}, {"words": 4}, {"hkv": 3}):
+        with pytest.raises(RuntimeError, match="capacity too small"):
+            call(**change)
+    call(hkv=2)
+    assert out.tolist() == [8, 8, 0, 0]
 
 
 class _HostBackend(MI355XMXFP4AttentionBackend):
