@@ -522,16 +522,19 @@ int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stri
                       int head_dim, int dtype, void* stream);
 
 /*
- * Host planner of mva_paged_decode_mxfp4 besides mva_decode_plan_listed: four
- * wavefronts share every (sequence, KV head), in an order made for num_cus CUs.
- * Unless always is nonzero it plans only where that is expected to be faster
- * than page ranges; otherwise, and for no sequences, the counts are 0.  items holds
- * num_seqs * num_kv_heads * 4 rows of 8 int32, wave_extra one entry more;
- * out_counts = {items, wavefronts, 0 partial slots, 0 merges}.
+ * Host planner of mva_paged_decode_mxfp4 besides mva_decode_plan_listed: pieces
+ * that four wavefronts share, whole segments (sequence, KV head) or cuts of
+ * them, in an order made for num_cus CUs.  Unless always is nonzero it plans
+ * only where that is expected to be faster than page ranges; otherwise, and for no
+ * sequences, the counts are 0.  With S = max(num_seqs * num_kv_heads, 3 * num_cus),
+ * items holds 4 * S rows of 8 int32, wave_extra 4 * S + 1 entries and merges
+ * num_seqs * num_kv_heads rows; out_counts = {items, wavefronts, partial
+ * slots, merges}.
  */
 int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq, int64_t first_q_row,
                            int num_kv_heads, int num_cus, int always, int32_t* items, int64_t item_rows,
-                           int32_t* wave_extra, int64_t wave_extra_len, int64_t* out_counts);
+                           int32_t* wave_extra, int64_t wave_extra_len, int32_t* merges, int64_t merge_rows,
+                           int64_t* out_counts);
 
 /*
  * mva_paged_decode over MXFP4 caches, with piece lists (wave_extra; no
@@ -540,9 +543,9 @@ int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_
  * fixed-shape launch of mva_paged_decode_graph: num_items, num_waves and
  * num_merges are then capacities.  The workspace is mva_paged_decode's.
  *
- * The plan may be mva_decode_plan_shared's, whose pieces have part_base -1:
- * wavefronts 4 i .. 4 i + 3 hold a quarter each of one segment and join in LDS
- * (all pieces of a launch, one a wavefront, or none).
+ * The plan may be mva_decode_plan_shared's, whose pieces have the complement
+ * of part_base: wavefronts 4 i .. 4 i + 3 hold a quarter each of one piece and join
+ * in LDS (all pieces of a launch, one a wavefront, or none).
  */
 int mva_paged_decode_mxfp4(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                            const void* v_cache, int64_t num_pages, int64_t page_stride_bytes,

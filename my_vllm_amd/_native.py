@@ -165,7 +165,7 @@ _SIGNATURES = {
         _i32,
         [
             _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32,  # block_counts, seqs, first_seq, first_q_row, heads, cus, always
-            _c_void_p, _i64, _c_void_p, _i64, _c_void_p,  # items, item_rows, wave_extra, its length, out_counts
+            _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,  # items, wave_extra, merges, lengths, counts
         ],
     ),
     "mva_decode_plan_listed": (

@@ -309,21 +309,30 @@ def plan_decode_listed(
     return items[:num_items], wave_extra, waves, slots, merges[:num_merges]
 
 
+def shared_decode_capacity(num_seqs: int, num_kv_heads: int, num_cus: int) -> int:
+    """Most wavefronts of a :func:`plan_decode_shared` plan."""
+    return ops.MXFP4_SHARE_WAVES * max(num_seqs * num_kv_heads, 3 * num_cus)
+
+
 def plan_decode_shared(block_counts: np.ndarray | tuple[int, ...], first_seq: int, first_q_row: int,
-                       num_kv_heads: int, num_cus: int, always: bool = False) -> tuple[np.ndarray, np.ndarray]:
-    """(items, wave_extra) of an MXFP4 decode launch in which four wavefronts share
-    each (sequence, KV head) and join in LDS, from the library's native planner
-    ``mva_decode_plan_shared``.  Unless ``always``, the plan is empty where page
-    ranges (:func:`plan_decode_listed`) are expected to be faster."""
+                       num_kv_heads: int, num_cus: int,
+                       always: bool = False) -> tuple[np.ndarray, np.ndarray, int, int, np.ndarray]:
+    """(items, wave_extra, waves, partial slots, merges) of an MXFP4 decode launch in
+    which four wavefronts share each piece and join in LDS, from the library's native
+    planner ``mva_decode_plan_shared``.  Unless ``always``, the plan is empty where
+    page ranges (:func:`plan_decode_listed`) are expected to be faster."""
     counts = _plan_counts(block_counts)
-    rows = counts.size * int(num_kv_heads) * ops.MXFP4_SHARE_WAVES
+    hkv, num_cus = int(num_kv_heads), int(num_cus)
+    rows = shared_decode_capacity(counts.size, hkv, num_cus)
     items = np.empty((rows, ops.DECODE_ITEM_INTS), np.int32)
+    merges = np.empty((counts.size * hkv, ops.DECODE_ITEM_INTS), np.int32)
     wave_extra = np.empty(rows + 1, np.int32)
     out = np.zeros(4, np.int64)
-    _native.call("mva_decode_plan_shared", counts.ctypes.data, counts.size, int(first_seq), int(first_q_row),
-                 int(num_kv_heads), int(num_cus), int(always), items.ctypes.data, rows, wave_extra.ctypes.data, wave_extra.size,
-                 out.ctypes.data)
-    return items[:out[0]], wave_extra[:out[0] + 1]
+    _native.call("mva_decode_plan_shared", counts.ctypes.data, counts.size, int(first_seq), int(first_q_row), hkv,
+                 num_cus, int(always), items.ctypes.data, rows, wave_extra.ctypes.data, wave_extra.size,
+                 merges.ctypes.data, merges.shape[0], out.ctypes.data)
+    num_items, waves, slots, num_merges = (int(x) for x in out)
+    return items[:num_items], wave_extra[:waves + 1], waves, slots, merges[:num_merges]
 
 
 def make_decode_plan_listed(
@@ -1348,18 +1357,16 @@ class MI355XSplitAttentionBackend(MI355XAttentionBackend):
     default_attention_mode = "split"
 
 
-# A decode launch over an MXFP4 cache: (wavefronts per CU, wavefronts per
-# workgroup) of batches below and from _MXFP4_LARGE_BYTES of K and V.  Twelve
-# wavefronts, whose priorities keep the three of a SIMD level, fill a CU's LDS;
-# eight leave fewer split-K chunks and start sooner.  Call, microseconds, 12 / 8:
-# 56 sequences of 8192-32768 tokens at 64 / 8 heads (1.4 GB) 251 / 264, 28
-# (0.7 GB) 117 / 122, 14 (0.4 GB) 70.0 / 65.6; 64 of 128-2048 at 16 / 8 26.4 /
-# 23.6; one of 30001 at 32 / 8 20.0 / 17.1.
-_MXFP4_LARGE_BYTES = 512 << 20
+# Page ranges of a decode launch over an MXFP4 cache: (wavefronts per CU, wavefronts
+# per workgroup) below and from _MXFP4_LARGE_BYTES of K and V.  Twelve wavefronts in one
+# workgroup, whose priorities keep the three of a SIMD level, fill a CU's LDS; eight
+# start sooner.  Call, microseconds, 8 / 12: 56 sequences of 8192-32768 tokens at 64 / 8
+# heads (1.4 GB) 256 / 245, 48 of 10000 at 32 / 8 (0.52 GB) 109 / 102, 96 of 8000 at 16 / 4
+# (0.42 GB) 91.5 / 86.0, 32 of 10000 at 32 / 8 (0.35 GB) 74.5 / 72.6, 14 of 8192-32768 at
+# 64 / 8 (0.32 GB) 71.0 / 75.2, 32 of 100-6000 at 32 / 8 (0.11 GB) 33.7 / 36.0.
+_MXFP4_LARGE_BYTES = 384 << 20
 _MXFP4_WAVES = ((8, 4), (12, 12))
-# Pages a range has at least, two tiles.  Ranges of one / four / sixteen pages:
-# one sequence of 30000 tokens at 8 / 1 heads 24.6 / 13.6 / 15.5, eight of
-# 256-1024 at 16 / 8 12.9 / 12.6 / 16.3.
+# Pages a range has at least, two tiles.
 _MXFP4_RANGE_PAGES = 4
 
 
@@ -1400,31 +1407,29 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
             raise ValueError("decode over an MXFP4 cache runs piece lists or shared segments only")
         return "listed"
 
-    def _decode_ranges(self, decode_counts: np.ndarray, device: torch.device) -> tuple[int, int]:
-        return mxfp4_decode_ranges(int(decode_counts.sum()), self.num_kv_heads, device, self.decode_waves_override)
-
     def _plan_decode_lists(self, decode_counts: np.ndarray, first_seq: int, first_q_row: int, device: torch.device):
         forced = self.decode_schedule_override
         if forced == "shared" or (forced is None and self.decode_waves_override is None):
-            items, wave_extra = plan_decode_shared(decode_counts, first_seq, first_q_row, self.num_kv_heads,
-                                                   _num_cus(device), forced is not None)
-            if items.shape[0]:
-                no_merges = np.zeros((0, ops.DECODE_ITEM_INTS), np.int32)
-                return items, wave_extra, items.shape[0], 0, no_merges, 0, ops.MXFP4_SHARE_WAVES
-        return super()._plan_decode_lists(decode_counts, first_seq, first_q_row, device)
+            plan = plan_decode_shared(decode_counts, first_seq, first_q_row, self.num_kv_heads, _num_cus(device),
+                                      forced is not None)
+            if plan[2]:
+                return (*plan, 0, ops.MXFP4_SHARE_WAVES)
+        groups, per_group = mxfp4_decode_ranges(int(decode_counts.sum()), self.num_kv_heads, device,
+                                                self.decode_waves_override)
+        return (*plan_decode_listed(decode_counts, first_seq, first_q_row, self.num_kv_heads, groups,
+                                    self._max_piece_pages), groups, per_group)
 
     def _decode_graph_capacities(self, batch_size: int, total_pages: int, device: torch.device):
-        groups, waves_per_group = mxfp4_decode_ranges(total_pages, self.num_kv_heads, device,
-                                                      self.decode_waves_override)
+        groups, _ = mxfp4_decode_ranges(total_pages, self.num_kv_heads, device, self.decode_waves_override)
         caps = graph_decode_capacities(batch_size, total_pages, self.num_kv_heads, groups)
-        # A step may be a plan of shared segments.  Workgroups of twelve wavefronts
-        # only where one for each CU holds it: a CU takes no second one.
-        shared = batch_size * self.num_kv_heads * ops.MXFP4_SHARE_WAVES
-        if shared > 12 * _num_cus(device):
-            waves_per_group = 4
-        for name in ("item_capacity", "wave_capacity"):
-            caps[name] = max(caps[name], shared)
-        return groups, waves_per_group, caps
+        # Workgroups of four, whichever plan a step has: of twelve, an empty or short
+        # one holds a CU's LDS.  Replays, microseconds, of four / twelve: 64 sequences
+        # of 128-2048 at 16 / 8 heads 23.4 / 33.2, 56 of 8192-32768 at 64 / 8 265 / 245.
+        shared = shared_decode_capacity(batch_size, self.num_kv_heads, _num_cus(device))
+        for name, most in (("item_capacity", shared), ("wave_capacity", shared),
+                           ("part_slot_capacity", shared // ops.MXFP4_SHARE_WAVES // self.num_kv_heads)):
+            caps[name] = max(caps[name], most)
+        return groups, ops.MXFP4_SHARE_WAVES, caps
 
     def _validate_inputs(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
         if _native.host_ops().forward_inputs_ok_mxfp4(q, k_cache, v_cache, _native.DTYPE_CODES[self.dtype],

@@ -188,90 +188,166 @@ extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_s
   return 0;
 }
 
-// A segment (sequence, KV head) for every four wavefronts, which join in LDS: no
-// partials, no merges.  A wavefront takes a contiguous quarter of the segment's tiles
-// (two pages).
+namespace mva {
+namespace {
+
+// ---- pieces shared by four wavefronts (MXFP4 caches) ----
 //
-// Order: workgroups go to CUs in turn, and a CU holds three at a time.  Where all fit at
-// once, the longest num_cus segments come first, shortest of them first, then the
-// next num_cus longest first, and so on: every CU gets a long and a short one.  With
-// more, longest first, as the later ones go where there is room.  Longest first /
-// alternating, call in microseconds: 16 / 8 heads, 64 sequences of 128-2048 23.3 /
-// 20.6; 32 / 8, 64 of 100-6000 54.3 / 46.9, 80 of 1000-4000 52.6 / 50.2; 40 / 8, 200
-// of 128-4096 (1600 segments) 96.2 / 98.3.
-//
-// Unless `always`, only where that is faster than page ranges.  The unit is one tile of
-// each of the four wavefronts.  The longest queue of a CU, the segments handed out
-// longest first to the least loaded, takes M units of about 0.8 us after 5 us; ranges
-// take the mean A of a CU's units and 10 us, of which 4 are the merge kernel.  Measured
-// (call, microseconds, ranges / shared) on both sides of M <= 7 + A:
-//   32 / 8 heads, 8 sequences of 1000         M  8  A  2   12.3 / 10.9
-//   32 / 8, 32 of 1000                        M  8  A  8   16.6 / 12.3
-//   32 / 8, 200 of 100-200                    M  9  A  8   22.4 / 15.5
-//   16 / 8, 64 of 128-2048                    M 18  A 18   27.8 / 20.6
-//   32 / 8, 90 of 4000                        M 94  A 89   90.0 / 83.7
-//   32 / 8, one of 1200                       M 10  A  0    9.6 / 12.2
-//   32 / 8, 8 of 1800                         M 14  A  4   14.6 / 17.0
-//   16 / 4, 37 of 300-3000                    M 23  A  7   19.3 / 23.6
-//   32 / 8, 24 of 6000                        M 47  A 35   41.5 / 45.5
-//   16 / 4, 96 of 8000                        M 125 A 94   91.5 / 93.9
+// Each workgroup's four wavefronts take a quarter of one piece and join in LDS:
+// a quarter of the partials, and no wavefront goes from one piece to another, which
+// leaves it idle for a memory round trip or three.
+
+constexpr int kShareWaves = 4;
+constexpr int kTilePages = 2;   // pages a wavefront takes at a time
+constexpr int kSharesPerCu = 3;  // workgroups a CU holds at once
+
+struct Share {
+  int64_t begin, end;  // tiles of the sequence
+  int32_t seq, chunk, of;
+  int64_t tiles() const { return end - begin; }
+};
+
+// Every sequence cut into pieces of about `target` tiles, longest pieces first.
+std::vector<Share> cut_shares(const int64_t* counts, int64_t n, double target) {
+  std::vector<Share> shares;
+  shares.reserve((size_t)n);
+  for (int64_t s = 0; s < n; ++s) {
+    const int64_t tiles = (counts[s] + kTilePages - 1) / kTilePages;
+    const int64_t of = std::max<int64_t>(1, (int64_t)((double)tiles / target + 0.5));
+    for (int64_t k = 0; k < of; ++k) {
+      const int64_t q = tiles / of, r = tiles % of;  // k * tiles / of without overflow
+      shares.push_back({k * q + k * r / of, (k + 1) * q + (k + 1) * r / of, (int32_t)s, (int32_t)k, (int32_t)of});
+    }
+  }
+  std::stable_sort(shares.begin(), shares.end(), [](const Share& x, const Share& y) { return x.tiles() > y.tiles(); });
+  return shares;
+}
+
+// Which of the sorted (piece, KV head) pairs workgroup i takes.  Workgroups go to the
+// CUs in turn.  Where all fit at once, the longest num_cus pairs come first, the shortest
+// of them first, then the next num_cus longest first, and so on: every CU gets long and
+// short ones.  With more, longest first, as the later ones go where there is room.
+// Longest first / alternating, call in microseconds: 16 / 8 heads, 64 sequences of
+// 128-2048 23.3 / 20.6; 32 / 8, 64 of 100-6000 54.3 / 46.9; 40 / 8, 200 of 128-4096
+// (1600 pairs) 96.2 / 98.3.
+int64_t share_of_workgroup(int64_t i, int64_t pairs, int64_t num_cus) {
+  const int64_t turn = i / num_cus;
+  if (pairs > kSharesPerCu * num_cus || turn % 2) return i;
+  return std::min(pairs, (turn + 1) * num_cus) - 1 - i % num_cus;
+}
+
+// The most tiles that a CU's workgroups have together, a wavefront's quarter of each.
+double longest_queue(const std::vector<Share>& shares, int64_t hkv, int64_t num_cus) {
+  const int64_t pairs = (int64_t)shares.size() * hkv;
+  auto quarter = [&](int64_t at) { return (double)shares[(size_t)(at / hkv)].tiles() / kShareWaves; };
+  if (pairs <= kSharesPerCu * num_cus) {
+    double most = 0;
+    for (int64_t cu = 0; cu < std::min(num_cus, pairs); ++cu) {
+      double sum = 0;
+      for (int64_t i = cu; i < pairs; i += num_cus) sum += quarter(share_of_workgroup(i, pairs, num_cus));
+      most = std::max(most, sum);
+    }
+    return most;
+  }
+  std::priority_queue<double, std::vector<double>, std::greater<double>> load;
+  for (int64_t i = 0; i < num_cus; ++i) load.push(0);
+  double most = 0;
+  for (int64_t at = 0; at < pairs; ++at) {
+    const double sum = load.top() + quarter(at);
+    load.pop();
+    load.push(sum);
+    most = std::max(most, sum);
+  }
+  return most;
+}
+
+}  // namespace
+}  // namespace mva
+
+// Of the whole segments and of pieces for about one, two and three workgroups a CU (four
+// tiles or more each, one a wavefront), the cut with the least estimated time, or no
+// plan where page ranges come out below all of them.  The estimates, microseconds, with M
+// the longest queue of a CU and A the mean, in tiles a wavefront, fitted to graphs of calls:
+//   whole  4.2 + 0.87 M    32 / 8 heads, 8 sequences of 1000 10.9, 16 of 2400 21.2; 8 / 1, 250 of 2000-4000 31.8
+//   cut    8.2 + 0.87 M, 1 more above 32 pieces   32 / 8, one of 1000 7.9, 24 of 6000 39.3; 16 / 4, 96 of 8000 89.0
+//   ranges 10 + 0.85 A     64 / 8, 56 of 8192-32768 245, 28 137; 32 / 8, 40 of 12000 107
+// and 1.3 on the last two for the host's second launch (8 of 256-1024 at 16 / 8, whole / cut: 10.5 / 9.3 in a
+// graph, 9.3 / 11.1 call by call).  Ranges of eight wavefronts a CU against the plan taken: one of 30001 at 32 / 8
+// 17.7 / 16.3, 37 of 300-6000 at 16 / 4 24.2 / 22.4, 64 of 128-2048 at 16 / 8 28.1 / 22.0, 200 of 128-4096 at
+// 40 / 8 114.5 / 96.2, one of 8000 and 40 of 100-300 at 32 / 8 19.9 / 12.9.
 extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
                                       int64_t first_q_row, int num_kv_heads, int num_cus, int always, int32_t* items,
                                       int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
-                                      int64_t* out_counts) {
+                                      int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
   using namespace mva;
-  constexpr int kShare = 4, kTilePages = 2, kPerCu = 3;
   if (num_seqs < 0 || num_kv_heads <= 0 || num_cus <= 0 || out_counts == nullptr || wave_extra == nullptr ||
       wave_extra_len < 1)
     return set_error("decode plan: invalid arguments");
   for (int i = 0; i < 4; ++i) out_counts[i] = 0;
   wave_extra[0] = 0;
   if (num_seqs == 0) return 0;
-  if (block_counts == nullptr || items == nullptr) return set_error("decode plan: invalid arguments");
+  if (block_counts == nullptr || items == nullptr || merges == nullptr)
+    return set_error("decode plan: invalid arguments");
   if (!rows_fit_int32(first_seq, first_q_row, num_seqs))
     return set_error("decode plan: sequence or query row index out of int32 range");
-  if (page_offsets(block_counts, num_seqs).empty()) return -1;
-  if (num_seqs > std::numeric_limits<int32_t>::max() / kShare / num_kv_heads)
+  const std::vector<int64_t> offsets = page_offsets(block_counts, num_seqs);
+  if (offsets.empty()) return -1;
+  const int64_t hkv = num_kv_heads, cus = num_cus;
+  const int64_t at_once = kSharesPerCu * cus;
+  if (std::max(num_seqs * hkv, at_once) > std::numeric_limits<int32_t>::max() / kShareWaves)
     return set_error("decode plan: more than 2^31-1 pieces");
-  const int64_t segments = num_seqs * num_kv_heads, waves = segments * kShare;
-  std::vector<int32_t> order((size_t)num_seqs);
-  for (int64_t s = 0; s < num_seqs; ++s) order[(size_t)s] = (int32_t)s;
-  std::stable_sort(order.begin(), order.end(),
-                   [&](int32_t a, int32_t b) { return block_counts[a] > block_counts[b]; });
-  if (!always) {
-    auto units = [&](int32_t s) { return (double)((block_counts[s] + kTilePages - 1) / kTilePages) / kShare; };
-    double mean = 0;
-    for (int32_t s : order) mean += units(s) * num_kv_heads / num_cus;
-    const double most = 7 + mean;
-    if (units(order[0]) > most) return 0;
-    std::priority_queue<double, std::vector<double>, std::greater<double>> load;
-    for (int i = 0; i < num_cus; ++i) load.push(0);
-    for (int32_t s : order)
-      for (int h = 0; h < num_kv_heads; ++h) {
-        const double after = load.top() + units(s);
-        if (after > most) return 0;
-        load.pop();
-        load.push(after);
-      }
+  double tiles = 0;
+  for (int64_t s = 0; s < num_seqs; ++s) tiles += (double)((block_counts[s] + kTilePages - 1) / kTilePages);
+  const double mean = tiles * (double)hkv / (double)cus;  // tiles a CU
+  const double whole = std::numeric_limits<double>::infinity();
+  std::vector<Share> best;
+  double best_us = always ? whole : 11.3 + 0.85 * mean / kShareWaves;
+  for (const double target : {whole, mean, mean / 2, mean / 3}) {
+    std::vector<Share> shares = cut_shares(block_counts, num_seqs, std::max(target, (double)kShareWaves));
+    // Cut, at most what all CUs hold at once.
+    const bool is_cut = (int64_t)shares.size() > num_seqs;
+    if (is_cut && (int64_t)shares.size() * hkv > at_once) continue;
+    int32_t most_pieces = 1;
+    for (const Share& x : shares) most_pieces = std::max(most_pieces, x.of);
+    const double us = (is_cut ? 9.5 : 4.2) + (most_pieces > 32 ? 1 : 0) + 0.87 * longest_queue(shares, hkv, cus);
+    if (us >= best_us) continue;
+    best_us = us;
+    best = std::move(shares);
   }
+  const int64_t pairs = (int64_t)best.size() * hkv, waves = pairs * kShareWaves;
+  if (pairs == 0) return 0;
   if (waves > item_rows || wave_extra_len < waves + 1) return set_error("decode plan: item capacity too small");
-  // Place at = segment order[at / heads], head at % heads, sorted by length.
-  auto emit = [&](int64_t row, int64_t at) {
-    const int32_t s = order[(size_t)(at / num_kv_heads)];
-    const int64_t pages = block_counts[s], tiles = (pages + kTilePages - 1) / kTilePages;
-    for (int k = 0; k < kShare; ++k) {
-      const int64_t begin = tiles * k / kShare * kTilePages, end = tiles * (k + 1) / kShare * kTilePages;
-      write_piece(items + (row * kShare + k) * kItemInts, s, first_seq, first_q_row, begin, std::min(end, pages), k,
-                  kShare, -1, (int)(at % num_kv_heads));
+
+  std::vector<int32_t> part_base((size_t)num_seqs, 0);
+  for (const Share& x : best)
+    if (x.of > 1) part_base[(size_t)x.seq] = x.of;
+  int32_t slots = 0;
+  int64_t num_merges = 0;
+  for (int64_t s = 0; s < num_seqs; ++s) {
+    const int32_t of = part_base[(size_t)s];
+    part_base[(size_t)s] = slots;
+    slots += of;
+    if (of == 0) continue;
+    if (num_merges + hkv > merge_rows) return set_error("decode plan: merge capacity too small");
+    for (int h = 0; h < num_kv_heads; ++h)
+      write_piece(merges + num_merges++ * kItemInts, s, first_seq, first_q_row, 0, block_counts[s], 0, of,
+                  part_base[(size_t)s], h);
+  }
+  for (int64_t i = 0; i < pairs; ++i) {
+    const int64_t at = share_of_workgroup(i, pairs, cus);
+    const Share& x = best[(size_t)(at / hkv)];
+    const int64_t n = x.tiles(), pages = block_counts[x.seq];
+    for (int k = 0; k < kShareWaves; ++k) {
+      const int64_t begin = (x.begin + n * k / kShareWaves) * kTilePages;
+      const int64_t end = (x.begin + n * (k + 1) / kShareWaves) * kTilePages;
+      write_piece(items + (i * kShareWaves + k) * kItemInts, x.seq, first_seq, first_q_row, begin,
+                  std::min(end, pages), x.chunk, x.of, ~part_base[(size_t)x.seq], (int)(at % hkv));
     }
-  };
-  const bool at_once = segments <= (int64_t)kPerCu * num_cus;
-  for (int64_t turn = 0, first = 0; first < segments; ++turn, first += num_cus) {
-    const int64_t end = std::min(segments, first + num_cus);
-    for (int64_t i = first; i < end; ++i) emit(i, at_once && turn % 2 == 0 ? end - 1 - (i - first) : i);
   }
   std::fill(wave_extra, wave_extra + waves + 1, (int32_t)waves);
   out_counts[0] = out_counts[1] = waves;
+  out_counts[2] = slots;
+  out_counts[3] = num_merges;
   return 0;
 }
 

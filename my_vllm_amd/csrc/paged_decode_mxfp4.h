@@ -44,9 +44,9 @@ constexpr int kFp4TileVScales = kFp4TileKScales + kFp4TileTokens * kFp4RowScales
 constexpr int kFp4TileBytes = kFp4TileVScales + kFp4TileTokens * kFp4RowScales;  // 4352
 constexpr int kFp4TileBufs = 3;
 constexpr int kFp4WaveLdsBytes = kFp4TileBufs * kFp4TileBytes;  // 13056: twelve wavefronts in 160 KB
-// Wavefronts that share a segment, and where each leaves its m and l of 16 heads,
+// Wavefronts that share a piece, and where each leaves its m and l of 16 heads,
 // after its 16 rows of o.
-constexpr int kFp4ShareWaves = 4;
+constexpr int kFp4ShareWaves = 4;  // as the planner's
 constexpr int kFp4ShareMax = 16 * kHeadDim * 4;
 constexpr int kFp4ShareSum = kFp4ShareMax + 64;
 static_assert(kFp4ShareSum + 64 <= kFp4WaveLdsBytes, "a share fits its wavefront's LDS");
@@ -110,10 +110,10 @@ __device__ inline float groups_sum(float v) {
 // One wavefront, number `slot` of its workgroup, of a decode launch over piece
 // lists (see decode_wave); `group_lds` is kFp4WaveLdsBytes for each wavefront of the workgroup.
 //
-// Wavefronts 4 i .. 4 i + 3 of a launch may instead share a segment (sequence, KV
-// head): each has one piece, a quarter of its pages and part_base -1, and the four
-// join in LDS, without partials in memory and the merge kernel after it.  Either all
-// pieces of a launch are shared or none.
+// Wavefronts 4 i .. 4 i + 3 of a launch may instead share a piece: each has one
+// descriptor, with a quarter of the pages and the complement of part_base, and the four
+// join in LDS, with one partial for them, or none and no merge kernel where the piece is
+// a whole segment.  Either all pieces of a launch are shared or none.
 //
 // A piece goes in runs of up to 256 pages.  A run loads its queries and page table
 // words, copies its first three tiles, and then computes tile after tile, copying
@@ -298,8 +298,8 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
           __builtin_bit_cast(V8, __builtin_shufflevector(v0[mt], v1[mt], 0, 1, 2, 3, 4, 5, 6, 7)), pf, o[mt]);
   };
 
-  // A piece of a shared segment (part_base -1): the four wavefronts of its share
-  // group leave their o, m and l in LDS, over their tiles, and join them together.
+  // A quarter of a shared piece: its four wavefronts leave their o, m and l in LDS,
+  // over their tiles, and join them together, into the output or a partial.
   auto join_share = [&](float l_tot) __attribute__((always_inline)) {
     // Row c of this wavefront, 16-byte chunk ch at slot ch ^ c: 16 lanes of a
     // write take 16 slots.
@@ -331,6 +331,12 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
         sum += a * lds_ld16<f32x4>(first + w * kFp4WaveLdsBytes + g * 4 * kHeadDim + ((ch ^ g) << 4));
       }
       const float inv = den > 0.f ? 1.0f / den : 0.f;
+      if (X[4] > 1) {
+        const int64_t row = ((int64_t)(~X[5] + X[3]) * Hkv + X[7]) * G + g;
+        store16_device_untracked(p.part_o + row * kHeadDim + 4 * ch, __builtin_bit_cast(u32x4, sum * inv));
+        if (ch == 0) store4_device_untracked(&p.part_lse[row], den > 0.f ? m_use + fast_log2(den) : -INFINITY);
+        continue;
+      }
       V4 y;
 #pragma unroll
       for (int r = 0; r < 4; ++r) y[r] = (T)(sum[r] * inv);

@@ -18,9 +18,8 @@ int launch_decode_merge(const DecodeParams& p, const int32_t* merges, int64_t nu
 
 namespace {
 
-// kWaves wavefronts per workgroup, each with private LDS buffers.  Four neighbours
-// are neighbours of the launch; the next four of a workgroup are a grid further on, so
-// that a launch whose wavefronts are fewer than its capacity has them on all CUs.
+// kWaves wavefronts per workgroup, each with private LDS buffers; wavefront w of
+// workgroup b is decode wavefront b * kWaves + w.
 template <typename T, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))) void paged_decode_mxfp4_kernel(
     Fp4DecodeParams p) {
@@ -28,7 +27,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))
   // Tiles done by the wavefronts; one without work reads as far ahead.
   __shared__ int progress[kWaves];
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int wave = ((w >> 2) * (int)gridDim.x + (int)blockIdx.x) * 4 + (w & 3);
+  const int wave = (int)blockIdx.x * kWaves + w;
   if (kWaves == 12 && (threadIdx.x & 63) == 0) progress[w] = 0x3fffffff;
   if (wave >= p.num_waves) return;
   decode_wave_mxfp4<T>(p, wave, (lds_u8*)lds, kWaves == 12 ? progress : nullptr, w);

@@ -28,7 +28,7 @@ MAX_CHUNK_PAGES = 128
 # Piece length of a plan whose pieces are not cut any further (kAnyPiecePages):
 # paged_decode_mxfp4 takes pieces of any length, paged_decode of MAX_CHUNK_PAGES.
 ANY_PIECE_PAGES = 0x7fffffff
-# Wavefronts that share a segment of an MXFP4 decode plan (plan_decode_shared).
+# Wavefronts that share a piece of an MXFP4 decode plan (plan_decode_shared).
 MXFP4_SHARE_WAVES = 4
 # Query rows per prefill workgroup (kPrefillRows): G heads x 128 // G tokens.
 PREFILL_ROWS = 128

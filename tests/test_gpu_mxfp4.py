@@ -223,19 +223,18 @@ def test_decode(gpu, hq, hkv, dtype):
     _check(out, batch, k, v, dtype)
 
 
-@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("per_group", [4, 12])
 @pytest.mark.parametrize("waves", [8, 24, 64, 512])
-def test_decode_with_long_piece_lists(gpu, monkeypatch, waves, large):
+def test_decode_with_long_piece_lists(gpu, monkeypatch, waves, per_group):
     # Many pieces a wavefront, of every length modulo a tile, with one longer than a run of 256 pages; both
     # workgroup sizes.
     set_decode_planning(monkeypatch, waves=waves)
-    if large:
-        monkeypatch.setattr(attention_backend, "_MXFP4_LARGE_BYTES", 0)
+    monkeypatch.setattr(attention_backend, "_MXFP4_WAVES", ((8, per_group), (12, 12)))
     ctx = [1, 16, 17, 33, 48, 64, 65, 100, 113, 128, 129, 200, 8500, 5, 31, 47]
     batch = make_paged_batch(waves, [1] * len(ctx), ctx, 0, 16, 8)
     out, backend, plan, (_, _, k, v) = _forward(batch, gpu, BF16)
     assert plan.metadata.num_decode_waves <= max(waves, 8)
-    assert plan.metadata.decode_waves_per_group == (12 if large else 4)
+    assert plan.metadata.decode_waves_per_group == per_group
     if waves == 8:
         assert (plan.metadata.decode_items[:, 2] - plan.metadata.decode_items[:, 1]).max() > 512
     _check(out, batch, k, v, BF16)
@@ -571,9 +570,9 @@ def test_foreign_contract_family(gpu):
 @pytest.mark.parametrize("large", [False, True])
 @pytest.mark.parametrize("hq,hkv,dtype", [(8, 8, BF16), (16, 8, FP16), (32, 2, BF16), (24, 8, FP16), (5, 1, BF16)])
 def test_shared_segments_of_every_length(gpu, monkeypatch, hq, hkv, dtype, large):
-    """Four wavefronts a segment: lengths that leave some of them without pages, and long ones."""
+    """Four wavefronts a piece: lengths that leave some of them without pages, and long ones that are cut."""
     monkeypatch.setattr(MI355XMXFP4AttentionBackend, "decode_schedule_override", "shared")
-    ctx = [1, 15, 16, 17, 32, 33, 64, 65, 95, 96, 97, 128, 129, 300, 2047, 4500]
+    ctx = [1, 15, 16, 17, 32, 33, 64, 65, 95, 96, 97, 128, 129, 300, 2047, 9000]
     batch = make_paged_batch(hq, [1] * len(ctx), ctx, 0, hq, hkv, dtype=dtype)
     k, v = mxfp4.cache_of(batch.k_cache), mxfp4.cache_of(batch.v_cache)
     for cache, seed in ((k, 1), (v, 2)):
@@ -581,7 +580,7 @@ def test_shared_segments_of_every_length(gpu, monkeypatch, hq, hkv, dtype, large
     backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, dtype)
     plan = backend.build_plan(_on(batch.common, gpu))
     metadata = plan.metadata
-    assert metadata.num_decode_waves == len(ctx) * hkv * 4 and metadata.num_decode_merges == 0
+    assert metadata.num_decode_merges >= hkv and (metadata.decode_items[:, 5] < 0).all()
     q, kd, vd = batch.q.to(gpu), k.to(gpu), v.to(gpu)
     if not large:
         _check(backend.forward(q, None, None, kd, vd, plan), batch, k, v, dtype)
@@ -589,32 +588,32 @@ def test_shared_segments_of_every_length(gpu, monkeypatch, hq, hkv, dtype, large
     # The same plan in workgroups of twelve.
     out = torch.full_like(q, float("nan"))
     ops.paged_decode_mxfp4(q, kd, vd, metadata.block_tables, metadata.seq_lens, metadata.decode_items,
-                           metadata.num_decode_items, metadata.num_decode_waves, None, 0, 0, out,
-                           torch.empty(ops.decode_workspace_bytes(0, hkv, hq // hkv), dtype=torch.uint8, device=gpu),
+                           metadata.num_decode_items, metadata.num_decode_waves, metadata.decode_merges,
+                           metadata.num_decode_merges, metadata.num_decode_part_slots, out,
+                           torch.zeros(ops.decode_workspace_bytes(metadata.num_decode_part_slots, hkv, hq // hkv),
+                                       dtype=torch.uint8, device=gpu),
                            backend.softmax_scale, metadata.decode_wave_extra, 12)
     _check(out, batch, k, v, dtype)
     assert torch.equal(out, backend.forward(q, None, None, kd, vd, plan))
 
 
-@pytest.mark.parametrize("large", [False, True])
-def test_one_graph_replays_shared_and_listed_steps(gpu, monkeypatch, large):
-    """Steps of one captured launch whose plans are of either kind, in workgroups of 4 and of 12."""
-    if large:
-        monkeypatch.setattr(attention_backend, "_MXFP4_LARGE_BYTES", 0)
+def test_one_graph_replays_shared_and_listed_steps(gpu):
+    """Steps of one captured launch whose plans are of either kind."""
     hq, hkv, n, width = 16, 8, 6, 260
     backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, BF16)
     state = backend.create_full_decode_graph_state(n, n * width, gpu)
-    assert state.waves_per_group == (12 if large else 4)
     caches = torch.zeros(2, *ops.mxfp4_cache_shape(n * width, hkv), dtype=torch.uint8, device=gpu)
     q = torch.zeros(n, hq, 128, dtype=BF16, device=gpu)
     graph, kinds = None, []
-    for seed, ctx in enumerate(([100, 7, 64, 300, 16, 1], [4100, 30, 17, 1000, 1, 900], [500] * 6, [4160] * 6)):
+    for seed, (ctx, schedule) in enumerate((([100, 7, 64, 300, 16, 1], None), ([4100, 30, 17, 1000, 1, 900], "listed"),
+                                            ([500] * 6, "listed"), ([4160] * 6, None), ([4100, 1, 1, 2, 3, 50], None))):
+        backend.decode_schedule_override = schedule
         batch = make_paged_batch(seed, [1] * n, ctx, 0, hq, hkv)
         k, v = mxfp4.cache_of(batch.k_cache), mxfp4.cache_of(batch.v_cache)
         caches[0, :len(k)], caches[1, :len(v)] = k.to(gpu), v.to(gpu)
         q.copy_(batch.q)
         plan = backend.build_plan(_on(batch.common, gpu))
-        kinds.append(plan.metadata.num_decode_merges == 0)
+        kinds.append((bool((plan.metadata.decode_items[:, 5] < 0).all()), plan.metadata.num_decode_merges > 0))
         eager = backend.forward(q, None, None, caches[0], caches[1], plan).clone()
         _check(eager, batch, k, v, BF16)
         assert backend.full_decode_graph_metadata_fits(state, plan)
@@ -633,4 +632,4 @@ def test_one_graph_replays_shared_and_listed_steps(gpu, monkeypatch, large):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(state.output, eager)
-    assert kinds == [True, False, True, False]
+    assert kinds == [(True, False), (False, True), (False, True), (True, True), (True, True)]

@@ -5,7 +5,12 @@ import pytest
 import torch
 
 from my_vllm_amd import _native, ops
-from my_vllm_amd.attention_backend import MI355XMXFP4AttentionBackend, mxfp4_decode_ranges, plan_decode_shared
+from my_vllm_amd.attention_backend import (
+    MI355XMXFP4AttentionBackend,
+    mxfp4_decode_ranges,
+    plan_decode_shared,
+    shared_decode_capacity,
+)
 from my_vllm_amd.contract import AttentionRoute
 from my_vllm_amd.custom_op import CustomOpConfig
 from my_vllm_amd.layers import MXFP4KVCacheStore
@@ -192,7 +197,7 @@ def test_abi_prefill_refuses_before_any_launch(change, message):
 
 
 def test_decode_ranges():
-    # Ranges of four pages or more; twelve wavefronts a CU from half a gigabyte on.
+    # Ranges of four pages or more; twelve wavefronts a CU on large batches.
     assert mxfp4_decode_ranges(3, 8) == (1, 4)
     assert mxfp4_decode_ranges(41, 8) == (10, 4)
     assert mxfp4_decode_ranges(20000, 8) == (256, 4)
@@ -202,47 +207,75 @@ def test_decode_ranges():
     assert mxfp4_decode_ranges(4000, 300) == (10, 12)  # 2.6 GB
 
 
-def test_shared_plan_covers_every_segment():
-    counts = np.array([5, 1, 40, 8, 1, 129], np.int64)
-    items, wave_extra = plan_decode_shared(counts, 3, 7, 5, 256, always=True)
-    assert items.shape == (6 * 5 * 4, 8) and (wave_extra == len(items)).all() and wave_extra.size == len(items) + 1
+@pytest.mark.parametrize("counts,hkv,cus", [
+    ([5, 1, 40, 8, 1, 129], 5, 256),
+    ([1875], 8, 256),
+    ([2000, 1, 2, 3], 8, 256),
+    ([17] * 300, 8, 256),
+    ([9, 8, 7], 2, 1),
+    ([2 ** 20, 3], 16, 256),
+    ([300] * 37, 4, 304),
+])
+def test_shared_plans_cover_every_segment(counts, hkv, cus):
+    items, wave_extra, waves, slots, merges = plan_decode_shared(counts, 3, 7, hkv, cus, always=True)
+    assert items.shape == (waves, 8) and (wave_extra == waves).all() and wave_extra.size == waves + 1
+    assert len(items) <= shared_decode_capacity(len(counts), hkv, cus)
     groups = items.reshape(-1, 4, 8)
-    assert (groups[:, :, [0, 6, 7]] == groups[:, :1, [0, 6, 7]]).all()  # four of one segment
-    assert (groups[:, :, 3] == np.arange(4)).all() and (items[:, 4] == 4).all() and (items[:, 5] == -1).all()
-    assert (items[:, 6] - items[:, 0] == 4).all()
-    assert len({(s, h) for s, h in groups[:, 0, [0, 7]].tolist()}) == 30
-    for group in groups:
-        pages = counts[group[0, 0] - 3]
-        assert group[0, 1] == 0 and group[3, 2] == pages
-        assert (group[1:, 1] == group[:-1, 2]).all() and (group[:, 2] >= group[:, 1]).all()
-        assert (group[:, 1] % 2 == 0).all() or pages < 8  # whole tiles
-        assert (group[:, 2] - group[:, 1]).max() <= 2 * -(-pages // 8)
+    assert (groups[:, :, 3:] == groups[:, :1, 3:]).all() and (groups[:, :, 0] == groups[:, :1, 0]).all()
+    assert (groups[:, 1:, 1] == groups[:, :-1, 2]).all()  # quarters side by side
+    assert (items[:, 1] <= items[:, 2]).all() and (items[:, 6] - items[:, 0] == 4).all()
+    sizes = items[:, 2] - items[:, 1]
+    pieces = (groups[:, 3, 2] - groups[:, 0, 1] + 1) // 2  # tiles
+    assert (sizes.reshape(-1, 4) <= 2 * -(-pieces[:, None] // 4)).all()
+    ends = np.array(counts)[items[:, 0] - 3]
+    assert (items[:, 1] % 2 == 0).all() or (items[:, 1] <= ends).all()  # whole tiles
+    used = []
+    for s, pages in enumerate(counts):
+        for h in range(hkv):
+            own = groups[(groups[:, 0, 0] == s + 3) & (groups[:, 0, 7] == h)]
+            own = own[np.argsort(own[:, 0, 3])]
+            n = len(own)
+            assert own[:, 0, 3].tolist() == list(range(n)) and (own[:, 0, 4] == n).all()
+            assert own[0, 0, 1] == 0 and own[-1, 3, 2] == pages and (own[1:, 0, 1] == own[:-1, 3, 2]).all()
+            base = ~int(own[0, 0, 5])
+            assert base >= 0
+            merge = merges[(merges[:, 0] == s + 3) & (merges[:, 7] == h)]
+            assert len(merge) == (n > 1)
+            if n > 1:
+                assert merge[0].tolist() == [s + 3, 0, pages, 0, n, base, s + 7, h]
+                if h == 0:
+                    used += range(base, base + n)
+    assert used == list(range(slots))
 
 
 def test_shared_plan_order():
     # All at once: every CU's workgroups (4 CUs, places i, i + 4, i + 8) sum to about the same.
-    counts = np.array([10, 3, 7, 1, 12, 5, 9, 2, 8, 4], np.int64)
-    pages = counts[plan_decode_shared(counts, 0, 0, 1, 4, always=True)[0][::4, 0]]
-    assert pages.tolist() == [8, 9, 10, 12, 7, 5, 4, 3, 1, 2]
+    counts = np.array([10, 3, 7, 1, 12, 5, 9, 2, 8, 4], np.int64) * 2
+
+    def pages(cus):
+        items, _, waves, _, merges = plan_decode_shared(counts, 0, 0, 1, cus, always=True)
+        assert waves == 40 and len(merges) == 0
+        return (counts[items[::4, 0]] // 2).tolist()
+
+    assert pages(4) == [8, 9, 10, 12, 7, 5, 4, 3, 1, 2]
     # More than a CU holds: longest first.
-    pages = counts[plan_decode_shared(counts, 0, 0, 1, 3, always=True)[0][::4, 0]]
-    assert pages.tolist() == sorted(counts.tolist(), reverse=True)
+    assert pages(3) == sorted((counts // 2).tolist(), reverse=True)
 
 
-@pytest.mark.parametrize("counts,hkv,shared", [
-    ([1], 8, True),
-    ([33] * 8, 8, True),
-    ([63] * 32, 8, True),
-    ([13] * 200, 8, True),
-    ([2000], 8, False),
-    ([75], 8, False),
-    ([500] + [10] * 40, 8, False),
-    ([150] * 37, 4, False),
-    ([500] * 96, 4, False),  # 384 segments on 256 CUs: two on half of them
+@pytest.mark.parametrize("counts,hkv,pieces", [
+    ([1], 8, 8),
+    ([19], 8, 8),
+    ([63] * 32, 8, 256),
+    ([13] * 200, 8, 1600),
+    ([75], 8, 80),  # 38 tiles, ten pieces (9.5 to nearest, up)
+    ([1876], 8, 256),
+    ([500] + [10] * 40, 8, None),
+    ([8192] * 56, 8, 0),  # page ranges
+    ([750] * 40, 8, 0),
 ])
-def test_shared_plans_where_they_are_expected_to_be_faster(counts, hkv, shared):
-    items, wave_extra = plan_decode_shared(counts, 0, 0, hkv, 256)
-    assert len(items) == (len(counts) * hkv * 4 if shared else 0) and wave_extra.size == len(items) + 1
+def test_plans_taken(counts, hkv, pieces):
+    waves = plan_decode_shared(counts, 0, 0, hkv, 256)[2]
+    assert waves == 4 * pieces if pieces is not None else 4 * 8 * 41 < waves <= 4 * 768
 
 
 def test_shared_plan_refusals():
@@ -250,21 +283,21 @@ def test_shared_plan_refusals():
         plan_decode_shared([3, 0], 0, 0, 8, 256)
     with pytest.raises(RuntimeError, match="int32 range"):
         plan_decode_shared([3, 3], 2 ** 31 - 1, 0, 8, 256)
-    counts, items = np.array([4], np.int64), np.zeros((8, 8), np.int32)
-    extra, out = np.zeros(9, np.int32), np.zeros(4, np.int64)
+    counts, items = np.array([400], np.int64), np.zeros((3072, 8), np.int32)
+    extra, merges, out = np.zeros(3073, np.int32), np.zeros((4, 8), np.int32), np.zeros(4, np.int64)
 
-    def call(hkv=1, cus=256, rows=8, words=9):
+    def call(hkv=1, cus=256, rows=3072, words=3073, joins=4):
         _native.call("mva_decode_plan_shared", counts.ctypes.data, 1, 0, 0, hkv, cus, 1, items.ctypes.data, rows,
-                     extra.ctypes.data, words, out.ctypes.data)
+                     extra.ctypes.data, words, merges.ctypes.data, joins, out.ctypes.data)
 
     for change in ({"hkv": 0}, {"cus": 0}, {"words": 0}):
         with pytest.raises(RuntimeError, match="invalid arguments"):
             call(**change)
-    for change in ({"rows": 3}, {"words": 4}, {"hkv": 3}):
+    for change in ({"rows": 3}, {"words": 4}, {"joins": 0}, {"hkv": 5}):
         with pytest.raises(RuntimeError, match="capacity too small"):
             call(**change)
-    call(hkv=2)
-    assert out.tolist() == [8, 8, 0, 0]
+    call(hkv=4)
+    assert out.tolist() == [4 * 4 * 50, 4 * 4 * 50, 50, 4]
 
 
 class _HostBackend(MI355XMXFP4AttentionBackend):
