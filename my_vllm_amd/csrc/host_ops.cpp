@@ -417,6 +417,13 @@ PyObject* forward_inputs_ok(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- MXFP4 caches ----
+//
+// The module also loads over a library without these entry points (hence weak):
+// their calls then take the general path, which names the one that is missing.
+#pragma weak mva_kv_store_mxfp4
+#pragma weak mva_kv_load_mxfp4
+#pragma weak mva_paged_decode_mxfp4
+#pragma weak mva_paged_prefill_mxfp4
 
 constexpr int64_t kFp4Block = 1088;
 
@@ -441,6 +448,7 @@ bool aligned_rows(const Tensor& t) {
 // (key, value, k_cache, v_cache, slot_mapping): True when launched.
 PyObject* store_kvcache_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
+    if (&mva_kv_store_mxfp4 == nullptr) return none();
     if (n != 5) return none();
     const Tensor *k = plain(a[0]), *v = plain(a[1]), *kc = plain(a[2]), *vc = plain(a[3]), *slots = plain(a[4]);
     if (!k || !v || !slots || !head_rows(*k, *k) || !head_rows(*v, *k) || k->sizes() != v->sizes() ||
@@ -461,6 +469,7 @@ PyObject* store_kvcache_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // (k_cache, v_cache, slot_mapping, MVA_DTYPE_* of the rows): (key, value).
 PyObject* load_kvcache_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
+    if (&mva_kv_load_mxfp4 == nullptr) return none();
     int64_t code;
     if (n != 4 || !as_int(a[3], &code) || (code != MVA_DTYPE_BF16 && code != MVA_DTYPE_F16)) return none();
     const Tensor *kc = plain(a[0]), *vc = plain(a[1]), *slots = plain(a[2]);
@@ -503,6 +512,7 @@ struct PagedFp4 : Paged {
 //  workspace, scale, wave_extra, waves_per_group): True when launched.
 PyObject* paged_decode_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
+    if (&mva_paged_decode_mxfp4 == nullptr) return none();
     PagedFp4 p;
     int64_t items_n, waves, merges_n, slots_n, per_group;
     double scale;
@@ -529,6 +539,7 @@ PyObject* paged_decode_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 //  max_tiles, workspace, out, scale, planned): True when launched.
 PyObject* paged_prefill_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
+    if (&mva_paged_prefill_mxfp4 == nullptr) return none();
     PagedFp4 p;
     int64_t seqs, tiles;
     double scale;

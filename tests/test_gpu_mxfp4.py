@@ -4,6 +4,9 @@ What the cache holds is compared exactly, bytes and values.  Attention is held
 to the bound that tests/_mxfp4.py derives from the roundings made.
 """
 
+import shutil
+import subprocess
+import sys
 import types
 
 import pytest
@@ -633,3 +636,44 @@ def test_one_graph_replays_shared_and_listed_steps(gpu):
             torch.cuda.synchronize()
             assert torch.equal(state.output, eager)
     assert kinds == [(True, False), (False, True), (False, True), (True, True), (True, True)]
+
+
+GIL_CALLS = """
+import importlib.machinery, importlib.util, sys
+import torch
+
+loader = importlib.machinery.ExtensionFileLoader("mva_host", sys.argv[1])
+host = importlib.util.module_from_spec(importlib.util.spec_from_loader("mva_host", loader))
+loader.exec_module(host)
+i32 = dict(dtype=torch.int32, device="cuda")
+q, kv = (torch.zeros(4, n, 128, dtype=torch.bfloat16, device="cuda") for n in (8, 2))
+cache, ws = torch.zeros(2, 2, 1088, dtype=torch.uint8, device="cuda"), torch.zeros(64, dtype=torch.uint8, device="cuda")
+ints, bt = torch.zeros(8, **i32), torch.zeros(4, 2, **i32)
+for name, args in (("store_kvcache_mxfp4", (kv, kv, cache, cache, ints[:4])),
+                   ("load_kvcache_mxfp4", (cache, cache, ints, 0)),
+                   ("paged_decode_mxfp4", (q, cache, cache, bt, ints, None, ints, 1, 1, ints, 0, 0, q, ws, 0.1, ints, 4)),
+                   ("paged_prefill_mxfp4", (q, cache, cache, bt, ints, ints, 1, 1, ws, q, 0.1, False))):
+    got = getattr(host, name)(*args)
+    assert (got is None) if sys.argv[2] == "absent" else (got is not None), name
+print("done")
+"""
+
+
+@pytest.mark.parametrize("library", ["present", "absent"])
+def test_launches_release_the_gil(gpu, tmp_path, library):
+    # Beside a stand-in for the C library whose entry points fail if their thread holds the GIL.  One
+    # without them leaves the calls to the general path.
+    names = ("mva_silu_and_mul", "mva_rms_norm", "mva_fused_add_rms_norm", "mva_qk_norm_rope_store",
+             "mva_paged_decode", "mva_paged_decode_store", "mva_paged_prefill", "mva_paged_prefill_run",
+             "mva_paged_mixed", "mva_paged_mixed_run")
+    if library == "present":
+        names += ("mva_kv_store_mxfp4", "mva_kv_load_mxfp4", "mva_paged_decode_mxfp4", "mva_paged_prefill_mxfp4")
+    source = tmp_path / "stand_in.c"
+    source.write_text("extern int PyGILState_Check(void);\n"
+                      'const char* mva_last_error(void) { return "the launch holds the GIL"; }\n'
+                      + "".join(f"int {name}(void) {{ return PyGILState_Check(); }}\n" for name in names))
+    subprocess.run(["gcc", "-shared", "-fPIC", str(source), "-o", str(tmp_path / _native.LIB_PATH.name)], check=True)
+    module = shutil.copy(_native.HOST_PATH, tmp_path)
+    run = subprocess.run([sys.executable, "-c", GIL_CALLS, str(module), library], capture_output=True, text=True,
+                         timeout=100)
+    assert "done" in run.stdout, run.stderr
