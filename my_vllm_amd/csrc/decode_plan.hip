@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <exception>
 #include <functional>
 #include <limits>
 #include <queue>
@@ -261,8 +262,6 @@ double longest_queue(const std::vector<Share>& shares, int64_t hkv, int64_t num_
   return most;
 }
 
-}  // namespace
-}  // namespace mva
 
 // Of the whole segments and of pieces for about one, two and three workgroups a CU (four
 // tiles or more each, one a wavefront), the cut with the least estimated time, or no
@@ -275,11 +274,9 @@ double longest_queue(const std::vector<Share>& shares, int64_t hkv, int64_t num_
 // graph, 9.3 / 11.1 call by call).  Ranges of eight wavefronts a CU against the plan taken: one of 30001 at 32 / 8
 // 17.7 / 16.3, 37 of 300-6000 at 16 / 4 24.2 / 22.4, 64 of 128-2048 at 16 / 8 28.1 / 22.0, 200 of 128-4096 at
 // 40 / 8 114.5 / 96.2, one of 8000 and 40 of 100-300 at 32 / 8 19.9 / 12.9.
-extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
-                                      int64_t first_q_row, int num_kv_heads, int num_cus, int always, int32_t* items,
-                                      int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
-                                      int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
-  using namespace mva;
+int plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq, int64_t first_q_row,
+                int num_kv_heads, int num_cus, int always, int32_t* items, int64_t item_rows, int32_t* wave_extra,
+                int64_t wave_extra_len, int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
   if (num_seqs < 0 || num_kv_heads <= 0 || num_cus <= 0 || out_counts == nullptr || wave_extra == nullptr ||
       wave_extra_len < 1)
     return set_error("decode plan: invalid arguments");
@@ -304,9 +301,9 @@ extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_s
   double best_us = always ? whole : 11.3 + 0.85 * mean / kShareWaves;
   for (const double target : {whole, mean, mean / 2, mean / 3}) {
     std::vector<Share> shares = cut_shares(block_counts, num_seqs, std::max(target, (double)kShareWaves));
-    // Cut, at most what all CUs hold at once.
+    // Cut, into at most what all CUs hold at once.
     const bool is_cut = (int64_t)shares.size() > num_seqs;
-    if (is_cut && (int64_t)shares.size() * hkv > at_once) continue;
+    if (target != whole && (!is_cut || (int64_t)shares.size() * hkv > at_once)) continue;
     int32_t most_pieces = 1;
     for (const Share& x : shares) most_pieces = std::max(most_pieces, x.of);
     const double us = (is_cut ? 9.5 : 4.2) + (most_pieces > 32 ? 1 : 0) + 0.87 * longest_queue(shares, hkv, cus);
@@ -349,6 +346,21 @@ extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_s
   out_counts[2] = slots;
   out_counts[3] = num_merges;
   return 0;
+}
+
+}  // namespace
+}  // namespace mva
+
+extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
+                                      int64_t first_q_row, int num_kv_heads, int num_cus, int always, int32_t* items,
+                                      int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
+                                      int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
+  try {
+    return mva::plan_shared(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_cus, always, items,
+                            item_rows, wave_extra, wave_extra_len, merges, merge_rows, out_counts);
+  } catch (const std::exception&) {
+    return mva::set_error("decode plan: out of memory");
+  }
 }
 
 extern "C" int64_t mva_decode_plan_claims_rows(int64_t num_seqs, int64_t total_pages, int num_kv_heads,

@@ -35,7 +35,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(3))
 
 template <typename T>
 int launch(const Fp4DecodeParams& p, int waves_per_group, hipStream_t s) {
-  const uint32_t blocks = (uint32_t)((p.num_waves + waves_per_group - 1) / waves_per_group);
+  if (p.num_waves > (int)(0xffffffffu / 64) - 12)  // a launch has fewer than 2^32 threads
+    return set_error("paged attention mxfp4: too many wavefronts");
+  const uint32_t blocks = ((uint32_t)p.num_waves + waves_per_group - 1) / waves_per_group;
   switch (waves_per_group) {
     case 4: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 4>), dim3(blocks), dim3(256), 0, s, p); break;
     case 12: hipLaunchKernelGGL((paged_decode_mxfp4_kernel<T, 12>), dim3(blocks), dim3(768), 0, s, p); break;
@@ -62,7 +64,9 @@ extern "C" int mva_paged_decode_mxfp4(const void* q, int64_t q_token_stride, int
   if (wave_extra == nullptr && num_items > 0) return set_error("paged attention mxfp4: piece lists (wave_extra) needed");
   if (((uint64_t)page_stride_bytes | (uint64_t)head_stride_bytes) % 16)
     return set_error("paged attention mxfp4: cache strides must be 16-byte aligned");
-  if (page_stride_bytes < 0 || page_stride_bytes > 0xffffffffLL)
+  if (page_stride_bytes < 0 || head_stride_bytes < 0)
+    return set_error("paged attention mxfp4: cache strides must not be negative");
+  if (page_stride_bytes > 0xffffffffLL)
     return set_error("paged attention mxfp4: pages must lie less than 4 GiB apart");
   if (dtype != kBF16 && dtype != kF16) return set_error("paged attention: dtype must be bf16 or fp16");
   Fp4DecodeParams p;

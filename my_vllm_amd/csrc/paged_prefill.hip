@@ -890,6 +890,8 @@ extern "C" int mva_paged_prefill_mxfp4(const void* q, int64_t q_token_stride, in
                                        void* stream) {
   if (((uint64_t)page_stride_bytes | (uint64_t)head_stride_bytes) % 16)
     return set_error("paged attention mxfp4: cache strides must be 16-byte aligned");
+  if (page_stride_bytes < 0 || head_stride_bytes < 0)
+    return set_error("paged attention mxfp4: cache strides must not be negative");
   Fp4PrefillParams p;
   const int rc = fill_prefill_params(p, q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, 0, 0,
                                      block_tables, block_table_stride, seq_lens, query_start_loc, num_seqs, out,

@@ -219,12 +219,13 @@ __device__ __attribute__((always_inline)) inline bool settle_piece(int32_t* plan
 // phase of the wave converts them (exactly) and writes the rows to the page's
 // place in LDS, four groups of four conversions and a 16-byte write between the
 // phase's last MFMAs, whose issue slots the vector ALU does not need (at its first
-// ones: 1% slower).  Loads go out
-// at the end of an M phase, so that they have two phases to arrive: group 0
-// loads K(t+2) after M(t) and writes it in M(t+1), phase 2t+2; group 1 loads
-// V(t+2) after M(t) and writes it in M(t+1), phase 2t+3.  Either is after the
-// last read of the buffer (phase 2t-1, 2t+1) and two phases before the first
-// (2t+4, 2t+6).
+// ones: 1% slower).  Loads go out at the end of an M phase, so that they have two
+// phases to arrive: group 0 loads K(t+2) after M(t) and writes it in M(t+1),
+// phase 2t+2; group 1 loads V(t+2) after M(t) and writes it in M(t+1), phase 2t+3.
+// Either is after the last read of the buffer (phase 2t-1, 2t+1) and two phases
+// before the first (2t+4, 2t+6).  Kernel, microseconds, this cache / 16 bits: 16
+// sequences of 64-2048 new tokens over prefixes at 32 / 8 heads 369 / 340 (0.92 / 1.0
+// PFLOP/s), 512 tokens over 7168 75 / 70, one prompt of 333 16.7 / 16.3.
 template <typename T, int kGrp, bool kFixed, bool kPieces, typename P>
 __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(const P& p, int32_t* plan,
                                                                              int h0, int rank, lds_u8* tiles, lds_i32* nextq) {

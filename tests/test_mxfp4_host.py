@@ -121,6 +121,7 @@ def _abi_store(**change):
     ({"khs": 132}, "16-byte aligned"),
     ({"ps": 2180}, "16-byte aligned"),
     ({"vc": 24}, "16-byte aligned"),
+    ({"ps": -2176}, "not be negative"),
 ])
 @pytest.mark.parametrize("name", ["mva_kv_store_mxfp4", "mva_kv_load_mxfp4"])
 def test_abi_refuses_before_any_launch(name, change, message):
@@ -159,6 +160,8 @@ def _abi_decode(**change):
     ({"wsb": 1024}, "workspace too small"),
     ({"per": 8}, "waves_per_group"),
     ({"ps": 1 << 33}, "less than 4 GiB apart"),
+    ({"ps": -2176}, "not be negative"),
+    ({"n": 1 << 27, "waves": 1 << 27}, "too many wavefronts"),
 ])
 def test_abi_decode_refuses_before_any_launch(change, message):
     with pytest.raises(RuntimeError, match=message):
@@ -176,6 +179,7 @@ def _abi_prefill(**change):
 @pytest.mark.parametrize("change,message", [
     ({"ps": 2184}, "16-byte aligned"),
     ({"hs": 1090}, "16-byte aligned"),
+    ({"hs": -1088}, "not be negative"),
     ({"dtype": 2}, "bf16 or fp16"),
     ({"dim": 64}, "head_dim must be 128"),
     ({"page": 32}, "page_size must be 16"),
