@@ -1391,7 +1391,10 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
     ``ops.store_kvcache_mxfp4`` (``layers.MXFP4KVCacheStore``), which
     :meth:`forward_with_kv_store` calls.  DECODE and its graphs, PREFILL and
     WARMUP run as on the base; a MIXED batch runs as prefill + decode launches
-    (route MIXED_SPLIT) in both attention modes."""
+    (route MIXED_SPLIT) in both attention modes.
+
+    A NaN group of V reaches the queries that see it and, in a prefill launch,
+    those before it whose tile of queries and keys holds both."""
 
     backend_name = "mi355x_mxfp4"
     _max_piece_pages = ops.ANY_PIECE_PAGES

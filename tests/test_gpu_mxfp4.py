@@ -677,3 +677,53 @@ def test_launches_release_the_gil(gpu, tmp_path, library):
     run = subprocess.run([sys.executable, "-c", GIL_CALLS, str(module), library], capture_output=True, text=True,
                          timeout=100)
     assert "done" in run.stdout, run.stderr
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """Two backends' decode and prefill steps side by side on two streams: each as alone."""
+    sides = []
+    for seed, (hq, hkv) in enumerate(((32, 8), (16, 4))):
+        dec = make_paged_batch(seed, [1] * 40, decode_lengths(seed, 40, 1, 3000), 0, hq, hkv)
+        pre = make_paged_batch(seed, [300, 500], [700, 500], 2, hq, hkv)
+        backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, BF16)
+        steps = []
+        for batch in (dec, pre):
+            kd, vd, _, _ = cache_pool(batch, gpu)
+            q, plan = batch.q.to(gpu), backend.build_plan(_on(batch.common, gpu))
+            alone = backend.forward(q, None, None, kd, vd, plan).clone()
+            steps.append((q, kd, vd, plan, alone))
+        sides.append((backend, torch.cuda.Stream(), steps))
+    torch.cuda.synchronize()
+    found = []
+    for _ in range(10):
+        for which in (0, 1):
+            for backend, stream, steps in sides:
+                q, kd, vd, plan, alone = steps[which]
+                with torch.cuda.stream(stream):
+                    found.append((backend.forward(q, None, None, kd, vd, plan).clone(), alone))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in found)
+
+
+def test_padding_rows_and_rows_behind_the_last_stay(gpu):
+    """Slots of -1 and tokens behind a call's last leave the cache and the output buffer alone."""
+    rows = torch.randn(70, 8, 128, device=gpu).to(BF16)
+    cache = torch.full((2, 6, 8, 1088), 0x5a, dtype=torch.uint8, device=gpu)
+    slots = torch.full((70,), -1, dtype=torch.int32, device=gpu)
+    slots[:3] = torch.tensor([17, 40, 95])
+    ops.store_kvcache_mxfp4(rows, rows, cache[0], cache[1], slots)
+    want = torch.full((6, 8, 1088), 0x5a, dtype=torch.uint8)
+    mxfp4.store(rows[:3].cpu(), want, [17, 40, 95])
+    assert torch.equal(cache[0].cpu(), want) and torch.equal(cache[1].cpu(), want)
+    batch = make_paged_batch(5, [1] * 4, [20, 300, 16, 900], 0, 16, 8)
+    kd, vd, k, v = cache_pool(batch, gpu)
+    backend = MI355XMXFP4AttentionBackend(16, 8, 128, 16, BF16)
+    m = backend.build_plan(_on(batch.common, gpu)).metadata
+    out = torch.full((7, 16, 128), 2.0, dtype=BF16, device=gpu)
+    ops.paged_decode_mxfp4(batch.q.to(gpu), kd, vd, m.block_tables, m.seq_lens, m.decode_items, m.num_decode_items,
+                           m.num_decode_waves, m.decode_merges, m.num_decode_merges, m.num_decode_part_slots, out,
+                           torch.zeros(ops.decode_workspace_bytes(m.num_decode_part_slots, 8, 2), dtype=torch.uint8,
+                                       device=gpu), backend.softmax_scale, m.decode_wave_extra,
+                           m.decode_waves_per_group)
+    _check(out[:4], batch, k, v, BF16)
+    assert (out[4:] == 2.0).all()

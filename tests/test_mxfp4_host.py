@@ -287,10 +287,10 @@ def test_shared_plan_refusals():
         plan_decode_shared([3, 0], 0, 0, 8, 256)
     with pytest.raises(RuntimeError, match="int32 range"):
         plan_decode_shared([3, 3], 2 ** 31 - 1, 0, 8, 256)
-    counts, items = np.array([400], np.int64), np.zeros((3072, 8), np.int32)
-    extra, merges, out = np.zeros(3073, np.int32), np.zeros((4, 8), np.int32), np.zeros(4, np.int64)
+    counts, items = np.array([400], np.int64), np.zeros((4096, 8), np.int32)
+    extra, merges, out = np.zeros(4097, np.int32), np.zeros((4, 8), np.int32), np.zeros(4, np.int64)
 
-    def call(hkv=1, cus=256, rows=3072, words=3073, joins=4):
+    def call(hkv=1, cus=256, rows=4096, words=4097, joins=4):
         _native.call("mva_decode_plan_shared", counts.ctypes.data, 1, 0, 0, hkv, cus, 1, items.ctypes.data, rows,
                      extra.ctypes.data, words, merges.ctypes.data, joins, out.ctypes.data)
 
