@@ -216,16 +216,6 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
       vw[i] = lds_ld16<u32x4>(buf + kFp4TileV + i * kFp4ScaleOffset + voff);
       vs[i] = buf[kFp4TileVScales + 64 * i + lane];
     }
-    f32x4 sc[2];  // sc[i][r] = S[token 4 q4 + r of page i][g = c]
-#pragma unroll
-    for (int i = 0; i < 2; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // The two pages' sums in turn: one alone is a chain of dependent MFMAs.
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) sc[i] = Elem<T>::mfma16(fp4_unpack8<T>(kw[i][j], ks[i]), qf[j], sc[i]);
-      if (j & 1) __builtin_amdgcn_sched_barrier(0);  // not all conversions at once: registers
-    }
     // Rows of page i over the tile's codes, and their transposed reads.  LDS works
     // in order for a wavefront: the reads of codes above come before the first
     // page's writes, its transposed reads before the second page's writes.
@@ -247,10 +237,24 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) v[mt] = lds_ld_tr16(buf + (vread ^ (32 * mt)));
     };
+    // The first page's rows are on their way while the scores are computed (after them:
+    // 0.05 us a tile more for a wavefront alone on its SIMD, 200 sequences of 128-4096 at
+    // 40 / 8 heads 100 against 97 us).  A second place for the other page's, so that both
+    // are on their way, was slower: two workgroups a CU instead of three.
     s16x4 v0[8], v1[8];
     wave_lds_fence();
     write_v(0);
     wave_lds_fence();
+    f32x4 sc[2];  // sc[i][r] = S[token 4 q4 + r of page i][g = c]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // The two pages' sums in turn: one alone is a chain of dependent MFMAs.
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc[i] = Elem<T>::mfma16(fp4_unpack8<T>(kw[i][j], ks[i]), qf[j], sc[i]);
+      if (j & 1) __builtin_amdgcn_sched_barrier(0);  // not all conversions at once: registers
+    }
     read_v(v0);
     wave_lds_fence();
     write_v(1);
