@@ -6,7 +6,8 @@
 //   {seq, page_begin, page_end, chunk, n_chunks, part_base, q_row, kv_head}
 // where a segment cut into n_chunks > 1 pieces is split-K: chunk k of it
 // writes partial slot (part_base + k) * Hkv + kv_head.  The merge list is the
-// chunk-0 piece of every split segment, in piece order.
+// chunk-0 piece of every split segment, in piece order.  A third planner, for the
+// MXFP4 decode kernel, makes pieces that four wavefronts share (below).
 //
 // No device code and no HIP calls: these run on the host once per step and
 // only fill caller-provided arrays.

@@ -288,6 +288,25 @@ def test_nan_groups_reach_the_rows_that_see_them(gpu):
     assert torch.equal(nan, expected)
 
 
+@pytest.mark.parametrize("schedule", ["shared", "listed"])
+def test_nan_groups_pass_the_joins(gpu, monkeypatch, schedule):
+    # In one chunk of several: through the joins in LDS and the merge.
+    monkeypatch.setattr(MI355XMXFP4AttentionBackend, "decode_schedule_override", schedule)
+    batch = make_paged_batch(12, [1, 1, 1], [5000, 5000, 90], 0, 16, 8)
+    table = batch.common.block_tables
+    batch.k_cache[table[0, 100], 3, 2, 5] = float("nan")
+    batch.v_cache[table[1, 311], 9, 4, 70] = float("inf")
+    batch.v_cache[table[2, 5], 9, 0, 127] = float("nan")  # the last token
+    out, _, plan, _ = _forward(batch, gpu, BF16, poison=False)
+    assert plan.metadata.num_decode_merges > 0
+    nan = torch.isnan(out.cpu())
+    expected = torch.zeros_like(nan)
+    expected[0, 4:6] = True
+    expected[1, 8:10, 64:96] = True
+    expected[2, 0:2, 96:] = True
+    assert torch.equal(nan, expected)
+
+
 @pytest.mark.parametrize("dtype,hq,hkv", [(BF16, 32, 8), (FP16, 16, 8), (BF16, 12, 4), (FP16, 8, 1), (BF16, 16, 1)])
 def test_prefill(gpu, dtype, hq, hkv):
     q = [1, 37, 130, 64, 2, 300]
