@@ -11,7 +11,7 @@
 //
 // Measured: 56 sequences of 8192-32768 tokens at 64 / 8 heads 246 us a call with its merge
 // (1.38 GB, 5.6 TB/s; a stream of the same pages into LDS without arithmetic reaches
-// 6.1), 64 of 128-2048 at 16 / 8 19.7 us (74 MB, 3.8 TB/s), 8 of 256-1024 9.3 us. The small
+// 6.1), 64 of 128-2048 at 16 / 8 19.2 us (74 MB, 3.9 TB/s), 8 of 256-1024 9.4 us. The small
 // ones are bound by a chain of memory latencies: launch, piece, page table, pages, and
 // 0.8 us a tile of a wavefront alone on its SIMD.
 //

@@ -702,8 +702,8 @@ def test_calls_on_two_streams_at_once(gpu):
     """Two backends' decode and prefill steps side by side on two streams: each as alone."""
     sides = []
     for seed, (hq, hkv) in enumerate(((32, 8), (16, 4))):
-        dec = make_paged_batch(seed, [1] * 40, decode_lengths(seed, 40, 1, 3000), 0, hq, hkv)
-        pre = make_paged_batch(seed, [300, 500], [700, 500], 2, hq, hkv)
+        dec = make_paged_batch(seed, [1] * 12, decode_lengths(seed, 12, 1, 2000), 0, hq, hkv)
+        pre = make_paged_batch(seed, [100, 300], [200, 300], 2, hq, hkv)
         backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, BF16)
         steps = []
         for batch in (dec, pre):
