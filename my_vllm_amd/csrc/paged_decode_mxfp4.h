@@ -199,7 +199,7 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
   V8 qf[4];
   f32x4 o[8];  // o[mt][r] = O^T[d = 16 mt + 4 q4 + r][g = c]
   float m, l;  // reference max (log2 domain) of g = c; this lane's share of the denominator
-  // `valid`: tokens of the tile that count; below 64 on an edge tile.
+  // `valid`: tokens of the tile that count; below 32 on an edge tile.
   auto compute = [&](lds_u8* buf, int valid) __attribute__((always_inline)) {
     const bool edge = valid < kFp4TileTokens;  // wave-uniform
     u32x4 vw[2];  // page i's codes of token lane / 4, group lane % 4
@@ -216,21 +216,25 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
       vw[i] = lds_ld16<u32x4>(buf + kFp4TileV + i * kFp4ScaleOffset + voff);
       vs[i] = buf[kFp4TileVScales + 64 * i + lane];
     }
+    // A branch, not selects (the asm keeps it one).
+    if (edge) {
+      int end = valid;
+      asm volatile("" : "+s"(end));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool live = kPageSize * i + vtok < end;
+        vs[i] = live ? vs[i] : 127u;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) vw[i][u] = live ? vw[i][u] : 0u;
+      }
+    }
     // Rows of page i over the tile's codes, and their transposed reads.  LDS works
     // in order for a wavefront: the reads of codes above come before the first
     // page's writes, its transposed reads before the second page's writes.
     auto write_v = [&](int i) __attribute__((always_inline)) {
-      u32x4 w = vw[i];
-      uint32_t byte = vs[i];
-      if (edge) {
-        const bool live = kPageSize * i + vtok < valid;
-        byte = live ? byte : 127u;
+      const float scale = fp4_scale(vs[i]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) w[u] = live ? w[u] : 0u;
-      }
-      const float scale = fp4_scale(byte);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) lds_st16(buf + (vwrite ^ (16 * u)), fp4_unpack8<T>(w[u], scale));
+      for (int u = 0; u < 4; ++u) lds_st16(buf + (vwrite ^ (16 * u)), fp4_unpack8<T>(vw[i][u], scale));
     };
     // v[mt]: dimension 16 mt + c of tokens 4 q4 .. + 3 of the page.
     auto read_v = [&](s16x4 (&v)[8]) __attribute__((always_inline)) {
@@ -261,11 +265,13 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
     wave_lds_fence();
     read_v(v1);
     if (edge) {
+      int end = valid;
+      asm volatile("" : "+s"(end));
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (kPageSize * i + 4 * q4 + r >= valid) sc[i][r] = -INFINITY;
+          if (kPageSize * i + 4 * q4 + r >= end) sc[i][r] = -INFINITY;
     }
     // P = 2^(S * scale - m), packed, and this lane's sum of it.
     V8 pf;
@@ -314,17 +320,21 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
   auto join_share = [&](float l_tot) __attribute__((always_inline)) {
     // Row c of this wavefront, 16-byte chunk ch at slot ch ^ c: 16 lanes of a
     // write take 16 slots.
+    int row = c, part = q4;
+    asm volatile("" : "+v"(row), "+v"(part));  // addresses made here, not held in registers through the stream
     if (q_lane) {
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) lds_st16(lds + c * 4 * kHeadDim + (((4 * mt + q4) ^ c) << 4), o[mt]);
-      if (q4 == 0) {
-        *(lds_f32*)(lds + kFp4ShareMax + 4 * c) = m;
-        *(lds_f32*)(lds + kFp4ShareSum + 4 * c) = l_tot;
+      for (int mt = 0; mt < 8; ++mt) lds_st16(lds + row * 4 * kHeadDim + (((4 * mt + part) ^ row) << 4), o[mt]);
+      if (part == 0) {
+        *(lds_f32*)(lds + kFp4ShareMax + 4 * row) = m;
+        *(lds_f32*)(lds + kFp4ShareSum + 4 * row) = l_tot;
       }
     }
     __syncthreads();
     lds_u8* const first = group_lds + (slot & ~(kFp4ShareWaves - 1)) * kFp4WaveLdsBytes;
-    for (int i = (slot & (kFp4ShareWaves - 1)) * 64 + lane; i < G * (kHeadDim / 4); i += 64 * kFp4ShareWaves) {
+    int thread = lane;
+    asm volatile("" : "+v"(thread));
+    for (int i = (slot & (kFp4ShareWaves - 1)) * 64 + thread; i < G * (kHeadDim / 4); i += 64 * kFp4ShareWaves) {
       const int g = i >> 5, ch = i & 31;
       float mw[kFp4ShareWaves], top = -INFINITY;
 #pragma unroll
@@ -343,9 +353,9 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
       }
       const float inv = den > 0.f ? 1.0f / den : 0.f;
       if (X[4] > 1) {
-        const int64_t row = ((int64_t)(~X[5] + X[3]) * Hkv + X[7]) * G + g;
-        store16_device_untracked(p.part_o + row * kHeadDim + 4 * ch, __builtin_bit_cast(u32x4, sum * inv));
-        if (ch == 0) store4_device_untracked(&p.part_lse[row], den > 0.f ? m_use + fast_log2(den) : -INFINITY);
+        const int64_t at = ((int64_t)(~X[5] + X[3]) * Hkv + X[7]) * G + g;
+        store16_device_untracked(p.part_o + at * kHeadDim + 4 * ch, __builtin_bit_cast(u32x4, sum * inv));
+        if (ch == 0) store4_device_untracked(&p.part_lse[at], den > 0.f ? m_use + fast_log2(den) : -INFINITY);
         continue;
       }
       V4 y;
@@ -367,10 +377,10 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
     const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
     const int h = X[7];
     if (!q_lane) return;
-    int hc = h * G + c;
-    asm volatile("" : "+v"(hc));  // its address is made here, not held in registers through the stream
+    int hc = h * G + c, part = q4;
+    asm volatile("" : "+v"(hc), "+v"(part));  // as above
     if (X[4] == 1) {
-      T* op = (T*)p.out + (int64_t)X[6] * p.out_tok_stride + (int64_t)hc * p.out_head_stride + 4 * q4;
+      T* op = (T*)p.out + (int64_t)X[6] * p.out_tok_stride + (int64_t)hc * p.out_head_stride + 4 * part;
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) {
         V4 w;
@@ -381,10 +391,10 @@ __device__ void decode_wave_mxfp4(const Fp4DecodeParams& p, int wave, lds_u8* gr
       return;
     }
     const int64_t row = (int64_t)(X[5] + X[3]) * Hkv * G + hc;
-    float* po = p.part_o + row * kHeadDim + 4 * q4;
+    float* po = p.part_o + row * kHeadDim + 4 * part;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) store16_device_untracked(po + 16 * mt, __builtin_bit_cast(u32x4, o[mt] * inv));
-    if (q4 == 0) store4_device_untracked(&p.part_lse[row], l_tot > 0.f ? m + fast_log2(l_tot) : -INFINITY);
+    if (part == 0) store4_device_untracked(&p.part_lse[row], l_tot > 0.f ? m + fast_log2(l_tot) : -INFINITY);
   };
 
   int done = 0;
