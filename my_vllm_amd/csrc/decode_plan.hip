@@ -268,13 +268,13 @@ double longest_queue(const std::vector<Share>& shares, int64_t hkv, int64_t num_
 // tiles or more each, one a wavefront), the cut with the least estimated time, or no
 // plan where page ranges come out below all of them.  The estimates, microseconds, with M
 // the longest queue of a CU and A the mean, in tiles a wavefront, fitted to graphs of calls:
-//   whole  4.2 + 0.87 M    32 / 8 heads, 8 sequences of 1000 10.9, 16 of 2400 21.2; 8 / 1, 250 of 2000-4000 31.8
-//   cut    8.2 + 0.87 M, 1 more above 32 pieces   32 / 8, one of 1000 7.9, 24 of 6000 39.3; 16 / 4, 96 of 8000 89.0
-//   ranges 10 + 0.85 A     64 / 8, 56 of 8192-32768 245, 28 137; 32 / 8, 40 of 12000 107
-// and 1.3 on the last two for the host's second launch (8 of 256-1024 at 16 / 8, whole / cut: 10.5 / 9.3 in a
+//   whole  4.2 + 0.82 M    32 / 8 heads, 8 sequences of 1000 10.3, 16 of 2400 19.8; 8 / 1, 250 of 2000-4000 30.0
+//   cut    8.2 + 0.82 M, 1 more above 32 pieces   32 / 8, one of 1000 7.8, 24 of 6000 38.9; 16 / 4, 96 of 8000 87.9
+//   ranges 10 + 0.83 A     64 / 8, 56 of 8192-32768 245, 28 137; 32 / 8, 24 of 6000 39.8, 40 of 12000 107
+// and 1.3 on the last two for the host's second launch (8 of 256-1024 at 16 / 8, whole / cut: 9.9 / 9.2 in a
 // graph, 9.3 / 11.1 call by call).  Ranges of eight wavefronts a CU against the plan taken: one of 30001 at 32 / 8
-// 17.7 / 16.3, 37 of 300-6000 at 16 / 4 24.2 / 22.4, 64 of 128-2048 at 16 / 8 28.1 / 22.0, 200 of 128-4096 at
-// 40 / 8 114.5 / 96.2, one of 8000 and 40 of 100-300 at 32 / 8 19.9 / 12.9.
+// 17.3 / 15.8, 37 of 300-6000 at 16 / 4 23.9 / 22.1, 64 of 128-2048 at 16 / 8 27.6 / 21.7, 200 of 128-4096 at
+// 40 / 8 114 / 96, one of 8000 and 40 of 100-300 at 32 / 8 19.9 / 12.8.
 int plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq, int64_t first_q_row,
                 int num_kv_heads, int num_cus, int always, int32_t* items, int64_t item_rows, int32_t* wave_extra,
                 int64_t wave_extra_len, int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
@@ -299,7 +299,7 @@ int plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq
   const double mean = tiles * (double)hkv / (double)cus;  // tiles a CU
   const double whole = std::numeric_limits<double>::infinity();
   std::vector<Share> best;
-  double best_us = always ? whole : 11.3 + 0.85 * mean / kShareWaves;
+  double best_us = always ? whole : 11.3 + 0.83 * mean / kShareWaves;
   for (const double target : {whole, mean, mean / 2, mean / 3}) {
     std::vector<Share> shares = cut_shares(block_counts, num_seqs, std::max(target, (double)kShareWaves));
     // Cut, into at most what all CUs hold at once.
@@ -307,7 +307,7 @@ int plan_shared(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq
     if (target != whole && (!is_cut || (int64_t)shares.size() * hkv > at_once)) continue;
     int32_t most_pieces = 1;
     for (const Share& x : shares) most_pieces = std::max(most_pieces, x.of);
-    const double us = (is_cut ? 9.5 : 4.2) + (most_pieces > 32 ? 1 : 0) + 0.87 * longest_queue(shares, hkv, cus);
+    const double us = (is_cut ? 9.5 : 4.2) + (most_pieces > 32 ? 1 : 0) + 0.82 * longest_queue(shares, hkv, cus);
     if (us >= best_us) continue;
     best_us = us;
     best = std::move(shares);

@@ -11,9 +11,9 @@
 //
 // Measured: 56 sequences of 8192-32768 tokens at 64 / 8 heads 246 us a call with its merge
 // (1.38 GB, 5.6 TB/s; a stream of the same pages into LDS without arithmetic reaches
-// 6.1), 64 of 128-2048 at 16 / 8 19.2 us (74 MB, 3.9 TB/s), 8 of 256-1024 9.4 us. The small
-// ones are bound by a chain of memory latencies: launch, piece, page table, pages, and
-// 0.8 us a tile of a wavefront alone on its SIMD.
+// 6.1), 64 of 128-2048 at 16 / 8 18.6 us (74 MB, 4.0 TB/s), 8 of 256-1024 9.1 us.  The small
+// ones are bound by a chain of latencies: launch, piece, page table, pages, and 0.75 us a
+// tile of a wavefront alone on its SIMD (155 vector instructions, V through LDS).
 //
 //  * K: a lane reads the 16 bytes of one token's 32-element group, which is
 //    also what one scale covers, and converts them to the query's type with
