@@ -22,6 +22,7 @@ backend-owned output buffer:
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from types import MappingProxyType
 from typing import Any
@@ -560,6 +561,8 @@ class MI355XAttentionBackendMixin:
         self._route_counts = {route.value: 0 for route in self.route_type}
         self._output_buffer: torch.Tensor | None = None
         self._workspace: torch.Tensor | None = None
+        # The decode workspace of a captured step: its capture and stream, and it.
+        self._captured_workspace: tuple[tuple, torch.Tensor] | None = None
         self._prefill_workspace: torch.Tensor | None = None
         # The metadata whose device tile plan the prefill workspace holds:
         # the first prefill launch of a step plans, the other layers reuse it.
@@ -861,12 +864,28 @@ class MI355XAttentionBackendMixin:
         plan = self.plan_type(batch_type, route, common, metadata)
         self._prefill_planned_for = None  # a new step plans its prefill tiles again
         self._captured_plan = None
+        self._captured_workspace = None
         self._planned_route = route.value
         self._route_counts[route.value] += 1
         return plan
 
     # ---- buffers ---------------------------------------------------------------
+    def _capture_of(self, device: torch.device) -> tuple | None:
+        """(number of the graph capture, stream) that torch's current stream of
+        ``device`` is in, or None."""
+        if device.type != "cuda":
+            return None
+        index = torch.cuda.current_device() if device.index is None else device.index
+        with torch.cuda.device(index) if index != torch.cuda.current_device() else nullcontext():
+            if not torch.cuda.is_current_stream_capturing():
+                return None
+        return _native.host_ops().capture_id(index), _native.stream_handle(device)
+
     def _get_reusable_attention_output(self, q: torch.Tensor) -> torch.Tensor:
+        # A graph writes its outputs at every replay: they come from its own pool,
+        # as an eager step may replace the buffer below at any time.
+        if self._capture_of(q.device) is not None:
+            return torch.empty_like(q)
         required = q.size(0)
         buffer = self._output_buffer
         if (
@@ -926,8 +945,22 @@ class MI355XAttentionBackendMixin:
             self._captured_plan = (key, metadata, workspace)
 
     def _get_workspace(self, nbytes: int, device: torch.device) -> torch.Tensor | None:
+        """The decode workspace of the launch that follows.
+
+        A graph has one of its own, from its pool, for the layers captured on one
+        stream: an eager step that needs more partials replaces the backend's, and
+        replays of two graphs may overlap.  Its counters are cleared inside the
+        graph, once a replay (2 us)."""
         if nbytes <= 0:
             return None
+        capture = self._capture_of(device)
+        if capture is not None:
+            held = self._captured_workspace
+            if held is None or not capture[0] or held[0] != capture or held[1].numel() < nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                ws[:ops.decode_workspace_bytes(0, 1, 1)].zero_()
+                self._captured_workspace = held = (capture, ws)
+            return held[1]
         ws = self._workspace
         if ws is None or ws.numel() < nbytes or ws.device != device:
             # Zeroed once: the kernels leave their counters at zero on exit.
@@ -1108,7 +1141,8 @@ class MI355XAttentionBackendMixin:
     def fused_store_error(self) -> bool:
         """Whether a folded decode store since the last call met a row whose
         slot was not its sequence's last position (written after the
-        attention; reads the device and clears the word)."""
+        attention; reads the device and clears the word).  A captured step's
+        word lies in its graph's own workspace and is not read here."""
         if self._workspace is None:
             return False
         return ops.decode_store_error(self._workspace)
