@@ -102,6 +102,9 @@ class MI355XAttentionMetadata:
     mixed_prefill_max_tiles: int = 0
     mixed_prefill_workgroups: int = 0
     mixed_split_reason: str | None = None
+    # Whether the decode plan is one for MXFP4 caches: longer pieces than the
+    # 16-bit kernels take, or pieces that four wavefronts share.
+    mxfp4: bool = False
 
     @property
     def is_cacheless(self) -> bool:
@@ -448,6 +451,7 @@ class MI355XFullDecodeGraphState:
     output: torch.Tensor
     plan: Any = None
     staging_turn: int = 0
+    mxfp4: bool = False  # as the metadata's
 
     def views(self):
         """(counts, items, wave_extra, merges) views of the device plan buffer."""
@@ -527,8 +531,9 @@ class MI355XAttentionBackendMixin:
     # after each fused launch (a device read) and raise if a row's slot was
     # not its sequence's last position.
     check_fused_store: bool = False
-    # Longest piece of a decode plan with piece lists.
+    # Longest piece of a decode plan with piece lists, and whether the caches are MXFP4.
     _max_piece_pages = ops.MAX_CHUNK_PAGES
+    _mxfp4 = False
 
     def __init__(
         self,
@@ -835,6 +840,7 @@ class MI355XAttentionBackendMixin:
             mixed_prefill_max_tiles=mixed_prefill_max_tiles,
             mixed_prefill_workgroups=mixed_prefill_workgroups,
             mixed_split_reason=split_reason if mixed and not one_launch else None,
+            mxfp4=self._mxfp4,
         )
 
     def build_plan(self, common, metadata: MI355XAttentionMetadata | None = None):
@@ -1086,6 +1092,8 @@ class MI355XAttentionBackendMixin:
         common = plan.common
         if q.size(0) != common.num_query_tokens:
             raise ValueError("query token count does not match the attention plan")
+        if metadata.mxfp4 and not self._mxfp4 and common.num_decode_seqs:
+            raise ValueError("the plan's decode pieces were made for an MXFP4 cache")
 
         output = self._get_reusable_attention_output(q)
         if route is Route.DECODE:
@@ -1183,6 +1191,7 @@ class MI355XAttentionBackendMixin:
             staging_ready=[None, None],
             workspace=torch.zeros(ws_bytes, dtype=torch.uint8, device=graph_device),
             output=torch.empty(batch_size, self.num_q_heads, self.head_dim, dtype=self.dtype, device=graph_device),
+            mxfp4=self._mxfp4,
             **caps,
         )
 
@@ -1193,6 +1202,8 @@ class MI355XAttentionBackendMixin:
             return False
         metadata = plan.metadata
         if not isinstance(metadata, MI355XAttentionMetadata) or metadata.is_cacheless:
+            return False
+        if state.mxfp4 != self._mxfp4 or (metadata.mxfp4 and not self._mxfp4):
             return False
         common = plan.common
         if common.num_prefill_seqs != 0 or common.num_prefill_tokens != 0:
@@ -1259,6 +1270,8 @@ class MI355XAttentionBackendMixin:
             raise TypeError("invalid MI355X decode graph state")
         if state.plan is None:
             raise RuntimeError("decode graph state must be planned before activation")
+        if state.mxfp4 != self._mxfp4:
+            raise ValueError("the decode graph state was made for another kind of cache")
         if self._active_graph_state is not None:
             raise RuntimeError("a decode graph state is already active")
         self._active_graph_state = state
@@ -1432,6 +1445,7 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
 
     backend_name = "mi355x_mxfp4"
     _max_piece_pages = ops.ANY_PIECE_PAGES
+    _mxfp4 = True
 
     def _store_rows(self, k, v, k_cache, v_cache, slot_mapping) -> None:
         ops.store_kvcache_mxfp4(k, v, k_cache, v_cache, slot_mapping)

@@ -1,0 +1,72 @@
+"""CPU: decode plans and graph states of MXFP4 and of 16-bit caches are kept apart."""
+
+import types
+
+import pytest
+import torch
+
+from my_vllm_amd import ops
+from my_vllm_amd.attention_backend import (
+    MI355XAttentionBackend,
+    MI355XFullDecodeGraphState,
+    MI355XMXFP4AttentionBackend,
+)
+from workloads import make_paged_batch
+
+
+class _Host16(MI355XAttentionBackend):
+    require_device_metadata = False
+
+
+class _HostFp4(MI355XMXFP4AttentionBackend):
+    require_device_metadata = False
+
+
+def _backends(monkeypatch, mode=None):
+    """A backend of either kind whose launches are only recorded."""
+    calls = []
+    for cls in (_Host16, _HostFp4):
+        monkeypatch.setattr(cls, "_validate_inputs", lambda self, q, k, v: None)
+        monkeypatch.setattr(cls, "_get_workspace", lambda self, nbytes, device: None)
+        monkeypatch.setattr(cls, "_run_prefill", lambda self, *a: calls.append("prefill"))
+        monkeypatch.setattr(cls, "_run_decode", lambda self, *a: calls.append("decode"))
+        monkeypatch.setattr(cls, "_run_mixed", lambda self, *a: calls.append("mixed"))
+    return _Host16(16, 4, 128, 16, torch.bfloat16, mode), _HostFp4(16, 4, 128, 16, torch.bfloat16, mode), calls
+
+
+@pytest.mark.parametrize("prefills,runs", [(0, ["decode"]), (1, ["prefill", "decode"]), (3, ["prefill"])])
+def test_a_decode_plan_for_mxfp4_caches_runs_over_those_only(monkeypatch, prefills, runs):
+    wide, fp4, calls = _backends(monkeypatch, "split")
+    q_lens = [5] * prefills + [1] * (3 - prefills)
+    common = make_paged_batch(1, q_lens, [40, 90, 5000], prefills, 16, 4).common
+    plan = fp4.build_plan(common)
+    q, cache = torch.zeros(sum(q_lens), 16, 128, dtype=torch.bfloat16), torch.zeros(1)
+    fp4.forward(q, None, None, cache, cache, plan)
+    assert calls == runs
+    if prefills == 3:  # the tile plans are the same
+        wide.forward(q, None, None, cache, cache, plan)
+        assert calls == 2 * runs
+        return
+    with pytest.raises(ValueError, match="MXFP4"):
+        wide.forward(q, None, None, cache, cache, plan)
+    if prefills == 0:  # nor with the store folded in
+        kv = torch.zeros(3, 4, 128, dtype=torch.bfloat16)
+        with pytest.raises(ValueError, match="MXFP4"):
+            wide.forward_with_kv_store(q, kv, kv, cache, cache, common.slot_mapping, plan)
+    assert calls == runs
+    wide.forward(q, None, None, cache, cache, wide.build_plan(common))
+    assert calls == 2 * runs
+
+
+def _state(mxfp4):
+    names = [f for f in MI355XFullDecodeGraphState.__dataclass_fields__ if f not in ("plan", "staging_turn", "mxfp4")]
+    return MI355XFullDecodeGraphState(**dict.fromkeys(names), plan=types.SimpleNamespace(), mxfp4=mxfp4)
+
+
+def test_graph_states_belong_to_one_kind_of_cache(monkeypatch):
+    wide, fp4, _ = _backends(monkeypatch)
+    for own, other, mxfp4 in ((wide, fp4, False), (fp4, wide, True)):
+        with pytest.raises(ValueError, match="another kind of cache"):
+            other.activate_full_decode_graph(_state(mxfp4))
+        own.activate_full_decode_graph(_state(mxfp4))
+        own.deactivate_full_decode_graph()
