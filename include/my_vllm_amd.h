@@ -201,8 +201,7 @@ int mva_paged_decode(const void* q, int64_t q_token_stride, int64_t q_head_strid
  * G = min(num_groups, total pages) near-equal ranges (range g = pages
  * [g*T/G, (g+1)*T/G)); wavefront g*num_kv_heads + h streams KV head h of
  * range g, one piece per sequence the range touches, cut further to at most
- * max_piece_pages (1 .. 128, or INT_MAX for mva_paged_decode_mxfp4: no
- * further cut).  wave_extra gets G*num_kv_heads + 1 entries
+ * max_piece_pages (1 .. 128).  wave_extra gets G*num_kv_heads + 1 entries
  * (the mva_paged_decode argument).  item_rows must be at least
  * mva_decode_plan_listed_rows(...), an upper bound on the rows written.
  */
@@ -522,8 +521,20 @@ int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stri
                       int head_dim, int dtype, void* stream);
 
 /*
- * Host planner of mva_paged_decode_mxfp4 besides mva_decode_plan_listed: pieces
- * that four wavefronts share, whole segments (sequence, KV head) or cuts of
+ * Host planners of mva_paged_decode_mxfp4 (besides mva_decode_plan_listed).
+ * Their plans are for it alone: no other decode takes pieces beyond 128 pages,
+ * or shared ones.
+ *
+ * Page ranges as mva_decode_plan_listed's, not cut further.  item_rows must be
+ * at least (num_seqs + num_groups) * num_kv_heads.
+ */
+int mva_decode_plan_listed_mxfp4(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
+                                 int64_t first_q_row, int num_kv_heads, int num_groups, int32_t* items,
+                                 int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len, int32_t* merges,
+                                 int64_t merge_rows, int64_t* out_counts);
+
+/*
+ * Pieces that four wavefronts share, whole segments (sequence, KV head) or cuts of
  * them, in an order made for num_cus CUs.  Unless always is nonzero it plans
  * only where that is expected to be faster than page ranges; otherwise, and for no
  * sequences, the counts are 0.  With S = max(num_seqs * num_kv_heads, 3 * num_cus),

@@ -161,6 +161,13 @@ _SIGNATURES = {
         ],
     ),
     "mva_decode_plan_listed_rows": (_i64, [_i64, _i64, _i32, _i32, _i32]),
+    "mva_decode_plan_listed_mxfp4": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64, _i64, _i32, _i32,  # block_counts, seqs, first_seq, first_q_row, heads, groups
+            _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,  # items, wave_extra, merges, lengths, counts
+        ],
+    ),
     "mva_decode_plan_shared": (
         _i32,
         [
@@ -252,7 +259,7 @@ _SIGNATURES = {
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 # The C ABI revision these signatures describe (mva_abi_version()).
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -290,25 +290,45 @@ def plan_decode_listed(
     :func:`ops.decode_merge_list` would give it), from the library's native
     planner ``mva_decode_plan_listed``."""
     counts = _plan_counts(block_counts)
-    if max_piece_pages != ops.ANY_PIECE_PAGES and not 1 <= max_piece_pages <= ops.MAX_CHUNK_PAGES:
-        raise ValueError("piece length must be in [1, 128] pages, or ANY_PIECE_PAGES")
+    if not 1 <= max_piece_pages <= ops.MAX_CHUNK_PAGES:
+        raise ValueError("piece length must be in [1, 128] pages")
+    rows = _native.query("mva_decode_plan_listed_rows", counts.size, int(counts.sum()), int(num_kv_heads),
+                         max(1, int(num_groups)), int(max_piece_pages))
+    return _plan_listed("mva_decode_plan_listed", counts, first_seq, first_q_row, num_kv_heads, num_groups, int(rows),
+                        int(max_piece_pages))
+
+
+def plan_decode_listed_mxfp4(
+    block_counts: np.ndarray | tuple[int, ...],
+    first_seq: int,
+    first_q_row: int,
+    num_kv_heads: int,
+    num_groups: int,
+) -> tuple[np.ndarray, np.ndarray, int, int, np.ndarray]:
+    """:func:`plan_decode_listed` for a decode launch over MXFP4 caches, which alone
+    takes it: pieces are as long as their ranges (``mva_decode_plan_listed_mxfp4``)."""
+    counts = _plan_counts(block_counts)
+    rows = (counts.size + max(1, int(num_groups))) * int(num_kv_heads)
+    return _plan_listed("mva_decode_plan_listed_mxfp4", counts, first_seq, first_q_row, num_kv_heads, num_groups, rows)
+
+
+def _plan_listed(planner: str, counts: np.ndarray, first_seq: int, first_q_row: int, num_kv_heads: int,
+                 num_groups: int, rows: int, *piece_pages: int):
     n = counts.size
     if n == 0:
         empty = np.zeros((0, ops.DECODE_ITEM_INTS), np.int32)
         return empty, np.zeros(1, np.int32), 0, 0, empty
     hkv = int(num_kv_heads)
-    total = int(counts.sum())
     num_groups = max(1, int(num_groups))
-    rows = int(_native.query("mva_decode_plan_listed_rows", n, total, hkv, num_groups, int(max_piece_pages)))
     if rows < 0:
         raise ValueError("invalid decode plan arguments")
     items = np.empty((rows, ops.DECODE_ITEM_INTS), np.int32)
     merges = np.empty((n * hkv, ops.DECODE_ITEM_INTS), np.int32)
-    wave_extra = np.empty(min(num_groups, total) * hkv + 1, np.int32)
+    wave_extra = np.empty(min(num_groups, int(counts.sum())) * hkv + 1, np.int32)
     out = np.zeros(4, np.int64)
-    _native.call("mva_decode_plan_listed", counts.ctypes.data, n, int(first_seq), int(first_q_row), hkv,
-                 num_groups, int(max_piece_pages), items.ctypes.data, rows, wave_extra.ctypes.data,
-                 wave_extra.size, merges.ctypes.data, merges.shape[0], out.ctypes.data)
+    _native.call(planner, counts.ctypes.data, n, int(first_seq), int(first_q_row), hkv, num_groups, *piece_pages,
+                 items.ctypes.data, rows, wave_extra.ctypes.data, wave_extra.size, merges.ctypes.data,
+                 merges.shape[0], out.ctypes.data)
     num_items, waves, slots, num_merges = (int(x) for x in out)
     return items[:num_items], wave_extra, waves, slots, merges[:num_merges]
 
@@ -324,7 +344,7 @@ def plan_decode_shared(block_counts: np.ndarray | tuple[int, ...], first_seq: in
     """(items, wave_extra, waves, partial slots, merges) of an MXFP4 decode launch in
     which four wavefronts share each piece and join in LDS, from the library's native
     planner ``mva_decode_plan_shared``.  Unless ``always``, the plan is empty where
-    page ranges (:func:`plan_decode_listed`) are expected to be faster."""
+    page ranges (:func:`plan_decode_listed_mxfp4`) are expected to be faster."""
     counts = _plan_counts(block_counts)
     hkv, num_cus = int(num_kv_heads), int(num_cus)
     rows = shared_decode_capacity(counts.size, hkv, num_cus)
@@ -531,8 +551,7 @@ class MI355XAttentionBackendMixin:
     # after each fused launch (a device read) and raise if a row's slot was
     # not its sequence's last position.
     check_fused_store: bool = False
-    # Longest piece of a decode plan with piece lists, and whether the caches are MXFP4.
-    _max_piece_pages = ops.MAX_CHUNK_PAGES
+    # Whether the caches are MXFP4.
     _mxfp4 = False
 
     def __init__(
@@ -680,8 +699,10 @@ class MI355XAttentionBackendMixin:
         """(items, wave_extra, waves, partial slots, merges, page ranges, wavefronts
         per workgroup) of a decode launch with piece lists."""
         groups, waves_per_group = self._decode_ranges(decode_counts, device)
-        return (*plan_decode_listed(decode_counts, first_seq, first_q_row, self.num_kv_heads, groups,
-                                    self._max_piece_pages), groups, waves_per_group)
+        return (*self._plan_ranges(decode_counts, first_seq, first_q_row, groups), groups, waves_per_group)
+
+    def _plan_ranges(self, counts: np.ndarray, first_seq: int, first_q_row: int, groups: int):
+        return plan_decode_listed(counts, first_seq, first_q_row, self.num_kv_heads, groups)
 
     def _decode_graph_capacities(self, batch_size: int, total_pages: int, device: torch.device):
         """(page ranges, wavefronts per workgroup, capacities) of a captured
@@ -1243,8 +1264,7 @@ class MI355XAttentionBackendMixin:
         # KV heads): replays run what an eager launch runs.
         if host is None or host[3] > state.groups:
             counts = np.diff(np.asarray(metadata.kv_indptr, dtype=np.int64))
-            items, wave_extra, _, _, merges = plan_decode_listed(counts, 0, 0, self.num_kv_heads, state.groups,
-                                                                 self._max_piece_pages)
+            items, wave_extra, _, _, merges = self._plan_ranges(counts, 0, 0, state.groups)
         else:
             items, wave_extra, merges, _ = host
         # Staging buffers alternate: the one refilled now was last copied two
@@ -1444,7 +1464,6 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
     those before it whose tile of queries and keys holds both."""
 
     backend_name = "mi355x_mxfp4"
-    _max_piece_pages = ops.ANY_PIECE_PAGES
     _mxfp4 = True
 
     def _store_rows(self, k, v, k_cache, v_cache, slot_mapping) -> None:
@@ -1467,8 +1486,10 @@ class MI355XMXFP4AttentionBackendMixin(MI355XAttentionBackendMixin):
                 return (*plan, 0, ops.MXFP4_SHARE_WAVES)
         groups, per_group = mxfp4_decode_ranges(int(decode_counts.sum()), self.num_kv_heads, device,
                                                 self.decode_waves_override)
-        return (*plan_decode_listed(decode_counts, first_seq, first_q_row, self.num_kv_heads, groups,
-                                    self._max_piece_pages), groups, per_group)
+        return (*self._plan_ranges(decode_counts, first_seq, first_q_row, groups), groups, per_group)
+
+    def _plan_ranges(self, counts: np.ndarray, first_seq: int, first_q_row: int, groups: int):
+        return plan_decode_listed_mxfp4(counts, first_seq, first_q_row, self.num_kv_heads, groups)
 
     def _decode_graph_capacities(self, batch_size: int, total_pages: int, device: torch.device):
         groups, _ = mxfp4_decode_ranges(total_pages, self.num_kv_heads, device, self.decode_waves_override)
@@ -1591,5 +1612,6 @@ __all__ = [
     "plan_decode_claims",
     "plan_decode_shared",
     "plan_decode_listed",
+    "plan_decode_listed_mxfp4",
     "resident_decode_waves",
 ]

@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kItemInts = 8;
 constexpr int kMaxPiecePages = 128;  // the decode kernel's longest piece
-constexpr int kAnyPiecePages = 0x7fffffff;  // piece lists not cut further: the MXFP4 decode kernel takes any length
+constexpr int kAnyPiecePages = 0x7fffffff;  // not cut further: the MXFP4 decode kernel takes any length
 
 struct Piece {
   int64_t begin, end;  // absolute page offsets in the batch
@@ -84,7 +84,7 @@ int64_t collect_merges(const int32_t* items, int64_t num_items, int32_t* merges,
 extern "C" int64_t mva_decode_plan_listed_rows(int64_t num_seqs, int64_t total_pages, int num_kv_heads,
                                                int num_groups, int max_piece_pages) {
   if (num_seqs < 0 || total_pages < 0 || num_kv_heads <= 0 || num_groups <= 0 || max_piece_pages < 1 ||
-      (max_piece_pages > mva::kMaxPiecePages && max_piece_pages != mva::kAnyPiecePages))
+      max_piece_pages > mva::kMaxPiecePages)
     return -1;
   if (num_seqs == 0) return 0;
   const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(num_groups, total_pages));
@@ -94,17 +94,17 @@ extern "C" int64_t mva_decode_plan_listed_rows(int64_t num_seqs, int64_t total_p
   return (groups + num_seqs + total_pages / max_piece_pages) * num_kv_heads;
 }
 
-extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
-                                      int64_t first_q_row, int num_kv_heads, int num_groups, int max_piece_pages,
-                                      int32_t* items, int64_t item_rows, int32_t* wave_extra,
-                                      int64_t wave_extra_len, int32_t* merges, int64_t merge_rows,
-                                      int64_t* out_counts) {
-  using namespace mva;
+namespace mva {
+namespace {
+
+// Page ranges with pieces of at most max_piece_pages.
+int plan_listed(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq, int64_t first_q_row,
+                int num_kv_heads, int num_groups, int max_piece_pages, int32_t* items, int64_t item_rows,
+                int32_t* wave_extra, int64_t wave_extra_len, int32_t* merges, int64_t merge_rows,
+                int64_t* out_counts) {
   if (num_seqs < 0 || num_kv_heads <= 0 || num_groups <= 0 || out_counts == nullptr || wave_extra == nullptr ||
       wave_extra_len < 1)
     return set_error("decode plan: invalid arguments");
-  if (max_piece_pages < 1 || (max_piece_pages > kMaxPiecePages && max_piece_pages != kAnyPiecePages))
-    return set_error("decode plan: piece length must be in [1, 128] pages, or unlimited (INT_MAX)");
   for (int i = 0; i < 4; ++i) out_counts[i] = 0;
   if (num_seqs == 0) {
     wave_extra[0] = 0;
@@ -188,6 +188,29 @@ extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_s
   out_counts[2] = slots;
   out_counts[3] = num_merges;
   return 0;
+}
+
+}  // namespace
+}  // namespace mva
+
+extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
+                                      int64_t first_q_row, int num_kv_heads, int num_groups, int max_piece_pages,
+                                      int32_t* items, int64_t item_rows, int32_t* wave_extra,
+                                      int64_t wave_extra_len, int32_t* merges, int64_t merge_rows,
+                                      int64_t* out_counts) {
+  if (max_piece_pages < 1 || max_piece_pages > mva::kMaxPiecePages)
+    return mva::set_error("decode plan: piece length must be in [1, 128] pages");
+  return mva::plan_listed(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_groups, max_piece_pages,
+                          items, item_rows, wave_extra, wave_extra_len, merges, merge_rows, out_counts);
+}
+
+extern "C" int mva_decode_plan_listed_mxfp4(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
+                                            int64_t first_q_row, int num_kv_heads, int num_groups, int32_t* items,
+                                            int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
+                                            int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
+  return mva::plan_listed(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_groups,
+                          mva::kAnyPiecePages, items, item_rows, wave_extra, wave_extra_len, merges, merge_rows,
+                          out_counts);
 }
 
 namespace mva {

@@ -25,9 +25,6 @@ PAGE_SIZE = 16
 DECODE_ITEM_INTS = 8
 # Longest piece one decode work item may cover (kMaxChunkPages).
 MAX_CHUNK_PAGES = 128
-# Piece length of a plan whose pieces are not cut any further (kAnyPiecePages):
-# paged_decode_mxfp4 takes pieces of any length, paged_decode of MAX_CHUNK_PAGES.
-ANY_PIECE_PAGES = 0x7fffffff
 # Wavefronts that share a piece of an MXFP4 decode plan (plan_decode_shared).
 MXFP4_SHARE_WAVES = 4
 # Query rows per prefill workgroup (kPrefillRows): G heads x 128 // G tokens.
@@ -1073,7 +1070,7 @@ def paged_decode_mxfp4(
 ) -> None:
     """:func:`paged_decode` over MXFP4 caches, with piece lists (``wave_extra``),
     pieces of any length and 4 or 12 wavefronts to a workgroup.  The pieces are
-    those of ``mva_decode_plan_listed`` or of ``mva_decode_plan_shared``.
+    those of ``mva_decode_plan_listed_mxfp4`` or of ``mva_decode_plan_shared``.
 
     With ``counts`` (int32 ``[3]`` on the device) it is the fixed-shape launch
     of :func:`paged_decode_graph`: ``counts`` holds this step's ``{num_items,

@@ -2,15 +2,20 @@
 
 import types
 
+import numpy as np
 import pytest
 import torch
 
-from my_vllm_amd import ops
+from my_vllm_amd import _native
 from my_vllm_amd.attention_backend import (
     MI355XAttentionBackend,
     MI355XFullDecodeGraphState,
     MI355XMXFP4AttentionBackend,
+    plan_decode_listed,
+    plan_decode_listed_mxfp4,
 )
+from tests import _decode_plan_spec
+from tests._decode_plan_spec import listed_plan_spec, merge_list_spec
 from workloads import make_paged_batch
 
 
@@ -70,3 +75,30 @@ def test_graph_states_belong_to_one_kind_of_cache(monkeypatch):
             other.activate_full_decode_graph(_state(mxfp4))
         own.activate_full_decode_graph(_state(mxfp4))
         own.deactivate_full_decode_graph()
+
+
+def test_only_the_mxfp4_planner_leaves_pieces_longer_than_128_pages():
+    counts = np.array([300, 2, 900], np.int64)
+    unlimited = 2 ** 31 - 1
+    with pytest.raises(ValueError, match=r"\[1, 128\]"):
+        plan_decode_listed(counts, 0, 0, 8, 2, unlimited)
+    assert _native.query("mva_decode_plan_listed_rows", 3, 1202, 8, 2, unlimited) == -1
+    items, extra, out = np.zeros((100, 8), np.int32), np.zeros(100, np.int32), np.zeros(4, np.int64)
+    with pytest.raises(RuntimeError, match=r"\[1, 128\]"):
+        _native.call("mva_decode_plan_listed", counts.ctypes.data, 3, 0, 0, 8, 2, unlimited, items.ctypes.data, 100,
+                     extra.ctypes.data, 100, 0, 0, out.ctypes.data)
+    assert (plan_decode_listed(counts, 0, 0, 8, 2)[0][:, 2] - plan_decode_listed(counts, 0, 0, 8, 2)[0][:, 1]).max() <= 128
+
+
+@pytest.mark.parametrize("counts,hkv,groups", [([300, 2, 900], 8, 2), ([1], 1, 5), ([7, 1, 1, 40], 3, 4),
+                                               ([5] * 50, 2, 1000), ([100000, 3], 8, 384)])
+def test_mxfp4_page_ranges(monkeypatch, counts, hkv, groups):
+    monkeypatch.setattr(_decode_plan_spec, "MAX_CHUNK_PAGES", 1 << 30)
+    counts = np.array(counts, np.int64)
+    items, extra, waves, slots, merges = plan_decode_listed_mxfp4(counts, 4, 9, hkv, groups)
+    want = listed_plan_spec(counts, 4, 9, hkv, groups, int(counts.sum()))
+    assert np.array_equal(items, want[0]) and np.array_equal(extra, want[1]) and (waves, slots) == want[2:4]
+    assert np.array_equal(merges, merge_list_spec(want[0]))
+    assert len(items) <= (len(counts) + groups) * hkv
+    empty = plan_decode_listed_mxfp4(np.zeros(0, np.int64), 0, 0, hkv, groups)
+    assert empty[0].shape == (0, 8) and empty[1].tolist() == [0] and empty[2:4] == (0, 0)
