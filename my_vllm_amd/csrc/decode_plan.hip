@@ -25,6 +25,17 @@ namespace mva {
 namespace {
 
 constexpr int kItemInts = 8;
+
+// `plan`'s status; a C++ exception (no memory) becomes an error of the C ABI.
+template <typename F>
+int guarded(F plan) {
+  try {
+    return plan();
+  } catch (const std::exception&) {
+    return set_error("decode plan: out of memory");
+  }
+}
+
 constexpr int kMaxPiecePages = 128;  // the decode kernel's longest piece
 constexpr int kAnyPiecePages = 0x7fffffff;  // not cut further: the MXFP4 decode kernel takes any length
 
@@ -200,17 +211,21 @@ extern "C" int mva_decode_plan_listed(const int64_t* block_counts, int64_t num_s
                                       int64_t* out_counts) {
   if (max_piece_pages < 1 || max_piece_pages > mva::kMaxPiecePages)
     return mva::set_error("decode plan: piece length must be in [1, 128] pages");
-  return mva::plan_listed(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_groups, max_piece_pages,
-                          items, item_rows, wave_extra, wave_extra_len, merges, merge_rows, out_counts);
+  return mva::guarded([&] {
+    return mva::plan_listed(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_groups, max_piece_pages,
+                            items, item_rows, wave_extra, wave_extra_len, merges, merge_rows, out_counts);
+  });
 }
 
 extern "C" int mva_decode_plan_listed_mxfp4(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
                                             int64_t first_q_row, int num_kv_heads, int num_groups, int32_t* items,
                                             int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
                                             int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
-  return mva::plan_listed(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_groups,
-                          mva::kAnyPiecePages, items, item_rows, wave_extra, wave_extra_len, merges, merge_rows,
-                          out_counts);
+  return mva::guarded([&] {
+    return mva::plan_listed(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_groups,
+                            mva::kAnyPiecePages, items, item_rows, wave_extra, wave_extra_len, merges, merge_rows,
+                            out_counts);
+  });
 }
 
 namespace mva {
@@ -379,12 +394,10 @@ extern "C" int mva_decode_plan_shared(const int64_t* block_counts, int64_t num_s
                                       int64_t first_q_row, int num_kv_heads, int num_cus, int always, int32_t* items,
                                       int64_t item_rows, int32_t* wave_extra, int64_t wave_extra_len,
                                       int32_t* merges, int64_t merge_rows, int64_t* out_counts) {
-  try {
+  return mva::guarded([&] {
     return mva::plan_shared(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_cus, always, items,
                             item_rows, wave_extra, wave_extra_len, merges, merge_rows, out_counts);
-  } catch (const std::exception&) {
-    return mva::set_error("decode plan: out of memory");
-  }
+  });
 }
 
 extern "C" int64_t mva_decode_plan_claims_rows(int64_t num_seqs, int64_t total_pages, int num_kv_heads,
@@ -394,12 +407,13 @@ extern "C" int64_t mva_decode_plan_claims_rows(int64_t num_seqs, int64_t total_p
   return (total_pages / min_piece_pages + num_seqs) * num_kv_heads;
 }
 
-extern "C" int mva_decode_plan_claims(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
-                                      int64_t first_q_row, int num_kv_heads, int64_t num_waves,
-                                      double pieces_per_wave, int min_piece_pages, int max_piece_pages,
-                                      int32_t* items, int64_t item_rows, int32_t* merges, int64_t merge_rows,
-                                      int64_t* out_counts) {
-  using namespace mva;
+namespace mva {
+namespace {
+
+int plan_claims(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq, int64_t first_q_row,
+                int num_kv_heads, int64_t num_waves, double pieces_per_wave, int min_piece_pages,
+                int max_piece_pages, int32_t* items, int64_t item_rows, int32_t* merges, int64_t merge_rows,
+                int64_t* out_counts) {
   if (num_seqs < 0 || num_kv_heads <= 0 || out_counts == nullptr)
     return set_error("decode plan: invalid arguments");
   if (!(1 <= min_piece_pages && min_piece_pages <= max_piece_pages && max_piece_pages <= kMaxPiecePages))
@@ -464,4 +478,18 @@ extern "C" int mva_decode_plan_claims(const int64_t* block_counts, int64_t num_s
   out_counts[2] = slots;
   out_counts[3] = num_merges;
   return 0;
+}
+
+}  // namespace
+}  // namespace mva
+
+extern "C" int mva_decode_plan_claims(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
+                                      int64_t first_q_row, int num_kv_heads, int64_t num_waves,
+                                      double pieces_per_wave, int min_piece_pages, int max_piece_pages,
+                                      int32_t* items, int64_t item_rows, int32_t* merges, int64_t merge_rows,
+                                      int64_t* out_counts) {
+  return mva::guarded([&] {
+    return mva::plan_claims(block_counts, num_seqs, first_seq, first_q_row, num_kv_heads, num_waves, pieces_per_wave,
+                            min_piece_pages, max_piece_pages, items, item_rows, merges, merge_rows, out_counts);
+  });
 }
