@@ -492,7 +492,7 @@ int mva_paged_mixed_run(const void* q, int64_t q_token_stride, int64_t q_head_st
  * 64*t (element 2i in the low four bits of byte i), then its four E8M0 scales
  * (2^(byte - 127), 255: NaN), one for 32 elements, at byte 1024 + 4*t.  Blocks
  * lie page_stride_bytes / head_stride_bytes apart (multiples of 16, K and V
- * alike).  Reduced-precision caches have no counterpart in the reference.
+ * alike) and do not overlap.  Reduced-precision caches have no counterpart in the reference.
  */
 
 /*

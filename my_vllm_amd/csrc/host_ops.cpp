@@ -435,8 +435,14 @@ bool fp4_caches(const Tensor* kc, const Tensor* vc, c10::Device device) {
     return false;
   for (const Tensor* c : {kc, vc})
     if (c->scalar_type() != at::kByte || c->device() != device) return false;
-  for (int d : {0, 1})
-    if (kc->size(d) > 1 && kc->stride(d) < kFp4Block) return false;
+  // No two blocks overlap: in the order of their strides, a row of blocks ends before the next begins.
+  const int inner = kc->size(1) > 1 && (kc->size(0) <= 1 || kc->stride(1) <= kc->stride(0)) ? 1 : 0;
+  int64_t end = kFp4Block;
+  for (int d : {inner, 1 - inner}) {
+    if (kc->size(d) <= 1) continue;
+    if (kc->stride(d) < end) return false;
+    end += kc->stride(d) * (kc->size(d) - 1);
+  }
   return device.index() == c10::hip::current_device();
 }
 

@@ -909,7 +909,12 @@ def _check_mxfp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, device: to
             raise TypeError(f"{name} must be a uint8 [pages, num_kv_heads, {MXFP4_PAGE_BYTES}] MXFP4 cache")
         if cache.device != device:
             raise RuntimeError(f"{name} must be on the device of the other tensors")
-        if cache.stride(2) != 1 or any(cache.size(d) > 1 and cache.stride(d) < MXFP4_PAGE_BYTES for d in (0, 1)):
+        # In either order of pages and heads, a row of blocks ends before the next begins.
+        apart, end = True, MXFP4_PAGE_BYTES
+        for stride, size in sorted((cache.stride(d), cache.size(d)) for d in (0, 1) if cache.size(d) > 1):
+            apart = apart and stride >= end
+            end += stride * (size - 1)
+        if cache.stride(2) != 1 or not apart:
             raise ValueError(f"{name} blocks must be contiguous and apart")
     if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
         raise ValueError("k_cache and v_cache must share shape and layout")
