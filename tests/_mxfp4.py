@@ -55,3 +55,20 @@ def poison_stale(cache: torch.Tensor, block_tables, kv_lengths, seed: int) -> No
                                     cache[..., :1024].unflatten(-1, (16, 64))).flatten(-2)
     cache[..., 1024:] = torch.where(stale, torch.tensor(255, dtype=torch.uint8),
                                     cache[..., 1024:].unflatten(-1, (16, 4))).flatten(-2)
+
+
+def random_cache(pages: int, heads: int, seed: int) -> torch.Tensor:
+    """A cache of arbitrary codes under scales of 2^-5 .. 1 (CPU)."""
+    gen = torch.Generator().manual_seed(seed)
+    cache = torch.randint(0, 256, (pages, heads, mxfp4.BLOCK), generator=gen, dtype=torch.uint8)
+    cache[..., 1024:] = torch.randint(122, 128, (pages, heads, 64), generator=gen, dtype=torch.uint8)
+    return cache
+
+
+def subnormal_bound(keys: int, value: float, p_dtype: torch.dtype) -> float:
+    """What :func:`attention_bound` leaves out: a probability below the type's normal
+    range, relative to a reference that the largest of its row reaches, is rounded by
+    up to half a subnormal step, so the average of ``keys`` values of at most
+    ``value`` by that often as much."""
+    info = torch.finfo(p_dtype)
+    return keys * value * info.tiny * info.eps / 2
