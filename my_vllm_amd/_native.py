@@ -265,6 +265,7 @@ _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 _load_error: Exception | None = None
 _host: ModuleType | None = None
+_capture_id = None  # its capture_id
 
 
 def load_library() -> ctypes.CDLL:
@@ -316,7 +317,7 @@ def load_library() -> ctypes.CDLL:
 def host_ops() -> ModuleType:
     """The native launch path (csrc/host_ops.cpp), loaded once; RuntimeError if
     it is missing or of another ABI revision."""
-    global _host
+    global _host, _capture_id
     if _host is not None:
         return _host
     load_library()  # the module binds to the library already in the process
@@ -332,7 +333,7 @@ def host_ops() -> ModuleType:
     if module.ABI_VERSION != ABI_VERSION:
         raise RuntimeError(f"{HOST_PATH} has C ABI revision {module.ABI_VERSION}, this package expects "
                            f"{ABI_VERSION}; re{rebuild}")
-    _host = module
+    _host, _capture_id = module, module.capture_id
     return module
 
 
@@ -359,6 +360,13 @@ def call(name: str, *args) -> None:
 def query(name: str, *args):
     """Call an entry point that returns a value rather than a status."""
     return getattr(load_library(), name)(*args)
+
+
+def capture_id(device_index: int) -> int:
+    """Number of the graph capture that torch's current stream of a device is in, or 0."""
+    if _capture_id is None:
+        host_ops()
+    return _capture_id(device_index)
 
 
 def stream_handle(device: torch.device) -> int:

@@ -22,7 +22,6 @@ backend-owned output buffer:
 
 from __future__ import annotations
 
-from contextlib import nullcontext
 from dataclasses import dataclass
 from types import MappingProxyType
 from typing import Any
@@ -585,7 +584,9 @@ class MI355XAttentionBackendMixin:
         self._route_counts = {route.value: 0 for route in self.route_type}
         self._output_buffer: torch.Tensor | None = None
         self._workspace: torch.Tensor | None = None
-        # The decode workspace of a captured step: its capture and stream, and it.
+        # The capture and stream that the current forward is in, or None; the decode
+        # workspace of a captured step: its capture and stream, and it.
+        self._captured: tuple | None = None
         self._captured_workspace: tuple[tuple, torch.Tensor] | None = None
         self._prefill_workspace: torch.Tensor | None = None
         # The metadata whose device tile plan the prefill workspace holds:
@@ -898,20 +899,16 @@ class MI355XAttentionBackendMixin:
 
     # ---- buffers ---------------------------------------------------------------
     def _capture_of(self, device: torch.device) -> tuple | None:
-        """(number of the graph capture, stream) that torch's current stream of
-        ``device`` is in, or None."""
-        if device.type != "cuda":
-            return None
-        index = torch.cuda.current_device() if device.index is None else device.index
-        with torch.cuda.device(index) if index != torch.cuda.current_device() else nullcontext():
-            if not torch.cuda.is_current_stream_capturing():
-                return None
-        return _native.host_ops().capture_id(index), _native.stream_handle(device)
+        """(number of the graph capture, stream) that torch's current stream of a
+        tensor's GPU is in, or None."""
+        capture = _native.capture_id(device.index) if device.index is not None else 0
+        return (capture, _native.stream_handle(device)) if capture else None
 
     def _get_reusable_attention_output(self, q: torch.Tensor) -> torch.Tensor:
         # A graph writes its outputs at every replay: they come from its own pool,
         # as an eager step may replace the buffer below at any time.
-        if self._capture_of(q.device) is not None:
+        self._captured = self._capture_of(q.device)
+        if self._captured is not None:
             return torch.empty_like(q)
         required = q.size(0)
         buffer = self._output_buffer
@@ -924,7 +921,8 @@ class MI355XAttentionBackendMixin:
         ):
             buffer = torch.empty_like(q)
             self._output_buffer = buffer
-        return buffer[:required]
+        # (A view of all of it costs the host half as much this way.)
+        return buffer[:required] if required < buffer.size(0) else buffer.detach()
 
     def _get_prefill_workspace(self, max_tiles: int, device: torch.device) -> torch.Tensor:
         nbytes = ops.prefill_workspace_bytes(max_tiles)
@@ -954,7 +952,7 @@ class MI355XAttentionBackendMixin:
         back, the pool would hand it to the next captured allocation."""
         versions = self._plan_versions(metadata)
         if torch.cuda.is_current_stream_capturing():
-            key = (_native.host_ops().capture_id(device.index), _native.stream_handle(device), versions)
+            key = (_native.capture_id(device.index), _native.stream_handle(device), versions)
             held, self._captured_plan = self._captured_plan, None
             if key[0] and held is not None and held[0] == key and held[1] is metadata:
                 return held[2], True, key
@@ -980,10 +978,10 @@ class MI355XAttentionBackendMixin:
         graph, once a replay (2 us)."""
         if nbytes <= 0:
             return None
-        capture = self._capture_of(device)
+        capture = self._captured
         if capture is not None:
             held = self._captured_workspace
-            if held is None or not capture[0] or held[0] != capture or held[1].numel() < nbytes:
+            if held is None or held[0] != capture or held[1].numel() < nbytes:
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
                 ws[:ops.decode_workspace_bytes(0, 1, 1)].zero_()
                 self._captured_workspace = held = (capture, ws)
