@@ -301,10 +301,10 @@ double longest_queue(const std::vector<Share>& shares, int64_t hkv, int64_t num_
   return most;
 }
 
-
-// Of the whole segments and of pieces for about one, two and three workgroups a CU (four
-// tiles or more each, one a wavefront), the cut with the least estimated time, or no
-// plan where page ranges come out below all of them.  The estimates, microseconds, with M
+// Of the whole segments and of pieces for about one, two and three workgroups a CU, the
+// cut with the least estimated time, or no plan where page ranges come out below all of
+// them.  Pieces aim at four tiles or more, one a wavefront; rounded to nearest they have
+// three at least, which leaves one of the four wavefronts without pages.  The estimates, microseconds, with M
 // the longest queue of a CU and A the mean, in tiles a wavefront, fitted to graphs of calls:
 //   whole  4.2 + 0.82 M    32 / 8 heads, 8 sequences of 1000 10.3, 16 of 2400 19.8; 8 / 1, 250 of 2000-4000 30.0
 //   cut    8.2 + 0.82 M, 1 more above 32 pieces   32 / 8, one of 1000 7.8, 24 of 6000 38.9; 16 / 4, 96 of 8000 87.9

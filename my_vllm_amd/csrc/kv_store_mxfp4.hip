@@ -14,9 +14,11 @@
 // two lane exchanges away.  A workgroup takes 16 or 64 tokens of one head, so the
 // codes of consecutive tokens leave as whole lines.
 //
-// Measured, 8 KV heads, K and V: 16384 tokens at random slots stored in 17.9 us and read
-// back in 22.2 (85 MB each: 4.7 and 3.8 TB/s, where a large copy reaches 4.7); 30001
-// of one sequence read back in 24.6 us; 61 in 2.7 and 2.4 us, launch latency.
+// Measured, kernels, 8 KV heads, K and V, microseconds, with all data in memory / in the
+// 256 MB last-level cache (one set of rows and results again and again): 16384 tokens (85
+// MB) in runs of 1024 slots stored in 18.9 / 15.5 and read back in 21.5 / 14.7, at random slots
+// 25.9 / 16.8 and 28.2 / 18.2; 30001 of one sequence (156 MB) 30.3 / 24.5 and 34.9 / 24.2: 4.5
+// TB/s from memory, where a large copy reaches 4.7.  61 tokens 2.7 and 2.8, launch latency.
 #include "mva_capi.h"
 #include "mxfp4.h"
 

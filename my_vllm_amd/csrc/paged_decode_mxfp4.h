@@ -9,8 +9,8 @@
 // flight while one is computed, up to twelve wavefronts per CU.  (Tiles of four pages in
 // two buffers, eight wavefronts: 275 us for the largest batch below.)
 //
-// Measured: 56 sequences of 8192-32768 tokens at 64 / 8 heads 246 us a call with its merge
-// (1.38 GB, 5.6 TB/s; a stream of the same pages into LDS without arithmetic reaches
+// Measured: 56 sequences of 8192-32768 tokens at 64 / 8 heads 249 us a call with its merge
+// (1.38 GB, 5.5 TB/s; a stream of the same pages into LDS without arithmetic reaches
 // 6.1), 64 of 128-2048 at 16 / 8 18.6 us (74 MB, 4.0 TB/s), 8 of 256-1024 9.1 us.  The small
 // ones are bound by a chain of latencies: launch, piece, page table, pages, and 0.75 us a
 // tile of a wavefront alone on its SIMD (155 vector instructions, V through LDS).

@@ -223,9 +223,9 @@ __device__ __attribute__((always_inline)) inline bool settle_piece(int32_t* plan
 // phases to arrive: group 0 loads K(t+2) after M(t) and writes it in M(t+1),
 // phase 2t+2; group 1 loads V(t+2) after M(t) and writes it in M(t+1), phase 2t+3.
 // Either is after the last read of the buffer (phase 2t-1, 2t+1) and two phases
-// before the first (2t+4, 2t+6).  Kernel, microseconds, this cache / 16 bits: 16
-// sequences of 64-2048 new tokens over prefixes at 32 / 8 heads 369 / 340 (0.92 / 1.0
-// PFLOP/s), 512 tokens over 7168 75 / 70, one prompt of 333 16.7 / 16.3.
+// before the first (2t+4, 2t+6).  Call, microseconds, this cache / 16 bits: 16
+// sequences of 64-2048 new tokens over prefixes at 32 / 8 heads 362 / 350 (0.94 / 0.98
+// PFLOP/s), 512 tokens over 7168 71.8 / 68.2, one prompt of 333 16.1 / 15.7.
 template <typename T, int kGrp, bool kFixed, bool kPieces, typename P>
 __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(const P& p, int32_t* plan,
                                                                              int h0, int rank, lds_u8* tiles, lds_i32* nextq) {
@@ -291,11 +291,9 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
   const uint32_t voff = (uint32_t)(((lane >> 2) * p.tok_stride + 8 * (lane & 3)) * (int64_t)sizeof(T));
   auto kbuf = [&](int x) { return tiles + (x % kPrefillPPBufs) * kPrefillTileBytes; };
   auto vbuf = [&](int x) { return tiles + (kPrefillPPBufs + x % kPrefillPPBufs) * kPrefillTileBytes; };
-  // This wave's page of K (group 0) or V (group 1) of KV head `head`, global
-  // tile x.
   // MXFP4: the page in registers (its codes and scale byte, and the place of its
-  // rows).  K: this lane holds group lane / 16 of token lane %
-  // 16 and writes chunk u of four at 256 u, 16 lanes side by side.  V: group g =
+  // rows).  K: this lane holds group lane / 16 of token lane % 16
+  // and writes chunk u of four at 256 u, 16 lanes side by side.  V: group g =
   // lane % 4 of token lane / 4; a row's chunks are neighbours there, so lanes of
   // one token take them in different orders, u ^ g, to write to different banks.
   u32x4 held_w = {};
@@ -332,6 +330,8 @@ __device__ __attribute__((always_inline)) inline void prefill_items_pingpong(con
       held = false;
     }
   };
+  // This wave's page of K (group 0) or V (group 1) of KV head `head`, global
+  // tile x.
   auto copy_page = [&](int x, int page, int head) __attribute__((always_inline)) {
     if constexpr (kFp4) {
       // A second page at one time (only items of one or two tiles ask for it)
