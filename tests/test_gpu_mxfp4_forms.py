@@ -141,6 +141,41 @@ def test_prefill_of_many_short_prompts(gpu, dtype, kv):
     assert_within(out, expected, _bound(expected, spread, largest, kv, dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("hq", [8, 16, 32])
+def test_prefill_nan_groups(gpu, hq, dtype):
+    # A NaN of K reaches the queries that see it and no other; one of V also those before it
+    # in its tile of queries (256 rows over a KV head's query heads) and keys (64).
+    n, hkv = 300, 8
+    batch, caches = _prefill_case(hq, [n], [n], hq, hkv, dtype)
+    backend = MI355XMXFP4AttentionBackend(hq, hkv, 128, 16, dtype)
+    plan = backend.build_plan(_on(batch.common, gpu))
+    q = batch.q.to(gpu)
+
+    def run():
+        return backend.forward(q, None, None, caches[0].to(gpu), caches[1].to(gpu), plan).cpu()
+
+    clean = run()
+    assert torch.isfinite(clean).all()
+    table, group = batch.common.block_tables[0], hq // hkv
+    caches[0][table[100 // 16], 3, 1024 + 4 * (100 % 16) + 1] = 255
+    out = run()
+    heads = torch.zeros(hq, dtype=torch.bool)
+    heads[3 * group:4 * group] = True
+    assert torch.isnan(out[100:, heads]).all()
+    assert torch.equal(out[:100], clean[:100]) and torch.equal(out[100:, ~heads], clean[100:, ~heads])
+    caches[0][table[100 // 16], 3, 1024 + 4 * (100 % 16) + 1] = 124
+    clean = run()
+    caches[1][table[290 // 16], 3, 1024 + 4 * (290 % 16) + 2] = 255
+    out, dims = run(), slice(64, 96)
+    assert torch.isnan(out[290:, heads, dims]).all()
+    # Queries 256 .. 299 are in the last tile, and keys 256 .. 299 in theirs.
+    assert torch.equal(out[:256], clean[:256])
+    assert torch.equal(out[:, ~heads], clean[:, ~heads])
+    rest = [d for d in range(128) if d not in range(64, 96)]
+    assert torch.equal(out[:, heads][..., rest], clean[:, heads][..., rest])
+
+
 # ---- fp16: probabilities in fp16, MIXED steps and captured decode ------------------------
 
 FEW_KEYS = [2, 3, 4, 5, 7, 15, 16, 17, 31, 33, 64, 65]
