@@ -526,7 +526,7 @@ int mva_kv_load_mxfp4(void* key, int64_t key_token_stride, int64_t key_head_stri
  * or shared ones.
  *
  * Page ranges as mva_decode_plan_listed's, not cut further.  item_rows must be
- * at least (num_seqs + num_groups) * num_kv_heads.
+ * at least (num_seqs + min(num_groups, total pages)) * num_kv_heads.
  */
 int mva_decode_plan_listed_mxfp4(const int64_t* block_counts, int64_t num_seqs, int64_t first_seq,
                                  int64_t first_q_row, int num_kv_heads, int num_groups, int32_t* items,

@@ -307,7 +307,7 @@ def plan_decode_listed_mxfp4(
     """:func:`plan_decode_listed` for a decode launch over MXFP4 caches, which alone
     takes it: pieces are as long as their ranges (``mva_decode_plan_listed_mxfp4``)."""
     counts = _plan_counts(block_counts)
-    rows = (counts.size + max(1, int(num_groups))) * int(num_kv_heads)
+    rows = (counts.size + max(1, min(int(num_groups), int(counts.sum())))) * int(num_kv_heads)
     return _plan_listed("mva_decode_plan_listed_mxfp4", counts, first_seq, first_q_row, num_kv_heads, num_groups, rows)
 
 

@@ -102,3 +102,10 @@ def test_mxfp4_page_ranges(monkeypatch, counts, hkv, groups):
     assert len(items) <= (len(counts) + groups) * hkv
     empty = plan_decode_listed_mxfp4(np.zeros(0, np.int64), 0, 0, hkv, groups)
     assert empty[0].shape == (0, 8) and empty[1].tolist() == [0] and empty[2:4] == (0, 0)
+
+
+def test_more_ranges_than_pages():
+    # As many rows as the pages can need, not as the ranges asked for.
+    few = plan_decode_listed_mxfp4([3, 1], 0, 0, 8, 4)
+    many = plan_decode_listed_mxfp4([3, 1], 0, 0, 8, 2 ** 31 - 1)
+    assert all(np.array_equal(a, b) for a, b in zip(few, many))
