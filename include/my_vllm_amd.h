@@ -580,6 +580,65 @@ int mva_paged_prefill_mxfp4(const void* q, int64_t q_token_stride, int64_t q_hea
                             int64_t out_token_stride, int64_t out_head_stride, int num_q_heads, int num_kv_heads,
                             int head_dim, int page_size, float softmax_scale, int dtype, void* stream);
 
+/*
+ * ---- decode over selected pages -------------------------------------------------
+ *
+ * page_bounds is a dense [num_pages][num_kv_heads][2][128] array of the cache's
+ * element type: for a full page the smallest (0) and the largest (1) value of
+ * each channel of its 16 keys.
+ *
+ * mva_update_page_bounds writes the bounds of every page that a step's new
+ * tokens complete, from the K cache that already holds them: of sequence s the
+ * pages that end at a position in [seq_lens[s] - new tokens, seq_lens[s]).
+ * query_start_loc ([num_seqs + 1]) gives the new tokens; without it (NULL)
+ * every sequence has one and num_tokens equals num_seqs.  num_tokens bounds
+ * query_start_loc[num_seqs]: tokens from there on are not looked at.  Pages
+ * beyond the table or the cache are skipped.  A NaN in a channel makes both of
+ * its bounds NaN.
+ */
+int mva_update_page_bounds(const void* k_cache, int64_t num_pages, int64_t page_stride, int64_t token_stride,
+                           void* page_bounds, const int32_t* block_tables, int64_t block_table_stride,
+                           int64_t table_width, const int32_t* seq_lens, const int32_t* query_start_loc,
+                           int64_t num_seqs, int64_t num_tokens, int num_kv_heads, int head_dim, int page_size,
+                           int dtype, void* stream);
+
+/* Bytes of the workspace of mva_select_pages and mva_paged_decode_selected
+ * (either takes it; neither needs it cleared), or -1. */
+int64_t mva_selection_workspace_bytes(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t table_width,
+                                      int64_t num_selected);
+
+/*
+ * Chooses at most num_selected pages for each row s (one query, q [num_seqs]
+ * [num_q_heads][128]) and KV head h: all pages of a row of no more; else its
+ * first sink_pages, its last recent_pages (>= 1) and, of those between, the
+ * ones of the highest score
+ *   sum_d P[d] hi[d] + N[d] lo[d],  P = sum_g max(q_g, 0),  N = sum_g min(q_g, 0)
+ * over the queries g of the KV head, in 64 bits; NaN ranks above everything,
+ * ties go to the lowest place.  tables (dense [num_seqs][num_kv_heads]
+ * [num_selected]) gets their page ids in the order of their places, -1 after
+ * the last; lens ([num_seqs]) the tokens they hold, those of the last page
+ * counted to the row's end.  A row of seq_lens <= 0 gets no page and 0.
+ */
+int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* page_bounds,
+                     int64_t num_pages, const int32_t* block_tables, int64_t block_table_stride, int64_t table_width,
+                     const int32_t* seq_lens, int64_t num_seqs, int64_t num_selected, int64_t sink_pages,
+                     int64_t recent_pages, int32_t* tables, int32_t* lens, void* workspace, int64_t workspace_bytes,
+                     int num_q_heads, int num_kv_heads, int head_dim, int page_size, int dtype, void* stream);
+
+/*
+ * Attention of one query a row over the first lens[s] tokens of the pages
+ * tables[s][h][0 ..], a list for each row and KV head of at most num_selected
+ * pages (strides in elements; the lists themselves dense).  Rows of lens <= 0
+ * give zeros.
+ */
+int mva_paged_decode_selected(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                              const void* v_cache, int64_t num_pages, int64_t page_stride, int64_t token_stride,
+                              const int32_t* tables, int64_t seq_table_stride, int64_t head_table_stride,
+                              const int32_t* lens, int64_t num_seqs, int64_t num_selected, void* out,
+                              int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                              int64_t workspace_bytes, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                              float softmax_scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -160,6 +160,35 @@ _SIGNATURES = {
             _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p,
         ],
     ),
+    "mva_update_page_bounds": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64, _i64, _c_void_p,  # k_cache, num_pages, page and token strides, page_bounds
+            _c_void_p, _i64, _i64, _c_void_p, _c_void_p,  # block_tables, stride, width, seq_lens, query_start_loc
+            _i64, _i64, _i32, _i32, _i32, _i32, _c_void_p,  # seqs, tokens, KV heads, head_dim, page, dtype, stream
+        ],
+    ),
+    "mva_selection_workspace_bytes": (_i64, [_i64, _i32, _i32, _i64, _i64]),
+    "mva_select_pages": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64, _c_void_p, _i64,  # q and its strides, page_bounds, num_pages
+            _c_void_p, _i64, _i64, _c_void_p, _i64,  # block_tables, stride, width, seq_lens, seqs
+            _i64, _i64, _i64, _c_void_p, _c_void_p,  # selected, sink and recent pages, tables, lens
+            _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p,  # workspace, bytes, heads, dim, page, dtype, stream
+        ],
+    ),
+    "mva_paged_decode_selected": (
+        _i32,
+        [
+            _c_void_p, _i64, _i64,  # q, q_token_stride, q_head_stride
+            _c_void_p, _c_void_p, _i64, _i64, _i64,  # k_cache, v_cache, num_pages, page_stride, token_stride
+            _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # tables, row and head strides, lens, seqs, selected
+            _c_void_p, _i64, _i64,  # out, out_token_stride, out_head_stride
+            _c_void_p, _i64,  # workspace, workspace_bytes
+            _i32, _i32, _i32, _i32, _f32, _i32, _c_void_p,  # heads, head_dim, page, scale, dtype, stream
+        ],
+    ),
     "mva_decode_plan_listed_rows": (_i64, [_i64, _i64, _i32, _i32, _i32]),
     "mva_decode_plan_listed_mxfp4": (
         _i32,
@@ -259,7 +288,7 @@ _SIGNATURES = {
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 # The C ABI revision these signatures describe (mva_abi_version()).
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -471,6 +471,7 @@ class MI355XFullDecodeGraphState:
     plan: Any = None
     staging_turn: int = 0
     mxfp4: bool = False  # as the metadata's
+    selects: bool = False  # whether it is of a backend that selects pages
 
     def views(self):
         """(counts, items, wave_extra, merges) views of the device plan buffer."""
@@ -552,6 +553,8 @@ class MI355XAttentionBackendMixin:
     check_fused_store: bool = False
     # Whether the caches are MXFP4.
     _mxfp4 = False
+    # Whether decode rows attend to selected pages (and need no decode plan).
+    _selects = False
 
     def __init__(
         self,
@@ -775,7 +778,7 @@ class MI355XAttentionBackendMixin:
         mixed = bool(common.num_prefill_seqs and common.num_decode_seqs)
         split_reason = self._batch_mixed_reason(common) if mixed else None
         one_launch = mixed and split_reason is None
-        if common.num_decode_seqs:
+        if common.num_decode_seqs and not self._selects:
             decode_counts = counts[common.num_prefill_seqs:]
             wave_extra = None
             if one_launch and self.decode_waves_override is None and self.decode_schedule_override != "claims":
@@ -1113,6 +1116,8 @@ class MI355XAttentionBackendMixin:
             raise ValueError("query token count does not match the attention plan")
         if metadata.mxfp4 and not self._mxfp4 and common.num_decode_seqs:
             raise ValueError("the plan's decode pieces were made for an MXFP4 cache")
+        if metadata.decode_items is None and common.num_decode_seqs and not self._selects:
+            raise ValueError("the plan has no decode pieces: a backend that selects pages made it")
 
         output = self._get_reusable_attention_output(q)
         if route is Route.DECODE:
@@ -1222,7 +1227,7 @@ class MI355XAttentionBackendMixin:
         metadata = plan.metadata
         if not isinstance(metadata, MI355XAttentionMetadata) or metadata.is_cacheless:
             return False
-        if state.mxfp4 != self._mxfp4 or (metadata.mxfp4 and not self._mxfp4):
+        if state.mxfp4 != self._mxfp4 or (metadata.mxfp4 and not self._mxfp4) or bool(state.selects) != self._selects:
             return False
         common = plan.common
         if common.num_prefill_seqs != 0 or common.num_prefill_tokens != 0:
@@ -1290,6 +1295,8 @@ class MI355XAttentionBackendMixin:
             raise RuntimeError("decode graph state must be planned before activation")
         if state.mxfp4 != self._mxfp4:
             raise ValueError("the decode graph state was made for another kind of cache")
+        if bool(state.selects) != self._selects:
+            raise ValueError("the decode graph state was made for another kind of decode")
         if self._active_graph_state is not None:
             raise RuntimeError("a decode graph state is already active")
         self._active_graph_state = state
@@ -1562,6 +1569,155 @@ class MI355XMXFP4AttentionBackend(MI355XMXFP4AttentionBackendMixin, AttentionBac
     """gfx950 backend over an MXFP4 cache ("mi355x_mxfp4")."""
 
 
+# --------------------------------------------------------------------------
+# Decode over selected pages.
+# --------------------------------------------------------------------------
+
+
+class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
+    """The backend whose decode rows attend to a part of their pages.
+
+    For every layer the caller keeps, beside its 16-bit caches, ``page_bounds``
+    (``ops.page_bounds_shape``, the cache's dtype).  A decode row of more than
+    ``selected_pages`` pages attends, for each KV head, to its first
+    ``sink_pages``, its last ``recent_pages`` and the pages whose bounds score
+    highest for its queries (``ops.select_pages``); a shorter row attends to all
+    of its pages, as on the base.  Prefill is dense.  A MIXED batch runs as
+    prefill + decode launches (route MIXED_SPLIT) in both attention modes.
+
+    :meth:`forward_with_kv_store` stores the step's rows, brings the bounds up to
+    date and attends.  A caller that stores the rows itself (the fused prologue)
+    calls :meth:`update_page_bounds` before :meth:`forward`, in prefill steps too.
+    Decode needs no plan of work: graph states hold tables and lengths only."""
+
+    backend_name = "mi355x_sparse"
+    _selects = True
+    default_selected_pages = 128
+    default_sink_pages = 1
+    default_recent_pages = 4
+
+    def __init__(
+        self,
+        num_q_heads: int,
+        num_kv_heads: int,
+        head_dim: int,
+        block_size: int,
+        dtype: torch.dtype,
+        attention_mode: str | None = None,
+        selected_pages: int | None = None,
+        sink_pages: int | None = None,
+        recent_pages: int | None = None,
+    ) -> None:
+        super().__init__(num_q_heads, num_kv_heads, head_dim, block_size, dtype, attention_mode)
+        self.selected_pages = self.default_selected_pages if selected_pages is None else selected_pages
+        self.sink_pages = self.default_sink_pages if sink_pages is None else sink_pages
+        self.recent_pages = self.default_recent_pages if recent_pages is None else recent_pages
+        for name, least in (("selected_pages", 1), ("sink_pages", 0), ("recent_pages", 1)):
+            value = getattr(self, name)
+            if isinstance(value, bool) or not isinstance(value, int):
+                raise TypeError(f"{name} must be an int")
+            if value < least:
+                raise ValueError(f"{name} must be at least {least}")
+        if self.sink_pages + self.recent_pages > self.selected_pages:
+            raise ValueError("sink_pages + recent_pages must be at most selected_pages")
+        # The page bounds of the layer that forward runs.
+        self._page_bounds: torch.Tensor | None = None
+
+    def _backend_mixed_reason(self) -> str | None:
+        return "MIXED batches with selected pages run as prefill + decode launches"
+
+    def forward_with_kv_store(self, q, k, v, k_cache, v_cache, slot_mapping, plan, store=None,
+                              page_bounds=None) -> torch.Tensor:
+        """The step's K/V rows into the caches (``store``, or ``ops.store_kvcache``),
+        :meth:`update_page_bounds`, then :meth:`forward`."""
+        if _has_cache(k_cache) and page_bounds is None:
+            raise ValueError("a backend that selects pages needs page_bounds")
+        (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
+        if _has_cache(k_cache):
+            self.update_page_bounds(k_cache, page_bounds, plan)
+        return self.forward(q, k, v, k_cache, v_cache, plan, page_bounds=page_bounds)
+
+    def update_page_bounds(self, k_cache, page_bounds, plan) -> None:
+        """The bounds of the pages that the plan's step completes
+        (``ops.update_page_bounds``); ``k_cache`` holds the step's rows."""
+        state = self._active_graph_state
+        if state is not None:
+            ops.update_page_bounds(k_cache, page_bounds, state.block_tables_buffer, state.seq_lens_buffer)
+            return
+        metadata = plan_metadata(plan, MI355XAttentionMetadata, self.backend_name, self.plan_type)
+        if metadata.is_cacheless:
+            raise ValueError("page bounds require page metadata")
+        common = plan.common
+        if common.num_prefill_seqs == 0:
+            ops.update_page_bounds(k_cache, page_bounds, metadata.block_tables, metadata.seq_lens)
+            return
+        ops.update_page_bounds(k_cache, page_bounds, metadata.block_tables, metadata.seq_lens,
+                               metadata.query_start_loc, common.num_query_tokens)
+
+    def forward(self, q, k, v, k_cache, v_cache, plan, page_bounds=None) -> torch.Tensor:
+        """As the base's; steps with decode rows need ``page_bounds``."""
+        self._page_bounds = page_bounds
+        try:
+            return super().forward(q, k, v, k_cache, v_cache, plan)
+        finally:
+            self._page_bounds = None
+
+    def _attend(self, q, k_cache, v_cache, block_tables, seq_lens, out) -> None:
+        if self._page_bounds is None:
+            raise ValueError("decode over selected pages needs page_bounds")
+        if self._page_bounds.size(0) != k_cache.size(0):
+            raise ValueError("page_bounds must have the cache's number of pages")
+        nbytes = ops.selection_workspace_bytes(q.size(0), self.num_q_heads, self.num_kv_heads, block_tables.size(1),
+                                               self.selected_pages)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        tables, lens = ops.select_pages(q, self._page_bounds, block_tables, seq_lens, self.selected_pages,
+                                        self.sink_pages, self.recent_pages, workspace=workspace)
+        ops.paged_decode_selected(q, k_cache, v_cache, tables, lens, self.softmax_scale, out=out, workspace=workspace)
+
+    def _run_decode(self, q, k_cache, v_cache, common, metadata: MI355XAttentionMetadata, output) -> None:
+        first, rows = common.num_prefill_seqs, common.num_prefill_tokens
+        self._attend(q[rows:], k_cache, v_cache, metadata.block_tables[first:], metadata.seq_lens[first:],
+                     output[rows:])
+
+    # ---- full-decode HIP graph: tables and lengths are all that a step changes ----
+    def create_full_decode_graph_state(self, batch_size: int, page_indices_capacity: int, device):
+        if any(isinstance(x, bool) or not isinstance(x, int) for x in (batch_size, page_indices_capacity)):
+            raise TypeError("batch_size and page_indices_capacity must be ints")
+        if batch_size <= 0 or page_indices_capacity < batch_size:
+            raise ValueError("graph state requires positive batch and page capacity")
+        graph_device = torch.device(device)
+        if graph_device.type != "cuda":
+            raise ValueError("full decode graph state must be on CUDA")
+        width = page_indices_capacity // batch_size
+        return MI355XFullDecodeGraphState(
+            batch_size=batch_size,
+            page_indices_capacity=page_indices_capacity,
+            groups=0, waves_per_group=0, item_capacity=0, wave_capacity=0, merge_capacity=0, part_slot_capacity=0,
+            block_tables_buffer=torch.zeros((batch_size, width), dtype=torch.int32, device=graph_device),
+            seq_lens_buffer=torch.ones(batch_size, dtype=torch.int32, device=graph_device),
+            plan_buffer=torch.zeros(0, dtype=torch.int32, device=graph_device),
+            plan_staging=[], staging_ready=[],
+            workspace=torch.zeros(0, dtype=torch.uint8, device=graph_device),
+            output=torch.empty(batch_size, self.num_q_heads, self.head_dim, dtype=self.dtype, device=graph_device),
+            selects=True,
+        )
+
+    def plan_full_decode_graph(self, state, plan) -> None:
+        if not self.full_decode_graph_metadata_fits(state, plan):
+            raise ValueError("attention plan does not fit full decode graph state")
+        tables = plan.metadata.block_tables
+        state.block_tables_buffer[:, : tables.size(1)].copy_(tables)
+        state.seq_lens_buffer.copy_(plan.metadata.seq_lens)
+        state.plan = plan
+
+    def _run_decode_graph(self, q, k_cache, v_cache, state: MI355XFullDecodeGraphState) -> None:
+        self._attend(q, k_cache, v_cache, state.block_tables_buffer, state.seq_lens_buffer, state.output)
+
+
+class MI355XSparseAttentionBackend(MI355XSparseAttentionBackendMixin, AttentionBackend):
+    """gfx950 backend whose decode rows attend to selected pages ("mi355x_sparse")."""
+
+
 def integrate(registry: Any, base: type, plan_type: type, route_type: type, batch_type_enum: type,
               common_type: type, names: tuple[str, str] = ("mi355x", "mi355x_split")) -> tuple[type, type]:
     """Build the backend on another contract's classes and register it.
@@ -1596,15 +1752,34 @@ def integrate_mxfp4(registry: Any, base: type, plan_type: type, route_type: type
     return backend
 
 
+def integrate_sparse(registry: Any, base: type, plan_type: type, route_type: type, batch_type_enum: type,
+                     common_type: type, name: str = "mi355x_sparse", selected_pages: int | None = None,
+                     sink_pages: int | None = None, recent_pages: int | None = None) -> type:
+    """:func:`integrate` for the backend whose decode rows attend to selected
+    pages.  Another contract's registry constructs it without the page numbers,
+    so those given here become the class's."""
+    given = {"default_selected_pages": selected_pages, "default_sink_pages": sink_pages,
+             "default_recent_pages": recent_pages}
+    backend = type("MI355XSparseBackend", (MI355XSparseAttentionBackendMixin, base),
+                   {"__module__": __name__, "backend_name": name, "plan_type": plan_type, "route_type": route_type,
+                    "batch_type_enum": batch_type_enum, "common_type": common_type,
+                    **{key: value for key, value in given.items() if value is not None}})
+    registry.register(name, backend)
+    return backend
+
+
 __all__ = [
     "MI355XAttentionBackend",
     "MI355XAttentionBackendMixin",
     "MI355XAttentionMetadata",
     "MI355XMXFP4AttentionBackend",
     "MI355XMXFP4AttentionBackendMixin",
+    "MI355XSparseAttentionBackend",
+    "MI355XSparseAttentionBackendMixin",
     "MI355XSplitAttentionBackend",
     "integrate",
     "integrate_mxfp4",
+    "integrate_sparse",
     "make_decode_plan",
     "make_decode_plan_listed",
     "plan_decode_claims",

@@ -1,0 +1,25 @@
+// Sizes that the page selection and the attention over selected pages share.
+//
+// Workspace: [partials of the attention][score keys of the selection].  The
+// partials come first: the attention knows its own sizes only.
+#pragma once
+
+#include <cstdint>
+
+namespace mva {
+
+constexpr int kPageTokens = 16;
+constexpr int kMaxQueryGroup = 16;
+
+inline int64_t align_up256(int64_t x) { return (x + 255) & ~int64_t(255); }
+
+// Whether a selection of `num_selected` pages a row can be made at all.
+inline bool selection_sizes_ok(int64_t num_seqs, int hq, int hkv, int64_t num_selected) {
+  return num_seqs >= 0 && num_seqs <= 0x7fffffffLL && hkv > 0 && hq > 0 && hq % hkv == 0 && hq / hkv <= kMaxQueryGroup &&
+         num_seqs * hq <= 0x7fffffffLL && num_selected > 0 && num_selected <= (1 << 24);
+}
+
+// Bytes of the attention's partials.
+int64_t selection_part_bytes(int64_t num_seqs, int hq, int hkv, int64_t num_selected);
+
+}  // namespace mva

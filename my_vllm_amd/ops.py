@@ -1142,3 +1142,278 @@ def paged_prefill_mxfp4(
         q.shape[1], k_cache.shape[1], q.shape[2], PAGE_SIZE, float(softmax_scale),
         _native.dtype_code(q.dtype), _native.stream_handle(q.device),
     )
+
+
+# ---- decode over selected pages ---------------------------------------------------
+
+
+def page_bounds_shape(num_pages: int, num_kv_heads: int) -> tuple[int, int, int, int]:
+    """Shape of a layer's page bounds, in the cache's dtype: for every full page
+    of ``num_pages`` and KV head the smallest (index 0) and the largest (index 1)
+    value of each channel of its 16 keys; 1/16 of the room of K and V."""
+    return int(num_pages), int(num_kv_heads), 2, HEAD_DIM
+
+
+def _check_cache(name: str, cache: torch.Tensor, device: torch.device, dtype: torch.dtype) -> None:
+    if cache.device != device:
+        raise RuntimeError(f"{name} must be on the device of the other tensors")
+    if cache.dtype != dtype:
+        raise TypeError(f"{name} must have the dtype of the other tensors")
+    if cache.dim() != 4 or cache.size(1) != PAGE_SIZE or cache.size(3) != HEAD_DIM:
+        raise ValueError(f"{name} must be [pages, {PAGE_SIZE}, num_kv_heads, {HEAD_DIM}]")
+    # Each page's rows, and each row's heads, lie apart: [pages, tokens] in either order.
+    row = cache.size(2) * HEAD_DIM
+    apart, end = cache.stride(3) == 1 and (cache.size(2) <= 1 or cache.stride(2) == HEAD_DIM), row
+    for stride, size in sorted((cache.stride(d), cache.size(d)) for d in (0, 1) if cache.size(d) > 1):
+        apart = apart and stride >= end
+        end += stride * (size - 1)
+    if not apart:
+        raise ValueError(f"{name} must hold packed heads in rows that do not overlap")
+
+
+def _check_page_bounds(page_bounds: torch.Tensor, num_kv_heads: int, device: torch.device, dtype: torch.dtype) -> None:
+    if page_bounds.device != device:
+        raise RuntimeError("page_bounds must be on the device of the other tensors")
+    if page_bounds.dtype != dtype:
+        raise TypeError("page_bounds must have the cache's dtype")
+    if page_bounds.dim() != 4 or page_bounds.shape[1:] != (num_kv_heads, 2, HEAD_DIM):
+        raise ValueError(f"page_bounds must be [pages, num_kv_heads, 2, {HEAD_DIM}]")
+    if not page_bounds.is_contiguous():
+        raise ValueError("page_bounds must be contiguous")
+
+
+def _check_rows_metadata(device: torch.device, block_tables: torch.Tensor, seq_lens: torch.Tensor) -> None:
+    for name, t, dims in (("block_tables", block_tables, 2), ("seq_lens", seq_lens, 1)):
+        if t.device != device:
+            raise RuntimeError(f"{name} must be on the device of the other tensors")
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+        if t.dim() != dims:
+            raise ValueError(f"{name} must have {dims} dimension{'s' if dims > 1 else ''}")
+    if block_tables.size(0) != seq_lens.size(0):
+        raise ValueError("block_tables must have one row per sequence")
+    if block_tables.size(1) > 1 and block_tables.stride(1) != 1:
+        raise ValueError("block table rows must be dense")
+    if seq_lens.size(0) > 1 and seq_lens.stride(0) != 1:
+        raise ValueError("seq_lens must be dense")
+
+
+def _check_queries(q: torch.Tensor) -> None:
+    if not q.is_cuda:
+        raise RuntimeError("expected CUDA tensors")
+    if q.dtype not in _native.DTYPE_CODES:
+        raise TypeError("queries must be bfloat16 or float16")
+    if q.dim() != 3 or q.size(2) != HEAD_DIM or q.stride(2) != 1:
+        raise ValueError(f"queries must be [rows, num_q_heads, {HEAD_DIM}] with unit inner stride")
+
+
+def _check_groups(num_q_heads: int, num_kv_heads: int) -> None:
+    if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads or num_q_heads // num_kv_heads > 16:
+        raise ValueError("the query heads must be 1 to 16 for each KV head")
+
+
+def _positive(name: str, value: int, least: int) -> int:
+    if isinstance(value, bool) or not isinstance(value, int):
+        raise TypeError(f"{name} must be an int")
+    if value < least:
+        raise ValueError(f"{name} must be at least {least}")
+    return value
+
+
+def update_page_bounds(
+    k_cache: torch.Tensor,
+    page_bounds: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor | None = None,
+    num_tokens: int | None = None,
+) -> None:
+    """Write the bounds of the pages that a step's new tokens complete, in place.
+
+    Called after the step's rows are in ``k_cache`` (``[P, 16, Hkv, 128]`` bf16 or
+    fp16): for sequence ``s`` the pages that end at one of its new positions
+    ``[seq_lens[s] - new, seq_lens[s])``.  ``query_start_loc`` (``[S + 1]``) counts
+    the new tokens and ``num_tokens`` is their number; without them every
+    sequence has one.  ``page_bounds`` is a contiguous tensor of
+    :func:`page_bounds_shape`.  A page that is not full has no bounds (none are
+    read: the last page of a row is always selected); a page without new tokens,
+    such as a shared prefix's, keeps the ones that it has.  A NaN in a channel
+    makes both of its bounds NaN."""
+    if not k_cache.is_cuda:
+        raise RuntimeError("update_page_bounds expects CUDA tensors")
+    if k_cache.dtype not in _native.DTYPE_CODES:
+        raise TypeError("update_page_bounds takes bfloat16 or float16 caches")
+    device = k_cache.device
+    _check_cache("k_cache", k_cache, device, k_cache.dtype)
+    _check_page_bounds(page_bounds, k_cache.size(2), device, k_cache.dtype)
+    if page_bounds.size(0) != k_cache.size(0):
+        raise ValueError("page_bounds must have the cache's number of pages")
+    _check_rows_metadata(device, block_tables, seq_lens)
+    num_seqs = seq_lens.size(0)
+    if query_start_loc is None:
+        if num_tokens is not None and num_tokens != num_seqs:
+            raise ValueError("without query_start_loc every sequence has one new token")
+        num_tokens = num_seqs
+    else:
+        if query_start_loc.device != device or query_start_loc.dtype != torch.int32:
+            raise RuntimeError("query_start_loc must be an int32 tensor on the device of the other tensors")
+        if query_start_loc.shape != (num_seqs + 1,) or (num_seqs and query_start_loc.stride(0) != 1):
+            raise ValueError("query_start_loc must be dense and hold one more entry than there are sequences")
+        if num_tokens is None:
+            raise ValueError("query_start_loc needs num_tokens")
+        _positive("num_tokens", num_tokens, 0)
+    if num_tokens == 0 or k_cache.numel() == 0 or block_tables.numel() == 0:
+        return
+    _call_on(
+        device, "mva_update_page_bounds",
+        k_cache.data_ptr(), k_cache.size(0), k_cache.stride(0), k_cache.stride(1), page_bounds.data_ptr(),
+        block_tables.data_ptr(), block_tables.stride(0), block_tables.size(1), seq_lens.data_ptr(),
+        query_start_loc.data_ptr() if query_start_loc is not None else 0, num_seqs, num_tokens,
+        k_cache.size(2), HEAD_DIM, PAGE_SIZE, _native.dtype_code(k_cache.dtype), _native.stream_handle(device),
+    )
+
+
+@functools.lru_cache(maxsize=256)
+def selection_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, table_width: int,
+                              num_selected: int) -> int:
+    """Bytes of a workspace for :func:`select_pages` and :func:`paged_decode_selected`
+    over block tables of ``table_width`` pages.  Calls that share one must not
+    overlap; it needs no clearing."""
+    nbytes = int(_native.query("mva_selection_workspace_bytes", num_seqs, num_q_heads, num_kv_heads, table_width,
+                               num_selected))
+    if nbytes < 0:
+        raise ValueError("invalid page selection sizes")
+    return nbytes
+
+
+def _selection_workspace(workspace: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+    if workspace is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor on the device of the other tensors")
+    if workspace.numel() < nbytes:
+        raise ValueError(f"workspace must have {nbytes} bytes")
+    return workspace
+
+
+def select_pages(
+    q: torch.Tensor,
+    page_bounds: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    num_selected: int,
+    sink_pages: int = 1,
+    recent_pages: int = 1,
+    *,
+    workspace: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Choose the pages that each row's query attends to, for every KV head.
+
+    ``q`` is ``[S, Hq, 128]``, one query a row (a sequence with several new
+    tokens has a row for each, with its own ``seq_lens``); ``page_bounds`` those of
+    :func:`update_page_bounds`.  A row of at most ``num_selected`` pages keeps them
+    all.  Any other keeps its first ``sink_pages``, its last ``recent_pages`` (at
+    least one: the last page may be partly filled) and, of those between, the
+    ones of the highest score ``sum_d P[d] max[d] + N[d] min[d]``, with ``P`` and
+    ``N`` the sums of the positive and of the negative parts of the KV head's
+    queries: no key of the page has a larger product with them, summed over the
+    queries.  Scores are held in 64 bits; NaN ranks above everything, ties go to
+    the lowest place.
+
+    Returns ``(tables, lens)``: int32 ``[S, Hkv, num_selected]`` page ids in the
+    order of their places, -1 after a row's last, and int32 ``[S]`` the tokens
+    that they hold, for :func:`paged_decode_selected`.  A row of ``seq_lens`` 0
+    gets no page."""
+    _check_queries(q)
+    device, dtype = q.device, q.dtype
+    if page_bounds.dim() != 4:
+        raise ValueError(f"page_bounds must be [pages, num_kv_heads, 2, {HEAD_DIM}]")
+    num_seqs, num_q_heads, num_kv_heads = q.size(0), q.size(1), page_bounds.size(1)
+    _check_groups(num_q_heads, num_kv_heads)
+    _check_page_bounds(page_bounds, num_kv_heads, device, dtype)
+    _check_rows_metadata(device, block_tables, seq_lens)
+    if seq_lens.size(0) != num_seqs:
+        raise ValueError("seq_lens and block_tables must have a row for every query")
+    _positive("num_selected", num_selected, 1)
+    _positive("sink_pages", sink_pages, 0)
+    _positive("recent_pages", recent_pages, 1)
+    if sink_pages + recent_pages > num_selected:
+        raise ValueError("sink_pages + recent_pages must be at most num_selected")
+    width = block_tables.size(1)
+    if num_seqs and (width == 0 or page_bounds.size(0) == 0):
+        raise ValueError("page selection needs pages")
+    tables = torch.empty((num_seqs, num_kv_heads, num_selected), dtype=torch.int32, device=device)
+    lens = torch.empty(num_seqs, dtype=torch.int32, device=device)
+    workspace = _selection_workspace(
+        workspace, selection_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, width, num_selected), device)
+    if num_seqs == 0:
+        return tables, lens
+    q = _aligned_rows(q)
+    _call_on(
+        device, "mva_select_pages",
+        q.data_ptr(), q.stride(0), q.stride(1), page_bounds.data_ptr(), page_bounds.size(0),
+        block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), num_seqs,
+        num_selected, sink_pages, recent_pages, tables.data_ptr(), lens.data_ptr(),
+        workspace.data_ptr(), workspace.numel(), num_q_heads, num_kv_heads, HEAD_DIM, PAGE_SIZE,
+        _native.dtype_code(dtype), _native.stream_handle(device),
+    )
+    return tables, lens
+
+
+def paged_decode_selected(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    tables: torch.Tensor,
+    lens: torch.Tensor,
+    softmax_scale: float,
+    *,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of one query a row over its selected pages; returns ``out``
+    (``[S, Hq, 128]``, new unless given).
+
+    ``tables`` (int32 ``[S, Hkv, n]``, rows dense) lists pages of the 16-bit caches
+    (``[P, 16, Hkv, 128]``) for each row and KV head; ``lens`` (int32 ``[S]``) counts
+    the tokens they hold: all pages of a list but its last are full.  A row of
+    ``lens`` 0 gives zeros."""
+    _check_queries(q)
+    device, dtype = q.device, q.dtype
+    for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _check_cache(name, cache, device, dtype)
+    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+        raise ValueError("k_cache and v_cache must share shape and layout")
+    num_seqs, num_q_heads, num_kv_heads = q.size(0), q.size(1), k_cache.size(2)
+    _check_groups(num_q_heads, num_kv_heads)
+    for name, t in (("tables", tables), ("lens", lens)):
+        if t.device != device:
+            raise RuntimeError(f"{name} must be on the device of the other tensors")
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+    if tables.dim() != 3 or tables.shape[:2] != (num_seqs, num_kv_heads) or tables.size(2) == 0:
+        raise ValueError("tables must be [rows, num_kv_heads, pages]")
+    if tables.size(2) > 1 and tables.stride(2) != 1:
+        raise ValueError("tables must hold dense lists")
+    if lens.shape != (num_seqs,) or (num_seqs > 1 and lens.stride(0) != 1):
+        raise ValueError("lens must be dense, one for every row")
+    if out is None:
+        out = torch.empty(q.shape, dtype=dtype, device=device)
+    elif out.device != device or out.dtype != dtype or out.shape != q.shape or out.stride(2) != 1:
+        raise ValueError("out must have the queries' shape, dtype and device, with unit inner stride")
+    if num_seqs == 0:
+        return out
+    if k_cache.size(0) == 0:
+        raise ValueError("attention needs cache pages")
+    workspace = _selection_workspace(
+        workspace, selection_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, 0, tables.size(2)), device)
+    q = _aligned_rows(q)
+    _call_on(
+        device, "mva_paged_decode_selected",
+        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.size(0),
+        k_cache.stride(0), k_cache.stride(1), tables.data_ptr(), tables.stride(0), tables.stride(1), lens.data_ptr(),
+        num_seqs, tables.size(2), out.data_ptr(), out.stride(0), out.stride(1),
+        workspace.data_ptr(), workspace.numel(), num_q_heads, num_kv_heads, HEAD_DIM, PAGE_SIZE,
+        float(softmax_scale), _native.dtype_code(dtype), _native.stream_handle(device),
+    )
+    return out
