@@ -1622,6 +1622,8 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
             raise ValueError("sink_pages + recent_pages must be at most selected_pages")
         # The page bounds of the layer that forward runs.
         self._page_bounds: torch.Tensor | None = None
+        # Workspaces of eager steps, by GPU and stream.
+        self._stream_workspaces: dict[tuple, torch.Tensor] = {}
 
     def _backend_mixed_reason(self) -> str | None:
         return "MIXED batches with selected pages run as prefill + decode launches"
@@ -1662,20 +1664,36 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
         finally:
             self._page_bounds = None
 
+    def _get_workspace(self, nbytes: int, device: torch.device) -> torch.Tensor:
+        """The workspace of the layer that follows: a graph's own, from its pool, for
+        the layers captured on one stream, else one of the current stream.  Its
+        counters are cleared when it is made (in a graph, once a replay)."""
+        capture = self._capture_of(device)
+        if capture is not None:
+            held = self._captured_workspace
+            if held is None or held[0] != capture or held[1].numel() < nbytes:
+                self._captured_workspace = held = (capture, ops.new_selection_workspace(nbytes, device))
+            return held[1]
+        key = (device.index, _native.stream_handle(device))
+        workspace = self._stream_workspaces.get(key)
+        if workspace is None or workspace.numel() < nbytes:
+            self._stream_workspaces[key] = workspace = ops.new_selection_workspace(nbytes, device)
+        return workspace
+
     def _attend(self, q, k_cache, v_cache, block_tables, seq_lens, out) -> None:
         if self._page_bounds is None:
             raise ValueError("decode over selected pages needs page_bounds")
-        if self._page_bounds.size(0) != k_cache.size(0):
-            raise ValueError("page_bounds must have the cache's number of pages")
         nbytes = ops.selection_workspace_bytes(q.size(0), self.num_q_heads, self.num_kv_heads, block_tables.size(1),
                                                self.selected_pages)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        tables, lens = ops.select_pages(q, self._page_bounds, block_tables, seq_lens, self.selected_pages,
-                                        self.sink_pages, self.recent_pages, workspace=workspace)
-        ops.paged_decode_selected(q, k_cache, v_cache, tables, lens, self.softmax_scale, out=out, workspace=workspace)
+        ops.sparse_decode(q, self._page_bounds, k_cache, v_cache, block_tables, seq_lens, self.softmax_scale,
+                          self.selected_pages, self.sink_pages, self.recent_pages, out=out,
+                          workspace=self._get_workspace(nbytes, q.device))
 
     def _run_decode(self, q, k_cache, v_cache, common, metadata: MI355XAttentionMetadata, output) -> None:
         first, rows = common.num_prefill_seqs, common.num_prefill_tokens
+        if first == 0:
+            self._attend(q, k_cache, v_cache, metadata.block_tables, metadata.seq_lens, output)
+            return
         self._attend(q[rows:], k_cache, v_cache, metadata.block_tables[first:], metadata.seq_lens[first:],
                      output[rows:])
 

@@ -578,6 +578,168 @@ PyObject* forward_inputs_ok_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- decode over selected pages ----
+
+constexpr int64_t kPage = 16;
+
+// A 16-bit cache [pages, 16, heads, 128] of q's type on its device, its rows of
+// packed heads apart, pages outermost.
+bool selectable(const Tensor* c, const Tensor& like) {
+  if (!c || c->dim() != 4 || c->scalar_type() != like.scalar_type() || c->device() != like.device() ||
+      c->size(0) == 0 || c->size(1) != kPage || c->size(3) != kHeadDim || c->stride(3) != 1 ||
+      c->stride(2) != kHeadDim || c->size(2) == 0)
+    return false;
+  const int64_t row = c->size(2) * kHeadDim;
+  return c->stride(1) >= row && c->stride(0) >= (kPage - 1) * c->stride(1) + row;
+}
+bool bounds_of_heads(const Tensor* b, const Tensor& like, int64_t heads) {
+  return b && b->dim() == 4 && b->scalar_type() == like.scalar_type() && b->device() == like.device() &&
+         b->size(0) > 0 && b->size(1) == heads && b->size(2) == 2 && b->size(3) == kHeadDim && b->is_contiguous();
+}
+bool table_rows(const Tensor* bt, const Tensor* sl, const Tensor& like) {
+  return bt && sl && bt->dim() == 2 && sl->dim() == 1 && bt->scalar_type() == at::kInt &&
+         sl->scalar_type() == at::kInt && bt->device() == like.device() && sl->device() == like.device() &&
+         bt->size(0) == sl->size(0) && bt->size(0) > 0 && bt->size(1) > 0 && bt->stride(1) == 1 && sl->is_contiguous();
+}
+bool queries_of(const Tensor* q) {
+  return q && dtype_code(*q) >= 0 && head_rows(*q, *q) && q->size(0) > 0 && aligned_rows(*q) &&
+         q->device().index() == c10::hip::current_device();
+}
+bool workspace_for(const Tensor* ws, const Tensor& q, int64_t heads, int64_t width, int64_t selected) {
+  const int64_t need = mva_selection_workspace_bytes(q.size(0), (int)q.size(1), (int)heads, width, selected);
+  return ws && ws->scalar_type() == at::kByte && ws->device() == q.device() && ws->is_contiguous() && need >= 0 &&
+         ws->numel() >= need;
+}
+bool groups(const Tensor& q, int64_t heads) {
+  return heads > 0 && q.size(1) > 0 && q.size(1) % heads == 0 && q.size(1) / heads <= 16;
+}
+bool page_numbers(PyObject* const* a, int64_t (&v)[3]) {
+  for (int i = 0; i < 3; ++i)
+    if (PyBool_Check(a[i]) || !as_int(a[i], &v[i])) return false;
+  return v[1] >= 0 && v[2] >= 1 && v[0] <= (int64_t(1) << 24) && v[1] <= v[0] && v[2] <= v[0] - v[1];
+}
+
+// (k_cache, page_bounds, block_tables, seq_lens, query_start_loc | None,
+//  num_tokens | None): True when launched.
+PyObject* update_page_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 6) return none();
+    const Tensor *kc = plain(a[0]), *bounds = plain(a[1]), *bt = plain(a[2]), *sl = plain(a[3]);
+    const Tensor* qsl = a[4] == Py_None ? nullptr : plain(a[4]);
+    if (!kc || dtype_code(*kc) < 0 || !selectable(kc, *kc) || !bounds_of_heads(bounds, *kc, kc->size(2)) ||
+        bounds->size(0) != kc->size(0) || !table_rows(bt, sl, *kc) ||
+        kc->device().index() != c10::hip::current_device())
+      return none();
+    const int64_t seqs = sl->size(0);
+    int64_t tokens = seqs;
+    if (a[4] != Py_None) {
+      if (!qsl || qsl->scalar_type() != at::kInt || qsl->device() != kc->device() || qsl->dim() != 1 ||
+          qsl->size(0) != seqs + 1 || !qsl->is_contiguous() || PyBool_Check(a[5]) || !as_int(a[5], &tokens) ||
+          tokens <= 0)
+        return none();
+    } else if (a[5] != Py_None) {
+      return none();
+    }
+    void* const stream = stream_of(*kc);
+    const int status = unlocked(
+        mva_update_page_bounds, ptr(*kc), kc->size(0), kc->stride(0), kc->stride(1), ptr(*bounds), words(bt),
+        bt->stride(0), bt->size(1), words(sl), words(qsl), seqs, tokens, (int)kc->size(2), kHeadDim, (int)kPage,
+        dtype_code(*kc), stream);
+    return launched("mva_update_page_bounds", status);
+  });
+}
+
+int select(const Tensor& q, const Tensor& bounds, const Tensor& bt, const Tensor& sl, const int64_t (&pages)[3],
+           const Tensor& tables, const Tensor& lens, const Tensor& ws, void* stream) {
+  return unlocked(mva_select_pages, ptr(q), q.stride(0), q.stride(1), ptr(bounds), bounds.size(0), words(&bt),
+                  bt.stride(0), bt.size(1), words(&sl), q.size(0), pages[0], pages[1], pages[2], (int32_t*)ptr(tables),
+                  (int32_t*)ptr(lens), ptr(ws), ws.numel(), (int)q.size(1), (int)bounds.size(1), kHeadDim, (int)kPage,
+                  dtype_code(q), stream);
+}
+int attend(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& tables, const Tensor& lens, double scale,
+           const Tensor& out, const Tensor& ws, void* stream) {
+  return unlocked(mva_paged_decode_selected, ptr(q), q.stride(0), q.stride(1), ptr(kc), ptr(vc), kc.size(0),
+                  kc.stride(0), kc.stride(1), words(&tables), tables.stride(0), tables.stride(1), words(&lens),
+                  q.size(0), tables.size(2), ptr(out), out.stride(0), out.stride(1), ptr(ws), ws.numel(),
+                  (int)q.size(1), (int)kc.size(2), kHeadDim, (int)kPage, (float)scale, dtype_code(q), stream);
+}
+
+// (q, page_bounds, block_tables, seq_lens, num_selected, sink_pages, recent_pages,
+//  workspace): (tables, lens).
+PyObject* select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int64_t pages[3];
+    if (n != 8 || !page_numbers(a + 4, pages)) return none();
+    const Tensor *q = plain(a[0]), *bounds = plain(a[1]), *bt = plain(a[2]), *sl = plain(a[3]), *ws = plain(a[7]);
+    if (!queries_of(q) || !bounds || bounds->dim() != 4 || !groups(*q, bounds->size(1)) ||
+        !bounds_of_heads(bounds, *q, bounds->size(1)) || !table_rows(bt, sl, *q) || sl->size(0) != q->size(0) ||
+        !workspace_for(ws, *q, bounds->size(1), bt->size(1), pages[0]))
+      return none();
+    const auto options = sl->options().requires_grad(false);
+    const Tensor tables = at::empty({q->size(0), bounds->size(1), pages[0]}, options);
+    const Tensor lens = at::empty({q->size(0)}, options);
+    const int status = select(*q, *bounds, *bt, *sl, pages, tables, lens, *ws, stream_of(*q));
+    if (status != 0) return launched("mva_select_pages", status, nullptr);
+    PyObject* pair = PyTuple_New(2);
+    if (pair == nullptr) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(tables));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(lens));
+    return pair;
+  });
+}
+
+// (q, k_cache, v_cache, tables, lens, scale, out | None, workspace): out.
+PyObject* paged_decode_selected(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    double scale;
+    if (n != 8 || !as_float(a[5], &scale)) return none();
+    const Tensor *q = plain(a[0]), *kc = plain(a[1]), *vc = plain(a[2]), *tables = plain(a[3]), *lens = plain(a[4]);
+    const Tensor *given = a[6] == Py_None ? nullptr : plain(a[6]), *ws = plain(a[7]);
+    if (!queries_of(q) || !selectable(kc, *q) || !selectable(vc, *q) || kc->sizes() != vc->sizes() ||
+        kc->strides() != vc->strides() || !groups(*q, kc->size(2)) || !tables || !lens ||
+        tables->scalar_type() != at::kInt || tables->device() != q->device() || tables->dim() != 3 ||
+        tables->size(0) != q->size(0) || tables->size(1) != kc->size(2) || tables->size(2) == 0 ||
+        tables->stride(2) != 1 || lens->scalar_type() != at::kInt || lens->device() != q->device() ||
+        lens->dim() != 1 || lens->size(0) != q->size(0) || !lens->is_contiguous() ||
+        !workspace_for(ws, *q, kc->size(2), 0, tables->size(2)))
+      return none();
+    if (a[6] != Py_None && (!given || given->sizes() != q->sizes() || !head_rows(*given, *q))) return none();
+    const Tensor out = given ? *given : at::empty(q->sizes(), q->options().requires_grad(false));
+    const int status = attend(*q, *kc, *vc, *tables, *lens, scale, out, *ws, stream_of(*q));
+    if (given && status == 0) {
+      Py_INCREF(a[6]);
+      return a[6];
+    }
+    return launched("mva_paged_decode_selected", status, out);
+  });
+}
+
+// (q, page_bounds, k_cache, v_cache, block_tables, seq_lens, scale, num_selected,
+//  sink_pages, recent_pages, out, workspace): True when launched.
+PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    double scale;
+    int64_t pages[3];
+    if (n != 12 || !as_float(a[6], &scale) || !page_numbers(a + 7, pages)) return none();
+    const Tensor *q = plain(a[0]), *bounds = plain(a[1]), *kc = plain(a[2]), *vc = plain(a[3]), *bt = plain(a[4]);
+    const Tensor *sl = plain(a[5]), *out = plain(a[10]), *ws = plain(a[11]);
+    if (!queries_of(q) || !selectable(kc, *q) || !selectable(vc, *q) || kc->sizes() != vc->sizes() ||
+        kc->strides() != vc->strides() || !groups(*q, kc->size(2)) || !bounds_of_heads(bounds, *q, kc->size(2)) ||
+        bounds->size(0) != kc->size(0) || !table_rows(bt, sl, *q) || sl->size(0) != q->size(0) || !out ||
+        out->sizes() != q->sizes() || !head_rows(*out, *q) ||
+        !workspace_for(ws, *q, kc->size(2), bt->size(1), pages[0]))
+      return none();
+    const auto options = sl->options().requires_grad(false);
+    const Tensor tables = at::empty({q->size(0), kc->size(2), pages[0]}, options);
+    const Tensor lens = at::empty({q->size(0)}, options);
+    void* const stream = stream_of(*q);
+    int status = select(*q, *bounds, *bt, *sl, pages, tables, lens, *ws, stream);
+    if (status != 0) return launched("mva_select_pages", status);
+    status = attend(*q, *kc, *vc, tables, lens, scale, *out, *ws, stream);
+    return launched("mva_paged_decode_selected", status);
+  });
+}
+
 // (device index): number of the graph capture that torch's current stream of
 // the device is in, or 0.
 PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -600,7 +762,9 @@ PyMethodDef kMethods[] = {MVA_METHOD(silu_and_mul),       MVA_METHOD(rms_norm), 
                           MVA_METHOD(paged_mixed),        MVA_METHOD(forward_inputs_ok), MVA_METHOD(capture_id),
                           MVA_METHOD(store_kvcache_mxfp4), MVA_METHOD(load_kvcache_mxfp4),
                           MVA_METHOD(paged_decode_mxfp4), MVA_METHOD(paged_prefill_mxfp4),
-                          MVA_METHOD(forward_inputs_ok_mxfp4),
+                          MVA_METHOD(forward_inputs_ok_mxfp4), MVA_METHOD(update_page_bounds),
+                          MVA_METHOD(select_pages),       MVA_METHOD(paged_decode_selected),
+                          MVA_METHOD(sparse_decode),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "mva_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

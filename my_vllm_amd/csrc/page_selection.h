@@ -1,7 +1,9 @@
 // Sizes that the page selection and the attention over selected pages share.
 //
-// Workspace: [partials of the attention][score keys of the selection].  The
-// partials come first: the attention knows its own sizes only.
+// Workspace: [arrival counters of the selection][of the attention][partials of
+// the attention][score keys of the selection].  The counters lie at one place
+// whatever the sizes: they are zero between launches, of any sizes.  The partials
+// come before the keys: the attention knows its own sizes only.
 #pragma once
 
 #include <cstdint>
@@ -10,6 +12,10 @@ namespace mva {
 
 constexpr int kPageTokens = 16;
 constexpr int kMaxQueryGroup = 16;
+
+// (row, KV head) pairs of a launch whose workgroups count themselves in.
+constexpr int kSelectionCounters = 4096;
+constexpr int64_t kSelectionHeaderBytes = 2 * kSelectionCounters * 4;
 
 inline int64_t align_up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 

@@ -30,22 +30,40 @@ struct SelectedParams {
   int64_t out_head_stride;
   float* part_lse;  // [S][Hkv][parts][G]
   float* part_o;    // [S][Hkv][parts][G][128]
+  int* counters;    // [S][Hkv], zero between launches
   int num_kv_heads;
   int group;
   float scale_log2;
 };
 
-constexpr int kSelWaves = 8;
-constexpr int kSelWaveLds = 2 * kDecodePageBytes;
+constexpr int kSelWaves = 4;       // wavefronts of a workgroup
+constexpr int kSelGroupsPerCu = 3;  // workgroups that a CU holds
+constexpr int kJoinRow = kHeadDim + 4;  // floats of a joined row in LDS: its 16 rows start in different banks
 
-// One workgroup per (row, KV head, part); its wavefronts take the part's pages
-// in turns, each with a running maximum and sum of its own, and join in LDS.
+// A page of one KV head in registers.  k[j]: lane (q4, c) channels 32 j + 8 q4 .. + 7
+// of token c, the A operand of S^T = K Q^T; v[e]: channels 8 c .. 8 c + 7 of token
+// 4 q4 + e, so that halves of v[0 .. 3] make the A operand of O^T += V^T P^T
+// whose rows are the channels 8 m + i, m the row of the matrix instruction.
 template <typename T>
-__global__ __launch_bounds__(64 * kSelWaves) void selected_decode_kernel(SelectedParams p) {
+struct PageRegs {
+  typename Elem<T>::v8 k[4];
+  u32x4 v[4];
+};
+
+// One workgroup per (row, part of its pages, KV head).  Its wavefronts take the
+// part's pages in turns, each with a running maximum and sum of its own, and
+// join in LDS; the row's last workgroup joins the parts.
+//
+// Pages come straight into registers, two ahead of the arithmetic, in pieces of
+// 16 bytes a lane that are contiguous over 64 (K) or 256 bytes (V); no
+// LDS is filled, so a CU holds 12 wavefronts with two pages each.
+template <typename T>
+__global__ __launch_bounds__(64 * kSelWaves, kSelGroupsPerCu) void selected_decode_kernel(SelectedParams p) {
   typedef typename Elem<T>::v8 V8;
   typedef typename Elem<T>::v4 V4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds_all[kSelWaves * kSelWaveLds];
+  __shared__ __attribute__((aligned(16))) float join_o[kSelWaves][16][kJoinRow];
   __shared__ float join_m[kSelWaves][16], join_l[kSelWaves][16];
+  __shared__ int join_last;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int q4 = lane >> 4, c = lane & 15;
@@ -55,7 +73,10 @@ __global__ __launch_bounds__(64 * kSelWaves) void selected_decode_kernel(Selecte
   const int G = p.group;
   const int len = sload(p.lens, s);
   const int pages = len <= 0 ? 0 : min((int)(((int64_t)len + kPageSize - 1) / kPageSize), p.num_selected);
-  const int begin = (int)((int64_t)pages * part / p.parts), end = (int)((int64_t)pages * (part + 1) / p.parts);
+  // Parts of a row of few pages: no more than it has groups of kSelWaves pages.
+  const int parts = min(p.parts, max(1, (pages + kSelWaves - 1) / kSelWaves));
+  if (part >= parts) return;
+  const int begin = (int)((int64_t)pages * part / parts), end = (int)((int64_t)pages * (part + 1) / parts);
   const int32_t* table = p.tables + s * p.seq_table_stride + h * p.head_table_stride;
 
   V8 qf[4];
@@ -63,72 +84,114 @@ __global__ __launch_bounds__(64 * kSelWaves) void selected_decode_kernel(Selecte
   for (int j = 0; j < 4; ++j) {
     qf[j] = V8{};
     if (c < G)
-      qf[j] = ld16<V8>((const T*)p.q + s * p.q_tok_stride + (int64_t)(h * G + c) * p.q_head_stride + 32 * q4 + 8 * j);
+      qf[j] = ld16<V8>((const T*)p.q + s * p.q_tok_stride + (int64_t)(h * G + c) * p.q_head_stride + 32 * j + 8 * q4);
   }
-  f32x4 o[8];
+  f32x4 o[8];  // o[i][r] = O[g = c][channel 32 q4 + 8 r + i]
 #pragma unroll
-  for (int mt = 0; mt < 8; ++mt) o[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int i = 0; i < 8; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY;  // reference maximum of the scaled scores (log2), per g = c
+  float l = 0.f;        // this lane's share of the running sum
 
-  for (int i = begin + wave; i < end; i += kSelWaves) {
-    int id = sload(table, i);
-    if (id < 0 || id >= p.num_pages) id = 0;
-    const int64_t base = (int64_t)id * p.page_stride + h * kHeadDim;
-    const int left = len - i * kPageSize;  // tokens from this page on
-    // K rows as the A operand, straight from memory: lane (q4, c) token c.
+  // Byte offsets in a page, one register each beside the page's address in scalar ones.
+  const uint32_t tok = (uint32_t)p.tok_stride * 2;
+  const uint32_t k_off = c * tok + 16 * q4;
+  uint32_t v_off[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v_off[e] = (4 * q4 + e) * tok + 16 * c;
+  auto load = [&](PageRegs<T>& r, int id) __attribute__((always_inline)) {
+    const int64_t base = ((int64_t)id * p.page_stride + h * kHeadDim) * 2;
+    const uint8_t* const k = (const uint8_t*)p.k_cache + base;
+    const uint8_t* const v = (const uint8_t*)p.v_cache + base;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.k[j] = ld16<V8>(k + 64 * j + (size_t)k_off);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.v[e] = ld16<u32x4>(v + (size_t)v_off[e]);
+  };
+  // `left`: tokens of the row from this page on (16 or more unless it is the last one).
+  auto compute = [&](PageRegs<T>& r, int left, auto may_end) __attribute__((always_inline)) {
     f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const V8 k = ld16<V8>((const T*)p.k_cache + base + c * p.tok_stride + 32 * q4 + 8 * j);
-      sc = Elem<T>::mfma16(k, qf[j], sc);
-    }
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (4 * q4 + r >= left) sc[r] = -INFINITY;
-      tmax = fmaxf(tmax, sc[r]);
-    }
-    tmax = wave_max16(tmax) * p.scale_log2;
-    const float m_new = fmaxf(m, tmax);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = fast_exp2(m - m_use);
-    m = m_new;
-    l *= alpha;
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) o[mt] *= alpha;
-    V4 pf;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float pr = fast_exp2(sc[r] * p.scale_log2 - m_use);
-      l += pr;
-      pf[r] = (T)pr;
-    }
-    // V^T operands element by element: lane (q4, c) tokens 4 q4 .. + 3, channel 16 mt + c.
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-      V4 v;
+    for (int j = 0; j < 4; ++j) sc = Elem<T>::mfma16(r.k[j], qf[j], sc);
+    // sc[e] = S[token 4 q4 + e][g = c].  Rows behind the last token, whatever they hold, do not count.
+    if (decltype(may_end)::value && left < kPageSize) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int t = 4 * q4 + e;
-        v[e] = t < left ? ((const T*)p.v_cache)[base + t * p.tok_stride + 16 * mt + c] : (T)0.f;
+        if (4 * q4 + e >= left) {
+          sc[e] = -INFINITY;
+          r.v[e] = u32x4{0u, 0u, 0u, 0u};
+        }
       }
-      o[mt] = Elem<T>::mfma16k16(v, pf, o[mt]);
     }
+    const float tmax = wave_max16(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]))) * p.scale_log2;
+    // The reference is the maximum so far: the largest P are near 1, where the operand's type rounds them least.
+    if (__any(tmax > m)) {
+      const float m_new = fmaxf(m, tmax);
+      const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] *= alpha;
+    }
+    const float m_use = m == -INFINITY ? 0.f : m;
+    V4 pf;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float pr = fast_exp2(sc[e] * p.scale_log2 - m_use);
+      l += pr;
+      pf[e] = (T)pr;  // the operand's type: half a step of it
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const u32x2 lo = {__builtin_amdgcn_perm(r.v[1][w], r.v[0][w], 0x05040100u),
+                        __builtin_amdgcn_perm(r.v[3][w], r.v[2][w], 0x05040100u)};
+      const u32x2 hi = {__builtin_amdgcn_perm(r.v[1][w], r.v[0][w], 0x07060302u),
+                        __builtin_amdgcn_perm(r.v[3][w], r.v[2][w], 0x07060302u)};
+      o[2 * w] = Elem<T>::mfma16k16(__builtin_bit_cast(V4, lo), pf, o[2 * w]);
+      o[2 * w + 1] = Elem<T>::mfma16k16(__builtin_bit_cast(V4, hi), pf, o[2 * w + 1]);
+    }
+  };
+
+  // This wavefront's pages begin + wave + kSelWaves * k, 64 ids at a time.
+  const int mine = end - begin > wave ? (end - begin - wave + kSelWaves - 1) / kSelWaves : 0;
+  for (int k0 = 0; k0 < mine; k0 += 64) {
+    const int n = min(64, mine - k0);
+    const int at = begin + wave + kSelWaves * k0;
+    int ids = table[at + kSelWaves * min(lane, n - 1)];
+    if (ids < 0 || ids >= p.num_pages) ids = 0;
+    PageRegs<T> a, b;
+    load(a, __builtin_amdgcn_readlane(ids, 0));
+    for (int k = 1; k < n; ++k) {
+      load(b, __builtin_amdgcn_readlane(ids, k));
+      compute(a, kPageSize, std::false_type{});
+      a = b;
+    }
+    compute(a, len - (at + kSelWaves * (n - 1)) * kPageSize, std::true_type{});
   }
 
-  // Join the wavefronts: o[mt][r] = O[g = c][d = 16 mt + 4 q4 + r].
   const float l_tot = wave_sum16(l);
   if (q4 == 0) {
     join_m[wave][c] = m;
     join_l[wave][c] = l_tot;
   }
-  float* mine = (float*)(lds_all + wave * kSelWaveLds);  // [g][128]
+  if (c < G) {
 #pragma unroll
-  for (int mt = 0; mt < 8; ++mt)
-    if (c < G) *(f32x4*)(mine + c * kHeadDim + 16 * mt + 4 * q4) = o[mt];
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4)
+        *(f32x4*)&join_o[wave][c][32 * q4 + 8 * r + i] = f32x4{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]};
+    }
+  }
   __syncthreads();
-  for (int v = threadIdx.x; v < G * (kHeadDim / 4); v += 64 * kSelWaves) {
-    const int g = v / (kHeadDim / 4), d = v % (kHeadDim / 4) * 4;
+  // Four channels of a query a thread, kSelWaves * 2 queries at a time.
+  const int g0 = threadIdx.x / (kHeadDim / 4), d = threadIdx.x % (kHeadDim / 4) * 4;
+  const int64_t slot0 = (s * p.num_kv_heads + h) * p.parts * G;
+  auto write = [&](int g, f32x4 acc, float inv) {
+    V4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(acc[e] * inv);
+    *(V4*)((T*)p.out + s * p.out_tok_stride + (int64_t)(h * G + g) * p.out_head_stride + d) = y;
+  };
+  for (int g = g0; g < G; g += 2 * kSelWaves) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kSelWaves; ++w) top = fmaxf(top, join_m[w][g]);
@@ -139,55 +202,72 @@ __global__ __launch_bounds__(64 * kSelWaves) void selected_decode_kernel(Selecte
     for (int w = 0; w < kSelWaves; ++w) {
       const float f = fast_exp2(join_m[w][g] - use);
       sum += f * join_l[w][g];
-      acc += f * *(const f32x4*)((const float*)(lds_all + w * kSelWaveLds) + g * kHeadDim + d);
+      acc += f * *(const f32x4*)&join_o[w][g][d];
     }
     const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-    if (p.parts == 1) {
-      V4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(acc[e] * inv);
-      *(V4*)((T*)p.out + s * p.out_tok_stride + (int64_t)(h * G + g) * p.out_head_stride + d) = y;
+    if (parts == 1) {
+      write(g, acc, inv);
     } else {
-      const int64_t slot = ((s * p.num_kv_heads + h) * p.parts + part) * G + g;
-      *(f32x4*)(p.part_o + slot * kHeadDim + d) = acc * inv;
-      if (d == 0) p.part_lse[slot] = sum > 0.f ? use + fast_log2(sum) : -INFINITY;
+      const int64_t slot = slot0 + part * G + g;
+      store16_device_untracked(p.part_o + slot * kHeadDim + d, __builtin_bit_cast(u32x4, acc * inv));
+      if (d == 0) store4_device_untracked(p.part_lse + slot, sum > 0.f ? use + fast_log2(sum) : -INFINITY);
     }
   }
-}
-
-// One wavefront per (row, query head): the parts of a row joined.
-template <typename T>
-__global__ __launch_bounds__(256) void selected_merge_kernel(SelectedParams p, int64_t rows) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (s, h, g)
-  if (row >= rows) return;
-  const int g = (int)(row % p.group);
-  const int64_t sh = row / p.group;
-  float top = -INFINITY;
-  for (int k = 0; k < p.parts; ++k) top = fmaxf(top, p.part_lse[(sh * p.parts + k) * p.group + g]);
-  const float use = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, a = 0.f, b = 0.f;
-  for (int k = 0; k < p.parts; ++k) {
-    const int64_t slot = (sh * p.parts + k) * p.group + g;
-    const float f = fast_exp2(p.part_lse[slot] - use);
-    sum += f;
-    a += f * p.part_o[slot * kHeadDim + 2 * lane];
-    b += f * p.part_o[slot * kHeadDim + 2 * lane + 1];
+  if (parts == 1) return;
+  // Parts meet in memory: stores that reach it, counted in once they have, and
+  // loads that come from there.
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int* counter = p.counters + s * p.num_kv_heads + h;
+    const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    join_last = last;
   }
-  const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-  T* out = (T*)p.out + sh / p.num_kv_heads * p.out_tok_stride +
-           (sh % p.num_kv_heads * p.group + g) * p.out_head_stride + 2 * lane;
-  out[0] = (T)(a * inv);
-  out[1] = (T)(b * inv);
+  __syncthreads();
+  if (!join_last) return;
+  constexpr int kAtOnce = 8;
+  for (int g = g0; g < G; g += 2 * kSelWaves) {
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, sum = 0.f;
+    for (int k = 0; k < parts; k += kAtOnce) {
+      float lse[kAtOnce];
+      f32x4 rows[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int64_t slot = slot0 + min(k + i, parts - 1) * G + g;
+        lse[i] = part_load<true>(p.part_lse + slot);
+        rows[i] = part_load4<true>(p.part_o + slot * kHeadDim + d);
+      }
+      float most = top;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (k + i >= parts) lse[i] = -INFINITY;
+        most = fmaxf(most, lse[i]);
+      }
+      const float use = most == -INFINITY ? 0.f : most;
+      const float alpha = fast_exp2(top - use);
+      top = most;
+      sum *= alpha;
+      acc *= alpha;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float f = fast_exp2(lse[i] - use);
+        sum += f;
+        acc += f * rows[i];
+      }
+    }
+    write(g, acc, sum > 0.f ? 1.0f / sum : 0.f);
+  }
 }
 
-// Parts a row's pages are cut into, one workgroup each: enough workgroups for
-// 256 CUs, as long as every wavefront has a page.
+// Parts a row's pages are cut into, one workgroup each: as many workgroups as
+// the GPU holds, as long as every wavefront has a page.
 int selected_parts(int64_t num_seqs, int hkv, int64_t num_selected) {
   const int64_t rows = num_seqs * hkv;
   const int64_t most = (num_selected + kSelWaves - 1) / kSelWaves;
-  const int64_t want = rows > 0 ? (256 + rows - 1) / rows : 1;
-  return (int)(want < most ? want : most);
+  const int64_t want = rows > 0 ? 256 * kSelGroupsPerCu / rows : 1;
+  return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 }  // namespace
@@ -221,29 +301,29 @@ extern "C" int mva_paged_decode_selected(const void* q, int64_t q_token_stride, 
        (uint64_t)(q_token_stride * 2) | (uint64_t)(q_head_stride * 2) | (uint64_t)(page_stride * 2) |
        (uint64_t)(token_stride * 2)) % 16)
     return set_error("selected attention: q / cache buffers and strides must be 16-byte aligned");
+  if (token_stride < 0 || token_stride > (1 << 26))
+    return set_error("selected attention: a page's tokens must lie less than 2^26 elements apart");
   if (((uint64_t)(uintptr_t)out | (uint64_t)(out_token_stride * 2) | (uint64_t)(out_head_stride * 2)) % 8)
     return set_error("selected attention: output buffer and strides must be 8-byte aligned");
   const int parts = selected_parts(num_seqs, num_kv_heads, num_selected);
   if (parts > 1 && (workspace == nullptr || (uint64_t)(uintptr_t)workspace % 16 ||
-                    workspace_bytes < selection_part_bytes(num_seqs, num_q_heads, num_kv_heads, num_selected)))
+                    workspace_bytes < kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads,
+                                                                                   num_kv_heads, num_selected)))
     return set_error("selected attention: workspace missing, too small or unaligned");
   const int64_t blocks = num_seqs * num_kv_heads * parts;
   if (blocks > 0xffffffffLL / (64 * kSelWaves)) return set_error("selected attention: too many rows for one launch");
   const int64_t slots = num_seqs * num_q_heads * parts;
-  SelectedParams p = {q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, page_stride, token_stride, tables,
-                      seq_table_stride, head_table_stride, lens, (int)num_selected, parts, out, out_token_stride,
-                      out_head_stride, (float*)workspace, (float*)((uint8_t*)workspace + align_up256(slots * 4)),
-                      num_kv_heads, num_q_heads / num_kv_heads, softmax_scale * 1.4426950408889634f};
+  uint8_t* const ws = (uint8_t*)workspace;
+  float* const part_lse = (float*)(ws + kSelectionHeaderBytes);
+  const SelectedParams p = {q, q_token_stride, q_head_stride, k_cache, v_cache, num_pages, page_stride, token_stride,
+                            tables, seq_table_stride, head_table_stride, lens, (int)num_selected, parts, out,
+                            out_token_stride, out_head_stride, part_lse,
+                            (float*)((uint8_t*)part_lse + align_up256(slots * 4)), (int*)ws + kSelectionCounters,
+                            num_kv_heads, num_q_heads / num_kv_heads, softmax_scale * 1.4426950408889634f};
   const hipStream_t st = (hipStream_t)stream;
-  const int64_t rows = num_seqs * num_q_heads;
-  if (dtype == kBF16) {
+  if (dtype == kBF16)
     hipLaunchKernelGGL(selected_decode_kernel<__bf16>, dim3((uint32_t)blocks), dim3(64 * kSelWaves), 0, st, p);
-    if (parts > 1)
-      hipLaunchKernelGGL(selected_merge_kernel<__bf16>, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st, p, rows);
-  } else {
+  else
     hipLaunchKernelGGL(selected_decode_kernel<_Float16>, dim3((uint32_t)blocks), dim3(64 * kSelWaves), 0, st, p);
-    if (parts > 1)
-      hipLaunchKernelGGL(selected_merge_kernel<_Float16>, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st, p, rows);
-  }
   return check_launch("selected_decode");
 }

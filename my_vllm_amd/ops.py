@@ -1147,6 +1147,10 @@ def paged_prefill_mxfp4(
 # ---- decode over selected pages ---------------------------------------------------
 
 
+# Counters at the start of a selection workspace (kSelectionHeaderBytes).
+SELECTION_HEADER_BYTES = 32768
+
+
 def page_bounds_shape(num_pages: int, num_kv_heads: int) -> tuple[int, int, int, int]:
     """Shape of a layer's page bounds, in the cache's dtype: for every full page
     of ``num_pages`` and KV head the smallest (index 0) and the largest (index 1)
@@ -1239,6 +1243,8 @@ def update_page_bounds(
     read: the last page of a row is always selected); a page without new tokens,
     such as a shared prefix's, keeps the ones that it has.  A NaN in a channel
     makes both of its bounds NaN."""
+    if _native.host_ops().update_page_bounds(k_cache, page_bounds, block_tables, seq_lens, query_start_loc, num_tokens):
+        return
     if not k_cache.is_cuda:
         raise RuntimeError("update_page_bounds expects CUDA tensors")
     if k_cache.dtype not in _native.DTYPE_CODES:
@@ -1277,8 +1283,9 @@ def update_page_bounds(
 def selection_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, table_width: int,
                               num_selected: int) -> int:
     """Bytes of a workspace for :func:`select_pages` and :func:`paged_decode_selected`
-    over block tables of ``table_width`` pages.  Calls that share one must not
-    overlap; it needs no clearing."""
+    over block tables of ``table_width`` pages.  Zero it once when it is made: the
+    kernels leave its counters at zero.  Calls that share one, of whatever sizes,
+    must not overlap."""
     nbytes = int(_native.query("mva_selection_workspace_bytes", num_seqs, num_q_heads, num_kv_heads, table_width,
                                num_selected))
     if nbytes < 0:
@@ -1286,9 +1293,16 @@ def selection_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int
     return nbytes
 
 
+def new_selection_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """A workspace of ``nbytes`` (:func:`selection_workspace_bytes`), its counters cleared."""
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    workspace[:SELECTION_HEADER_BYTES].zero_()
+    return workspace
+
+
 def _selection_workspace(workspace: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
     if workspace is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return new_selection_workspace(nbytes, device)
     if workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 tensor on the device of the other tensors")
     if workspace.numel() < nbytes:
@@ -1324,6 +1338,10 @@ def select_pages(
     order of their places, -1 after a row's last, and int32 ``[S]`` the tokens
     that they hold, for :func:`paged_decode_selected`.  A row of ``seq_lens`` 0
     gets no page."""
+    fast = _native.host_ops().select_pages(q, page_bounds, block_tables, seq_lens, num_selected, sink_pages,
+                                           recent_pages, workspace)
+    if fast is not None:
+        return fast
     _check_queries(q)
     device, dtype = q.device, q.dtype
     if page_bounds.dim() != 4:
@@ -1378,6 +1396,9 @@ def paged_decode_selected(
     (``[P, 16, Hkv, 128]``) for each row and KV head; ``lens`` (int32 ``[S]``) counts
     the tokens they hold: all pages of a list but its last are full.  A row of
     ``lens`` 0 gives zeros."""
+    fast = _native.host_ops().paged_decode_selected(q, k_cache, v_cache, tables, lens, softmax_scale, out, workspace)
+    if fast is not None:
+        return fast
     _check_queries(q)
     device, dtype = q.device, q.dtype
     for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
@@ -1417,3 +1438,31 @@ def paged_decode_selected(
         float(softmax_scale), _native.dtype_code(dtype), _native.stream_handle(device),
     )
     return out
+
+
+def sparse_decode(
+    q: torch.Tensor,
+    page_bounds: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    softmax_scale: float,
+    num_selected: int,
+    sink_pages: int = 1,
+    recent_pages: int = 1,
+    *,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`select_pages` and :func:`paged_decode_selected` over what it chose, in
+    one call; ``page_bounds`` has the caches' number of pages."""
+    if out is not None and _native.host_ops().sparse_decode(q, page_bounds, k_cache, v_cache, block_tables, seq_lens,
+                                                            softmax_scale, num_selected, sink_pages, recent_pages,
+                                                            out, workspace):
+        return out
+    if page_bounds.size(0) != k_cache.size(0):
+        raise ValueError("page_bounds must have the cache's number of pages")
+    tables, lens = select_pages(q, page_bounds, block_tables, seq_lens, num_selected, sink_pages, recent_pages,
+                                workspace=workspace)
+    return paged_decode_selected(q, k_cache, v_cache, tables, lens, softmax_scale, out=out, workspace=workspace)

@@ -341,6 +341,7 @@ def test_one_workspace_serves_calls_of_other_sizes(gpu):
     table, q = tables_for(counts, sum(counts), 3), queries(3, 8, BF16, 4)
     nbytes = ops.selection_workspace_bytes(3, 8, 2, table.shape[1], 20)
     workspace = torch.full((nbytes + 4096,), 0xff, dtype=torch.uint8, device=gpu)
+    workspace[:ops.SELECTION_HEADER_BYTES] = 0
     outs = []
     for n in (20, 7, 20):
         tables, kept = ops.select_pages(q.to(gpu), bounds_of(k).to(gpu), table.to(gpu), _ints(lens, gpu), n, 1, 1,
@@ -351,7 +352,7 @@ def test_one_workspace_serves_calls_of_other_sizes(gpu):
         assert torch.equal(tables.cpu(), want[0]) and torch.equal(kept.cpu(), want[1])
         _check_attention(outs[-1], q, k, v, *want, BF16)
     assert torch.equal(outs[0], outs[2])
-    assert (workspace[nbytes:] == 0xff).all()
+    assert (workspace[nbytes:] == 0xff).all() and (workspace[:ops.SELECTION_HEADER_BYTES] == 0).all()
 
 
 def test_calls_on_two_streams_and_captured_ones(gpu):
