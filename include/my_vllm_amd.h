@@ -604,7 +604,7 @@ int mva_update_page_bounds(const void* k_cache, int64_t num_pages, int64_t page_
 
 /* Bytes of the workspace of mva_select_pages and mva_paged_decode_selected
  * (either takes it, for these sizes or smaller ones), or -1.  Zero it once: the
- * kernels leave its counters, the first 32768 bytes, at zero.  Launches that
+ * kernels leave its counters, the first 8192 bytes, at zero.  Launches that
  * share it must not overlap. */
 int64_t mva_selection_workspace_bytes(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t table_width,
                                       int64_t num_selected);

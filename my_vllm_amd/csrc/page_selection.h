@@ -14,7 +14,7 @@ constexpr int kPageTokens = 16;
 constexpr int kMaxQueryGroup = 16;
 
 // (row, KV head) pairs of a launch whose workgroups count themselves in.
-constexpr int kSelectionCounters = 4096;
+constexpr int kSelectionCounters = 1024;
 constexpr int64_t kSelectionHeaderBytes = 2 * kSelectionCounters * 4;
 
 inline int64_t align_up256(int64_t x) { return (x + 255) & ~int64_t(255); }

@@ -154,18 +154,19 @@ __device__ inline uint64_t order_key(double score) {
   return (int64_t)b < 0 ? ~b : b | (uint64_t(1) << 63);
 }
 
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 512;
 constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kBatch = 16;       // pages that a wavefront scores at a time
-constexpr int kShortKeys = 512;  // keys held in LDS where one workgroup scores a row
-constexpr int kKeyRegs = 8;      // keys that a thread of the choice holds in registers
+constexpr int kSelectGroups = 2 * 256;  // workgroups that the GPU holds, two on each of its CUs
+static_assert(kSelectGroups <= kSelectionCounters, "a row in several workgroups has a counter");
+constexpr int kBatch = 16;        // pages that a wavefront scores at a time
+constexpr int kShortKeys = 8192;  // keys held in LDS where one workgroup scores a row
+constexpr int kKeyRegs = 4;       // keys that a thread of the choice holds in registers
 
 // Workgroup state of the choice.
 struct ChoiceLds {
   uint64_t keys[kShortKeys];
-  int hist[256];
-  int found[3];
-  uint32_t differ[kSelectWaves][2];
+  int hist[3][256];  // in turns
+  uint64_t differ[kSelectWaves];
   int last;
   int counts[kSelectWaves * kKeyRegs];
 };
@@ -179,104 +180,130 @@ __device__ inline uint64_t key_load(const uint64_t* a) {
   return __hip_atomic_load(a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Adds up eight values of 32 lanes each: of v[i] the sum over the lanes of this
-// half, in the lanes of index i = lane / 4 % 8 (bits 4, 3, 2 from the top).
-__device__ inline double sums_of_8(double (&v)[8], int lane) {
+// The value of the lane whose number differs in bit X (within 32 lanes).
+template <int X>
+__device__ inline double across(double v) {
+  const u32x2 b = __builtin_bit_cast(u32x2, v);
+  u32x2 r;
 #pragma unroll
-  for (int step = 0; step < 3; ++step) {
-    const int x = 16 >> step, n = 4 >> step;
-    const bool up = lane & x;
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const double send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
-      v[i] = keep + __shfl_xor(send, x);
-    }
+  for (int e = 0; e < 2; ++e) {
+    if constexpr (X == 1) r[e] = __builtin_amdgcn_update_dpp(0, b[e], 0xb1, 0xf, 0xf, true);       // quad_perm 1 0 3 2
+    else if constexpr (X == 2) r[e] = __builtin_amdgcn_update_dpp(0, b[e], 0x4e, 0xf, 0xf, true);  // quad_perm 2 3 0 1
+    else if constexpr (X == 8) r[e] = __builtin_amdgcn_update_dpp(0, b[e], 0x128, 0xf, 0xf, true);  // row_ror 8
+    else r[e] = __builtin_amdgcn_ds_swizzle(b[e], X << 10 | 0x1f);
   }
-  v[0] += __shfl_xor(v[0], 2);
-  return v[0] + __shfl_xor(v[0], 1);
+  return __builtin_bit_cast(double, r);
+}
+template <int X>
+__device__ inline double halves(double a, double b, bool up) {
+  return (up ? b : a) + across<X>(up ? a : b);
 }
 
-// The place-th key and page of the pages between the ends.
+// Adds up eight values of 32 lanes each: of v[i] the sum over the lanes of this
+// half, in the lanes of index i = lane / 4 % 8 (bits 4, 3, 2 from the top).
+__device__ inline double sums_of_8(const double (&v)[8], int lane) {
+  const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4;
+  const double x0 = halves<16>(v[0], v[4], b4), x1 = halves<16>(v[1], v[5], b4);
+  const double x2 = halves<16>(v[2], v[6], b4), x3 = halves<16>(v[3], v[7], b4);
+  const double y0 = halves<8>(x0, x2, b3), y1 = halves<8>(x1, x3, b3);
+  double z = halves<4>(y0, y1, b2);
+  z += across<2>(z);
+  return z + across<1>(z);
+}
+
+// Within a wavefront by DPP: of lane l the value of lane l - 1, 2, 4, 8 of its row of
+// 16, then of the rows before; 0 where there is none.
+template <int Ctrl, int Rows>
+__device__ inline int from_before(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, Ctrl, Rows, 0xf, true);
+}
+template <typename Op>
+__device__ inline int wave_scan(int x, Op op) {
+  x = op(x, from_before<0x111, 0xf>(x));
+  x = op(x, from_before<0x112, 0xf>(x));
+  x = op(x, from_before<0x114, 0xf>(x));
+  x = op(x, from_before<0x118, 0xf>(x));
+  x = op(x, from_before<0x142, 0xa>(x));  // the last lane of the row before, into rows 1 and 3
+  return op(x, from_before<0x143, 0xc>(x));  // lane 31, into rows 2 and 3
+}
+__device__ inline int wave_scan_add(int x) {
+  return wave_scan(x, [](int a, int b) { return a + b; });
+}
+__device__ inline uint32_t wave_or(uint32_t x) {
+  return __builtin_amdgcn_readlane(wave_scan((int)x, [](int a, int b) { return a | b; }), 63);
+}
+
+// The pages between the ends: their keys, in memory or (nullptr) in LDS, and ids.
 struct Scored {
-  const uint64_t* keys;  // in memory, or nullptr: in LDS
-  const int32_t* row;    // page ids from the first one between the ends on
+  const uint64_t* keys;
+  const int32_t* row;
   int64_t count;
+  __device__ uint64_t key(const ChoiceLds& lds, int64_t j) const {
+    return keys == nullptr ? lds.keys[j] : key_load(keys + j);
+  }
 };
 
 // The threshold of the `want` largest keys: a key is taken if key >> shift is
 // above `top`, and the first `want` (as returned) of those that equal it.
-// each(f) calls f(key) for every key of this thread.
+// each(f) calls f(key) for every key of this thread; `some` is any of the keys.
 //
 // Digit by digit from the highest bit in which keys differ, each by a histogram
 // of the keys that agree with the digits before, until a digit's keys are all
-// taken.
+// taken.  Every wavefront reads the histogram for itself, so a digit costs one
+// barrier; the next one's is cleared meanwhile.
 template <typename Each>
 __device__ inline void threshold(Each each, uint64_t some, ChoiceLds& lds, int& want, uint64_t& top, int& shift) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint64_t differ = 0;
   each([&](uint64_t key) { differ |= key ^ some; });
-  uint32_t lo = (uint32_t)differ, hi = (uint32_t)(differ >> 32);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) {
-    lo |= __shfl_xor(lo, x);
-    hi |= __shfl_xor(hi, x);
-  }
-  if (lane == 0) {
-    lds.differ[wave][0] = lo;
-    lds.differ[wave][1] = hi;
-  }
-  lds.hist[tid] = 0;
+  differ = (uint64_t)wave_or((uint32_t)(differ >> 32)) << 32 | wave_or((uint32_t)differ);
+  if (lane == 0) lds.differ[wave] = differ;
+  if (tid < 256) lds.hist[0][tid] = 0;
   __syncthreads();
   differ = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) differ |= (uint64_t)lds.differ[w][1] << 32 | lds.differ[w][0];
+  for (int w = 0; w < kSelectWaves; ++w) differ |= lds.differ[w];
   int end = differ ? 64 - __builtin_clzll(differ) : 0;  // bits from here up are the same in all keys
   shift = end;
   top = end == 64 ? 0 : some >> end;
   bool all = false;
-  while (shift > 0 && !all) {
+  for (int turn = 0; shift > 0 && !all; turn = turn == 2 ? 0 : turn + 1) {
+    int* const hist = lds.hist[turn];
     end = shift;
     shift = end > 8 ? end - 8 : 0;
     const uint64_t mask = (uint64_t(1) << (end - shift)) - 1;
     each([&](uint64_t key) {
-      if (end == 64 || key >> end == top) atomicAdd(&lds.hist[(int)(key >> shift & mask)], 1);
+      if (end == 64 || key >> end == top) atomicAdd(&hist[(int)(key >> shift & mask)], 1);
     });
+    if (tid < 256) lds.hist[turn == 2 ? 0 : turn + 1][tid] = 0;  // last read two barriers ago
     __syncthreads();
-    if (wave == 0) {
-      // Lane l holds digits 255 - 4l down to 252 - 4l.
-      int mine[4], sum = 0;
+    // Lane l holds digits 252 - 4l .. 255 - 4l; `before`: keys of larger digits.
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const i32x4 mine = *(const i32x4*)&hist[252 - 4 * lane];
+    const int sum = mine[0] + mine[1] + mine[2] + mine[3];
+    int before = wave_scan_add(sum) - sum;
+    const uint64_t holds = __ballot(before < want && before + sum >= want);
+    int digit = 255 - 4 * lane, keys = mine[3];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += mine[i] = lds.hist[255 - 4 * lane - i];
-      int before = sum;
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) {
-        const int other = __shfl_up(before, x);
-        if (lane >= x) before += other;
-      }
-      before -= sum;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (before < want && before + mine[i] >= want) {
-          lds.found[0] = 255 - 4 * lane - i;
-          lds.found[1] = want - before;
-          lds.found[2] = mine[i];
-        }
-        before += mine[i];
+    for (int i = 2; i >= 0; --i) {
+      if (before + keys < want) {
+        before += keys;
+        digit = 252 - 4 * lane + i;
+        keys = mine[i];
       }
     }
-    __syncthreads();
-    top = top << (end - shift) | (uint64_t)lds.found[0];
-    want = lds.found[1];
-    all = lds.found[2] == want;
-    lds.hist[tid] = 0;
-    __syncthreads();
+    const int from = __builtin_ctzll(holds);
+    want -= __builtin_amdgcn_readlane(before, from);
+    top = top << (end - shift) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(digit, from);
+    all = __builtin_amdgcn_readlane(keys, from) == want;
   }
 }
 
 // Chooses `want` of the scored pages and lists them in the order of their
 // places; all threads of the workgroup, the keys visible to them.
 __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds& lds) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint64_t below = (uint64_t(1) << lane) - 1;
   uint64_t top;
   int shift;
@@ -289,18 +316,17 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
       key[i] = 0;
       id[i] = 0;
       if (j < r.count) {
-        key[i] = r.keys == nullptr ? lds.keys[j & (kShortKeys - 1)] : key_load(r.keys + j);
+        key[i] = r.key(lds, j);
         id[i] = r.row[j];
       }
     }
-    const uint64_t some = r.keys == nullptr ? lds.keys[0] : key_load(r.keys);
     threshold(
         [&](auto f) {
 #pragma unroll
           for (int i = 0; i < kKeyRegs; ++i)
             if (i * kSelectThreads + tid < r.count) f(key[i]);
         },
-        some, lds, want, top, shift);
+        r.key(lds, 0), lds, want, top, shift);
     // Keys above and at the threshold, low and high half: first of each 64 places, then before each.
     uint64_t gts[kKeyRegs], eqs[kKeyRegs];
 #pragma unroll
@@ -313,13 +339,7 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
     }
     __syncthreads();
     int mine = lane < kSelectWaves * kKeyRegs ? lds.counts[lane] : 0;
-    const int own = mine;
-#pragma unroll
-    for (int x = 1; x < kSelectWaves * kKeyRegs; x <<= 1) {
-      const int other = __shfl_up(mine, x);
-      if (lane >= x) mine += other;
-    }
-    mine -= own;
+    mine = wave_scan_add(mine) - mine;
 #pragma unroll
     for (int i = 0; i < kKeyRegs; ++i) {
       const int before = __builtin_amdgcn_readlane(mine, i * kSelectWaves + wave);
@@ -330,13 +350,13 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
   }
   threshold(
       [&](auto f) {
-        for (int64_t j = tid; j < r.count; j += kSelectThreads) f(key_load(r.keys + j));
+        for (int64_t j = tid; j < r.count; j += kSelectThreads) f(r.key(lds, j));
       },
-      key_load(r.keys), lds, want, top, shift);
+      r.key(lds, 0), lds, want, top, shift);
   int above = 0, equal = 0;  // over the places before this block
   for (int64_t base = 0; base < r.count; base += kSelectThreads) {
     const int64_t j = base + tid;
-    const uint64_t key = j < r.count ? key_load(r.keys + j) >> shift : 0;
+    const uint64_t key = j < r.count ? r.key(lds, j) >> shift : 0;
     const uint64_t gts = __ballot(j < r.count && key > top), eqs = __ballot(j < r.count && key == top);
     if (lane == 0) {
       lds.counts[2 * wave] = __popcll(gts);
@@ -402,39 +422,73 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
 
   const int piece = lane & 31, half = lane >> 5;
   double w[8] = {};
-  for (int g = 0; g < p.group; ++g) {
-    const V8 q = ld16<V8>((const T*)p.q + s * p.q_tok_stride + (int64_t)(h * p.group + g) * p.q_head_stride +
-                          8 * (piece & 15));
+  auto weights = [&]() __attribute__((always_inline)) {
+    const float sign = piece < 16 ? -1.f : 1.f;  // the negative or the positive parts
+    const T* q = (const T*)p.q + s * p.q_tok_stride + (int64_t)h * p.group * p.q_head_stride + 8 * (piece & 15);
+    for (int g = 0; g < p.group; g += 4) {
+      V8 v[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = (float)q[e];
-      // A NaN stays in both parts.
-      w[e] += (double)(piece < 16 ? (x > 0.f ? 0.f : x) : (x < 0.f ? 0.f : x));
+      for (int i = 0; i < 4; ++i) v[i] = ld16<V8>(q + min(g + i, p.group - 1) * p.q_head_stride);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (g + i >= p.group) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = (float)v[i][e] * sign;
+          w[e] += (double)(x <= 0.f ? 0.f : x);  // a NaN stays in both parts
+        }
+      }
     }
-  }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] *= sign;
+  };
+  // This wavefront's pages, 16 at a time, the next ones loaded before the
+  // present ones are scored; their ids 256 at a time.
   const uint8_t* bounds = p.bounds + h * 512 + piece * 16;
-  for (int64_t base = first + wave * kBatch; base < last; base += kSelectWaves * kBatch) {
-    int id = row[min(base + (lane & 15), last - 1)];
-    if (id < 0 || id >= p.num_pages) id = 0;
-    V8 box[8];
+  const int64_t begin = first + wave * (int64_t)(chunk / kSelectWaves);
+  const int64_t mine = min(begin + chunk / kSelectWaves, last);
+  for (int64_t base = begin; base < mine; base += 4 * 64) {
+    uint32_t ids[4];  // times the heads: pages' first rows of 512 bytes
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t a = __builtin_amdgcn_readlane(id, 2 * i), b = __builtin_amdgcn_readlane(id, 2 * i + 1);
-      box[i] = ld16<V8>(bounds + (half ? b : a) * ((int64_t)p.num_kv_heads * 512));
+    for (int i = 0; i < 4; ++i) {
+      const int id = row[min(base + 64 * i + lane, mine - 1)];
+      ids[i] = (uint32_t)(id < 0 || id >= p.num_pages ? 0 : id) * (uint32_t)p.num_kv_heads;
     }
-    double sum[8];
+    const int batches = (int)((min(mine - base, (int64_t)256) + kBatch - 1) / kBatch);
+    auto load = [&](V8 (&box)[8], int t) __attribute__((always_inline)) {
+      const int of = t >> 2, at = (t & 3) * kBatch;
+      const uint32_t id = of == 0 ? ids[0] : of == 1 ? ids[1] : of == 2 ? ids[2] : ids[3];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum[i] = 0.0;
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = __builtin_amdgcn_readlane(id, at + 2 * i), b = __builtin_amdgcn_readlane(id, at + 2 * i + 1);
+        box[i] = ld16<V8>(bounds + ((uint64_t)(half ? b : a) << 9));
+      }
+    };
+    auto score = [&](const V8 (&box)[8], int t) __attribute__((always_inline)) {
+      double sum[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[i] = __builtin_fma((double)(float)box[i][e], w[e], sum[i]);
+      for (int i = 0; i < 8; ++i) {
+        sum[i] = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[i] = __builtin_fma((double)(float)box[i][e], w[e], sum[i]);
+      }
+      const uint64_t key = order_key(sums_of_8(sum, lane));
+      const int64_t place = base + t * kBatch + 2 * (piece >> 2) + half;
+      if ((lane & 3) == 0 && place < mine) {
+        if (in_lds) lds.keys[place] = key;
+        else key_store(keys + place, key);
+      }
+    };
+    V8 box[8], next[8];
+    load(box, 0);
+    if (base == begin) weights();
+    for (int t = 1; t < batches; ++t) {
+      load(next, t);
+      score(box, t - 1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) box[i] = next[i];
     }
-    const uint64_t key = order_key(sums_of_8(sum, lane));
-    const int64_t place = base + 2 * (piece >> 2) + half;
-    if ((lane & 3) == 0 && place < last) {
-      if (in_lds) lds.keys[place] = key;
-      else key_store(keys + place, key);
-    }
+    score(box, batches - 1);
   }
   if (parts > 1) {
     // This wavefront's keys have reached memory before the workgroup counts itself in.
@@ -523,6 +577,7 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
   if (((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)page_bounds | (uint64_t)(uintptr_t)workspace |
        (uint64_t)(q_token_stride * 2) | (uint64_t)(q_head_stride * 2)) % 16)
     return set_error("page selection: q, bounds, workspace and strides must be 16-byte aligned");
+  if (num_pages * num_kv_heads > 0xffffffffLL) return set_error("page selection: too many pages");
   const int64_t rows = num_seqs * num_kv_heads;
   uint8_t* const ws = (uint8_t*)workspace;
   const SelectParams p = {
@@ -530,11 +585,11 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
       table_width, seq_lens, num_seqs, (int)num_selected, (int)sink_pages, (int)recent_pages, tables, lens,
       (uint64_t*)(ws + kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_kv_heads, num_selected)),
       (int*)ws, num_kv_heads, num_q_heads / num_kv_heads};
-  // Chunks: as small as 64 pages (16 a wavefront) as long as that makes no more
-  // workgroups than the GPU holds at a time; one a row beyond the counters.
+  // Chunks: as small as 128 pages (16 a wavefront) as long as that makes no more
+  // workgroups than the GPU holds at a time.
   const int64_t most = table_width - sink_pages - recent_pages;
-  int64_t chunk = 64;
-  while (chunk < most && (rows > kSelectionCounters || rows * ((most + chunk - 1) / chunk) > 2048)) chunk *= 2;
+  int64_t chunk = kBatch * kSelectWaves;
+  while (chunk < most && rows * ((most + chunk - 1) / chunk) > kSelectGroups) chunk *= 2;
   const int64_t chunks = most > chunk && table_width > num_selected ? (most + chunk - 1) / chunk : 1;
   const int64_t blocks = rows * chunks;
   if (blocks > 0xffffffffLL / kSelectThreads) return set_error("page selection: too many rows for one launch");

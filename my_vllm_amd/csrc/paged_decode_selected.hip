@@ -38,6 +38,10 @@ struct SelectedParams {
 
 constexpr int kSelWaves = 4;       // wavefronts of a workgroup
 constexpr int kSelGroupsPerCu = 3;  // workgroups that a CU holds
+// Pages of a part, at least.  A part more costs the join more than the pages it
+// takes off the others' streams: 128 pages of one row at 32 / 8 heads in parts of
+// 4, 8, 16 and 32 pages take 10.4, 7.9, 7.6 and 9.8 us.
+constexpr int kPartPages = 16;
 constexpr int kJoinRow = kHeadDim + 4;  // floats of a joined row in LDS: its 16 rows start in different banks
 
 // A page of one KV head in registers.  k[j]: lane (q4, c) channels 32 j + 8 q4 .. + 7
@@ -73,8 +77,7 @@ __global__ __launch_bounds__(64 * kSelWaves, kSelGroupsPerCu) void selected_deco
   const int G = p.group;
   const int len = sload(p.lens, s);
   const int pages = len <= 0 ? 0 : min((int)(((int64_t)len + kPageSize - 1) / kPageSize), p.num_selected);
-  // Parts of a row of few pages: no more than it has groups of kSelWaves pages.
-  const int parts = min(p.parts, max(1, (pages + kSelWaves - 1) / kSelWaves));
+  const int parts = min(p.parts, max(1, (pages + kPartPages - 1) / kPartPages));  // fewer for a row of few pages
   if (part >= parts) return;
   const int begin = (int)((int64_t)pages * part / parts), end = (int)((int64_t)pages * (part + 1) / parts);
   const int32_t* table = p.tables + s * p.seq_table_stride + h * p.head_table_stride;
@@ -261,11 +264,13 @@ __global__ __launch_bounds__(64 * kSelWaves, kSelGroupsPerCu) void selected_deco
   }
 }
 
+static_assert(256 * kSelGroupsPerCu <= kSelectionCounters, "a row in several parts has a counter");
+
 // Parts a row's pages are cut into, one workgroup each: as many workgroups as
-// the GPU holds, as long as every wavefront has a page.
+// the GPU holds, as long as a part has kPartPages pages.
 int selected_parts(int64_t num_seqs, int hkv, int64_t num_selected) {
   const int64_t rows = num_seqs * hkv;
-  const int64_t most = (num_selected + kSelWaves - 1) / kSelWaves;
+  const int64_t most = (num_selected + kPartPages - 1) / kPartPages;
   const int64_t want = rows > 0 ? 256 * kSelGroupsPerCu / rows : 1;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }

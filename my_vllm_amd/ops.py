@@ -1148,7 +1148,7 @@ def paged_prefill_mxfp4(
 
 
 # Counters at the start of a selection workspace (kSelectionHeaderBytes).
-SELECTION_HEADER_BYTES = 32768
+SELECTION_HEADER_BYTES = 8192
 
 
 def page_bounds_shape(num_pages: int, num_kv_heads: int) -> tuple[int, int, int, int]:
