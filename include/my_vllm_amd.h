@@ -619,7 +619,8 @@ int64_t mva_selection_workspace_bytes(int64_t num_seqs, int num_q_heads, int num
  * ties go to the lowest place.  tables (dense [num_seqs][num_kv_heads]
  * [num_selected]) gets their page ids in the order of their places, -1 after
  * the last; lens ([num_seqs]) the tokens they hold, those of the last page
- * counted to the row's end.  A row of seq_lens <= 0 gets no page and 0.
+ * counted to the row's end.  A row of seq_lens <= 0 gets no page and 0; one longer
+ * than its table counts as long as the table.
  */
 int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* page_bounds,
                      int64_t num_pages, const int32_t* block_tables, int64_t block_table_stride, int64_t table_width,
@@ -630,8 +631,10 @@ int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q_head_strid
 /*
  * Attention of one query a row over the first lens[s] tokens of the pages
  * tables[s][h][0 ..], a list for each row and KV head of at most num_selected
- * pages (strides in elements; the lists themselves dense).  Rows of lens <= 0
- * give zeros.
+ * pages (strides in elements; the lists themselves dense).  All pages of a list
+ * but its last are full.  An id outside the cache reads page 0.  Rows of lens <= 0
+ * give zeros.  softmax_scale must be positive; tokens of a page must lie less than
+ * 2^26 elements apart.
  */
 int mva_paged_decode_selected(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                               const void* v_cache, int64_t num_pages, int64_t page_stride, int64_t token_stride,

@@ -1632,10 +1632,10 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
                               page_bounds=None) -> torch.Tensor:
         """The step's K/V rows into the caches (``store``, or ``ops.store_kvcache``),
         :meth:`update_page_bounds`, then :meth:`forward`."""
-        if _has_cache(k_cache) and page_bounds is None:
-            raise ValueError("a backend that selects pages needs page_bounds")
-        (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
         if _has_cache(k_cache):
+            if page_bounds is None:
+                raise ValueError("a backend that selects pages needs page_bounds")
+            (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
             self.update_page_bounds(k_cache, page_bounds, plan)
         return self.forward(q, k, v, k_cache, v_cache, plan, page_bounds=page_bounds)
 

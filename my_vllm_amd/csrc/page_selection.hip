@@ -46,43 +46,69 @@ __device__ inline s16x8v nan_mask(s16x8v b) {
 
 constexpr int kBoundsTokens = 16;  // tokens whose pages one wavefront looks after
 
+// The sequence of each token first + lane (lanes below kBoundsTokens), the
+// token's place in it and the sequence's new tokens, from starts [S + 1] that do
+// not fall; all lanes.
+struct TokenOf {
+  int64_t seq;
+  int place, count;
+};
+__device__ inline TokenOf token_of(const int32_t* starts, int64_t num_seqs, int64_t first, int lane) {
+  // A sequence that starts at or before `first`, less than 62 from the last one
+  // that does: 64 starts a step.
+  int64_t lo = 0, hi = num_seqs;
+  while (hi - lo > 62) {
+    const int64_t step = (hi - lo + 63) / 64;
+    const int64_t at = lo + lane * step;
+    const int below = __popcll(__ballot(at < hi && starts[min(at, hi - 1)] <= first));
+    lo += max(below - 1, 0) * step;
+    hi = min(hi, lo + step);
+  }
+  // The starts from there on tell each token's sequence.
+  const int mine = starts[min(lo + lane, num_seqs)];
+  int later = 0;
+#pragma unroll
+  for (int k = 0; k < kBoundsTokens; ++k) {
+    const int n = __popcll(__ballot(lane > 0 && lo + lane < num_seqs && mine <= first + k));
+    if (lane == k) later = n;
+  }
+  if (__any(lane < kBoundsTokens && later >= 62)) {
+    // It may lie beyond the starts that were read: each lane searches for itself.
+    lo = 0, hi = num_seqs;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (starts[mid] <= first + lane) lo = mid;
+      else hi = mid;
+    }
+    return {lo, (int)(first + lane - starts[lo]), starts[lo + 1] - starts[lo]};
+  }
+  const int start = __shfl(mine, later), end = __shfl(mine, later + 1);
+  return {lo + later, (int)(first + lane - start), end - start};
+}
+
 // One wavefront per (16 tokens of the step, KV head).  Lane t finds the page
 // that token t completes, if any; then, page by page, lane (r, c) = (lane / 16,
 // lane % 16) reads channels 8c .. 8c + 7 of rows r, r + 4, r + 8 and r + 12.
 template <int kInf>
 __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsParams p) {
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t chunk = unit / p.num_kv_heads;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t first = unit / p.num_kv_heads * kBoundsTokens;
   const int h = (int)(unit % p.num_kv_heads);
-  if (chunk * kBoundsTokens >= p.num_tokens) return;
-  int64_t page = -1;
-  const int64_t t = chunk * kBoundsTokens + lane;
-  if (lane < kBoundsTokens && t < p.num_tokens) {
-    int64_t s = t, place = 0, count = 1;
-    if (p.query_start_loc != nullptr) {
-      // The last sequence that starts at or before token t.
-      int64_t lo = 0, hi = p.num_seqs;
-      while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (p.query_start_loc[mid] <= t) lo = mid;
-        else hi = mid;
-      }
-      s = lo;
-      place = t - p.query_start_loc[s];
-      count = (int64_t)p.query_start_loc[s + 1] - p.query_start_loc[s];
-    }
-    if (place >= 0 && place < count) {
-      const int64_t pos = (int64_t)p.seq_lens[s] - count + place;
-      if (pos >= 0 && pos % kPageTokens == kPageTokens - 1 && pos / kPageTokens < p.width) {
-        page = p.block_tables[s * p.bt_stride + pos / kPageTokens];
-        if (page >= p.num_pages) page = -1;
-      }
+  if (first >= p.num_tokens) return;
+  TokenOf of = {first + lane, 0, 1};
+  if (p.query_start_loc != nullptr) of = token_of(p.query_start_loc, p.num_seqs, first, lane);
+  int page = -1;
+  if (lane < kBoundsTokens && first + lane < p.num_tokens && of.place >= 0 && of.place < of.count) {
+    const int64_t pos = (int64_t)p.seq_lens[of.seq] - of.count + of.place;
+    if (pos >= 0 && pos % kPageTokens == kPageTokens - 1 && pos / kPageTokens < p.width) {
+      page = p.block_tables[of.seq * p.bt_stride + pos / kPageTokens];
+      if (page >= p.num_pages) page = -1;
     }
   }
   for (uint64_t todo = __ballot(page >= 0); todo != 0; todo &= todo - 1) {
     const int from = __builtin_ctzll(todo);
-    const int64_t id = __shfl((int)page, from);
+    const int64_t id = __builtin_amdgcn_readlane(page, from);
     const int r = lane >> 4, c = lane & 15;
     const uint8_t* src = p.k_cache + id * p.page_stride + r * p.tok_stride + h * 256 + c * 16;
     s16x8v rows[4];

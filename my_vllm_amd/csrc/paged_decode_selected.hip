@@ -300,6 +300,8 @@ extern "C" int mva_paged_decode_selected(const void* q, int64_t q_token_stride, 
       head_table_stride < 0)
     return set_error("selected attention: invalid sizes");
   if (num_pages <= 0 || num_pages > 0x7fffffffLL) return set_error("selected attention: empty or oversized KV cache");
+  if (!(softmax_scale > 0.f && softmax_scale < INFINITY))
+    return set_error("selected attention: softmax_scale must be positive and finite");
   if (num_seqs == 0) return 0;
   if (!q || !k_cache || !v_cache || !tables || !lens || !out) return set_error("selected attention: null buffer");
   if (((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)k_cache | (uint64_t)(uintptr_t)v_cache |

@@ -104,6 +104,20 @@ def test_bounds_of_a_layer_of_a_pool_and_wider_tables(gpu):
     assert torch.equal(got.cpu(), selection.page_bounds(cache, before, table, lens, new))
 
 
+def test_bounds_among_many_empty_sequences(gpu):
+    # More sequences without new tokens between two with some than the kernel reads starts at a time.
+    for seqs, at in ((70, (0, 69)), (300, (3, 150, 299)), (5000, (0, 1, 64, 65, 2500, 4999))):
+        new = [0] * seqs
+        for i, s in enumerate(at):
+            new[s] = 16 + i
+        lens = [32 + i % 16 if n else 1 for i, n in enumerate(new)]
+        cache = keys(64, 1, BF16, seqs)
+        table = torch.randint(0, 64, (seqs, 3), generator=torch.Generator().manual_seed(seqs)).to(torch.int32)
+        before = torch.zeros(64, 1, 2, 128, dtype=BF16)
+        got = _update(gpu, cache.to(gpu), before, table, lens, new)
+        assert torch.equal(got.cpu(), selection.page_bounds(cache, before, table, lens, new))
+
+
 # ---- selection -------------------------------------------------------------------
 
 
@@ -138,6 +152,20 @@ def test_selected_pages_of_long_rows(gpu, pages):
     table = tables_for(counts, sum(counts), pages + 1)
     for n in (7, 128, pages // 2 + 1):
         _check_selection(gpu, queries(2, 4, BF16, pages + 2), bounds_of(cache), table, lens, n, 1, 2)
+
+
+# Rows enough that each has one workgroup: its keys in registers, in LDS and in memory.
+@pytest.mark.parametrize("pages", [300, 2300, 8300])
+def test_selected_pages_of_many_rows(gpu, pages):
+    q = queries(3, 2, BF16, pages)
+    cache = keys(pages, 1, BF16, pages + 1)
+    table = tables_for([pages], pages, pages + 2)
+    lens = [16 * pages, 16 * pages - 5, 16 * (pages - pages // 3) + 1]
+    want = selection.select_pages(q, bounds_of(cache), table.expand(3, pages), lens, 50, 2, 3)
+    rows = torch.arange(3).repeat(180)
+    got = _select(gpu, q[rows], bounds_of(cache), table.expand(len(rows), pages).contiguous(),
+                  [lens[i] for i in rows.tolist()], 50, 2, 3)
+    assert torch.equal(got[0], want[0][rows]) and torch.equal(got[1], want[1][rows])
 
 
 @pytest.mark.parametrize("n,sink,recent", [(9, 1, 1), (40, 0, 3), (150, 2, 2)])
@@ -240,6 +268,22 @@ def test_attention_over_lists_of_pages(gpu, hq, hkv, dtype, lens, n):
     out = ops.paged_decode_selected(q.to(gpu), k.to(gpu), v.to(gpu), tables.to(gpu), _ints(lens, gpu), SCALE)
     _check_attention(out, q, k, v, tables, lens, dtype)
     assert all((out[s] == 0).all() for s, length in enumerate(lens) if length == 0)
+
+
+# One, two and three parts a row, rows of few pages among them, and lists of more
+# than 64 pages a wavefront.
+@pytest.mark.parametrize("rows,hkv,n", [(100, 8, 300), (97, 8, 40), (45, 8, 61), (30, 8, 70), (257, 1, 33)])
+def test_attention_of_many_rows(gpu, rows, hkv, n):
+    kinds = [16 * n - 3, 16 * n, 200, 16 * (n // 2) + 9]
+    counts = page_counts(kinds)
+    total = max(counts) + 20
+    k, v = keys(total, hkv, FP16, 1), keys(total, hkv, FP16, 2)
+    q, tables = queries(4, 2 * hkv, FP16, 3), _lists(counts, hkv, total, n, 4)
+    of = torch.arange(rows) % 4
+    out = ops.paged_decode_selected(q[of].to(gpu), k.to(gpu), v.to(gpu), tables[of].to(gpu),
+                                    _ints([kinds[i] for i in of.tolist()], gpu), SCALE)
+    _check_attention(out[:4], q, k, v, tables, kinds, FP16)
+    assert torch.equal(out, out[:4][of.to(gpu)])
 
 
 def test_rows_behind_the_last_token_do_not_show(gpu):

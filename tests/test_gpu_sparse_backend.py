@@ -139,8 +139,7 @@ def test_warmup_runs_without_bounds(gpu):
         slot_mapping=torch.full((50,), -1, dtype=torch.int32, device=gpu), max_q_len=30, max_kv_len=30, trusted=True)
     q, k, v = (queries(50, n, BF16, n).to(gpu) for n in (16, 8, 8))
     empty = k.new_empty(0)
-    got = backend.forward_with_kv_store(q, k, v, empty, empty, common.slot_mapping, backend.build_plan(common),
-                                        store=lambda *a: None)
+    got = backend.forward_with_kv_store(q, k, v, empty, empty, common.slot_mapping, backend.build_plan(common))
     assert torch.equal(got, dense.forward(q, k, v, empty, empty, dense.build_plan(common)))
 
 
@@ -282,6 +281,8 @@ def test_operators_refuse(gpu):
     _refused(ValueError, "lens", attend, q, k, k, lists, lens[:2], 1.0)
     _refused(ValueError, "out must", attend, q, k, k, lists, lens, 1.0, out=q[:2])
     _refused(ValueError, "pages", attend, q, k[:0], k[:0], lists, lens, 1.0)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        _refused(RuntimeError, "softmax_scale", attend, q, k, k, lists, lens, scale)
     # No rows: nothing to do.
     none = select(q[:0], bounds, table[:0], lens[:0], 4)
     assert none[0].shape == (0, 2, 4) and attend(q[:0], k, k, none[0], none[1], 1.0).shape == (0, 8, 128)

@@ -128,6 +128,7 @@ def test_bounds_entry_refuses(change, message):
 @pytest.mark.parametrize("change,message", [
     ({21: 64}, "head_dim"), ({22: 8}, "page_size"), ({24: 2}, "dtype"), ({19: 9}, "sizes"), ({13: 0}, "sizes"),
     ({9: -1}, "sizes"), ({5: 0}, "empty"), ({3: 0}, "null"), ({14: 0}, "null"), ({0: 0x1004}, "aligned"),
+    ({7: 1 << 27}, "2\\^26"), ({23: 0.0}, "softmax_scale"), ({23: math.nan}, "softmax_scale"),
     ({6: 16 * 1024 + 1}, "aligned"), ({14: 0x1004}, "aligned"), ({17: 0}, "workspace"), ({18: 100}, "workspace"),
 ])
 def test_attention_entry_refuses(change, message):
