@@ -73,6 +73,13 @@ __device__ inline void st16(void* p, V v) {
   *reinterpret_cast<V*>(p) = v;
 }
 
+// 16 bytes that this launch reads once: non-temporal if kOnce.
+template <typename V, bool kOnce>
+__device__ inline V ld16_stream(const void* p) {
+  if constexpr (kOnce) return __builtin_bit_cast(V, __builtin_nontemporal_load((const u32x4*)p));
+  else return ld16<V>(p);
+}
+
 // LDS (address space 3) byte pointer.  Kernels pass LDS buffers around with
 // this type so every access compiles to ds_* instructions (a generic pointer
 // would compile to flat_* loads with 64-bit addresses).

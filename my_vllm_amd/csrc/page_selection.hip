@@ -44,6 +44,7 @@ __device__ inline s16x8v nan_mask(s16x8v b) {
   return (b & (short)0x7fff) > (short)kInf;
 }
 
+constexpr int64_t kRowBytes = 256;  // 128 channels
 constexpr int kBoundsTokens = 16;  // tokens whose pages one wavefront looks after
 
 // The sequence of each token first + lane (lanes below kBoundsTokens), the
@@ -413,7 +414,7 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
 // Products and sums are in 64 bits: products of 16-bit values are exact there
 // and sums of them nearly so, so that which page is taken does not hang on the
 // order of a sum.
-template <typename T>
+template <typename T, bool kOnce>
 __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p, int chunk, int chunks) {
   typedef typename Elem<T>::v8 V8;
   __shared__ ChoiceLds lds;
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t a = __builtin_amdgcn_readlane(id, at + 2 * i), b = __builtin_amdgcn_readlane(id, at + 2 * i + 1);
-        box[i] = ld16<V8>(bounds + ((uint64_t)(half ? b : a) << 9));
+        box[i] = ld16_stream<V8, kOnce>(bounds + ((uint64_t)(half ? b : a) << 9));
       }
     };
     auto score = [&](const V8 (&box)[8], int t) __attribute__((always_inline)) {
@@ -620,11 +621,11 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
   const int64_t blocks = rows * chunks;
   if (blocks > 0xffffffffLL / kSelectThreads) return set_error("page selection: too many rows for one launch");
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == kBF16)
-    hipLaunchKernelGGL(page_select_kernel<__bf16>, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p, (int)chunk,
-                       (int)chunks);
-  else
-    hipLaunchKernelGGL(page_select_kernel<_Float16>, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p,
-                       (int)chunk, (int)chunks);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p, (int)chunk, (int)chunks);
+  };
+  const bool once = read_once(rows * table_width * 2 * kRowBytes);
+  if (dtype == kBF16) once ? launch(page_select_kernel<__bf16, true>) : launch(page_select_kernel<__bf16, false>);
+  else once ? launch(page_select_kernel<_Float16, true>) : launch(page_select_kernel<_Float16, false>);
   return check_launch("page_select");
 }

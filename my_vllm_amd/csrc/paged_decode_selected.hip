@@ -44,10 +44,21 @@ constexpr int kSelGroupsPerCu = 3;  // workgroups that a CU holds
 constexpr int kPartPages = 16;
 constexpr int kJoinRow = kHeadDim + 4;  // floats of a joined row in LDS: its 16 rows start in different banks
 
-// A page of one KV head in registers.  k[j]: lane (q4, c) channels 32 j + 8 q4 .. + 7
-// of token c, the A operand of S^T = K Q^T; v[e]: channels 8 c .. 8 c + 7 of token
-// 4 q4 + e, so that halves of v[0 .. 3] make the A operand of O^T += V^T P^T
-// whose rows are the channels 8 m + i, m the row of the matrix instruction.
+// Lanes 0-31 of a, then of b; and lanes 32-63 of a, then of b.
+__device__ inline float lower_halves(float a, float b) {
+  return __uint_as_float(__builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false)[0]);
+}
+__device__ inline float upper_halves(float a, float b) {
+  return __uint_as_float(__builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false)[1]);
+}
+
+// A page of one KV head in registers, every load whole 128-byte lines.
+// k[i]: of token 8 (i % 2) + c % 8 the channels 64 (i / 2) + 32 (c / 8) + 8 q4 .. + 7,
+// an A operand of S^T = K Q^T whose rows 0-7 and 8-15 are the same tokens, over
+// the channels of one half of a line and of the other.
+// v[e]: channels 8 c .. 8 c + 7 of token 4 q4 + e, so that halves of v[0 .. 3] make
+// the A operand of O^T += V^T P^T whose rows are the channels 8 m + i, m the row of
+// the matrix instruction.
 template <typename T>
 struct PageRegs {
   typename Elem<T>::v8 k[4];
@@ -58,10 +69,9 @@ struct PageRegs {
 // part's pages in turns, each with a running maximum and sum of its own, and
 // join in LDS; the row's last workgroup joins the parts.
 //
-// Pages come straight into registers, two ahead of the arithmetic, in pieces of
-// 16 bytes a lane that are contiguous over 64 (K) or 256 bytes (V); no
+// Pages come straight into registers, the next one while one is computed; no
 // LDS is filled, so a CU holds 12 wavefronts with two pages each.
-template <typename T>
+template <typename T, bool kOnce>
 __global__ __launch_bounds__(64 * kSelWaves, kSelGroupsPerCu) void selected_decode_kernel(SelectedParams p) {
   typedef typename Elem<T>::v8 V8;
   typedef typename Elem<T>::v4 V4;
@@ -97,7 +107,7 @@ __global__ __launch_bounds__(64 * kSelWaves, kSelGroupsPerCu) void selected_deco
 
   // Byte offsets in a page, one register each beside the page's address in scalar ones.
   const uint32_t tok = (uint32_t)p.tok_stride * 2;
-  const uint32_t k_off = c * tok + 16 * q4;
+  const uint32_t k_off[2] = {(c & 7) * tok + 64 * (c >> 3) + 16 * q4, (8 + (c & 7)) * tok + 64 * (c >> 3) + 16 * q4};
   uint32_t v_off[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) v_off[e] = (4 * q4 + e) * tok + 16 * c;
@@ -106,15 +116,21 @@ __global__ __launch_bounds__(64 * kSelWaves, kSelGroupsPerCu) void selected_deco
     const uint8_t* const k = (const uint8_t*)p.k_cache + base;
     const uint8_t* const v = (const uint8_t*)p.v_cache + base;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r.k[j] = ld16<V8>(k + 64 * j + (size_t)k_off);
+    for (int i = 0; i < 4; ++i) r.k[i] = ld16_stream<V8, kOnce>(k + 128 * (i >> 1) + (size_t)k_off[i & 1]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r.v[e] = ld16<u32x4>(v + (size_t)v_off[e]);
+    for (int e = 0; e < 4; ++e) r.v[e] = ld16_stream<u32x4, kOnce>(v + (size_t)v_off[e]);
   };
   // `left`: tokens of the row from this page on (16 or more unless it is the last one).
   auto compute = [&](PageRegs<T>& r, int left, auto may_end) __attribute__((always_inline)) {
-    f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Rows 0-7 of near[u] and 8-15 of far[u] are the two halves of the scores of tokens 8 u .. 8 u + 7.
+    f32x4 near[2] = {}, far[2] = {}, sc;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sc = Elem<T>::mfma16(r.k[j], qf[j], sc);
+    for (int i = 0; i < 4; ++i) {
+      near[i & 1] = Elem<T>::mfma16(r.k[i], qf[i & 2], near[i & 1]);
+      far[i & 1] = Elem<T>::mfma16(r.k[i], qf[(i & 2) + 1], far[i & 1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sc[e] = lower_halves(near[0][e], near[1][e]) + upper_halves(far[0][e], far[1][e]);
     // sc[e] = S[token 4 q4 + e][g = c].  Rows behind the last token, whatever they hold, do not count.
     if (decltype(may_end)::value && left < kPageSize) {
 #pragma unroll
@@ -328,9 +344,11 @@ extern "C" int mva_paged_decode_selected(const void* q, int64_t q_token_stride, 
                             (float*)((uint8_t*)part_lse + align_up256(slots * 4)), (int*)ws + kSelectionCounters,
                             num_kv_heads, num_q_heads / num_kv_heads, softmax_scale * 1.4426950408889634f};
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == kBF16)
-    hipLaunchKernelGGL(selected_decode_kernel<__bf16>, dim3((uint32_t)blocks), dim3(64 * kSelWaves), 0, st, p);
-  else
-    hipLaunchKernelGGL(selected_decode_kernel<_Float16>, dim3((uint32_t)blocks), dim3(64 * kSelWaves), 0, st, p);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(64 * kSelWaves), 0, st, p);
+  };
+  const bool once = read_once(num_seqs * num_kv_heads * num_selected * 2 * kDecodePageBytes);
+  if (dtype == kBF16) once ? launch(selected_decode_kernel<__bf16, true>) : launch(selected_decode_kernel<__bf16, false>);
+  else once ? launch(selected_decode_kernel<_Float16, true>) : launch(selected_decode_kernel<_Float16, false>);
   return check_launch("selected_decode");
 }
