@@ -578,7 +578,12 @@ PyObject* forward_inputs_ok_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// ---- decode over selected pages ----
+// ---- decode over selected pages (entry points weak, as above) ----
+
+#pragma weak mva_update_page_bounds
+#pragma weak mva_selection_workspace_bytes
+#pragma weak mva_select_pages
+#pragma weak mva_paged_decode_selected
 
 constexpr int64_t kPage = 16;
 
@@ -623,7 +628,7 @@ bool page_numbers(PyObject* const* a, int64_t (&v)[3]) {
 //  num_tokens | None): True when launched.
 PyObject* update_page_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 6) return none();
+    if (&mva_update_page_bounds == nullptr || n != 6) return none();
     const Tensor *kc = plain(a[0]), *bounds = plain(a[1]), *bt = plain(a[2]), *sl = plain(a[3]);
     const Tensor* qsl = a[4] == Py_None ? nullptr : plain(a[4]);
     if (!kc || dtype_code(*kc) < 0 || !selectable(kc, *kc) || !bounds_of_heads(bounds, *kc, kc->size(2)) ||
@@ -669,7 +674,7 @@ int attend(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& ta
 PyObject* select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     int64_t pages[3];
-    if (n != 8 || !page_numbers(a + 4, pages)) return none();
+    if (&mva_select_pages == nullptr || n != 8 || !page_numbers(a + 4, pages)) return none();
     const Tensor *q = plain(a[0]), *bounds = plain(a[1]), *bt = plain(a[2]), *sl = plain(a[3]), *ws = plain(a[7]);
     if (!queries_of(q) || !bounds || bounds->dim() != 4 || !groups(*q, bounds->size(1)) ||
         !bounds_of_heads(bounds, *q, bounds->size(1)) || !table_rows(bt, sl, *q) || sl->size(0) != q->size(0) ||
@@ -692,7 +697,7 @@ PyObject* select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* paged_decode_selected(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     double scale;
-    if (n != 8 || !as_float(a[5], &scale)) return none();
+    if (&mva_paged_decode_selected == nullptr || n != 8 || !as_float(a[5], &scale)) return none();
     const Tensor *q = plain(a[0]), *kc = plain(a[1]), *vc = plain(a[2]), *tables = plain(a[3]), *lens = plain(a[4]);
     const Tensor *given = a[6] == Py_None ? nullptr : plain(a[6]), *ws = plain(a[7]);
     if (!queries_of(q) || !selectable(kc, *q) || !selectable(vc, *q) || kc->sizes() != vc->sizes() ||
@@ -720,7 +725,9 @@ PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     double scale;
     int64_t pages[3];
-    if (n != 12 || !as_float(a[6], &scale) || !page_numbers(a + 7, pages)) return none();
+    if (&mva_select_pages == nullptr || &mva_paged_decode_selected == nullptr || n != 12 ||
+        !as_float(a[6], &scale) || !page_numbers(a + 7, pages))
+      return none();
     const Tensor *q = plain(a[0]), *bounds = plain(a[1]), *kc = plain(a[2]), *vc = plain(a[3]), *bt = plain(a[4]);
     const Tensor *sl = plain(a[5]), *out = plain(a[10]), *ws = plain(a[11]);
     if (!queries_of(q) || !selectable(kc, *q) || !selectable(vc, *q) || kc->sizes() != vc->sizes() ||

@@ -73,11 +73,16 @@ __device__ inline void st16(void* p, V v) {
   *reinterpret_cast<V*>(p) = v;
 }
 
-// 16 bytes that this launch reads once: non-temporal if kOnce.
-template <typename V, bool kOnce>
-__device__ inline V ld16_stream(const void* p) {
-  if constexpr (kOnce) return __builtin_bit_cast(V, __builtin_nontemporal_load((const u32x4*)p));
-  else return ld16<V>(p);
+// 16 bytes that a launch reads once, as a decode step does a layer's cache: a
+// non-temporal load, which takes no room in the last-level cache, whose lines
+// other kernels have written to or will read.  Plain / non-temporal loads in
+// microseconds, attention over 84 MB of selected pages 22.4 / 21.4 after a kernel
+// that read 600 MB and 39.9 / 21.5 after one that wrote them; over 1.07 GB 187 / 168,
+// page scores of 324 MB 78 / 69.  Where the cache still holds the data they are
+// slower (three sets of 84 MB in turns: 19.4 / 20.5).
+template <typename V>
+__device__ inline V ld16_once(const void* p) {
+  return __builtin_bit_cast(V, __builtin_nontemporal_load((const u32x4*)p));
 }
 
 // LDS (address space 3) byte pointer.  Kernels pass LDS buffers around with

@@ -25,13 +25,6 @@ inline bool selection_sizes_ok(int64_t num_seqs, int hq, int hkv, int64_t num_se
          num_seqs * hq <= 0x7fffffffLL && num_selected > 0 && num_selected <= (1 << 24);
 }
 
-// Whether a launch that reads `bytes` once loads them non-temporally: more than
-// the last-level cache of 256 MiB keeps for the next reader.  Plain / non-temporal
-// loads, three sets of inputs in turns: scores of 324 MB 78 / 69 us, attention over
-// 1.07 GB 187 / 168 us; but attention over 84 MB, of which the cache still holds
-// a part, 19.4 / 20.5 us.
-inline bool read_once(int64_t bytes) { return bytes > (int64_t(256) << 20); }
-
 // Bytes of the attention's partials.
 int64_t selection_part_bytes(int64_t num_seqs, int hq, int hkv, int64_t num_selected);
 

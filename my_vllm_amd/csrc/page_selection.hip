@@ -44,7 +44,6 @@ __device__ inline s16x8v nan_mask(s16x8v b) {
   return (b & (short)0x7fff) > (short)kInf;
 }
 
-constexpr int64_t kRowBytes = 256;  // 128 channels
 constexpr int kBoundsTokens = 16;  // tokens whose pages one wavefront looks after
 
 // The sequence of each token first + lane (lanes below kBoundsTokens), the
@@ -90,6 +89,13 @@ __device__ inline TokenOf token_of(const int32_t* starts, int64_t num_seqs, int6
 // One wavefront per (16 tokens of the step, KV head).  Lane t finds the page
 // that token t completes, if any; then, page by page, lane (r, c) = (lane / 16,
 // lane % 16) reads channels 8c .. 8c + 7 of rows r, r + 4, r + 8 and r + 12.
+//
+// Bound by the reads of K where many pages are completed (16384 tokens at 8 KV
+// heads, 38 MB: 9.9 us, of them 1.8 of launch), by the chain starts - length - page id
+// - rows - bounds where few are (61 sequences of one token: 5.1 us).  16 tokens a
+// wavefront: of consecutive positions exactly one page's end.  Values are compared
+// as integers, two a lane's register; a search of the starts lane by lane took
+// 0.2 us longer at 61 sequences.
 template <int kInf>
 __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsParams p) {
   const int lane = threadIdx.x & 63;
@@ -409,12 +415,18 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
 // wavefronts score 16 pages at a time; the row's last workgroup to have scored
 // its pages chooses.
 //
+// Bound by the reads of the bounds on large batches (56 rows of 8192-32768 tokens at
+// 64 / 8 heads, 324 MB: 69 us, 4.7 TB/s over the launch; its reads alone 62).  Small ones are a chain of latencies (one row of 30001 tokens
+// at 32 / 8 heads, 7.7 MB: 9.6 us): launch and length 2.0, page ids 0.5, bounds 2.7,
+// keys counted in 1.4, choice 2.8.  Two launches with the keys in memory between
+// them and one page at a time took 132 and 35.5 us.
+//
 // Lanes 0-31 take one page's 512 bytes and lanes 32-63 the next one's, 16 bytes
 // a lane: lane % 32 / 16 the minima or the maxima, lane % 16 the channels.
 // Products and sums are in 64 bits: products of 16-bit values are exact there
 // and sums of them nearly so, so that which page is taken does not hang on the
 // order of a sum.
-template <typename T, bool kOnce>
+template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p, int chunk, int chunks) {
   typedef typename Elem<T>::v8 V8;
   __shared__ ChoiceLds lds;
@@ -488,7 +500,7 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t a = __builtin_amdgcn_readlane(id, at + 2 * i), b = __builtin_amdgcn_readlane(id, at + 2 * i + 1);
-        box[i] = ld16_stream<V8, kOnce>(bounds + ((uint64_t)(half ? b : a) << 9));
+        box[i] = ld16_once<V8>(bounds + ((uint64_t)(half ? b : a) << 9));
       }
     };
     auto score = [&](const V8 (&box)[8], int t) __attribute__((always_inline)) {
@@ -613,7 +625,10 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
       (uint64_t*)(ws + kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_kv_heads, num_selected)),
       (int*)ws, num_kv_heads, num_q_heads / num_kv_heads};
   // Chunks: as small as 128 pages (16 a wavefront) as long as that makes no more
-  // workgroups than the GPU holds at a time.
+  // workgroups than the GPU holds at a time.  One row of 30001 tokens at 8 KV heads
+  // in chunks of 128, 256 and 512 pages 9.5, 10.2 and 13.0 us; 448 (row, KV head)
+  // pairs of 512-2048 pages in one workgroup each 77 us, in chunks of 1024 pages 86,
+  // of 512 88.
   const int64_t most = table_width - sink_pages - recent_pages;
   int64_t chunk = kBatch * kSelectWaves;
   while (chunk < most && rows * ((most + chunk - 1) / chunk) > kSelectGroups) chunk *= 2;
@@ -621,11 +636,11 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
   const int64_t blocks = rows * chunks;
   if (blocks > 0xffffffffLL / kSelectThreads) return set_error("page selection: too many rows for one launch");
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p, (int)chunk, (int)chunks);
-  };
-  const bool once = read_once(rows * table_width * 2 * kRowBytes);
-  if (dtype == kBF16) once ? launch(page_select_kernel<__bf16, true>) : launch(page_select_kernel<__bf16, false>);
-  else once ? launch(page_select_kernel<_Float16, true>) : launch(page_select_kernel<_Float16, false>);
+  if (dtype == kBF16)
+    hipLaunchKernelGGL(page_select_kernel<__bf16>, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p, (int)chunk,
+                       (int)chunks);
+  else
+    hipLaunchKernelGGL(page_select_kernel<_Float16>, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p,
+                       (int)chunk, (int)chunks);
   return check_launch("page_select");
 }
