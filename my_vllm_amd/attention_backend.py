@@ -1674,7 +1674,7 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
             if held is None or held[0] != capture or held[1].numel() < nbytes:
                 self._captured_workspace = held = (capture, ops.new_selection_workspace(nbytes, device))
             return held[1]
-        key = (device.index, _native.stream_handle(device))
+        key = (device.index, _native.stream_of(device.index))
         workspace = self._stream_workspaces.get(key)
         if workspace is None or workspace.numel() < nbytes:
             self._stream_workspaces[key] = workspace = ops.new_selection_workspace(nbytes, device)

@@ -655,18 +655,18 @@ PyObject* update_page_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 int select(const Tensor& q, const Tensor& bounds, const Tensor& bt, const Tensor& sl, const int64_t (&pages)[3],
-           const Tensor& tables, const Tensor& lens, const Tensor& ws, void* stream) {
+           int32_t* tables, int32_t* lens, const Tensor& ws, void* stream) {
   return unlocked(mva_select_pages, ptr(q), q.stride(0), q.stride(1), ptr(bounds), bounds.size(0), words(&bt),
-                  bt.stride(0), bt.size(1), words(&sl), q.size(0), pages[0], pages[1], pages[2], (int32_t*)ptr(tables),
-                  (int32_t*)ptr(lens), ptr(ws), ws.numel(), (int)q.size(1), (int)bounds.size(1), kHeadDim, (int)kPage,
-                  dtype_code(q), stream);
+                  bt.stride(0), bt.size(1), words(&sl), q.size(0), pages[0], pages[1], pages[2], tables, lens, ptr(ws),
+                  ws.numel(), (int)q.size(1), (int)bounds.size(1), kHeadDim, (int)kPage, dtype_code(q), stream);
 }
-int attend(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& tables, const Tensor& lens, double scale,
-           const Tensor& out, const Tensor& ws, void* stream) {
+int attend(const Tensor& q, const Tensor& kc, const Tensor& vc, const int32_t* tables, int64_t row_stride,
+           int64_t head_stride, int64_t selected, const int32_t* lens, double scale, const Tensor& out,
+           const Tensor& ws, void* stream) {
   return unlocked(mva_paged_decode_selected, ptr(q), q.stride(0), q.stride(1), ptr(kc), ptr(vc), kc.size(0),
-                  kc.stride(0), kc.stride(1), words(&tables), tables.stride(0), tables.stride(1), words(&lens),
-                  q.size(0), tables.size(2), ptr(out), out.stride(0), out.stride(1), ptr(ws), ws.numel(),
-                  (int)q.size(1), (int)kc.size(2), kHeadDim, (int)kPage, (float)scale, dtype_code(q), stream);
+                  kc.stride(0), kc.stride(1), tables, row_stride, head_stride, lens, q.size(0), selected, ptr(out),
+                  out.stride(0), out.stride(1), ptr(ws), ws.numel(), (int)q.size(1), (int)kc.size(2), kHeadDim,
+                  (int)kPage, (float)scale, dtype_code(q), stream);
 }
 
 // (q, page_bounds, block_tables, seq_lens, num_selected, sink_pages, recent_pages,
@@ -683,7 +683,8 @@ PyObject* select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto options = sl->options().requires_grad(false);
     const Tensor tables = at::empty({q->size(0), bounds->size(1), pages[0]}, options);
     const Tensor lens = at::empty({q->size(0)}, options);
-    const int status = select(*q, *bounds, *bt, *sl, pages, tables, lens, *ws, stream_of(*q));
+    const int status = select(*q, *bounds, *bt, *sl, pages, (int32_t*)ptr(tables), (int32_t*)ptr(lens), *ws,
+                              stream_of(*q));
     if (status != 0) return launched("mva_select_pages", status, nullptr);
     PyObject* pair = PyTuple_New(2);
     if (pair == nullptr) return nullptr;
@@ -710,7 +711,8 @@ PyObject* paged_decode_selected(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return none();
     if (a[6] != Py_None && (!given || given->sizes() != q->sizes() || !head_rows(*given, *q))) return none();
     const Tensor out = given ? *given : at::empty(q->sizes(), q->options().requires_grad(false));
-    const int status = attend(*q, *kc, *vc, *tables, *lens, scale, out, *ws, stream_of(*q));
+    const int status = attend(*q, *kc, *vc, words(tables), tables->stride(0), tables->stride(1), tables->size(2),
+                              words(lens), scale, out, *ws, stream_of(*q));
     if (given && status == 0) {
       Py_INCREF(a[6]);
       return a[6];
@@ -736,13 +738,15 @@ PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         out->sizes() != q->sizes() || !head_rows(*out, *q) ||
         !workspace_for(ws, *q, kc->size(2), bt->size(1), pages[0]))
       return none();
-    const auto options = sl->options().requires_grad(false);
-    const Tensor tables = at::empty({q->size(0), kc->size(2), pages[0]}, options);
-    const Tensor lens = at::empty({q->size(0)}, options);
+    // One allocation for the lists and their lengths.
+    const int64_t rows = q->size(0), heads = kc->size(2);
+    const Tensor lists = at::empty({rows * (heads * pages[0] + 1)}, sl->options().requires_grad(false));
+    int32_t* const tables = (int32_t*)ptr(lists);
+    int32_t* const lens = tables + rows * heads * pages[0];
     void* const stream = stream_of(*q);
     int status = select(*q, *bounds, *bt, *sl, pages, tables, lens, *ws, stream);
     if (status != 0) return launched("mva_select_pages", status);
-    status = attend(*q, *kc, *vc, tables, lens, scale, *out, *ws, stream);
+    status = attend(*q, *kc, *vc, tables, heads * pages[0], pages[0], pages[0], lens, scale, *out, *ws, stream);
     return launched("mva_paged_decode_selected", status);
   });
 }
@@ -763,6 +767,17 @@ PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromUnsignedLongLong(id);
 }
 
+// (device index): hipStream_t of torch's current stream of the device, as an int.
+PyObject* stream_handle(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device;
+  if (n != 1 || !as_int(a[0], &device)) return PyErr_Format(PyExc_TypeError, "stream_handle takes a device index");
+  try {
+    return PyLong_FromVoidPtr((void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream());
+  } catch (const std::exception& error) {
+    return PyErr_Format(PyExc_RuntimeError, "%s", error.what());
+  }
+}
+
 #define MVA_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {MVA_METHOD(silu_and_mul),       MVA_METHOD(rms_norm),      MVA_METHOD(fused_add_rms_norm),
                           MVA_METHOD(qk_norm_rope_store), MVA_METHOD(paged_decode),  MVA_METHOD(paged_prefill),
@@ -771,7 +786,7 @@ PyMethodDef kMethods[] = {MVA_METHOD(silu_and_mul),       MVA_METHOD(rms_norm), 
                           MVA_METHOD(paged_decode_mxfp4), MVA_METHOD(paged_prefill_mxfp4),
                           MVA_METHOD(forward_inputs_ok_mxfp4), MVA_METHOD(update_page_bounds),
                           MVA_METHOD(select_pages),       MVA_METHOD(paged_decode_selected),
-                          MVA_METHOD(sparse_decode),
+                          MVA_METHOD(sparse_decode),      MVA_METHOD(stream_handle),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "mva_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
