@@ -6,7 +6,9 @@
 * ``attention_backend``: the gfx950 backend (``MI355XAttentionBackend``,
   ``MI355XSplitAttentionBackend``) and ``integrate``, which registers it in
   the reference's own registry; ``MI355XMXFP4AttentionBackend`` and
-  ``integrate_mxfp4``, the same over a KV cache held in 4 bits.
+  ``integrate_mxfp4``, the same over a KV cache held in 4 bits;
+  ``MI355XSparseAttentionBackend`` and ``integrate_sparse``, whose decode
+  attends to selected pages.
 * ``layers`` / ``providers``: drop-in ``SiluAndMul``, ``KVCacheStore``,
   ``RMSNorm`` and ``RotaryEmbedding`` operators on the gfx950 kernels, and
   the provider names that select them.

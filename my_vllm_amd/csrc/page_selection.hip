@@ -333,11 +333,14 @@ __device__ inline void threshold(Each each, uint64_t some, ChoiceLds& lds, int& 
 }
 
 // Chooses `want` of the scored pages and lists them in the order of their
-// places; all threads of the workgroup, the keys visible to them.
+// places; all threads of the workgroup, the keys visible to them.  Nothing is
+// written beyond `want` entries, whatever a launch that should not overlap does
+// to keys in memory.
 __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds& lds) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint64_t below = (uint64_t(1) << lane) - 1;
+  const int room = want;
   uint64_t top;
   int shift;
   if (r.count <= kKeyRegs * kSelectThreads) {
@@ -377,7 +380,8 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
     for (int i = 0; i < kKeyRegs; ++i) {
       const int before = __builtin_amdgcn_readlane(mine, i * kSelectWaves + wave);
       const int a = (before & 0xffff) + __popcll(gts[i] & below), b = (before >> 16) + __popcll(eqs[i] & below);
-      if ((gts[i] >> lane & 1) || ((eqs[i] >> lane & 1) && b < want)) out[a + min(b, want)] = id[i];
+      const int at = a + min(b, want);
+      if (((gts[i] >> lane & 1) || ((eqs[i] >> lane & 1) && b < want)) && at < room) out[at] = id[i];
     }
     return;
   }
@@ -406,7 +410,8 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
       above += lds.counts[2 * w];
       equal += lds.counts[2 * w + 1];
     }
-    if ((gts >> lane & 1) || ((eqs >> lane & 1) && b < want)) out[a + min(b, want)] = r.row[j];
+    const int at = a + min(b, want);
+    if (((gts >> lane & 1) || ((eqs >> lane & 1) && b < want)) && at < room) out[at] = r.row[j];
     __syncthreads();
   }
 }
@@ -416,10 +421,11 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
 // its pages chooses.
 //
 // Bound by the reads of the bounds on large batches (56 rows of 8192-32768 tokens at
-// 64 / 8 heads, 324 MB: 69 us, 4.7 TB/s over the launch; its reads alone 62).  Small ones are a chain of latencies (one row of 30001 tokens
-// at 32 / 8 heads, 7.7 MB: 9.6 us): launch and length 2.0, page ids 0.5, bounds 2.7,
-// keys counted in 1.4, choice 2.8.  Two launches with the keys in memory between
-// them and one page at a time took 132 and 35.5 us.
+// 64 / 8 heads, 324 MB: 69 us, 4.7 TB/s over the launch; its reads alone 62).  Small
+// ones are a chain of latencies (one row of 30001 tokens at 32 / 8 heads, 7.7 MB:
+// 9.6 us): launch and length 2.0, page ids 0.5, bounds 2.7, keys counted in 1.4,
+// choice 2.8.  Two launches with the keys in memory between them and one page at a
+// time took 132 and 35.5 us.
 //
 // Lanes 0-31 take one page's 512 bytes and lanes 32-63 the next one's, 16 bytes
 // a lane: lane % 32 / 16 the minima or the maxima, lane % 16 the channels.
@@ -563,7 +569,7 @@ extern "C" int mva_update_page_bounds(const void* k_cache, int64_t num_pages, in
   if (head_dim != 128 || page_size != kPageTokens) return set_error("page bounds: head_dim must be 128, page_size 16");
   if (dtype != kBF16 && dtype != kF16) return set_error("page bounds: dtype must be bf16 or fp16");
   if (num_kv_heads <= 0 || num_pages < 0 || num_pages > 0x7fffffffLL || num_seqs < 0 || num_tokens < 0 ||
-      table_width < 0 || block_table_stride < 0)
+      table_width < 0 || block_table_stride < 0 || page_stride < 0 || token_stride < 0)
     return set_error("page bounds: invalid sizes");
   if (query_start_loc == nullptr && num_tokens != num_seqs)
     return set_error("page bounds: without query_start_loc every sequence has one token");

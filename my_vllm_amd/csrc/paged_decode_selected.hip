@@ -326,7 +326,7 @@ extern "C" int mva_paged_decode_selected(const void* q, int64_t q_token_stride, 
     return set_error("selected attention: head_dim must be 128, page_size 16");
   if (dtype != kBF16 && dtype != kF16) return set_error("selected attention: dtype must be bf16 or fp16");
   if (!selection_sizes_ok(num_seqs, num_q_heads, num_kv_heads, num_selected) || seq_table_stride < 0 ||
-      head_table_stride < 0)
+      head_table_stride < 0 || page_stride < 0)
     return set_error("selected attention: invalid sizes");
   if (num_pages <= 0 || num_pages > 0x7fffffffLL) return set_error("selected attention: empty or oversized KV cache");
   if (!(softmax_scale > 0.f && softmax_scale < INFINITY))

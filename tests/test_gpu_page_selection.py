@@ -322,6 +322,16 @@ def test_out_strides_layers_of_a_pool_and_shared_lists(gpu):
     assert (whole[:, :4] == 7).all() and (whole[:, 12:] == 7).all()
 
 
+@pytest.mark.parametrize("rows,n", [(1, 128), (3, 40), (200, 20)])
+def test_out_may_be_the_queries(gpu, rows, n):
+    lens = [16 * n - s % 5 for s in range(rows)]
+    k, v = keys(n, 4, BF16, 1).to(gpu), keys(n, 4, BF16, 2).to(gpu)
+    tables = _lists([n], 4, n, n, 3).to(gpu).expand(rows, 4, n)
+    q = queries(rows, 16, BF16, 4).to(gpu)
+    want = ops.paged_decode_selected(q, k, v, tables, _ints(lens, gpu), SCALE)
+    assert torch.equal(ops.paged_decode_selected(q, k, v, tables, _ints(lens, gpu), SCALE, out=q), want)
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 def test_a_nan_or_infinite_key_or_value_shows(gpu, value):
     lens, n = [100, 90], 8

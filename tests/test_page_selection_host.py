@@ -115,7 +115,7 @@ def test_entries_of_no_rows_do_nothing():
 @pytest.mark.parametrize("change,message", [
     ({13: 64}, "head_dim"), ({14: 8}, "page_size"), ({15: 7}, "dtype"), ({12: 0}, "sizes"), ({1: -1}, "sizes"),
     ({11: -4}, "sizes"), ({9: 0}, "query_start_loc"), ({0: 0}, "null"), ({0: 0x1002}, "aligned"),
-    ({4: 0x1008}, "aligned"), ({3: 1023}, "aligned"), ({11: 1 << 40}, "too many"),
+    ({2: -1024}, "sizes"), ({3: -16}, "sizes"), ({4: 0x1008}, "aligned"), ({3: 1023}, "aligned"), ({11: 1 << 40}, "too many"),
 ])
 def test_bounds_entry_refuses(change, message):
     args = [0x1000, 10, 16 * 1024, 1024, 0x1000, 0x1000, 20, 20, 0x1000, 0x1000, 2, 7, 8, 128, 16, 0, 0]
@@ -127,7 +127,7 @@ def test_bounds_entry_refuses(change, message):
 
 @pytest.mark.parametrize("change,message", [
     ({21: 64}, "head_dim"), ({22: 8}, "page_size"), ({24: 2}, "dtype"), ({19: 9}, "sizes"), ({13: 0}, "sizes"),
-    ({9: -1}, "sizes"), ({5: 0}, "empty"), ({3: 0}, "null"), ({14: 0}, "null"), ({0: 0x1004}, "aligned"),
+    ({9: -1}, "sizes"), ({6: -1024}, "sizes"), ({5: 0}, "empty"), ({3: 0}, "null"), ({14: 0}, "null"), ({0: 0x1004}, "aligned"),
     ({7: 1 << 27}, "2\\^26"), ({23: 0.0}, "softmax_scale"), ({23: math.nan}, "softmax_scale"),
     ({6: 16 * 1024 + 1}, "aligned"), ({14: 0x1004}, "aligned"), ({17: 0}, "workspace"), ({18: 100}, "workspace"),
 ])
