@@ -621,12 +621,18 @@ int64_t mva_selection_workspace_bytes(int64_t num_seqs, int num_q_heads, int num
  * the last; lens ([num_seqs]) the tokens they hold, those of the last page
  * counted to the row's end.  A row of seq_lens <= 0 gets no page and 0; one longer
  * than its table counts as long as the table.
+ *
+ * With k_cache (or NULL) the launch also does what mva_update_page_bounds does for one
+ * token a sequence: a page that a row's last token completes is that row's last and
+ * is not scored.  It must not be a page that another row scores: the rows are
+ * different sequences then.  page_bounds is written.
  */
 int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* page_bounds,
                      int64_t num_pages, const int32_t* block_tables, int64_t block_table_stride, int64_t table_width,
                      const int32_t* seq_lens, int64_t num_seqs, int64_t num_selected, int64_t sink_pages,
-                     int64_t recent_pages, int32_t* tables, int32_t* lens, void* workspace, int64_t workspace_bytes,
-                     int num_q_heads, int num_kv_heads, int head_dim, int page_size, int dtype, void* stream);
+                     int64_t recent_pages, int32_t* tables, int32_t* lens, const void* k_cache, int64_t page_stride,
+                     int64_t token_stride, void* workspace, int64_t workspace_bytes, int num_q_heads,
+                     int num_kv_heads, int head_dim, int page_size, int dtype, void* stream);
 
 /*
  * Attention of one query a row over the first lens[s] tokens of the pages

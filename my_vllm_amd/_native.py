@@ -175,6 +175,7 @@ _SIGNATURES = {
             _c_void_p, _i64, _i64, _c_void_p, _i64,  # q and its strides, page_bounds, num_pages
             _c_void_p, _i64, _i64, _c_void_p, _i64,  # block_tables, stride, width, seq_lens, seqs
             _i64, _i64, _i64, _c_void_p, _c_void_p,  # selected, sink and recent pages, tables, lens
+            _c_void_p, _i64, _i64,  # k_cache, page and token strides
             _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p,  # workspace, bytes, heads, dim, page, dtype, stream
         ],
     ),

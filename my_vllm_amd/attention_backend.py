@@ -1620,8 +1620,10 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
                 raise ValueError(f"{name} must be at least {least}")
         if self.sink_pages + self.recent_pages > self.selected_pages:
             raise ValueError("sink_pages + recent_pages must be at most selected_pages")
-        # The page bounds of the layer that forward runs.
+        # The page bounds of the layer that forward runs, and whether its selection
+        # brings them up to date.
         self._page_bounds: torch.Tensor | None = None
+        self._update_bounds = False
         # Workspaces of eager steps, by GPU and stream.
         self._stream_workspaces: dict[tuple, torch.Tensor] = {}
 
@@ -1630,14 +1632,23 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
 
     def forward_with_kv_store(self, q, k, v, k_cache, v_cache, slot_mapping, plan, store=None,
                               page_bounds=None) -> torch.Tensor:
-        """The step's K/V rows into the caches (``store``, or ``ops.store_kvcache``),
-        :meth:`update_page_bounds`, then :meth:`forward`."""
-        if _has_cache(k_cache):
-            if page_bounds is None:
-                raise ValueError("a backend that selects pages needs page_bounds")
-            (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
+        """The step's K/V rows into the caches (``store``, or ``ops.store_kvcache``), the
+        bounds of the pages that they complete, then :meth:`forward`.  A step of decode
+        rows alone writes the bounds in the selection's launch."""
+        if not _has_cache(k_cache):
+            return self.forward(q, k, v, k_cache, v_cache, plan, page_bounds=page_bounds)
+        if page_bounds is None:
+            raise ValueError("a backend that selects pages needs page_bounds")
+        (store if store is not None else self._store_rows)(k, v, k_cache, v_cache, slot_mapping)
+        decode = self._active_graph_state is not None or (
+            isinstance(plan, self.plan_type) and plan.route is self.route_type.DECODE)
+        if not decode:
             self.update_page_bounds(k_cache, page_bounds, plan)
-        return self.forward(q, k, v, k_cache, v_cache, plan, page_bounds=page_bounds)
+        self._update_bounds = decode
+        try:
+            return self.forward(q, k, v, k_cache, v_cache, plan, page_bounds=page_bounds)
+        finally:
+            self._update_bounds = False
 
     def update_page_bounds(self, k_cache, page_bounds, plan) -> None:
         """The bounds of the pages that the plan's step completes
@@ -1687,7 +1698,7 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
                                                self.selected_pages)
         ops.sparse_decode(q, self._page_bounds, k_cache, v_cache, block_tables, seq_lens, self.softmax_scale,
                           self.selected_pages, self.sink_pages, self.recent_pages, out=out,
-                          workspace=self._get_workspace(nbytes, q.device))
+                          workspace=self._get_workspace(nbytes, q.device), update_bounds=self._update_bounds)
 
     def _run_decode(self, q, k_cache, v_cache, common, metadata: MI355XAttentionMetadata, output) -> None:
         first, rows = common.num_prefill_seqs, common.num_prefill_tokens

@@ -655,10 +655,12 @@ PyObject* update_page_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 int select(const Tensor& q, const Tensor& bounds, const Tensor& bt, const Tensor& sl, const int64_t (&pages)[3],
-           int32_t* tables, int32_t* lens, const Tensor& ws, void* stream) {
+           int32_t* tables, int32_t* lens, const Tensor* update, const Tensor& ws, void* stream) {
   return unlocked(mva_select_pages, ptr(q), q.stride(0), q.stride(1), ptr(bounds), bounds.size(0), words(&bt),
-                  bt.stride(0), bt.size(1), words(&sl), q.size(0), pages[0], pages[1], pages[2], tables, lens, ptr(ws),
-                  ws.numel(), (int)q.size(1), (int)bounds.size(1), kHeadDim, (int)kPage, dtype_code(q), stream);
+                  bt.stride(0), bt.size(1), words(&sl), q.size(0), pages[0], pages[1], pages[2], tables, lens,
+                  (const void*)(update ? ptr(*update) : nullptr), update ? update->stride(0) : 0,
+                  update ? update->stride(1) : 0, ptr(ws), ws.numel(), (int)q.size(1), (int)bounds.size(1), kHeadDim,
+                  (int)kPage, dtype_code(q), stream);
 }
 int attend(const Tensor& q, const Tensor& kc, const Tensor& vc, const int32_t* tables, int64_t row_stride,
            int64_t head_stride, int64_t selected, const int32_t* lens, double scale, const Tensor& out,
@@ -670,21 +672,25 @@ int attend(const Tensor& q, const Tensor& kc, const Tensor& vc, const int32_t* t
 }
 
 // (q, page_bounds, block_tables, seq_lens, num_selected, sink_pages, recent_pages,
-//  workspace): (tables, lens).
+//  workspace, k_cache | None): (tables, lens).
 PyObject* select_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     int64_t pages[3];
-    if (&mva_select_pages == nullptr || n != 8 || !page_numbers(a + 4, pages)) return none();
+    if (&mva_select_pages == nullptr || n != 9 || !page_numbers(a + 4, pages)) return none();
     const Tensor *q = plain(a[0]), *bounds = plain(a[1]), *bt = plain(a[2]), *sl = plain(a[3]), *ws = plain(a[7]);
     if (!queries_of(q) || !bounds || bounds->dim() != 4 || !groups(*q, bounds->size(1)) ||
         !bounds_of_heads(bounds, *q, bounds->size(1)) || !table_rows(bt, sl, *q) || sl->size(0) != q->size(0) ||
         !workspace_for(ws, *q, bounds->size(1), bt->size(1), pages[0]))
       return none();
+    const Tensor* update = a[8] == Py_None ? nullptr : plain(a[8]);
+    if (a[8] != Py_None && (!selectable(update, *q) || update->size(2) != bounds->size(1) ||
+                            update->size(0) != bounds->size(0)))
+      return none();
     const auto options = sl->options().requires_grad(false);
     const Tensor tables = at::empty({q->size(0), bounds->size(1), pages[0]}, options);
     const Tensor lens = at::empty({q->size(0)}, options);
-    const int status = select(*q, *bounds, *bt, *sl, pages, (int32_t*)ptr(tables), (int32_t*)ptr(lens), *ws,
-                              stream_of(*q));
+    const int status = select(*q, *bounds, *bt, *sl, pages, (int32_t*)ptr(tables), (int32_t*)ptr(lens), update,
+                              *ws, stream_of(*q));
     if (status != 0) return launched("mva_select_pages", status, nullptr);
     PyObject* pair = PyTuple_New(2);
     if (pair == nullptr) return nullptr;
@@ -722,13 +728,13 @@ PyObject* paged_decode_selected(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (q, page_bounds, k_cache, v_cache, block_tables, seq_lens, scale, num_selected,
-//  sink_pages, recent_pages, out, workspace): True when launched.
+//  sink_pages, recent_pages, out, workspace, update_bounds): True when launched.
 PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     double scale;
     int64_t pages[3];
-    if (&mva_select_pages == nullptr || &mva_paged_decode_selected == nullptr || n != 12 ||
-        !as_float(a[6], &scale) || !page_numbers(a + 7, pages))
+    if (&mva_select_pages == nullptr || &mva_paged_decode_selected == nullptr || n != 13 ||
+        !as_float(a[6], &scale) || !page_numbers(a + 7, pages) || !PyBool_Check(a[12]))
       return none();
     const Tensor *q = plain(a[0]), *bounds = plain(a[1]), *kc = plain(a[2]), *vc = plain(a[3]), *bt = plain(a[4]);
     const Tensor *sl = plain(a[5]), *out = plain(a[10]), *ws = plain(a[11]);
@@ -744,7 +750,7 @@ PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int32_t* const tables = (int32_t*)ptr(lists);
     int32_t* const lens = tables + rows * heads * pages[0];
     void* const stream = stream_of(*q);
-    int status = select(*q, *bounds, *bt, *sl, pages, tables, lens, *ws, stream);
+    int status = select(*q, *bounds, *bt, *sl, pages, tables, lens, a[12] == Py_True ? kc : nullptr, *ws, stream);
     if (status != 0) return launched("mva_select_pages", status);
     status = attend(*q, *kc, *vc, tables, heads * pages[0], pages[0], pages[0], lens, scale, *out, *ws, stream);
     return launched("mva_paged_decode_selected", status);

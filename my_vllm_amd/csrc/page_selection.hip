@@ -12,6 +12,8 @@
 #include "mva_common.h"
 #include "page_selection.h"
 
+#include <type_traits>
+
 namespace mva {
 namespace {
 
@@ -44,6 +46,7 @@ __device__ inline s16x8v nan_mask(s16x8v b) {
   return (b & (short)0x7fff) > (short)kInf;
 }
 
+constexpr int kInfBF16 = 0x7f80, kInfF16 = 0x7c00;  // bits of the infinities
 constexpr int kBoundsTokens = 16;  // tokens whose pages one wavefront looks after
 
 // The sequence of each token first + lane (lanes below kBoundsTokens), the
@@ -97,9 +100,7 @@ __device__ inline TokenOf token_of(const int32_t* starts, int64_t num_seqs, int6
 // as integers, two a lane's register; a search of the starts lane by lane took
 // 0.2 us longer at 61 sequences.
 template <int kInf>
-__global__ __launch_bounds__(256) void page_bounds_kernel(BoundsParams p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ inline void bounds_of_tokens(const BoundsParams& p, int64_t unit, int lane) {
   const int64_t first = unit / p.num_kv_heads * kBoundsTokens;
   const int h = (int)(unit % p.num_kv_heads);
   if (first >= p.num_tokens) return;
@@ -147,6 +148,12 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(BoundsParams p) {
     hi |= bad & (short)0x7fff;
     if (lane < 32) st16(p.bounds + ((id * p.num_kv_heads + h) * 2 + r) * 256 + c * 16, r == 0 ? lo : hi);
   }
+}
+
+template <int kInf>
+__global__ __launch_bounds__(256) void page_bounds_kernel(BoundsParams p) {
+  bounds_of_tokens<kInf>(p, (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+                         threadIdx.x & 63);
 }
 
 // ---- scores --------------------------------------------------------------------
@@ -427,17 +434,27 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
 // choice 2.8.  Two launches with the keys in memory between them and one page at a
 // time took 132 and 35.5 us.
 //
+// Workgroups from `blocks` on write the bounds of the pages that the rows' last
+// tokens complete.  Such a page is its row's last and is not scored, so a decode
+// step of different sequences needs no launch before this one for them.
+//
 // Lanes 0-31 take one page's 512 bytes and lanes 32-63 the next one's, 16 bytes
 // a lane: lane % 32 / 16 the minima or the maxima, lane % 16 the channels.
 // Products and sums are in 64 bits: products of 16-bit values are exact there
 // and sums of them nearly so, so that which page is taken does not hang on the
 // order of a sum.
 template <typename T>
-__global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p, int chunk, int chunks) {
+__global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p, int chunk, int chunks,
+                                                                    uint32_t blocks, BoundsParams update) {
   typedef typename Elem<T>::v8 V8;
   __shared__ ChoiceLds lds;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (blockIdx.x >= blocks) {
+    constexpr int kInf = std::is_same<T, __bf16>::value ? kInfBF16 : kInfF16;
+    bounds_of_tokens<kInf>(update, (int64_t)(blockIdx.x - blocks) * kSelectWaves + wave, lane);
+    return;
+  }
   const int h = (int)(blockIdx.x % p.num_kv_heads);
   const int part = (int)(blockIdx.x / p.num_kv_heads % chunks);
   const int64_t s = blockIdx.x / p.num_kv_heads / chunks;
@@ -560,6 +577,38 @@ int64_t selection_keys_bytes(int64_t num_seqs, int hkv, int64_t width) { return 
 
 }  // namespace mva
 
+namespace mva {
+namespace {
+
+// The parameters of an update of the bounds, or an error; p.num_tokens 0: nothing to do.
+int bounds_params(BoundsParams& p, const void* k_cache, int64_t num_pages, int64_t page_stride, int64_t token_stride,
+                  const void* page_bounds, const int32_t* block_tables, int64_t block_table_stride,
+                  int64_t table_width, const int32_t* seq_lens, const int32_t* query_start_loc, int64_t num_seqs,
+                  int64_t num_tokens, int num_kv_heads) {
+  if (num_kv_heads <= 0 || num_pages < 0 || num_pages > 0x7fffffffLL || num_seqs < 0 || num_tokens < 0 ||
+      table_width < 0 || block_table_stride < 0 || page_stride < 0 || token_stride < 0)
+    return set_error("page bounds: invalid sizes");
+  if (query_start_loc == nullptr && num_tokens != num_seqs)
+    return set_error("page bounds: without query_start_loc every sequence has one token");
+  p = {(const uint8_t*)k_cache, num_pages, page_stride * 2, token_stride * 2, (uint8_t*)page_bounds, block_tables,
+       block_table_stride, table_width, seq_lens, query_start_loc, num_seqs, num_tokens, num_kv_heads};
+  if (num_seqs == 0 || num_pages == 0 || table_width == 0) p.num_tokens = 0;
+  if (p.num_tokens == 0) return 0;
+  if (!k_cache || !page_bounds || !block_tables || !seq_lens) return set_error("page bounds: null buffer");
+  if (((uint64_t)(uintptr_t)k_cache | (uint64_t)(uintptr_t)page_bounds | (uint64_t)(page_stride * 2) |
+       (uint64_t)(token_stride * 2)) % 16)
+    return set_error("page bounds: cache and bounds must be 16-byte aligned");
+  return 0;
+}
+
+// Workgroups of `waves` wavefronts for an update.
+int64_t bounds_blocks(const BoundsParams& p, int waves) {
+  return ((p.num_tokens + kBoundsTokens - 1) / kBoundsTokens * p.num_kv_heads + waves - 1) / waves;
+}
+
+}  // namespace
+}  // namespace mva
+
 extern "C" int mva_update_page_bounds(const void* k_cache, int64_t num_pages, int64_t page_stride,
                                       int64_t token_stride, void* page_bounds, const int32_t* block_tables,
                                       int64_t block_table_stride, int64_t table_width, const int32_t* seq_lens,
@@ -568,24 +617,17 @@ extern "C" int mva_update_page_bounds(const void* k_cache, int64_t num_pages, in
   using namespace mva;
   if (head_dim != 128 || page_size != kPageTokens) return set_error("page bounds: head_dim must be 128, page_size 16");
   if (dtype != kBF16 && dtype != kF16) return set_error("page bounds: dtype must be bf16 or fp16");
-  if (num_kv_heads <= 0 || num_pages < 0 || num_pages > 0x7fffffffLL || num_seqs < 0 || num_tokens < 0 ||
-      table_width < 0 || block_table_stride < 0 || page_stride < 0 || token_stride < 0)
-    return set_error("page bounds: invalid sizes");
-  if (query_start_loc == nullptr && num_tokens != num_seqs)
-    return set_error("page bounds: without query_start_loc every sequence has one token");
-  if (num_seqs == 0 || num_tokens == 0 || num_pages == 0 || table_width == 0) return 0;
-  if (!k_cache || !page_bounds || !block_tables || !seq_lens) return set_error("page bounds: null buffer");
-  if (((uint64_t)(uintptr_t)k_cache | (uint64_t)(uintptr_t)page_bounds | (uint64_t)(page_stride * 2) |
-       (uint64_t)(token_stride * 2)) % 16)
-    return set_error("page bounds: cache and bounds must be 16-byte aligned");
-  const int64_t blocks = ((num_tokens + kBoundsTokens - 1) / kBoundsTokens * num_kv_heads + 3) / 4;
+  BoundsParams p;
+  if (const int rc = bounds_params(p, k_cache, num_pages, page_stride, token_stride, page_bounds, block_tables,
+                                   block_table_stride, table_width, seq_lens, query_start_loc, num_seqs, num_tokens,
+                                   num_kv_heads))
+    return rc;
+  if (p.num_tokens == 0) return 0;
+  const int64_t blocks = bounds_blocks(p, 4);
   if (blocks > 0xffffffffLL / 256) return set_error("page bounds: too many tokens for one launch");
-  const BoundsParams p = {(const uint8_t*)k_cache, num_pages, page_stride * 2, token_stride * 2, (uint8_t*)page_bounds,
-                          block_tables, block_table_stride, table_width, seq_lens, query_start_loc, num_seqs,
-                          num_tokens, num_kv_heads};
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == kBF16) hipLaunchKernelGGL(page_bounds_kernel<0x7f80>, dim3((uint32_t)blocks), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(page_bounds_kernel<0x7c00>, dim3((uint32_t)blocks), dim3(256), 0, st, p);
+  if (dtype == kBF16) hipLaunchKernelGGL(page_bounds_kernel<kInfBF16>, dim3((uint32_t)blocks), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(page_bounds_kernel<kInfF16>, dim3((uint32_t)blocks), dim3(256), 0, st, p);
   return check_launch("page_bounds");
 }
 
@@ -603,7 +645,7 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
                                 int64_t num_pages, const int32_t* block_tables, int64_t block_table_stride,
                                 int64_t table_width, const int32_t* seq_lens, int64_t num_seqs, int64_t num_selected,
                                 int64_t sink_pages, int64_t recent_pages, int32_t* tables, int32_t* lens,
-                                void* workspace, int64_t workspace_bytes, int num_q_heads, int num_kv_heads,
+                                const void* k_cache, int64_t page_stride, int64_t token_stride, void* workspace, int64_t workspace_bytes, int num_q_heads, int num_kv_heads,
                                 int head_dim, int page_size, int dtype, void* stream) {
   using namespace mva;
   if (head_dim != 128 || page_size != kPageTokens) return set_error("page selection: head_dim must be 128, page_size 16");
@@ -640,13 +682,21 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
   while (chunk < most && rows * ((most + chunk - 1) / chunk) > kSelectGroups) chunk *= 2;
   const int64_t chunks = most > chunk && table_width > num_selected ? (most + chunk - 1) / chunk : 1;
   const int64_t blocks = rows * chunks;
-  if (blocks > 0xffffffffLL / kSelectThreads) return set_error("page selection: too many rows for one launch");
+  BoundsParams update = {};
+  if (k_cache != nullptr) {
+    if (const int rc = bounds_params(update, k_cache, num_pages, page_stride, token_stride, page_bounds, block_tables,
+                                     block_table_stride, table_width, seq_lens, nullptr, num_seqs, num_seqs,
+                                     num_kv_heads))
+      return rc;
+  }
+  const int64_t all = blocks + (k_cache != nullptr ? bounds_blocks(update, kSelectWaves) : 0);
+  if (all > 0xffffffffLL / kSelectThreads) return set_error("page selection: too many rows for one launch");
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == kBF16)
-    hipLaunchKernelGGL(page_select_kernel<__bf16>, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p, (int)chunk,
-                       (int)chunks);
+    hipLaunchKernelGGL(page_select_kernel<__bf16>, dim3((uint32_t)all), dim3(kSelectThreads), 0, st, p, (int)chunk,
+                       (int)chunks, (uint32_t)blocks, update);
   else
-    hipLaunchKernelGGL(page_select_kernel<_Float16>, dim3((uint32_t)blocks), dim3(kSelectThreads), 0, st, p,
-                       (int)chunk, (int)chunks);
+    hipLaunchKernelGGL(page_select_kernel<_Float16>, dim3((uint32_t)all), dim3(kSelectThreads), 0, st, p, (int)chunk,
+                       (int)chunks, (uint32_t)blocks, update);
   return check_launch("page_select");
 }

@@ -1320,6 +1320,7 @@ def select_pages(
     recent_pages: int = 1,
     *,
     workspace: torch.Tensor | None = None,
+    k_cache: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Choose the pages that each row's query attends to, for every KV head.
 
@@ -1337,9 +1338,14 @@ def select_pages(
     Returns ``(tables, lens)``: int32 ``[S, Hkv, num_selected]`` page ids in the
     order of their places, -1 after a row's last, and int32 ``[S]`` the tokens
     that they hold, for :func:`paged_decode_selected`.  A row of ``seq_lens`` 0
-    gets no page."""
+    gets no page.
+
+    With ``k_cache``, which holds the step's rows, the launch also brings the bounds
+    up to date, as :func:`update_page_bounds` does for one new token a sequence.  The
+    rows must then be different sequences: a page that one of them completes is its
+    last, and no other may score it."""
     fast = _native.host_ops().select_pages(q, page_bounds, block_tables, seq_lens, num_selected, sink_pages,
-                                           recent_pages, workspace)
+                                           recent_pages, workspace, k_cache)
     if fast is not None:
         return fast
     _check_queries(q)
@@ -1360,6 +1366,10 @@ def select_pages(
     width = block_tables.size(1)
     if num_seqs and (width == 0 or page_bounds.size(0) == 0):
         raise ValueError("page selection needs pages")
+    if k_cache is not None:
+        _check_cache("k_cache", k_cache, device, dtype)
+        if k_cache.size(0) != page_bounds.size(0) or k_cache.size(2) != num_kv_heads:
+            raise ValueError("page_bounds must have the cache's number of pages and KV heads")
     tables = torch.empty((num_seqs, num_kv_heads, num_selected), dtype=torch.int32, device=device)
     lens = torch.empty(num_seqs, dtype=torch.int32, device=device)
     workspace = _selection_workspace(
@@ -1372,6 +1382,8 @@ def select_pages(
         q.data_ptr(), q.stride(0), q.stride(1), page_bounds.data_ptr(), page_bounds.size(0),
         block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), num_seqs,
         num_selected, sink_pages, recent_pages, tables.data_ptr(), lens.data_ptr(),
+        k_cache.data_ptr() if k_cache is not None else 0, k_cache.stride(0) if k_cache is not None else 0,
+        k_cache.stride(1) if k_cache is not None else 0,
         workspace.data_ptr(), workspace.numel(), num_q_heads, num_kv_heads, HEAD_DIM, PAGE_SIZE,
         _native.dtype_code(dtype), _native.stream_handle(device),
     )
@@ -1454,15 +1466,17 @@ def sparse_decode(
     *,
     out: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
+    update_bounds: bool = False,
 ) -> torch.Tensor:
-    """:func:`select_pages` and :func:`paged_decode_selected` over what it chose, in
-    one call; ``page_bounds`` has the caches' number of pages."""
+    """:func:`select_pages` (with ``k_cache`` if ``update_bounds``) and
+    :func:`paged_decode_selected` over what it chose, in one call; ``page_bounds`` has
+    the caches' number of pages."""
     if out is not None and _native.host_ops().sparse_decode(q, page_bounds, k_cache, v_cache, block_tables, seq_lens,
                                                             softmax_scale, num_selected, sink_pages, recent_pages,
-                                                            out, workspace):
+                                                            out, workspace, update_bounds):
         return out
     if page_bounds.size(0) != k_cache.size(0):
         raise ValueError("page_bounds must have the cache's number of pages")
     tables, lens = select_pages(q, page_bounds, block_tables, seq_lens, num_selected, sink_pages, recent_pages,
-                                workspace=workspace)
+                                workspace=workspace, k_cache=k_cache if update_bounds else None)
     return paged_decode_selected(q, k_cache, v_cache, tables, lens, softmax_scale, out=out, workspace=workspace)

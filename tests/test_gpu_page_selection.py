@@ -217,6 +217,42 @@ def test_values_at_the_ends_of_the_types(gpu):
             _check_selection(gpu, q, bounds, torch.arange(300, dtype=torch.int32)[None], [4800], 25, 1, 1)
 
 
+@pytest.mark.parametrize("hq,hkv,dtype", [(8, 8, BF16), (16, 1, FP16), (9, 3, BF16)])
+@pytest.mark.parametrize("rows", [1, 15, 40, 300])
+def test_selection_that_brings_the_bounds_up_to_date(gpu, hq, hkv, dtype, rows):
+    lens = [16 + 16 * (7 * s % 23) + (0, 0, 1, 15)[s % 4] for s in range(rows)]
+    counts = page_counts(lens)
+    cache = keys(sum(counts), hkv, dtype, rows)
+    table, q = tables_for(counts, sum(counts), rows + 1), queries(rows, hq, dtype, rows + 2)
+    # Pages that this step's tokens complete have none yet.
+    bounds = bounds_of(cache)
+    for s, length in enumerate(lens):
+        if length % 16 == 0:
+            bounds[table[s, counts[s] - 1].long()] = math.nan
+    for given in (cache.to(gpu), torch.stack((cache, cache), 1).to(gpu)[:, 1]):
+        got = bounds.to(gpu)
+        tables, kept = ops.select_pages(q.to(gpu), got, table.to(gpu), _ints(lens, gpu), 9, 1, 2, k_cache=given)
+        assert same(got, selection.page_bounds(cache, bounds, table, lens, [1] * rows)) and not got.isnan().any()
+        want = selection.select_pages(q, bounds_of(cache), table, lens, 9, 1, 2)
+        assert torch.equal(tables.cpu(), want[0]) and torch.equal(kept.cpu(), want[1])
+
+
+def test_lengths_beyond_the_tables_count_as_theirs(gpu):
+    cache = keys(40, 2, BF16, 1)
+    table = tables_for([20, 20], 40, 2)
+    long, full = [16 * 20 + 5, 2 ** 31 - 1], [16 * 20, 16 * 20]
+    q = queries(2, 4, BF16, 3)
+    got = _select(gpu, q, bounds_of(cache), table, long, 6, 1, 1)
+    want = selection.select_pages(q, bounds_of(cache), table, full, 6, 1, 1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # More tokens than a list's pages hold: all of its pages.
+    k, v = cache.to(gpu), keys(40, 2, BF16, 4).to(gpu)
+    lists = got[0].to(gpu)
+    outs = [ops.paged_decode_selected(q.to(gpu), k, v, lists, _ints(lens, gpu), SCALE)
+            for lens in ([96, 96], [97, 2 ** 31 - 1])]
+    assert torch.equal(*outs)
+
+
 def test_strided_queries_and_tables(gpu):
     # Queries as a view of the packed projection, tables as columns of a wider buffer.
     lens = [700, 16, 900]

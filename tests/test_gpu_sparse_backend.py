@@ -269,6 +269,9 @@ def test_operators_refuse(gpu):
     _refused(ValueError, "needs pages", select, q, bounds[:0], table, lens, 4)
     _refused(ValueError, "bytes", select, q, bounds, table, lens, 4,
              workspace=torch.empty(8, dtype=torch.uint8, device=gpu))
+    _refused(TypeError, "dtype", select, q, bounds, table, lens, 4, k_cache=k.half())
+    _refused(ValueError, "number of pages", select, q, bounds, table, lens, 4, k_cache=k[:5])
+    _refused(ValueError, "overlap", select, q, bounds, table, lens, 4, k_cache=k[:1].expand(6, 16, 2, 128))
     _refused(ValueError, "uint8", select, q, bounds, table, lens, 4, workspace=torch.empty(1 << 20, device=gpu))
     lists = table[:, None].expand(3, 2, 6)
     _refused(TypeError, "dtype", attend, q, k.half(), k, lists, lens, 1.0)

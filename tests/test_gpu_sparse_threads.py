@@ -28,10 +28,11 @@ table, lens, starts = torch.zeros(4, 2, **i32), torch.zeros(4, **i32), torch.zer
 lists, ws = torch.zeros(4, 2, 3, **i32), torch.zeros(64, dtype=torch.uint8, device="cuda")
 for name, args in (("update_page_bounds", (cache, bounds, table, lens, None, None)),
                    ("update_page_bounds", (cache, bounds, table, lens, starts, 4)),
-                   ("select_pages", (q, bounds, table, lens, 3, 1, 1, ws)),
+                   ("select_pages", (q, bounds, table, lens, 3, 1, 1, ws, None)),
+                   ("select_pages", (q, bounds, table, lens, 3, 1, 1, ws, cache)),
                    ("paged_decode_selected", (q, cache, cache, lists, lens, 0.1, None, ws)),
                    ("paged_decode_selected", (q, cache, cache, lists, lens, 0.1, q, ws)),
-                   ("sparse_decode", (q, bounds, cache, cache, table, lens, 0.1, 3, 1, 1, q, ws))):
+                   ("sparse_decode", (q, bounds, cache, cache, table, lens, 0.1, 3, 1, 1, q, ws, True))):
     assert getattr(host, name)(*args) is not None, name
 print("launched without the GIL")
 """

@@ -86,7 +86,8 @@ def test_oracle_attention_over_all_pages_is_dense_attention():
 def _select_args(**change):
     args = dict(q=0x1000, q_token_stride=1024, q_head_stride=128, page_bounds=0x1000, num_pages=10,
                 block_tables=0x1000, block_table_stride=20, table_width=20, seq_lens=0x1000, num_seqs=2,
-                num_selected=4, sink=1, recent=1, tables=0x1000, lens=0x1000, workspace=0x1000, bytes=1 << 30,
+                num_selected=4, sink=1, recent=1, tables=0x1000, lens=0x1000, k_cache=0, page_stride=0, token_stride=0,
+                workspace=0x1000, bytes=1 << 30,
                 hq=8, hkv=2, head_dim=128, page=16, dtype=0, stream=0)
     return list({**args, **change}.values())
 
@@ -99,6 +100,9 @@ def _select_args(**change):
     ({"q": 0}, "null"), ({"tables": 0}, "null"), ({"num_pages": 0}, "empty"), ({"table_width": 0}, "empty"),
     ({"q": 0x1008}, "aligned"), ({"page_bounds": 0x1008}, "aligned"), ({"q_head_stride": 129}, "aligned"),
     ({"num_seqs": 1 << 33}, "sizes"), ({"table_width": 1 << 40}, "sizes"), ({"block_table_stride": -20}, "sizes"),
+    ({"k_cache": 0x1008, "page_stride": 4096, "token_stride": 256}, "aligned"),
+    ({"k_cache": 0x1000, "page_stride": 4097, "token_stride": 256}, "aligned"),
+    ({"k_cache": 0x1000, "page_stride": -4096, "token_stride": 256}, "sizes"),
 ])
 def test_select_entry_refuses(change, message):
     with pytest.raises(RuntimeError, match=message):
