@@ -1688,7 +1688,8 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
         key = (device.index, _native.stream_of(device.index))
         workspace = self._stream_workspaces.get(key)
         if workspace is None or workspace.numel() < nbytes:
-            self._stream_workspaces[key] = workspace = ops.new_selection_workspace(nbytes, device)
+            # Room to grow in: the block tables do, by a page every 16 steps.
+            self._stream_workspaces[key] = workspace = ops.new_selection_workspace(max(nbytes * 5 // 4, 1 << 20), device)
         return workspace
 
     def _attend(self, q, k_cache, v_cache, block_tables, seq_lens, out) -> None:
