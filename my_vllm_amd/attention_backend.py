@@ -1709,6 +1709,9 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
         self._attend(q[rows:], k_cache, v_cache, metadata.block_tables[first:], metadata.seq_lens[first:],
                      output[rows:])
 
+    def _run_mixed(self, q, k_cache, v_cache, common, metadata: MI355XAttentionMetadata, output) -> None:
+        raise ValueError("the plan is for one dense MIXED launch: a backend that selects pages did not make it")
+
     # ---- full-decode HIP graph: tables and lengths are all that a step changes ----
     def create_full_decode_graph_state(self, batch_size: int, page_indices_capacity: int, device):
         if any(isinstance(x, bool) or not isinstance(x, int) for x in (batch_size, page_indices_capacity)):

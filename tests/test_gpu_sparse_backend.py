@@ -223,6 +223,17 @@ def test_plans_and_steps_that_do_not_fit_are_refused(gpu):
     want = sparse.forward(*args, plan, page_bounds=bounds).clone()
     assert torch.equal(sparse.forward(*args, dense.build_plan(batch.common), page_bounds=bounds), want)
     assert sparse._page_bounds is None
+    # Its MIXED plan does not: one launch, and dense; nor does this one's there.
+    mixed = make_paged_batch(6, [20, 1], [40, 300], 1, 16, 8, device=gpu, rng_device="cuda")
+    args, bounds = (mixed.q, None, None, mixed.k_cache, mixed.v_cache), bounds_of(mixed.k_cache)
+    assert dense.build_plan(mixed.common).route is AttentionRoute.MIXED_UNIFIED
+    with pytest.raises(ValueError, match="one dense MIXED launch"):
+        sparse.forward(*args, dense.build_plan(mixed.common), page_bounds=bounds)
+    with pytest.raises(ValueError, match="selects pages made it"):
+        dense.forward(*args, sparse.build_plan(mixed.common))
+    with pytest.raises(ValueError, match="needs page_bounds"):
+        sparse.forward(*args, sparse.build_plan(mixed.common))
+    sparse.forward(*args, sparse.build_plan(mixed.common), page_bounds=bounds)
 
 
 def _refused(error, message, call, *args, **more):
