@@ -430,7 +430,7 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
 // Bound by the reads of the bounds on large batches (56 rows of 8192-32768 tokens at
 // 64 / 8 heads, 324 MB: 69 us, 4.7 TB/s over the launch; its reads alone 62).  Small
 // ones are a chain of latencies (one row of 30001 tokens at 32 / 8 heads, 7.7 MB:
-// 9.6 us): launch and length 2.0, page ids 0.5, bounds 2.7, keys counted in 1.4,
+// 9.7 us): launch and length 2.0, page ids 0.5, bounds 2.7, keys counted in 1.4,
 // choice 2.8.  Two launches with the keys in memory between them and one page at a
 // time took 132 and 35.5 us.
 //

@@ -7,7 +7,7 @@
 // Bound by the reads of K and V: 64 rows of 256 pages at 64 / 8 heads (1.07 GB)
 // take 170 us, 6.3 TB/s.  Few pages are a chain of latencies: 1.8 us of launch, then
 // lengths, page ids, pages, the join of a row's parts through memory; 128 pages of
-// one row at 32 / 8 heads (8.4 MB) 7.5 us.
+// one row at 32 / 8 heads (8.4 MB) 7.8 us.
 //
 // Unlike the dense decode's ragged batches, lists are at most num_selected pages
 // long, so equal parts of them need no plan: a launch is fixed by its shapes, which
