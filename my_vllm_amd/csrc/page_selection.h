@@ -25,7 +25,7 @@ inline bool selection_sizes_ok(int64_t num_seqs, int hq, int hkv, int64_t num_se
          num_seqs * hq <= 0x7fffffffLL && num_selected > 0 && num_selected <= (1 << 24);
 }
 
-// Bytes of the attention's partials.
-int64_t selection_part_bytes(int64_t num_seqs, int hq, int hkv, int64_t num_selected);
+// Bytes kept for the attention's partials; they do not fall as any of the sizes grows.
+int64_t selection_part_bytes(int64_t num_seqs, int hq, int64_t num_selected);
 
 }  // namespace mva

@@ -637,7 +637,7 @@ extern "C" int64_t mva_selection_workspace_bytes(int64_t num_seqs, int num_q_hea
   if (!selection_sizes_ok(num_seqs, num_q_heads, num_kv_heads, num_selected) || table_width < 0 ||
       table_width > 0x7fffffffLL / kPageTokens)
     return -1;
-  return kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_kv_heads, num_selected) +
+  return kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_selected) +
          selection_keys_bytes(num_seqs, num_kv_heads, table_width);
 }
 
@@ -670,7 +670,7 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
   const SelectParams p = {
       q, q_token_stride, q_head_stride, (const uint8_t*)page_bounds, num_pages, block_tables, block_table_stride,
       table_width, seq_lens, num_seqs, (int)num_selected, (int)sink_pages, (int)recent_pages, tables, lens,
-      (uint64_t*)(ws + kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_kv_heads, num_selected)),
+      (uint64_t*)(ws + kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_selected)),
       (int*)ws, num_kv_heads, num_q_heads / num_kv_heads};
   // Chunks: as small as 128 pages (16 a wavefront) as long as that makes no more
   // workgroups than the GPU holds at a time.  One row of 30001 tokens at 8 KV heads

@@ -16,6 +16,8 @@
 #include "paged_decode.h"
 #include "page_selection.h"
 
+#include <algorithm>
+
 namespace mva {
 namespace {
 
@@ -306,8 +308,15 @@ int selected_parts(int64_t num_seqs, int hkv, int64_t num_selected) {
 
 }  // namespace
 
-int64_t selection_part_bytes(int64_t num_seqs, int hq, int hkv, int64_t num_selected) {
-  const int64_t slots = num_seqs * hq * selected_parts(num_seqs, hkv, num_selected);
+// Rows are cut into more parts the fewer they are, so that 64 rows can need less than
+// 48.  The bytes are therefore those of a bound that does not fall as any size grows:
+// in several parts a row, `parts` * rows is at most the workgroups that the GPU
+// holds, each of kMaxQueryGroup queries at most.
+int64_t selection_part_bytes(int64_t num_seqs, int hq, int64_t num_selected) {
+  const int64_t queries = num_seqs * hq;
+  const int64_t in_parts = queries * ((num_selected + kPartPages - 1) / kPartPages);
+  const int64_t resident = std::max(queries, (int64_t)256 * kSelGroupsPerCu * kMaxQueryGroup);
+  const int64_t slots = std::min(in_parts, resident);
   return align_up256(slots * 4) + align_up256(slots * kHeadDim * 4);
 }
 
@@ -343,8 +352,7 @@ extern "C" int mva_paged_decode_selected(const void* q, int64_t q_token_stride, 
     return set_error("selected attention: output buffer and strides must be 8-byte aligned");
   const int parts = selected_parts(num_seqs, num_kv_heads, num_selected);
   if (parts > 1 && (workspace == nullptr || (uint64_t)(uintptr_t)workspace % 16 ||
-                    workspace_bytes < kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads,
-                                                                                   num_kv_heads, num_selected)))
+                    workspace_bytes < kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_selected)))
     return set_error("selected attention: workspace missing, too small or unaligned");
   const int64_t blocks = num_seqs * num_kv_heads * parts;
   if (blocks > 0xffffffffLL / (64 * kSelWaves)) return set_error("selected attention: too many rows for one launch");

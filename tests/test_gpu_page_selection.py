@@ -445,6 +445,26 @@ def test_one_workspace_serves_calls_of_other_sizes(gpu):
     assert (workspace[nbytes:] == 0xff).all() and (workspace[:ops.SELECTION_HEADER_BYTES] == 0).all()
 
 
+def test_one_workspace_serves_a_batch_that_drains(gpu):
+    # Fewer rows are cut into more parts: 52 and 49 rows of 8 heads in one, 48 in two, 3 in eight.
+    lens = [16 * 130 - 7 * s for s in range(52)]
+    counts = page_counts(lens)
+    k, v = keys(max(counts), 8, BF16, 1), keys(max(counts), 8, BF16, 2)
+    table, q = torch.arange(max(counts), dtype=torch.int32).expand(52, -1).contiguous(), queries(52, 8, BF16, 3)
+    nbytes = ops.selection_workspace_bytes(52, 8, 8, table.shape[1], 120)
+    workspace = torch.full((nbytes + 4096,), 0xff, dtype=torch.uint8, device=gpu)
+    workspace[:ops.SELECTION_HEADER_BYTES] = 0
+    on_gpu = [t.to(gpu) for t in (q, bounds_of(k), k, v, table, _ints(lens, gpu))]
+    for rows in (52, 49, 48, 33, 3):
+        few = on_gpu[0][:rows], *on_gpu[1:4], on_gpu[4][:rows], on_gpu[5][:rows]
+        out = ops.sparse_decode(*few, SCALE, 120, 1, 4, out=torch.empty_like(few[0]), workspace=workspace[:nbytes])
+        assert torch.equal(out, ops.sparse_decode(*few, SCALE, 120, 1, 4))
+        if rows == 3:
+            want = selection.select_pages(q[:3], bounds_of(k), table[:3], lens[:3], 120, 1, 4)
+            _check_attention(out, q[:3], k, v, *want, BF16)
+    assert (workspace[nbytes:] == 0xff).all() and (workspace[:ops.SELECTION_HEADER_BYTES] == 0).all()
+
+
 def test_calls_on_two_streams_and_captured_ones(gpu):
     sets = []
     for seed in (1, 2):

@@ -155,6 +155,24 @@ def test_workspace_sizes():
             size(*bad)
 
 
+# Enough for fewer rows, heads, pages and columns: fewer rows are cut into more parts.
+@pytest.mark.parametrize("change", [{"num_seqs": n} for n in (1, 2, 31, 32, 47, 48, 49, 63)] + [
+    {"num_q_heads": 16}, {"num_q_heads": 8}, {"num_kv_heads": 4, "num_seqs": 33}, {"num_kv_heads": 4}, {"table_width": 0},
+    {"table_width": 1, "num_seqs": 13}, {"num_selected": 1}, {"num_selected": 17, "num_seqs": 40}])
+@pytest.mark.parametrize("width", [0, 200, 2048])
+def test_a_workspace_is_enough_for_smaller_sizes(change, width):
+    largest = dict(num_seqs=64, num_q_heads=64, num_kv_heads=8, table_width=width, num_selected=128)
+    smaller = {**largest, **{k: min(v, largest[k]) for k, v in change.items()}}
+    assert ops.selection_workspace_bytes(*smaller.values()) <= ops.selection_workspace_bytes(*largest.values())
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (32, 8), (64, 8), (16, 1), (16, 4)])
+@pytest.mark.parametrize("selected", [1, 16, 17, 128, 5000])
+def test_workspace_sizes_do_not_fall_as_rows_are_added(hq, hkv, selected):
+    sizes = [ops.selection_workspace_bytes(n, hq, hkv, 100, selected) for n in range(0, 1600)]
+    assert sizes == sorted(sizes)
+
+
 def test_operators_refuse_cpu_tensors():
     q, cache = torch.zeros(2, 8, 128, dtype=BF16), torch.zeros(4, 16, 2, 128, dtype=BF16)
     bounds, table, lens = torch.zeros(4, 2, 2, 128, dtype=BF16), torch.zeros(2, 4, dtype=torch.int32), torch.ones(
