@@ -1595,6 +1595,9 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
     default_selected_pages = 128
     default_sink_pages = 1
     default_recent_pages = 4
+    # Streams whose buffers are kept beside those of the one that ran last.
+    max_idle_streams = 8
+    _STREAM_BUFFERS = ("_output_buffer", "_selection_workspace", "_prefill_workspace")
 
     def __init__(
         self,
@@ -1624,8 +1627,11 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
         # brings them up to date.
         self._page_bounds: torch.Tensor | None = None
         self._update_bounds = False
-        # Workspaces of eager steps, by GPU and stream.
-        self._stream_workspaces: dict[tuple, torch.Tensor] = {}
+        # The eager steps' buffers: those of the GPU and stream that ran last, and the
+        # other streams' (_take_stream).
+        self._selection_workspace: torch.Tensor | None = None
+        self._stream: tuple | None = None
+        self._other_streams: dict[tuple, tuple] = {}
 
     def _backend_mixed_reason(self) -> str | None:
         return "MIXED batches with selected pages run as prefill + decode launches"
@@ -1675,9 +1681,34 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
         finally:
             self._page_bounds = None
 
+    def _take_stream(self, device: torch.device) -> None:
+        """Make the current stream's buffers the ones that eager steps write.
+
+        Steps on two streams may overlap, so each has an output, a selection
+        workspace and a prefill workspace of its own (and plans its prefill tiles
+        anew after a change of streams).  The buffers that have lain unused the
+        longest go once more than ``max_idle_streams`` streams have some: none was used on
+        another stream than its own, whose order their memory's next use keeps."""
+        stream = (device.index, _native.stream_of(device.index))
+        if stream == self._stream:
+            return
+        if self._stream is not None:
+            self._other_streams[self._stream] = tuple(getattr(self, name) for name in self._STREAM_BUFFERS)
+        buffers = self._other_streams.pop(stream, (None,) * len(self._STREAM_BUFFERS))
+        if len(self._other_streams) > self.max_idle_streams:
+            del self._other_streams[next(iter(self._other_streams))]
+        for name, buffer in zip(self._STREAM_BUFFERS, buffers):
+            setattr(self, name, buffer)
+        self._prefill_planned_for = None
+        self._stream = stream
+
+    def _get_reusable_attention_output(self, q: torch.Tensor) -> torch.Tensor:
+        self._take_stream(q.device)
+        return super()._get_reusable_attention_output(q)
+
     def _get_workspace(self, nbytes: int, device: torch.device) -> torch.Tensor:
         """The workspace of the layer that follows: a graph's own, from its pool, for
-        the layers captured on one stream, else one of the current stream.  Its
+        the layers captured on one stream, else that of the stream taken.  Its
         counters are cleared when it is made (in a graph, once a replay)."""
         capture = self._capture_of(device)
         if capture is not None:
@@ -1685,11 +1716,10 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
             if held is None or held[0] != capture or held[1].numel() < nbytes:
                 self._captured_workspace = held = (capture, ops.new_selection_workspace(nbytes, device))
             return held[1]
-        key = (device.index, _native.stream_of(device.index))
-        workspace = self._stream_workspaces.get(key)
+        workspace = self._selection_workspace
         if workspace is None or workspace.numel() < nbytes:
             # Room to grow in: the block tables do, by a page every 16 steps.
-            self._stream_workspaces[key] = workspace = ops.new_selection_workspace(max(nbytes * 5 // 4, 1 << 20), device)
+            self._selection_workspace = workspace = ops.new_selection_workspace(max(nbytes * 5 // 4, 1 << 20), device)
         return workspace
 
     def _attend(self, q, k_cache, v_cache, block_tables, seq_lens, out) -> None:
@@ -1744,6 +1774,7 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
         state.plan = plan
 
     def _run_decode_graph(self, q, k_cache, v_cache, state: MI355XFullDecodeGraphState) -> None:
+        self._take_stream(q.device)
         self._attend(q, k_cache, v_cache, state.block_tables_buffer, state.seq_lens_buffer, state.output)
 
 

@@ -200,6 +200,33 @@ def test_captured_decode_steps(gpu, stored):
         assert torch.equal(got, eager)
 
 
+def test_steps_on_two_streams(gpu):
+    # One backend, decode and prefill steps side by side on two streams: each as alone.
+    backend = MI355XSparseAttentionBackend(16, 4, 128, PAGE, BF16, selected_pages=20, recent_pages=2)
+    steps = []
+    for seed, (q_lens, kv_lens, prefills) in enumerate((([1] * 6, [3000, 40, 900, 16, 2222, 1500], 0),
+                                                        ([1] * 6, [2800, 700, 33, 1900, 5, 320], 0),
+                                                        ([300, 90], [700, 90], 2), ([120, 250], [120, 900], 2))):
+        batch = make_paged_batch(20 + seed, q_lens, kv_lens, prefills, 16, 4, device=gpu, rng_device="cuda")
+        steps.append((batch, bounds_of(batch.k_cache).contiguous()))
+
+    def run(batch, bounds, plan):
+        return backend.forward(batch.q, None, None, batch.k_cache, batch.v_cache, plan, page_bounds=bounds)
+
+    plans = [backend.build_plan(batch.common) for batch, _ in steps]
+    alone = [run(*step, plan).clone() for step, plan in zip(steps, plans)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for pair in ((0, 1), (2, 3), (0, 3)):
+            outs = []
+            for stream, i in zip(streams, pair):
+                with torch.cuda.stream(stream):
+                    outs.append(run(*steps[i], plans[i]))
+            torch.cuda.synchronize()
+            assert all(torch.equal(out, alone[i]) for out, i in zip(outs, pair))
+
+
 def test_plans_and_steps_that_do_not_fit_are_refused(gpu):
     batch = make_paged_batch(5, [1, 1], [300, 20], 0, 16, 8, device=gpu, rng_device="cuda")
     sparse, dense = (cls(16, 8, 128, 16, BF16) for cls in (MI355XSparseAttentionBackend, MI355XAttentionBackend))

@@ -231,6 +231,40 @@ def test_graph_states_belong_to_one_kind_of_decode(host_planning):
         own.deactivate_full_decode_graph()
 
 
+def test_each_eager_stream_has_buffers_of_its_own(monkeypatch):
+    # One backend whose steps run on two streams, played on the CPU: nothing that one writes is the other's.
+    backend, cpu = ab.MI355XSparseAttentionBackend(16, 8, 128, 16, BF16), torch.device("cpu")
+    stream = [0]
+    monkeypatch.setattr(_native, "stream_of", lambda device: stream[0])
+    q = torch.zeros(5, 16, 128, dtype=BF16)
+
+    def step(n):
+        stream[0] = n
+        return (backend._get_reusable_attention_output(q), backend._get_workspace(1 << 20, cpu),
+                backend._get_prefill_workspace(4, cpu))
+
+    def addresses(tensors):
+        return [t.data_ptr() for t in tensors]
+
+    first, second = step(1), step(2)
+    assert not set(addresses(first)) & set(addresses(second))
+    # Back on the first: its own again, and no tile plan counts as laid there.
+    backend._prefill_planned_for = object()
+    assert addresses(step(1)) == addresses(first) and backend._prefill_planned_for is None
+    assert addresses(step(1)) == addresses(first) and addresses(step(2)) == addresses(second)
+    # A decode step of a graph state has its output from the state.
+    taken = []
+    monkeypatch.setattr(backend, "_attend", lambda q, *_: taken.append(backend._get_workspace(1 << 20, q.device)))
+    stream[0] = 1
+    backend._run_decode_graph(q, None, None, types.SimpleNamespace(
+        block_tables_buffer=None, seq_lens_buffer=None, output=None))
+    assert taken[0] is first[1]
+    # As many streams as are in use at a time, not as many as ever were.
+    held = [step(n) for n in range(3, 40)]
+    assert len(backend._other_streams) <= 8 and addresses(step(38)) == addresses(held[-2])
+    assert backend._workspace is None  # the dense decode's, whose words mean something else
+
+
 def test_integrate_builds_on_another_contract(host_planning):
     registered = {}
     registry = types.SimpleNamespace(register=registered.__setitem__)
