@@ -346,7 +346,7 @@ extern "C" int mva_paged_decode_selected(const void* q, int64_t q_token_stride, 
        (uint64_t)(q_token_stride * 2) | (uint64_t)(q_head_stride * 2) | (uint64_t)(page_stride * 2) |
        (uint64_t)(token_stride * 2)) % 16)
     return set_error("selected attention: q / cache buffers and strides must be 16-byte aligned");
-  if (token_stride < 0 || token_stride > (1 << 26))
+  if (token_stride < 0 || token_stride >= (1 << 26))
     return set_error("selected attention: a page's tokens must lie less than 2^26 elements apart");
   if (((uint64_t)(uintptr_t)out | (uint64_t)(out_token_stride * 2) | (uint64_t)(out_head_stride * 2)) % 8)
     return set_error("selected attention: output buffer and strides must be 8-byte aligned");

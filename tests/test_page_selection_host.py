@@ -144,6 +144,14 @@ def test_attention_entry_refuses(change, message):
         _native.call("mva_paged_decode_selected", *args)
 
 
+def test_attention_entry_refuses_tokens_too_far_apart_from_the_first_on():
+    # 2^26 elements, and the largest stride below: that one is refused for its workspace alone.
+    for stride, message in ((1 << 26, "2\\^26"), ((1 << 26) - 8, "workspace")):
+        with pytest.raises(RuntimeError, match=message):
+            _native.call("mva_paged_decode_selected", 0x1000, 1024, 128, 0x1000, 0x1000, 10, 1 << 30, stride, 0x1000,
+                         160, 20, 0x1000, 2, 20, 0x1000, 1024, 128, 0, 0, 8, 8, 128, 16, 1.0, 0, 0)
+
+
 def test_workspace_sizes():
     size = ops.selection_workspace_bytes
     assert size(0, 8, 8, 10, 4) >= 0
