@@ -6,7 +6,9 @@
 //   score[s, h, j] = sum_d P[d] hi[j, h, d] + N[d] lo[j, h, d],
 //   P = sum_g max(q_g, 0),  N = sum_g min(q_g, 0),
 // is at least sum_g q_g . k for every key k of page j, and costs one dot
-// product of length 256 whatever G is.  Selected are the first `sink` pages,
+// product of length 256 whatever G is.  It stands for sum_g sum_d of the larger of
+// q_g lo and q_g hi; where a bound or a query is infinite, 0 of P or N times it would
+// not, and such pages are scored again.  Selected are the first `sink` pages,
 // the last `recent` and, of those between, the ones of the highest score.
 #include "mva_capi.h"
 #include "mva_common.h"
@@ -509,6 +511,12 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
   const uint8_t* bounds = p.bounds + h * 512 + piece * 16;
   const int64_t begin = first + wave * (int64_t)(chunk / kSelectWaves);
   const int64_t mine = min(begin + chunk / kSelectWaves, last);
+  bool odd = false;  // an infinity or a NaN among this lane's scores
+  auto put = [&](int64_t place, double score, bool writes) __attribute__((always_inline)) {
+    if (!writes || place >= mine) return;
+    if (in_lds) lds.keys[place] = order_key(score);
+    else key_store(keys + place, order_key(score));
+  };
   for (int64_t base = begin; base < mine; base += 4 * 64) {
     uint32_t ids[4];  // times the heads: pages' first rows of 512 bytes
 #pragma unroll
@@ -534,12 +542,9 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[i] = __builtin_fma((double)(float)box[i][e], w[e], sum[i]);
       }
-      const uint64_t key = order_key(sums_of_8(sum, lane));
-      const int64_t place = base + t * kBatch + 2 * (piece >> 2) + half;
-      if ((lane & 3) == 0 && place < mine) {
-        if (in_lds) lds.keys[place] = key;
-        else key_store(keys + place, key);
-      }
+      const double total = sums_of_8(sum, lane);
+      odd |= !__builtin_isfinite(total);
+      put(base + t * kBatch + 2 * (piece >> 2) + half, total, (lane & 3) == 0);
     };
     V8 box[8], next[8];
     load(box, 0);
@@ -551,6 +556,45 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
       for (int i = 0; i < 8; ++i) box[i] = next[i];
     }
     score(box, batches - 1);
+  }
+  if (__any(odd)) {
+    // Again, two pages at a time, for what an infinity makes of a weight that stands for no
+    // query: 0 times it is NaN above and nothing here, where it is a NaN only if a query or
+    // a bound is that 0.  Scores without infinities come out as they were, bit for bit.
+    uint32_t part = 0, zero = 0, infinite = 0;  // a bit a channel: queries that have this part, are 0, are infinite
+    const T* q = (const T*)p.q + s * p.q_tok_stride + (int64_t)h * p.group * p.q_head_stride + 8 * (piece & 15);
+#pragma unroll 1
+    for (int g = 0; g < p.group; ++g) {
+      const V8 v = ld16<V8>(q + g * p.q_head_stride);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = (float)v[e];
+        part |= (uint32_t)(piece < 16 ? !(x >= 0.f) : !(x <= 0.f)) << e;
+        zero |= (uint32_t)(x == 0.f) << e;
+        infinite |= (uint32_t)__builtin_isinf(x) << e;
+      }
+    }
+#pragma unroll 1
+    for (int64_t place = begin + half; place - half < mine; place += 2) {
+      const int id = row[min(place, mine - 1)];
+      const V8 box = ld16<V8>(bounds + ((uint64_t)((uint32_t)(id < 0 || id >= p.num_pages ? 0 : id) *
+                                                    (uint32_t)p.num_kv_heads) << 9));
+      double sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float x = (float)box[e];
+        const bool inf = __builtin_isinf(x), has = part >> e & 1;
+        if (inf ? zero >> e & 1 : x == 0.f && (infinite >> e & 1)) x = __builtin_nanf("");
+        else if (inf && !has) x = 0.f;
+        sum = __builtin_fma((double)x, w[e], sum);
+      }
+      sum += across<16>(sum);
+      sum += across<8>(sum);
+      sum += across<4>(sum);
+      sum += across<2>(sum);
+      sum += across<1>(sum);
+      put(place, sum, piece == 0);
+    }
   }
   if (parts > 1) {
     // This wavefront's keys have reached memory before the workgroup counts itself in.

@@ -30,16 +30,24 @@ def page_bounds(k_cache, bounds, block_tables, seq_lens, new_tokens) -> torch.Te
 
 
 def page_scores(q, bounds) -> np.ndarray:
-    """Scores of pages ``bounds [n, 2, 128]`` for the queries ``q [G, 128]`` of a KV head."""
+    """Scores of pages ``bounds [n, 2, 128]`` for the queries ``q [G, 128]`` of a KV
+    head: the sum over queries and channels of the larger of q min and q max (that of
+    max for a positive q, of min for a negative one); NaN if either product is."""
     queries = q.double().numpy()
     up = np.where(queries < 0, 0.0, queries).sum(0)
     down = np.where(queries > 0, 0.0, queries).sum(0)
     box = bounds.double().numpy()
-    with np.errstate(invalid="ignore", over="ignore"):
-        terms = np.concatenate((box[:, 1] * up, box[:, 0] * down), 1)
-    finite = np.isfinite(terms).all(1)
-    with np.errstate(invalid="ignore"):
-        return np.array([math.fsum(t) if ok else t.sum() for t, ok in zip(terms, finite)])
+    finite = np.isfinite(box).all((1, 2)) & np.isfinite(queries).all()
+    scores = np.zeros(len(box))
+    for j, ok in enumerate(finite):
+        if ok:  # the same sum, queries of one sign taken together
+            scores[j] = math.fsum(np.concatenate((box[j, 1] * up, box[j, 0] * down)))
+        else:
+            with np.errstate(invalid="ignore"):
+                low, high = queries * box[j, 0], queries * box[j, 1]
+                larger = np.where(queries < 0, low, high)
+                scores[j] = np.where(np.isnan(low) | np.isnan(high), math.nan, larger).sum()
+    return scores
 
 
 def chosen(scores, want: int) -> list[int]:

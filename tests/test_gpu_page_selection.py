@@ -203,6 +203,32 @@ def test_nan_and_infinities_rank(gpu):
     _check_selection(gpu, q, bounds, table, lens, 11, 2, 3)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("pages,rows", [(40, 6), (700, 6), (300, 180)])
+def test_infinities_count_as_products_with_the_queries(gpu, dtype, pages, rows):
+    # Whole numbers, so that finite scores are exact; a few infinite bounds, and queries
+    # of one sign, of both, zero, infinite and NaN in those channels.  Rows in several
+    # workgroups and in one.
+    gen = torch.Generator().manual_seed(pages)
+    bounds = torch.randint(-2, 3, (pages, 2, 2, 128), generator=gen).float()
+    values = torch.tensor([-math.inf, -2.0, 0.0, 1.0, math.inf])
+    odd = torch.randperm(pages, generator=gen)[:pages // 3]
+    bounds[odd, :, :, :2] = values[torch.randint(0, 5, (len(odd), 2, 2, 2), generator=gen)]
+    bounds = bounds.sort(2).values.to(dtype)
+    q = torch.randint(-2, 3, (6, 4, 128), generator=gen).float()  # two queries a KV head
+    q[:, :, :2] = torch.tensor([[[1.0, 3.0], [2.0, 1.0]], [[-1.0, 2.0], [-2.0, 0.0]], [[0.0, 1.0], [-1.0, -1.0]],
+                                [[-math.inf, 1.0], [1.0, 2.0]], [[math.nan, 1.0], [1.0, 1.0]],
+                                [[0.0, 0.0], [0.0, 0.0]]]).repeat(1, 2, 1)
+    q[4, :2] = 1.0  # NaN queries of one KV head only
+    lens = [16 * pages - s for s in range(6)]
+    table = torch.stack([torch.randperm(pages, generator=gen) for _ in range(6)]).to(torch.int32)
+    of = torch.arange(rows) % 6
+    for n in (4, 11, pages // 3, pages - 2):
+        want = selection.select_pages(q.to(dtype), bounds, table, lens, n, 1, 2)
+        got = _select(gpu, q[of].to(dtype), bounds, table[of].contiguous(), [lens[i] for i in of.tolist()], n, 1, 2)
+        assert torch.equal(got[0], want[0][of]) and torch.equal(got[1], want[1][of])
+
+
 def test_values_at_the_ends_of_the_types(gpu):
     for dtype in (BF16, FP16):
         top, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal

@@ -49,6 +49,32 @@ def test_oracle_scores_bound_every_key():
     assert not (torch.from_numpy(selection.page_scores(q[0], swapped)) >= products.amax(1)).all()
 
 
+def test_oracle_scores_of_infinities_are_the_products_of_the_queries():
+    # Whole numbers: every finite sum is exact.
+    gen = torch.Generator().manual_seed(3)
+    values = torch.tensor([-math.inf, -2.0, 0.0, 1.0, 3.0, math.inf])
+    box = values[torch.randint(0, 6, (4000, 2, 128), generator=gen)].sort(1).values
+    box[:, :, 3:] = torch.randint(-2, 3, (4000, 2, 125), generator=gen).float().sort(1).values
+    box[500:, :, 1:3] = box[500:, :, 5:7]  # one channel with an infinity in most
+    q = torch.zeros(2, 128)
+    kinds = set()
+    for a in (-1.0, 0.0, 2.0, math.inf, math.nan):
+        for b in (-3.0, 0.0, 1.0, -math.inf):
+            q[:, :3] = torch.tensor([[a], [b]])
+            q[:, 3:] = torch.randint(-2, 3, (2, 125), generator=gen).float()
+            got = selection.page_scores(q.to(BF16), box.to(BF16))
+            want = torch.maximum(q[:, None] * box[None, :, 0], q[:, None] * box[None, :, 1]).double().sum((0, 2)).numpy()
+            assert np.array_equal(got, want, equal_nan=True)
+            kinds |= {(math.isinf(a), *x) for x in zip(np.isnan(got).tolist(), np.isinf(got).tolist())}
+    assert len(kinds) == 5  # finite ones too, but of no infinite query
+    # A channel's -inf says nothing about a product with a positive query.
+    box = torch.zeros(1, 2, 128)
+    box[0, 0, 0], box[0, 1, 0] = -math.inf, 2.0
+    q = torch.zeros(2, 128)
+    q[:, 0] = torch.tensor([1.0, 3.0])
+    assert selection.page_scores(q, box).tolist() == [8.0]
+
+
 def test_oracle_choice_ranks_ties_and_nan():
     nan = math.nan
     assert selection.chosen([1.0, 3.0, 3.0, 2.0, 3.0], 2) == [1, 2]
