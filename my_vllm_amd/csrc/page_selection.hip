@@ -667,6 +667,8 @@ extern "C" int mva_update_page_bounds(const void* k_cache, int64_t num_pages, in
                                    num_kv_heads))
     return rc;
   if (p.num_tokens == 0) return 0;
+  // (Starts are 32-bit.  A product with the heads passes 64 bits for counts near 2^63.)
+  if (num_tokens > 0x7fffffffLL) return set_error("page bounds: too many tokens for one launch");
   const int64_t blocks = bounds_blocks(p, 4);
   if (blocks > 0xffffffffLL / 256) return set_error("page bounds: too many tokens for one launch");
   const hipStream_t st = (hipStream_t)stream;

@@ -170,6 +170,13 @@ def test_attention_entry_refuses(change, message):
         _native.call("mva_paged_decode_selected", *args)
 
 
+@pytest.mark.parametrize("tokens", [1 << 31, 1 << 62, (1 << 63) - 15, (1 << 63) - 1])
+def test_bounds_entry_refuses_token_counts_whose_grid_overflows(tokens):
+    with pytest.raises(RuntimeError, match="too many"):
+        _native.call("mva_update_page_bounds", 0x1000, 10, 16 * 1024, 1024, 0x1000, 0x1000, 20, 20, 0x1000, 0x1000, 2,
+                     tokens, 8, 128, 16, 0, 0)
+
+
 def test_attention_entry_refuses_tokens_too_far_apart_from_the_first_on():
     # 2^26 elements, and the largest stride below: that one is refused for its workspace alone.
     for stride, message in ((1 << 26, "2\\^26"), ((1 << 26) - 8, "workspace")):
