@@ -227,6 +227,93 @@ def test_steps_on_two_streams(gpu):
             assert all(torch.equal(out, alone[i]) for out, i in zip(outs, pair))
 
 
+def _steps(gpu, seeds, kinds):
+    for seed, (q_lens, kv_lens, prefills) in zip(seeds, kinds):
+        batch = make_paged_batch(seed, q_lens, kv_lens, prefills, 16, 4, device=gpu, rng_device="cuda")
+        yield batch, bounds_of(batch.k_cache).contiguous()
+
+
+def _forward(backend, step, plan=None):
+    batch, bounds = step
+    return backend.forward(batch.q, None, None, batch.k_cache, batch.v_cache, plan or backend.build_plan(batch.common),
+                           page_bounds=bounds)
+
+
+@pytest.mark.parametrize("eager_first", [True, False])
+@pytest.mark.parametrize("kind", [([1] * 5, [5000, 17, 90, 1000, 33], 0), ([40, 1, 1], [300, 3000, 2000], 1),
+                                  ([40, 70], [300, 3000], 2)])
+def test_replays_beside_eager_steps_that_grow_the_buffers(gpu, kind, eager_first):
+    step, large = _steps(gpu, (1, 2), (kind, ([1] * 70, [2000 + 7 * i for i in range(70)], 0)))
+    numbers = {"selected_pages": 33, "recent_pages": 2}
+    backend, other = (MI355XSparseAttentionBackend(16, 4, 128, PAGE, BF16, **numbers) for _ in range(2))
+    want, large_want = _forward(other, step).clone(), _forward(other, large).clone()
+    plan = backend.build_plan(step[0].common)
+    if eager_first:
+        assert torch.equal(_forward(backend, step, plan), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _forward(backend, step, plan).clone()
+    assert torch.equal(_forward(backend, large), large_want)
+    torch.cuda.synchronize()
+    # Whatever was given back is taken by these.
+    fresh = [torch.full((n << 20,), 0xa5, dtype=torch.uint8, device=gpu) for n in (1, 1, 2, 4, 8)]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all((t == 0xa5).all() for t in fresh)
+        assert torch.equal(_forward(backend, large), large_want) and torch.equal(_forward(backend, step), want)
+
+
+def test_two_graphs_of_one_backend_replay_at_once(gpu):
+    # Two layers each, of decode steps whose rows are cut into parts and whose choice counts workgroups in.
+    backend = MI355XSparseAttentionBackend(16, 4, 128, PAGE, BF16, selected_pages=60)
+    graphs = []
+    for step in _steps(gpu, (3, 4), (([1] * 3, [4000, 900, 25000], 0), ([1] * 6, [3000] * 6, 0))):
+        batch, bounds = step
+        plan = backend.build_plan(batch.common)
+        swapped = (type(batch)(**{**batch.__dict__, "k_cache": batch.v_cache, "v_cache": batch.k_cache}),
+                   bounds_of(batch.v_cache).contiguous())
+        want = [_forward(backend, s, plan).clone() for s in (step, swapped)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [_forward(backend, s, plan).clone() for s in (step, swapped)]
+        graphs.append((graph, outs, want, torch.cuda.Stream(), (step, swapped, plan)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, outs, _, stream, _ in graphs:
+            with torch.cuda.stream(stream):
+                for _ in range(4):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for _, outs, want, _, (step, _, plan) in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+            assert torch.equal(_forward(backend, step, plan), want[0])
+
+
+def test_a_sequence_that_a_batch_holds_twice(gpu):
+    # As padding that repeats a row does: the page that both complete is last in both.
+    runner = Runner(gpu, 16, 4, BF16, 60, 9)
+    runner.step([319, 100], 2)
+    common, slots = runner.batch([1, 1], 0)
+    k, v = runner.rows_of(2)
+    q = queries(2, 16, BF16, 5)
+    runner.host_store(k, v, slots, [1, 1])
+    of = torch.tensor([0, 1, 0, 0])
+    counts = tuple(common.block_counts[i] for i in of.tolist())
+    twice = CommonAttentionMetadata(**{
+        **common.__dict__, "num_decode_seqs": 4, "num_decode_tokens": 4, "block_counts": counts,
+        "num_kv_blocks": sum(counts), "query_start_loc": torch.arange(5, dtype=torch.int32, device=gpu),
+        **{name: getattr(common, name)[of.to(gpu)].contiguous() for name in ("seq_lens", "slot_mapping", "block_tables")}})
+    out = runner.backend.forward_with_kv_store(
+        q[of].to(gpu), k[of].to(gpu), v[of].to(gpu), runner.k_gpu, runner.v_gpu, twice.slot_mapping,
+        runner.backend.build_plan(twice), page_bounds=runner.bounds_gpu)
+    assert torch.equal(out[2], out[0]) and torch.equal(out[3], out[0])
+    runner.check(out[:2], q, [1, 1], 0)
+
+
 def test_plans_and_steps_that_do_not_fit_are_refused(gpu):
     batch = make_paged_batch(5, [1, 1], [300, 20], 0, 16, 8, device=gpu, rng_device="cuda")
     sparse, dense = (cls(16, 8, 128, 16, BF16) for cls in (MI355XSparseAttentionBackend, MI355XAttentionBackend))
