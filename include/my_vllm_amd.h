@@ -616,9 +616,9 @@ int64_t mva_selection_workspace_bytes(int64_t num_seqs, int num_q_heads, int num
  * ones of the highest score
  *   sum_d P[d] hi[d] + N[d] lo[d],  P = sum_g max(q_g, 0),  N = sum_g min(q_g, 0)
  * over the queries g of the KV head, in 64 bits; NaN ranks above everything,
- * ties go to the lowest place.  An infinite bound counts only for queries of its sign
- * (hi for positive ones, lo for negative ones); with a query of 0 it makes the score
- * NaN, as an infinite query does with a bound of 0.  tables (dense [num_seqs][num_kv_heads]
+ * ties go to the lowest place.  An infinite hi counts for positive queries alone, an
+ * infinite lo for negative ones; either makes the score NaN with a query of 0, as an
+ * infinite query does with a bound of 0.  tables (dense [num_seqs][num_kv_heads]
  * [num_selected]) gets their page ids in the order of their places, -1 after
  * the last; lens ([num_seqs]) the tokens they hold, those of the last page
  * counted to the row's end.  A row of seq_lens <= 0 gets no page and 0; one longer

@@ -1640,7 +1640,9 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
                               page_bounds=None) -> torch.Tensor:
         """The step's K/V rows into the caches (``store``, or ``ops.store_kvcache``), the
         bounds of the pages that they complete, then :meth:`forward`.  A step of decode
-        rows alone writes the bounds in the selection's launch."""
+        rows alone writes the bounds in the selection's launch: its rows are different
+        sequences, or one more than once at the same length (a row for each draft of
+        a sequence takes :meth:`update_page_bounds` and :meth:`forward`)."""
         if not _has_cache(k_cache):
             return self.forward(q, k, v, k_cache, v_cache, plan, page_bounds=page_bounds)
         if page_bounds is None:
@@ -1684,7 +1686,7 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
     def _take_stream(self, device: torch.device) -> None:
         """Make the current stream's buffers the ones that eager steps write.
 
-        Steps on two streams may overlap, so each has an output, a selection
+        Steps that one host thread issues on two streams may overlap, so each has an output, a selection
         workspace and a prefill workspace of its own (and plans its prefill tiles
         anew after a change of streams).  The buffers that have lain unused the
         longest go once more than ``max_idle_streams`` streams have some: none was used on

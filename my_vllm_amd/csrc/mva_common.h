@@ -73,13 +73,16 @@ __device__ inline void st16(void* p, V v) {
   *reinterpret_cast<V*>(p) = v;
 }
 
-// 16 bytes that a launch reads once, as a decode step does a layer's cache: a
-// non-temporal load, which takes no room in the last-level cache, whose lines
-// other kernels have written to or will read.  Plain / non-temporal loads in
-// microseconds, attention over 84 MB of selected pages 22.4 / 21.4 after a kernel
-// that read 600 MB and 39.9 / 21.5 after one that wrote them; over 1.07 GB 187 / 168,
-// page scores of 324 MB 78 / 69.  Where the cache still holds the data they are
-// slower (three sets of 84 MB in turns: 19.4 / 20.5).
+// 16 bytes of what a launch reads once for the most part, as a decode step does a
+// layer's cache: a non-temporal load, which takes no room in the last-level cache,
+// whose lines other kernels have written to or will read.  Plain / non-temporal loads
+// in microseconds, attention over 84 MB of selected pages 22.4 / 21.4 after a kernel
+// that read 600 MB and 39.9 / 21.5 after one that wrote them; over 1.07 GB 186 / 168,
+// page scores of 324 MB 79 / 70.  Where the cache still holds the data they are
+// slower (three sets in turns, 84 MB of attention 19.2 / 20.3, scores of 13 MB 12.4 /
+// 12.9), and where rows share all that they read: 64 rows that attend to the same
+// 256 pages 73.7 / 77.9; to the same 128 and 128 of their own 132.8 / 123.5, scores of 56
+// rows of 8192-32768 tokens whose first 8192 are shared 62.3 / 58.3.
 template <typename V>
 __device__ inline V ld16_once(const void* p) {
   return __builtin_bit_cast(V, __builtin_nontemporal_load((const u32x4*)p));

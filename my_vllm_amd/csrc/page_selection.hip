@@ -442,9 +442,11 @@ __device__ inline void choose(const Scored& r, int want, int32_t* out, ChoiceLds
 //
 // Lanes 0-31 take one page's 512 bytes and lanes 32-63 the next one's, 16 bytes
 // a lane: lane % 32 / 16 the minima or the maxima, lane % 16 the channels.
-// Products and sums are in 64 bits: products of 16-bit values are exact there
-// and sums of them nearly so, so that which page is taken does not hang on the
-// order of a sum.
+// Products and sums are in 64 bits and round there (P and N are sums of up to 16
+// queries, a score of 256 products), all in one order: pages of equal bounds have equal
+// scores wherever they lie, and scores whose sums are exact, as those of whole numbers
+// are, tie where they are equal.  Other scores may round apart by 2^-48 of the sum of
+// their terms' sizes (at most 28 roundings of 2^-53).  Sums in 32 bits instead take 67.2 us of the 69.9 and 11.4 of 13.0 at 37 rows.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParams p, int chunk, int chunks,
                                                                     uint32_t blocks, BoundsParams update) {
@@ -691,8 +693,9 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
                                 int64_t num_pages, const int32_t* block_tables, int64_t block_table_stride,
                                 int64_t table_width, const int32_t* seq_lens, int64_t num_seqs, int64_t num_selected,
                                 int64_t sink_pages, int64_t recent_pages, int32_t* tables, int32_t* lens,
-                                const void* k_cache, int64_t page_stride, int64_t token_stride, void* workspace, int64_t workspace_bytes, int num_q_heads, int num_kv_heads,
-                                int head_dim, int page_size, int dtype, void* stream) {
+                                const void* k_cache, int64_t page_stride, int64_t token_stride, void* workspace,
+                                int64_t workspace_bytes, int num_q_heads, int num_kv_heads, int head_dim,
+                                int page_size, int dtype, void* stream) {
   using namespace mva;
   if (head_dim != 128 || page_size != kPageTokens) return set_error("page selection: head_dim must be 128, page_size 16");
   if (dtype != kBF16 && dtype != kF16) return set_error("page selection: dtype must be bf16 or fp16");
@@ -719,10 +722,11 @@ extern "C" int mva_select_pages(const void* q, int64_t q_token_stride, int64_t q
       (uint64_t*)(ws + kSelectionHeaderBytes + selection_part_bytes(num_seqs, num_q_heads, num_selected)),
       (int*)ws, num_kv_heads, num_q_heads / num_kv_heads};
   // Chunks: as small as 128 pages (16 a wavefront) as long as that makes no more
-  // workgroups than the GPU holds at a time.  One row of 30001 tokens at 8 KV heads
-  // in chunks of 128, 256 and 512 pages 9.5, 10.2 and 13.0 us; 448 (row, KV head)
-  // pairs of 512-2048 pages in one workgroup each 77 us, in chunks of 1024 pages 86,
-  // of 512 88.
+  // workgroups than the GPU holds at a time.  In microseconds, chunks of 128, 256 and
+  // 512 pages: one row of 30001 tokens at 8 KV heads 9.7, 10.4 and 13.1; 8 rows of
+  // 1024-4096 at 8 heads 8.1, 8.5 and 9.1; 37 of 300-6000 at 4 heads (at most 3, 2 and 1
+  // workgroups a row) 13.0, 14.8 and 12.6.  448 (row, KV head) pairs of 512-2048 pages
+  // in one workgroup each 70, in chunks of 1024 pages 83, of 512 86.
   const int64_t most = table_width - sink_pages - recent_pages;
   int64_t chunk = kBatch * kSelectWaves;
   while (chunk < most && rows * ((most + chunk - 1) / chunk) > kSelectGroups) chunk *= 2;

@@ -1333,8 +1333,9 @@ def select_pages(
     ``N`` the sums of the positive and of the negative parts of the KV head's
     queries: no key of the page has a larger product with them, summed over the
     queries.  Scores are held in 64 bits; NaN ranks above everything, ties go to
-    the lowest place.  An infinite bound counts only for queries of its sign; with
-    a query of 0 it makes the score NaN, as an infinite query does with a bound of 0.
+    the lowest place.  An infinite maximum counts for positive queries alone, an
+    infinite minimum for negative ones; either makes the score NaN with a query of
+    0, as an infinite query does with a bound of 0.
 
     Returns ``(tables, lens)``: int32 ``[S, Hkv, num_selected]`` page ids in the
     order of their places, -1 after a row's last, and int32 ``[S]`` the tokens
