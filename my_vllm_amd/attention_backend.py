@@ -1686,11 +1686,12 @@ class MI355XSparseAttentionBackendMixin(MI355XAttentionBackendMixin):
     def _take_stream(self, device: torch.device) -> None:
         """Make the current stream's buffers the ones that eager steps write.
 
-        Steps that one host thread issues on two streams may overlap, so each has an output, a selection
-        workspace and a prefill workspace of its own (and plans its prefill tiles
-        anew after a change of streams).  The buffers that have lain unused the
-        longest go once more than ``max_idle_streams`` streams have some: none was used on
-        another stream than its own, whose order their memory's next use keeps."""
+        Steps that one host thread issues on two streams may overlap, so each has an
+        output, a selection workspace and a prefill workspace of its own (and plans
+        its prefill tiles anew after a change of streams).  The buffers that have lain
+        unused the longest go once more than ``max_idle_streams`` streams have some: none
+        was used on another stream than its own, whose order their memory's next use
+        keeps."""
         stream = (device.index, _native.stream_of(device.index))
         if stream == self._stream:
             return

@@ -563,6 +563,7 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectParam
     // Again, two pages at a time, for what an infinity makes of a weight that stands for no
     // query: 0 times it is NaN above and nothing here, where it is a NaN only if a query or
     // a bound is that 0.  Scores without infinities come out as they were, bit for bit.
+    __builtin_amdgcn_s_waitcnt(0);  // other lanes' keys at these places have been written
     uint32_t part = 0, zero = 0, infinite = 0;  // a bit a channel: queries that have this part, are 0, are infinite
     const T* q = (const T*)p.q + s * p.q_tok_stride + (int64_t)h * p.group * p.q_head_stride + 8 * (piece & 15);
 #pragma unroll 1
